@@ -274,7 +274,8 @@ def _append(state):
         if case['type'] == 'e4m3':
             # The smallest power of two that brings the row's largest magnitude to 448 or below.
             mantissa, power = torch.frexp(rows.abs().amax(-1))
-            byte = torch.where(mantissa <= 0.875, power - 9, power - 8).clamp(-126, 127) + 127
+            power = torch.where(mantissa <= 0.875, power - 9, power - 8)
+            byte = torch.where(mantissa == 0, -126, power.clamp(-126, 127)) + 127
             state['exponents'][where, :, inside, side] = byte.to(torch.uint8)
             rows = (rows * _power(254 - byte)[..., None]).to(torch.float8_e4m3fn).view(torch.uint8)
         pool[where, :, inside] = rows.to(pool.dtype)
