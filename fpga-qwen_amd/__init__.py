@@ -34,6 +34,25 @@ class Options(ctypes.Structure):
     _fields_ = [('decode_threads', ctypes.c_int), ('prefill_threads', ctypes.c_int), ('context', ctypes.c_int)]
 
 
+class PagedCache(ctypes.Structure):
+    """qwen_gpu_paged_cache: where a paged key-value cache's rows lie (device
+    pointers as integers, strides in elements)."""
+    _fields_ = [('keys', ctypes.c_void_p), ('values', ctypes.c_void_p), ('exponents', ctypes.c_void_p),
+                ('page_stride', ctypes.c_int64), ('head_stride', ctypes.c_int64), ('slot_stride', ctypes.c_int64),
+                ('pages', ctypes.c_int), ('page_size', ctypes.c_int), ('kv_heads', ctypes.c_int),
+                ('head_dim', ctypes.c_int), ('type', ctypes.c_int)]
+
+
+class PagedBatch(ctypes.Structure):
+    """qwen_gpu_paged_batch: the sequences of a call on a paged cache."""
+    _fields_ = [('table', ctypes.c_void_p), ('lengths', ctypes.c_void_p), ('offsets', ctypes.c_void_p),
+                ('seen', ctypes.c_void_p), ('weights', ctypes.c_void_p), ('positions', ctypes.c_void_p),
+                ('track_stride', ctypes.c_int64), ('sequences', ctypes.c_int), ('table_stride', ctypes.c_int),
+                ('max_length', ctypes.c_int), ('rows', ctypes.c_int), ('total_rows', ctypes.c_int)]
+
+
+PAGED_TYPES = {'f16': 0, 'bf16': 1, 'e4m3': 2}
+
 SIGNATURES = {
     'qwen_gpu_last_error': (ctypes.c_char_p, []),
     'qwen_gpu_create': (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(Options), ctypes.POINTER(ctypes.c_void_p)]),
@@ -96,6 +115,18 @@ SIGNATURES = {
     'qwen_gpu_op_gemv_time': (ctypes.c_int, [ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_void_p,
                                              ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, _c_float_p]),
     'qwen_gpu_op_copy': (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    'qwen_gpu_op_paged_workspace': (ctypes.c_int, [ctypes.POINTER(PagedCache), ctypes.POINTER(PagedBatch),
+                                                   ctypes.c_int, _c_size_p]),
+    'qwen_gpu_op_paged_append': (ctypes.c_int, [ctypes.POINTER(PagedCache), ctypes.POINTER(PagedBatch),
+                                                ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64,
+                                                ctypes.c_void_p]),
+    'qwen_gpu_op_paged_attention': (ctypes.c_int, [ctypes.POINTER(PagedCache), ctypes.POINTER(PagedBatch),
+                                                   ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float,
+                                                   ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
+                                                   ctypes.c_size_t, ctypes.c_void_p]),
+    'qwen_gpu_op_paged_evict': (ctypes.c_int, [ctypes.POINTER(PagedCache), ctypes.POINTER(PagedBatch), ctypes.c_int,
+                                               ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p,
+                                               ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     'qwen_gpu_time_kernel': (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, _c_float_p]),
 }
 
@@ -596,3 +627,132 @@ def gemm_static(a, w, c=None):
     _check(_LIB.qwen_gpu_op_gemm_static(ad.ptr, wd.ptr, cd.ptr, m, n, k, int(c is not None), None))
     synchronize()
     return cd.to_array(np.float32, m * n).reshape(m, n)
+
+
+class PagedKV:
+    """A paged key-value cache and its sequences (qwen_gpu_op_paged_*), NumPy
+    in and out. ``table`` [sequences, max_pages] names each sequence's pages
+    (-1: none yet) and belongs to the caller, who may change it between
+    calls; ``lengths`` are the cached rows of each sequence and ``seen`` the
+    tokens of its text, evicted ones too. Pools are [page][head][slot][d].
+    ``track`` keeps the weights and positions that evict() goes by."""
+
+    def __init__(self, sequences, pages, max_pages, page_size=16, kv_heads=8, head_dim=128, type='f16', track=False):
+        if type not in PAGED_TYPES:
+            raise ValueError(f'type must be one of {", ".join(PAGED_TYPES)}, got {type!r}')
+        if min(sequences, pages, max_pages, page_size, kv_heads, head_dim) < 1:
+            raise ValueError('a paged cache needs sequences, pages, slots, heads and channels')
+        self.kv_heads, self.head_dim, self.page_size, self.pages = kv_heads, head_dim, page_size, pages
+        self.table = np.full((sequences, max_pages), -1, np.int32)
+        self.lengths, self.seen = np.zeros(sequences, np.int32), np.zeros(sequences, np.int32)
+        self._counts = np.zeros(sequences, np.int32)
+        slots = max_pages * page_size
+        size = 1 if type == 'e4m3' else 2
+
+        def zeros(count, dtype):
+            return DeviceBuffer.from_array(np.zeros(count, dtype))
+
+        pool = pages * kv_heads * page_size * head_dim * size
+        self._keys, self._values = zeros(pool, np.uint8), zeros(pool, np.uint8)
+        self._exponents = zeros(pages * kv_heads * page_size * 2, np.uint8) if type == 'e4m3' else None
+        tracked = sequences * kv_heads * slots
+        self._weights = zeros(tracked, np.float32) if track else None
+        self._positions = zeros(tracked, np.int32) if track else None
+        self._workspace = None
+        self._cache = PagedCache(self._keys.ptr, self._values.ptr, self._exponents.ptr if self._exponents else None,
+                                 kv_heads * page_size * head_dim, page_size * head_dim, head_dim, pages, page_size,
+                                 kv_heads, head_dim, PAGED_TYPES[type])
+        self._slots = slots
+
+    def _batch(self, rows, total):
+        """The batch's description and the device arrays that it points to."""
+        if self.table.shape[1] * self.page_size != self._slots or self.table.shape[0] != self.lengths.size:
+            raise ValueError('table must keep its shape')
+        offsets = np.concatenate(([0], np.cumsum(self._counts))).astype(np.int32)
+        held = [DeviceBuffer.from_array(np.ascontiguousarray(x, np.int32))
+                for x in (self.table, self.lengths, offsets, self.seen)]
+        batch = PagedBatch(held[0].ptr, held[1].ptr, held[2].ptr, held[3].ptr,
+                           self._weights.ptr if self._weights else None,
+                           self._positions.ptr if self._positions else None, self._slots, self.lengths.size,
+                           self.table.shape[1], self._slots, rows, total)
+        return batch, held
+
+    def _space(self, batch, query_heads):
+        need = ctypes.c_size_t()
+        _check(_LIB.qwen_gpu_op_paged_workspace(ctypes.byref(self._cache), ctypes.byref(batch), query_heads,
+                                                ctypes.byref(need)))
+        if self._workspace is None or self._workspace.nbytes < need.value:
+            self._workspace = DeviceBuffer.from_array(np.zeros(need.value, np.uint8))
+        return self._workspace
+
+    def append(self, keys, values, counts=None):
+        """New rows [total, kv_heads, head_dim] behind the sequences' cached
+        ones: counts[s] rows of sequence s, one after the other (None: one
+        each). Their pages must be in the table."""
+        counts = np.ones(self.lengths.size, np.int32) if counts is None else np.asarray(counts, np.int32)
+        keys, values = np.ascontiguousarray(keys, np.float32), np.ascontiguousarray(values, np.float32)
+        shape = (int(counts.sum()), self.kv_heads, self.head_dim)
+        if counts.shape != self.lengths.shape or (counts < 0).any():
+            raise ValueError(f'need one count of new rows for each of {self.lengths.size} sequences')
+        if keys.shape != shape or values.shape != shape:
+            raise ValueError(f'keys and values must both be {shape}, got {keys.shape} and {values.shape}')
+        if (self.lengths + counts > self._slots).any():
+            raise ValueError(f'a sequence has more than {self._slots} rows')
+        self._counts = counts
+        self.lengths, self.seen = self.lengths + counts, self.seen + counts
+        if not shape[0]:
+            return
+        batch, held = self._batch(int(counts.max()), shape[0])
+        k, v = DeviceBuffer.from_array(keys), DeviceBuffer.from_array(values)
+        stride = self.kv_heads * self.head_dim
+        _check(_LIB.qwen_gpu_op_paged_append(ctypes.byref(self._cache), ctypes.byref(batch), k.ptr, stride, v.ptr,
+                                             stride, None))
+        synchronize()
+        del held
+
+    def attention(self, queries, scale=None):
+        """Attention of the rows appended last: queries [total, query_heads,
+        head_dim], the same out. scale None: head_dim^-0.5."""
+        queries = np.ascontiguousarray(queries, np.float32)
+        total = int(self._counts.sum())
+        if queries.ndim != 3 or queries.shape[0] != total or queries.shape[2] != self.head_dim:
+            raise ValueError(f'queries must be [{total}, query_heads, {self.head_dim}], got {queries.shape}')
+        if not total:
+            return np.zeros_like(queries)
+        heads = queries.shape[1]
+        batch, held = self._batch(int(self._counts.max()), total)
+        space, q, out = self._space(batch, heads), DeviceBuffer.from_array(queries), DeviceBuffer(queries.nbytes)
+        stride = heads * self.head_dim
+        _check(_LIB.qwen_gpu_op_paged_attention(ctypes.byref(self._cache), ctypes.byref(batch), q.ptr, stride, heads,
+                                                self.head_dim ** -0.5 if scale is None else scale, out.ptr, stride,
+                                                space.ptr, space.nbytes, None))
+        synchronize()
+        del held
+        return out.to_array(np.float32, queries.size).reshape(queries.shape)
+
+    def evict(self, keep, sinks=0, recent=0):
+        """Cuts every sequence to at most `keep` rows of each KV head (weights
+        and positions are changed in place). Pages behind the new lengths are
+        the caller's again."""
+        batch, held = self._batch(1, 0)
+        space, lengths = self._space(batch, self.kv_heads), DeviceBuffer(self.lengths.nbytes)
+        _check(_LIB.qwen_gpu_op_paged_evict(ctypes.byref(self._cache), ctypes.byref(batch), keep, sinks, recent,
+                                            lengths.ptr, batch.weights, batch.positions, space.ptr, space.nbytes,
+                                            None))
+        synchronize()
+        del held
+        self.lengths = lengths.to_array(np.int32, self.lengths.size)
+        self._counts = np.zeros_like(self._counts)
+
+    def _tracked(self, buffer, dtype):
+        if buffer is None:
+            raise ValueError('this cache does not track')
+        shape = (self.lengths.size, self.kv_heads, self._slots)
+        return buffer.to_array(dtype, int(np.prod(shape))).reshape(shape)
+
+    def weights(self):
+        """Accumulated attention weights [sequences, kv_heads, max_pages * page_size]."""
+        return self._tracked(self._weights, np.float32)
+
+    def positions(self):
+        return self._tracked(self._positions, np.int32)

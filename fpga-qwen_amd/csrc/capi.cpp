@@ -6,6 +6,7 @@
 #include "batch.hpp"
 #include "engine.hpp"
 #include "pack.hpp"
+#include "paged.hpp"
 #include "prefill.hpp"
 
 struct qwen_gpu_model {
@@ -466,6 +467,52 @@ int qwen_gpu_op_copy(const void* src, void* dst, size_t bytes, void* stream) {
         need(src, "src");
         need(dst, "dst");
         qwen_hip::launch_copy(src, dst, bytes, static_cast<hipStream_t>(stream));
+        hip_ok(hipGetLastError());
+    });
+}
+
+int qwen_gpu_op_paged_workspace(const qwen_gpu_paged_cache* cache, const qwen_gpu_paged_batch* batch, int query_heads,
+                                size_t* bytes) {
+    return guarded([&] {
+        need(cache, "cache");
+        need(batch, "batch");
+        need(bytes, "bytes");
+        *bytes = 0;
+        *bytes = qwen_hip::paged_workspace_bytes(*cache, *batch, query_heads);
+    });
+}
+
+int qwen_gpu_op_paged_append(const qwen_gpu_paged_cache* cache, const qwen_gpu_paged_batch* batch, const float* keys,
+                             int64_t key_stride, const float* values, int64_t value_stride, void* stream) {
+    return guarded([&] {
+        need(cache, "cache");
+        need(batch, "batch");
+        qwen_hip::launch_paged_append(*cache, *batch, keys, key_stride, values, value_stride,
+                                      static_cast<hipStream_t>(stream));
+        hip_ok(hipGetLastError());
+    });
+}
+
+int qwen_gpu_op_paged_attention(const qwen_gpu_paged_cache* cache, const qwen_gpu_paged_batch* batch,
+                                const float* queries, int64_t query_stride, int query_heads, float scale, float* out,
+                                int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream) {
+    return guarded([&] {
+        need(cache, "cache");
+        need(batch, "batch");
+        qwen_hip::launch_paged_attention(*cache, *batch, queries, query_stride, query_heads, scale, out, out_stride,
+                                         workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+        hip_ok(hipGetLastError());
+    });
+}
+
+int qwen_gpu_op_paged_evict(const qwen_gpu_paged_cache* cache, const qwen_gpu_paged_batch* batch, int keep, int sinks,
+                            int recent, int32_t* new_lengths, float* new_weights, int32_t* new_positions,
+                            void* workspace, size_t workspace_bytes, void* stream) {
+    return guarded([&] {
+        need(cache, "cache");
+        need(batch, "batch");
+        qwen_hip::launch_paged_evict(*cache, *batch, keep, sinks, recent, new_lengths, new_weights, new_positions,
+                                     workspace, workspace_bytes, static_cast<hipStream_t>(stream));
         hip_ok(hipGetLastError());
     });
 }

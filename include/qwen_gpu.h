@@ -272,6 +272,107 @@ int qwen_gpu_op_gemv_time(const uint16_t* tiled, size_t copy_stride, int copies,
 /* Plain 16-byte-per-thread device copy (bytes a multiple of 16). No reference
  * counterpart: a kernel of known traffic for calibrating HBM byte counters. */
 int qwen_gpu_op_copy(const void* src, void* dst, size_t bytes, void* stream);
+/* ---- Paged key-value cache (no reference counterpart) ----
+ *
+ * Keys and values of many sequences in pages of `page_size` slots. Sequence
+ * s holds its j-th cached row in slot j % page_size of page
+ * table[s * table_stride + j / page_size]; sequences may share pages that
+ * neither appends to nor evicts from. Element d of kv head h, slot i, page p
+ * lies at p * page_stride + h * head_stride + i * slot_stride + d (strides in
+ * elements, equal for keys and values, multiples of 16 bytes; both pointers
+ * aligned to 16 bytes; rows must not overlap). [page][head][slot][d] and
+ * [page][slot][head][d] are two such layouts, and a contiguous
+ * [head][position][d] cache is one with page_stride = page_size * head_dim.
+ *
+ * Everything else is indexed per sequence, so that shared pages share no
+ * state: row j of kv head h of sequence s has its accumulated attention
+ * weight and its position in the text at [(s * kv_heads + h) * track_stride
+ * + j] of `weights` and `positions`.
+ *
+ * The device reads table, lengths, offsets and seen when the launch runs, so
+ * a captured graph follows them. What they hold cannot be checked on the
+ * host and is bounded on the device instead: lengths are taken into 0 ..
+ * max_length; a slot whose page is not in 0 .. pages - 1 is neither written
+ * nor attended; rows outside 0 .. total_rows - 1 are neither read nor
+ * written; offsets must not fall (where they do, which of its rows a sequence
+ * gets is open). */
+#define QWEN_GPU_PAGED_F16 0
+#define QWEN_GPU_PAGED_BF16 1
+#define QWEN_GPU_PAGED_E4M3 2   /* rows of e4m3 * 2^(exponent byte - 127) */
+
+typedef struct qwen_gpu_paged_cache {
+    void* keys;
+    void* values;
+    uint8_t* exponents;         /* E4M3: [pages][kv_heads][page_size][2], of the key row and of the value row */
+    int64_t page_stride;
+    int64_t head_stride;
+    int64_t slot_stride;
+    int pages;
+    int page_size;              /* 1..65536 */
+    int kv_heads;               /* 1..1024 */
+    int head_dim;               /* 64, 128 or 256 */
+    int type;                   /* QWEN_GPU_PAGED_* */
+} qwen_gpu_paged_cache;
+
+typedef struct qwen_gpu_paged_batch {
+    const int32_t* table;       /* [sequences][table_stride] */
+    const int32_t* lengths;     /* [sequences]: cached rows, the new ones among them */
+    const int32_t* offsets;     /* [sequences + 1]: new rows offsets[s] .. offsets[s + 1] - 1 are sequence s's, at
+                                 * most `rows` of them; NULL: s has rows s * rows .. (s + 1) * rows - 1 */
+    const int32_t* seen;        /* [sequences]: tokens of the text so far, evicted ones too; NULL: lengths */
+    float* weights;             /* [sequences][kv_heads][track_stride], or NULL: not tracked */
+    int32_t* positions;         /* the same */
+    int64_t track_stride;       /* at least max_length where one of them is given */
+    int sequences;              /* 1..65536 */
+    int table_stride;           /* pages in a row of the table */
+    int max_length;             /* 1..table_stride * page_size, at most 2^24 */
+    int rows;                   /* 1..max_length: most new rows of a sequence */
+    int total_rows;             /* new rows of all sequences; sequences * rows where offsets is NULL */
+} qwen_gpu_paged_batch;
+
+/* Bytes of workspace (device memory, aligned to 16) that the attention and the eviction of
+ * this cache and batch need at most. The caller zeroes it once; every call
+ * leaves it ready for the next, of whatever shape it suffices for. Calls
+ * that may overlap need workspaces of their own. */
+int qwen_gpu_op_paged_workspace(const qwen_gpu_paged_cache* cache, const qwen_gpu_paged_batch* batch, int query_heads,
+                                size_t* bytes);
+/* The new rows' keys and values, FP32, rounded to the cache's type (to
+ * nearest, ties to even) in their slots: row i of sequence s's n goes to slot
+ * lengths[s] - n + i, a negative one nowhere. Head h of row r lies at keys +
+ * r * key_stride + h * head_dim, so a projection's rows are read where they
+ * are. E4M3: the exponent is the smallest (of -126 .. 127) that brings the row's largest
+ * finite magnitude to 448 or below; infinities and NaN become NaN. Where tracked,
+ * the slots' weights are set to 0 and their positions to seen[s] - n + i.
+ * No two rows of a call may go to one slot. */
+int qwen_gpu_op_paged_append(const qwen_gpu_paged_cache* cache, const qwen_gpu_paged_batch* batch, const float* keys,
+                             int64_t key_stride, const float* values, int64_t value_stride, void* stream);
+/* Attention of the new rows over the cached ones, which hold the new ones
+ * already: query head g of row r (at queries + r * query_stride + g *
+ * head_dim, FP32) reads kv head g / (query_heads / kv_heads). Row i of
+ * sequence s's n attends slots 0 .. lengths[s] - n + i with softmax(scale *
+ * q . k); a row that has none gives zeros. out is laid out like queries, with
+ * out_stride. With weights, weights[s][h][j] grows by the sum of slot j's
+ * softmax weights over h's query heads and s's new rows. Sums are FP32, in
+ * an order that depends on the call's shapes and lengths alone. Keys and values that a row attends are finite; those it
+ * does not attend may be anything. */
+int qwen_gpu_op_paged_attention(const qwen_gpu_paged_cache* cache, const qwen_gpu_paged_batch* batch,
+                                const float* queries, int64_t query_stride, int query_heads, float scale, float* out,
+                                int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
+/* Cuts every sequence longer than `keep` to `keep` rows, for each kv head by
+ * itself: rows at positions below `sinks` or from seen[s] - recent on stay
+ * (sinks + recent <= keep), then those of the largest weight, of equal ones
+ * the lowest slot (NaN counts as the lowest weight, -0 as 0). The kept rows
+ * in slots from keep on move, in their order, into the holes before it, so
+ * the rows no longer lie in the order of their positions: attention of the
+ * rows that are appended next does not depend on it. new_lengths[s] =
+ * min(lengths[s], keep), not the array `lengths`; new_weights and
+ * new_positions receive the first new_lengths[s] entries and may be the
+ * batch's own arrays (else they must not overlap them). weights and
+ * positions are needed; offsets, rows and total_rows are not used. The
+ * sequences' pages must be their own. */
+int qwen_gpu_op_paged_evict(const qwen_gpu_paged_cache* cache, const qwen_gpu_paged_batch* batch, int keep, int sinks,
+                            int recent, int32_t* new_lengths, float* new_weights, int32_t* new_positions,
+                            void* workspace, size_t workspace_bytes, void* stream);
 /* Average milliseconds of one standalone launch of a decode kernel on the
  * model's stream, timed with HIP events (which: 0 norm+QKV, 1 attention,
  * 2 O, 3 norm+gate/up, 4 down, 5 lm_head, 6 the fused FFN kernel and 7 the

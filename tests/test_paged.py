@@ -1,0 +1,162 @@
+"""What the paged cache's entry points refuse (CPU: every check of arguments
+comes before the device is used), and the arithmetic of their NumPy oracle."""
+import ctypes
+import sys
+from pathlib import Path
+
+import numpy as np
+import pytest
+
+sys.path.insert(0, str(Path(__file__).resolve().parent))
+import paged_reference as ref  # noqa: E402
+
+AT = 1 << 20  # stands for device memory; never used
+
+
+def cache(q, **more):
+    fields = dict(keys=AT, values=AT, exponents=None, page_stride=8 * 16 * 128, head_stride=16 * 128, slot_stride=128,
+                  pages=4, page_size=16, kv_heads=8, head_dim=128, type=0)
+    fields.update(more)
+    return q.PagedCache(**fields)
+
+
+def batch(q, **more):
+    fields = dict(table=AT, lengths=AT, offsets=None, seen=None, weights=AT, positions=AT, track_stride=64,
+                  sequences=2, table_stride=4, max_length=64, rows=1, total_rows=2)
+    fields.update(more)
+    return q.PagedBatch(**fields)
+
+
+def refused(package, message, c=None, b=None, op='append', **call):
+    lib = package.load_library()
+    c, b = c if c is not None else cache(package), b if b is not None else batch(package)
+    given = dict(k=AT, v=AT, k_stride=1024, v_stride=1024, q=AT, q_stride=2048, heads=16, out=AT, out_stride=2048,
+                 space=AT, bytes=1 << 30, keep=8, sinks=1, recent=1, n=2 * AT, w=AT, p=AT)
+    given.update(call)
+    g = given
+    if op == 'append':
+        status = lib.qwen_gpu_op_paged_append(c, b, g['k'], g['k_stride'], g['v'], g['v_stride'], None)
+    elif op == 'attention':
+        status = lib.qwen_gpu_op_paged_attention(c, b, g['q'], g['q_stride'], g['heads'], 0.1, g['out'], g['out_stride'],
+                                                 g['space'], g['bytes'], None)
+    else:
+        status = lib.qwen_gpu_op_paged_evict(c, b, g['keep'], g['sinks'], g['recent'], g['n'], g['w'], g['p'],
+                                             g['space'], g['bytes'], None)
+    assert status == 1
+    error = lib.qwen_gpu_last_error().decode()
+    assert message in error, error
+
+
+@pytest.mark.parametrize('op', ['append', 'attention', 'evict'])
+@pytest.mark.parametrize('message,fields', [
+    ('Null argument: keys', dict(keys=None)), ('Null argument: values', dict(values=None)),
+    ('Null argument: exponents', dict(type=2)), ('Unknown paged cache type', dict(type=3)),
+    ('head_dim must be', dict(head_dim=96)), ('head_dim must be', dict(head_dim=0)),
+    ('Page size must be', dict(page_size=0)), ('Page size must be', dict(page_size=65537)),
+    ('needs pages', dict(pages=0)), ('kv_heads must be', dict(kv_heads=0)), ('kv_heads must be', dict(kv_heads=1025)),
+    ('let rows overlap', dict(slot_stride=120)), ('let rows overlap', dict(head_stride=15 * 128)),
+    ('let rows overlap', dict(page_stride=0)), ('let rows overlap', dict(slot_stride=-128)),
+    ('let rows overlap', dict(page_stride=1 << 41)), ('multiples of 16 bytes', dict(page_stride=8 * 16 * 128 + 4))])
+def test_caches_refused(qpkg, op, message, fields):
+    refused(qpkg, message, cache(qpkg, **fields), op=op)
+
+
+@pytest.mark.parametrize('op', ['append', 'attention', 'evict'])
+@pytest.mark.parametrize('message,fields', [
+    ('Null argument: table', dict(table=None)), ('Null argument: lengths', dict(lengths=None)),
+    ('sequences must be', dict(sequences=0)), ('sequences must be', dict(sequences=65537)),
+    ('table needs entries', dict(table_stride=0)), ('max_length must be', dict(max_length=0)),
+    ('max_length must be', dict(max_length=65)), ('max_length must be', dict(max_length=1 << 25, table_stride=1 << 25)),
+    ('track_stride is below', dict(track_stride=63)), ('track_stride is too large', dict(track_stride=1 << 33))])
+def test_batches_refused(qpkg, op, message, fields):
+    refused(qpkg, message, b=batch(qpkg, **fields), op=op)
+
+
+@pytest.mark.parametrize('op', ['append', 'attention'])
+@pytest.mark.parametrize('message,fields', [
+    ('rows must be', dict(rows=0)), ('rows must be', dict(rows=65)), ('total_rows must be', dict(total_rows=3)),
+    ('total_rows must be', dict(total_rows=-1, offsets=AT)),
+    ('total_rows must be', dict(total_rows=(1 << 24) + 1, offsets=AT))])
+def test_new_rows_refused(qpkg, op, message, fields):
+    refused(qpkg, message, b=batch(qpkg, **fields), op=op)
+
+
+@pytest.mark.parametrize('op,message,call', [
+    ('append', 'Null argument: new keys', dict(k=None)), ('append', 'Null argument: new values', dict(v=None)),
+    ('append', 'stride below', dict(k_stride=1023)), ('append', 'stride below', dict(v_stride=-1)),
+    ('append', 'too large', dict(k_stride=1 << 33)),
+    ('attention', 'Null argument: queries', dict(q=None)), ('attention', 'Null argument: out', dict(out=None)),
+    ('attention', 'multiple of kv_heads', dict(heads=12)), ('attention', 'multiple of kv_heads', dict(heads=0)),
+    ('attention', 'stride below', dict(q_stride=2047)), ('attention', 'stride below', dict(out_stride=0)),
+    ('evict', 'Null argument: new_lengths', dict(n=None)), ('evict', 'Null argument: new_weights', dict(w=None)),
+    ('evict', 'Null argument: new_positions', dict(p=None)), ('evict', 'keep must be', dict(keep=0)),
+    ('evict', 'sinks + recent <= keep', dict(sinks=5, recent=4)), ('evict', 'sinks + recent <= keep', dict(sinks=-1)),
+    ('evict', 'sinks + recent <= keep', dict(recent=2 ** 31 - 1)), ('evict', 'overlaps lengths', dict(n=AT)),
+    ('evict', 'overlaps lengths', dict(n=AT + 4)), ('evict', 'overlaps weights', dict(w=AT + 4)),
+    ('evict', 'overlaps positions', dict(p=AT - 4))])
+def test_calls_refused(qpkg, op, message, call):
+    refused(qpkg, message, op=op, **call)
+
+
+def test_evict_needs_what_it_goes_by(qpkg):
+    refused(qpkg, 'Null argument: weights', b=batch(qpkg, weights=None), op='evict')
+    refused(qpkg, 'Null argument: positions', b=batch(qpkg, positions=None), op='evict')
+
+
+@pytest.mark.parametrize('op', ['append', 'attention', 'evict'])
+def test_host_memory_refused(qpkg, op):
+    """Pointers that no kernel could read end in an error, not in a fault."""
+    host = np.zeros(1 << 16, np.uint8)
+    at = host.ctypes.data + (-host.ctypes.data) % 16
+    refused(qpkg, 'Not device memory: keys', cache(qpkg, keys=at, values=at), op=op)
+
+
+def test_null_descriptions_refused(qpkg):
+    lib, c, b = qpkg.load_library(), cache(qpkg), batch(qpkg)
+    size = ctypes.c_size_t()
+    for status in (lib.qwen_gpu_op_paged_append(None, b, AT, 1024, AT, 1024, None),
+                   lib.qwen_gpu_op_paged_attention(c, None, AT, 2048, 16, 0.1, AT, 2048, AT, 1 << 30, None),
+                   lib.qwen_gpu_op_paged_evict(None, None, 8, 0, 0, AT, AT, AT, AT, 1 << 30, None),
+                   lib.qwen_gpu_op_paged_workspace(c, None, 16, ctypes.byref(size)),
+                   lib.qwen_gpu_op_paged_workspace(c, b, 16, None)):
+        assert status == 1 and 'Null argument' in lib.qwen_gpu_last_error().decode()
+
+
+def test_workspace_bytes(qpkg):
+    """Known without a device, and enough for the lists of half the longest sequence."""
+    lib, size = qpkg.load_library(), ctypes.c_size_t()
+    assert lib.qwen_gpu_op_paged_workspace(cache(qpkg), batch(qpkg), 16, ctypes.byref(size)) == 0
+    assert size.value >= 2 * 8 * 2 * 32 * 4
+    assert lib.qwen_gpu_op_paged_workspace(cache(qpkg), batch(qpkg), 12, ctypes.byref(size)) == 1
+    assert 'multiple of kv_heads' in lib.qwen_gpu_last_error().decode()
+
+
+def test_strides_of_single_axes_do_not_matter(qpkg):
+    """An axis of one entry is never stepped along."""
+    lib, size = qpkg.load_library(), ctypes.c_size_t()
+    c = cache(qpkg, pages=1, page_stride=-3, kv_heads=1, head_stride=1, page_size=16)
+    assert lib.qwen_gpu_op_paged_workspace(c, batch(qpkg), 4, ctypes.byref(size)) == 0
+
+
+def test_oracle_conversions():
+    """The oracle's roundings against NumPy's own and the E4M3 format's values."""
+    rng = np.random.default_rng(0)
+    x = (rng.standard_normal(2000) * np.exp2(rng.integers(-20, 20, 2000))).astype(np.float32)
+    bf16 = ref.from_bits(ref.to_bits(x, 'bf16'), 'bf16')
+    assert (np.abs(bf16 - x) <= np.abs(x) * 2.0 ** -8).all()
+    assert ref.E4M3[0x7e] == 448 and ref.E4M3[1] == 2.0 ** -9 and ref.E4M3[0x38] == 1 and ref.E4M3[0xb8] == -1
+    assert np.isnan(ref.E4M3[[0x7f, 0xff]]).all()
+    codes = np.array([c for c in range(256) if c & 127 != 127], np.uint8)
+    assert np.array_equal(ref.to_e4m3(ref.E4M3[codes]), codes)
+    assert ref.E4M3[ref.to_e4m3([17, 19, 463.9, 464, 2.0 ** -10, 3 * 2.0 ** -10])].tolist()[:3] == [16, 20, 448]
+    assert ref.to_e4m3([2.0 ** -10, 3 * 2.0 ** -10]).tolist() == [0, 2]
+    codes, byte = ref.quantise(np.array([[448, 1], [449, 1], [0, 0], [0.875, 0.4375]], np.float32))
+    assert (byte.astype(int) - 127).tolist() == [0, 1, -126, -9] and codes[0, 0] == 0x7e and codes[3, 0] == 0x7e
+
+
+def test_wrapper_checks_arguments(qpkg):
+    """Python's PagedKV refuses what it can see before it allocates."""
+    with pytest.raises(ValueError, match='type must be'):
+        qpkg.PagedKV(1, 1, 1, type='f32')
+    with pytest.raises(ValueError, match='needs sequences'):
+        qpkg.PagedKV(0, 1, 1)
