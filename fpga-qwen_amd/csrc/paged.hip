@@ -4,12 +4,15 @@
 #include <algorithm>
 #include <string>
 
+#include "decode_dev.hpp"
 #include "paged_dev.hpp"
 #include "qwen_common.hpp"
 
 namespace qwen_hip {
 
 namespace {
+constexpr int kEvictHead = 4;  // ints of a unit's moves before its lists
+
 void hip_check(hipError_t e) {
     if (e != hipSuccess) throw std::runtime_error(std::string("HIP error: ") + hipGetErrorString(e));
 }
@@ -126,6 +129,10 @@ void PagedDevice::check(const void* p, const char* what, unsigned alignment) con
     }
     require(a.type != hipMemoryTypeDevice || a.device == device_,
             std::string("On another device than the cache: ") + what);
+}
+
+size_t paged_moves_bytes(const qwen_gpu_paged_cache& c, const qwen_gpu_paged_batch& b, int64_t room) {
+    return size_t(b.sequences) * c.kv_heads * (2 * room + kEvictHead) * sizeof(int32_t);
 }
 
 // ---- append ----
@@ -277,6 +284,7 @@ namespace {
 
 constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64, kEvictBins = 2048;
 constexpr unsigned kEvictFixed = 0xffffffffu;
+constexpr int kEvictFew = 4, kEvictHeld = 8, kMoveRows = 64;
 
 // Weights as whole numbers of the same order; NaN is the lowest, -0 is 0.
 __device__ __forceinline__ unsigned weight_key(float w) {
@@ -285,29 +293,66 @@ __device__ __forceinline__ unsigned weight_key(float w) {
     return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 
+// The lanes' lowest value, in every lane.
+__device__ __forceinline__ uint64_t lowest_of_wave(uint64_t x) {
+    auto with = [&](double other) { x = min(x, __builtin_bit_cast(uint64_t, other)); };
+    with(dev::xor_lanes<32>(__builtin_bit_cast(double, x)));
+    with(dev::xor_lanes<16>(__builtin_bit_cast(double, x)));
+    with(dev::xor_lanes<8>(__builtin_bit_cast(double, x)));
+    with(dev::xor_lanes<4>(__builtin_bit_cast(double, x)));
+    with(dev::xor_lanes<2>(__builtin_bit_cast(double, x)));
+    with(dev::xor_lanes<1>(__builtin_bit_cast(double, x)));
+    return x;
+}
+
 struct EvictArgs {
     int keep, sinks, recent;
     int32_t* new_lengths;
     float* new_weights;
     int32_t* new_positions;
-    int32_t* moves;  // workspace: [sequences * kv_heads][2][room], holes then (from the last) sources
+    int32_t* moves;  // workspace, a unit: their number, padding, holes[room], sources[room] from the last
     int64_t room;
     int size;        // bytes of a row
     bool scaled;     // rows have exponents
 };
 
-// One workgroup per sequence and KV head. The threshold weight (the keep-th
-// largest) is found digit by digit, 11 + 11 + 10 bits from the top: a
-// histogram of the digit among the slots that share the digits so far, and
-// the digit at which the count from above reaches what is still wanted. Of
-// the slots at the threshold the first ones are kept. A hole's rank among
-// holes is its slot less the kept slots before it, and a kept slot's rank
-// needs the same count, so one running count gives both lists.
+// Moves one 16-byte piece of a row (keys, then values, of 2 * size bytes), and
+// with the first piece the row's exponents.
+__device__ __forceinline__ void move_piece(const PagedView& v, const EvictArgs& a, int s, int head, int from, int to,
+                                           int piece) {
+    const int half = a.size / 16;
+    const PageSlot to_at = page_slot(to, v.page_size, v.magic), from_at = page_slot(from, v.page_size, v.magic);
+    const int to_page = v.page_of(s, to_at.page), from_page = v.page_of(s, from_at.page);
+    if (to_page < 0 || from_page < 0) return;
+    char* const pool = piece < half ? v.keys : v.values;
+    const int64_t at = 16 * (piece < half ? piece : piece - half);
+    *reinterpret_cast<uint4_t*>(pool + v.row_at(to_page, head, to_at.slot) + at) =
+        *reinterpret_cast<const uint4_t*>(pool + v.row_at(from_page, head, from_at.slot) + at);
+    if (piece == 0 && a.scaled)
+        *reinterpret_cast<uint16_t*>(v.exponents + v.exponents_at(to_page, head, to_at.slot)) =
+            *reinterpret_cast<const uint16_t*>(v.exponents + v.exponents_at(from_page, head, from_at.slot));
+}
+
+// One workgroup per sequence and KV head chooses what stays, and moves it where
+// `MOVE` (few rows at most); else the next kernel does.
+//
+// A few rows too many (kEvictFew; every step of a cache of fixed length): the
+// lowest weight, of equal ones the last slot, is found that many times. More:
+// the threshold weight (the keep-th largest) is found digit by digit, 11 + 11
+// + 10 bits from the top: a histogram of the digit among the slots that share
+// the digits so far, and the digit at which the count from above reaches what
+// is still wanted. Of the slots at the threshold the first ones are kept. A
+// hole's rank among holes is its slot less the kept slots before it, and a
+// kept slot's rank needs the same count, so one running count gives both
+// lists. Up to kEvictHeld slots a thread's keys stay in registers.
+template <bool MOVE>
 __global__ __launch_bounds__(kEvictThreads) void paged_evict_kernel(PagedView v, EvictArgs a) {
     __shared__ int bins[kEvictBins];
-    __shared__ int2 wave_counts[2][kEvictWaves];
+    __shared__ int2 wave_counts[kEvictHeld][kEvictWaves];
+    __shared__ uint64_t lowest[2][kEvictWaves];
     __shared__ int found[2];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __shared__ int few_holes[kEvictFew], few_sources[kEvictFew];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int s = blockIdx.x / v.kv_heads, head = blockIdx.x - s * v.kv_heads;
     const int n = v.length(s), keep = a.keep;
     const int64_t track = v.track_at(s, head);
@@ -315,113 +360,260 @@ __global__ __launch_bounds__(kEvictThreads) void paged_evict_kernel(PagedView v,
     const int32_t* positions = v.positions + track;
     float* new_weights = a.new_weights + track;
     int32_t* new_positions = a.new_positions + track;
+    const bool copies = new_weights != weights || new_positions != positions;
+    int32_t* const moves = a.moves + int64_t(blockIdx.x) * (2 * a.room + kEvictHead);
     if (head == 0 && tid == 0) a.new_lengths[s] = min(n, keep);
+    if (!MOVE && tid == 0 && n <= keep) moves[0] = 0;
     if (n <= keep) {
-        for (int j = tid; j < n; j += kEvictThreads) {
+        for (int j = tid; copies && j < n; j += kEvictThreads) {
             new_weights[j] = weights[j];
             new_positions[j] = positions[j];
         }
         return;
     }
-    const int64_t late = int64_t(v.seen ? v.seen[s] : v.length(s)) - a.recent;
+    const int64_t late = int64_t(v.seen ? v.seen[s] : n) - a.recent;
     auto key_of = [&](int j) {
         const int p = positions[j];
-        return p < a.sinks || p >= late ? kEvictFixed : weight_key(weights[j]);
+        const float w = weights[j];
+        return p < a.sinks || p >= late ? kEvictFixed : weight_key(w);
     };
-
-    unsigned prefix = 0, known = 0;  // the threshold's digits so far, and which bits they are
-    int wanted = keep;               // slots still to be taken among those that share them
-    for (int digit = 0; digit < 3; ++digit) {
-        const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, width = digit == 2 ? 1024 : 2048;
-        for (int b = tid; b < kEvictBins; b += kEvictThreads) bins[b] = 0;
-        __syncthreads();
-        for (int j = tid; j < n; j += kEvictThreads) {
-            const unsigned key = key_of(j);
-            if ((key & known) == prefix) atomicAdd(&bins[(key >> shift) & (width - 1)], 1);
+    unsigned held[kEvictHeld];
+    const bool holds = n <= kEvictHeld * kEvictThreads;
+    if (holds) {
+        float w[kEvictHeld];
+        int p[kEvictHeld];
+#pragma unroll
+        for (int i = 0; i < kEvictHeld; ++i) {
+            const int j = min(i * kEvictThreads + tid, n - 1);
+            w[i] = weights[j];
+            p[i] = positions[j];
         }
-        __syncthreads();
-        // Thread t holds bins top - 2 t and the one below; counts from above.
-        const int upper = bins[kEvictBins - 1 - 2 * tid], lower = bins[kEvictBins - 2 - 2 * tid];
-        int sum = upper + lower;
-        for (int off = 1; off < 64; off *= 2) {
-            const int other = __shfl_up(sum, off);
-            if (lane >= off) sum += other;
+#pragma unroll
+        for (int i = 0; i < kEvictHeld; ++i) {
+            const int j = i * kEvictThreads + tid;
+            held[i] = p[i] < a.sinks || p[i] >= late ? kEvictFixed : weight_key(w[i]);
+            if (copies && j < keep) {
+                new_weights[j] = w[i];
+                new_positions[j] = p[i];
+            }
         }
-        if (lane == 63) wave_counts[0][wave].x = sum;
-        __syncthreads();
-        int above = sum - upper - lower;
-        for (int w = 0; w < wave; ++w) above += wave_counts[0][w].x;
-        if (above < wanted && above + upper + lower >= wanted) {
-            const bool second = above + upper < wanted;
-            found[0] = kEvictBins - 1 - 2 * tid - second;
-            found[1] = wanted - above - (second ? upper : 0);
-        }
-        __syncthreads();
-        prefix |= unsigned(found[0]) << shift;
-        known |= unsigned(width - 1) << shift;
-        wanted = found[1];
-        __syncthreads();
-    }
-
-    int32_t* const holes = a.moves + int64_t(blockIdx.x) * 2 * a.room;
-    int32_t* const sources = holes + a.room;
-    int above_before = 0, at_before = 0;
-    for (int begin = 0, turn = 0; begin < n; begin += kEvictThreads, turn ^= 1) {
-        const int j = begin + tid;
-        const unsigned key = j < n ? key_of(j) : 0u;
-        const bool above = j < n && key > prefix, at = j < n && key == prefix;
-        const unsigned long long above_mask = __ballot(above), at_mask = __ballot(at);
-        if (lane == 0) wave_counts[turn][wave] = int2{__popcll(above_mask), __popcll(at_mask)};
-        __syncthreads();
-        const unsigned long long before = (1ull << lane) - 1;
-        int above_rank = above_before + __popcll(above_mask & before), at_rank = at_before + __popcll(at_mask & before);
-        for (int w = 0; w < kEvictWaves; ++w) {
-            const int2 c = wave_counts[turn][w];
-            if (w < wave) above_rank += c.x, at_rank += c.y;
-            above_before += c.x;
-            at_before += c.y;
-        }
-        const bool kept = above || (at && at_rank < wanted);
-        const int rank = above_rank + min(at_rank, wanted);  // kept slots before this one
-        if (j == keep) found[0] = keep - rank;               // the rest of them have to move
-        if (j >= n) continue;
-        if (j >= keep) {
-            if (kept && keep - 1 - rank < a.room) sources[keep - 1 - rank] = j;
-        } else if (!kept) {
-            if (j - rank < a.room) holes[j - rank] = j;
-        } else {
+    } else if (copies) {
+        for (int j = tid; j < keep; j += kEvictThreads) {
             new_weights[j] = weights[j];
             new_positions[j] = positions[j];
         }
     }
-    __syncthreads();
-    const int moved = int(min(int64_t(found[0]), a.room));
-    for (int i = tid; i < moved; i += kEvictThreads) {
-        const int to = holes[i], from = sources[moved - 1 - i];
-        new_weights[to] = weights[from];
-        new_positions[to] = positions[from];
+    // f(slot, key) for all slots, this thread's among each 1024 in turn.
+    auto each = [&](auto f) {
+        if (holds) {
+#pragma unroll
+            for (int i = 0; i < kEvictHeld; ++i)
+                if (i * kEvictThreads + tid < n) f(i * kEvictThreads + tid, held[i]);
+        } else {
+            for (int j = tid; j < n; j += kEvictThreads) f(j, key_of(j));
+        }
+    };
+    int32_t *holes = moves + kEvictHead, *sources = holes + a.room;
+    int moved;
+
+    if (n - keep <= kEvictFew && holds) {
+        holes = few_holes;
+        sources = few_sources;
+        int gone[kEvictFew];
+#pragma unroll
+        for (int e = 0; e < kEvictFew; ++e) {
+            gone[e] = -1;
+            if (e >= n - keep) continue;
+            uint64_t low = ~0ull;
+            each([&](int j, unsigned key) {
+                bool out = false;
+#pragma unroll
+                for (int f = 0; f < e; ++f) out |= gone[f] == j;
+                const uint64_t x = uint64_t(key) << 32 | unsigned(~j);
+                if (!out && x < low) low = x;
+            });
+            low = lowest_of_wave(low);
+            if (lane == 0) lowest[e & 1][wave] = low;
+            __syncthreads();
+            low = lowest_of_wave(lowest[e & 1][lane % kEvictWaves]);
+            gone[e] = ~int(unsigned(low));
+        }
+        // The evicted slots before `keep` are the holes, the others' complement the sources, both in order.
+        moved = 0;
+        int behind = 0;
+#pragma unroll
+        for (int e = 0; e < kEvictFew; ++e) {
+            if (e >= n - keep) continue;
+            bool out = false;  // of slot keep + e
+            int rank = 0;      // holes before gone[e]
+#pragma unroll
+            for (int f = 0; f < kEvictFew; ++f) {
+                out |= gone[f] == keep + e;
+                rank += gone[f] >= 0 && gone[f] < gone[e];
+            }
+            if (gone[e] < keep) {
+                if (tid == 0) holes[rank] = gone[e];
+                ++moved;
+            }
+            if (!out) {
+                if (tid == 0) sources[behind] = keep + e;
+                ++behind;
+            }
+        }
+        __syncthreads();
+    } else {
+        unsigned prefix = 0, known = 0;  // the threshold's digits so far, and which bits they are
+        int wanted = keep;               // slots still to be taken among those that share them
+        for (int digit = 0; digit < 3; ++digit) {
+            const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, width = digit == 2 ? 1024 : 2048;
+            bins[tid] = bins[tid + kEvictThreads] = 0;
+            __syncthreads();
+            each([&](int, unsigned key) {
+                if ((key & known) == prefix) atomicAdd(&bins[(key >> shift) & (width - 1)], 1);
+            });
+            __syncthreads();
+            // Thread t holds the t-th pair of bins from the top; counts from above.
+            const int2 pair = reinterpret_cast<const int2*>(bins)[kEvictThreads - 1 - tid];
+            const int upper = pair.y, lower = pair.x, sum = scan_lanes(upper + lower);
+            if (lane == 63) wave_counts[0][wave].x = sum;
+            __syncthreads();
+            const int of_wave = lane < kEvictWaves && lane < wave ? wave_counts[0][lane].x : 0;
+            const int above = sum - upper - lower + __builtin_amdgcn_readlane(scan_lanes(of_wave), 63);
+            if (above < wanted && above + upper + lower >= wanted) {
+                const bool second = above + upper < wanted;
+                found[0] = kEvictBins - 1 - 2 * tid - second;
+                found[1] = wanted - above - (second ? upper : 0);
+            }
+            __syncthreads();
+            prefix |= unsigned(found[0]) << shift;
+            known |= unsigned(width - 1) << shift;
+            wanted = found[1];
+        }
+        // Slot j, with the slots before it above and at the threshold.
+        auto place = [&](int j, unsigned key, int above_rank, int at_rank) {
+            const bool kept = key > prefix || (key == prefix && at_rank < wanted);
+            const int rank = above_rank + min(at_rank, wanted);  // kept slots before this one
+            if (j == keep) found[0] = keep - rank;               // the rest of them have to move
+            if (j >= keep) {
+                if (kept && keep - 1 - rank < a.room) sources[keep - 1 - rank] = j;  // from the last
+            } else if (!kept) {
+                if (j - rank < a.room) holes[j - rank] = j;
+            }
+        };
+        const unsigned long long before = (1ull << lane) - 1;
+        __syncthreads();
+        if (holds) {
+            // The counts of every wave's part of every 1024 slots, then their running sums.
+#pragma unroll
+            for (int i = 0; i < kEvictHeld; ++i) {
+                const bool in = i * kEvictThreads + tid < n;
+                const int above = __popcll(__ballot(in && held[i] > prefix));
+                const int at = __popcll(__ballot(in && held[i] == prefix));
+                if (lane == 0) wave_counts[i][wave] = int2{above, at};
+            }
+            __syncthreads();
+            static_assert(kEvictHeld * kEvictWaves == 128, "two counts for each lane");
+            const int2 c0 = wave_counts[0][2 * lane], c1 = wave_counts[0][2 * lane + 1];
+            const int above_upto = scan_lanes(c0.x + c1.x), at_upto = scan_lanes(c0.y + c1.y);
+#pragma unroll
+            for (int i = 0; i < kEvictHeld; ++i) {
+                const int of = (i * kEvictWaves + wave) / 2;
+                int above_rank = __builtin_amdgcn_readlane(above_upto - c1.x - (wave & 1 ? 0 : c0.x), of);
+                int at_rank = __builtin_amdgcn_readlane(at_upto - c1.y - (wave & 1 ? 0 : c0.y), of);
+                const bool in = i * kEvictThreads + tid < n;
+                above_rank += __popcll(__ballot(in && held[i] > prefix) & before);
+                at_rank += __popcll(__ballot(in && held[i] == prefix) & before);
+                if (in) place(i * kEvictThreads + tid, held[i], above_rank, at_rank);
+            }
+        } else {
+            int above_before = 0, at_before = 0, turn = 0;
+            for (int begin = 0; begin < n; begin += kEvictThreads, turn ^= 1) {
+                const int j = begin + tid;
+                const unsigned key = j < n ? key_of(j) : 0u;
+                const unsigned long long above = __ballot(j < n && key > prefix), at = __ballot(j < n && key == prefix);
+                if (lane == 0) wave_counts[turn][wave] = int2{__popcll(above), __popcll(at)};
+                __syncthreads();
+                const int2 c = lane < kEvictWaves ? wave_counts[turn][lane] : int2{0, 0};
+                const int above_upto = scan_lanes(c.x), at_upto = scan_lanes(c.y);
+                const int above_rank = above_before + (wave ? __builtin_amdgcn_readlane(above_upto, wave - 1) : 0);
+                const int at_rank = at_before + (wave ? __builtin_amdgcn_readlane(at_upto, wave - 1) : 0);
+                if (j < n) place(j, key, above_rank + __popcll(above & before), at_rank + __popcll(at & before));
+                above_before += __builtin_amdgcn_readlane(above_upto, 63);
+                at_before += __builtin_amdgcn_readlane(at_upto, 63);
+            }
+        }
+        __syncthreads();
+        moved = int(min(int64_t(found[0]), a.room));
+        sources += moved - 1;
     }
-    // Rows move in pieces of 16 bytes: keys, then values.
-    const int pieces = a.size / 16, all = 2 * pieces;
-    for (int64_t i = tid; i < int64_t(moved) * all; i += kEvictThreads) {
-        const int m = int(i / all), piece = int(i - int64_t(m) * all);
-        const PageSlot to = page_slot(holes[m], v.page_size, v.magic);
-        const PageSlot from = page_slot(sources[moved - 1 - m], v.page_size, v.magic);
-        const int to_page = v.page_of(s, to.page), from_page = v.page_of(s, from.page);
-        if (to_page < 0 || from_page < 0) continue;
-        char* const pool = piece < pieces ? v.keys : v.values;
-        const int64_t at = 16 * (piece < pieces ? piece : piece - pieces);
-        *reinterpret_cast<uint4_t*>(pool + v.row_at(to_page, head, to.slot) + at) =
-            *reinterpret_cast<const uint4_t*>(pool + v.row_at(from_page, head, from.slot) + at);
-        if (piece == 0 && a.scaled)
-            *reinterpret_cast<uint16_t*>(v.exponents + v.exponents_at(to_page, head, to.slot)) =
-                *reinterpret_cast<const uint16_t*>(v.exponents + v.exponents_at(from_page, head, from.slot));
+    if constexpr (MOVE) {
+        const int order = sources == few_sources ? 1 : -1;  // the long list begins with the last source
+        for (int i = tid; i < moved; i += kEvictThreads) {
+            const int to = holes[i], from = sources[order * i];
+            new_weights[to] = weights[from];
+            new_positions[to] = positions[from];
+        }
+        const int pieces = a.size / 8;
+        for (int i = tid; i < moved * pieces; i += kEvictThreads) {
+            const int m = i / pieces;
+            move_piece(v, a, s, head, sources[order * m], holes[m], i - m * pieces);
+        }
+    } else {
+        if (tid == 0) moves[0] = moved;
+        if (sources == few_sources && tid < moved) {
+            moves[kEvictHead + tid] = few_holes[tid];
+            moves[kEvictHead + a.room + moved - 1 - tid] = few_sources[tid];
+        }
     }
 }
 
-int64_t evict_room(const qwen_gpu_paged_batch& b, int keep) { return std::min(keep, b.max_length - keep); }
-size_t evict_bytes(const qwen_gpu_paged_cache& c, const qwen_gpu_paged_batch& b, int64_t room) {
-    return size_t(b.sequences) * c.kv_heads * 2 * room * sizeof(int32_t);
+// The moves that the choice left, 64 rows a workgroup's turn: a lane of the
+// first wave finds where one row goes from and to, and moves its weight,
+// position and exponents; then all threads move the rows' pieces, four loads in flight each.
+__global__ __launch_bounds__(256) void paged_move_kernel(PagedView v, EvictArgs a) {
+    __shared__ int64_t from_at[kMoveRows], to_at[kMoveRows];
+    const int tid = threadIdx.x, s = blockIdx.x / v.kv_heads, head = blockIdx.x - s * v.kv_heads;
+    const int32_t* const moves = a.moves + int64_t(blockIdx.x) * (2 * a.room + kEvictHead);
+    const int64_t track = v.track_at(s, head);
+    const int moved = moves[0];
+    const int32_t *const holes = moves + kEvictHead, *const sources = holes + a.room + moved - 1;
+    const int pieces = a.size / 8, shift = 31 - __builtin_clz(unsigned(pieces)), half = pieces / 2;  // powers of two
+    const int piece = tid & (pieces - 1), together = 256 >> shift;
+    char* const pool = (piece < half ? v.keys : v.values) + 16 * (piece & (half - 1));
+    for (int m0 = blockIdx.y * kMoveRows; m0 < moved; m0 += int(gridDim.y) * kMoveRows) {
+        const int rows = min(kMoveRows, moved - m0);
+        if (tid < rows) {
+            const int hole = holes[m0 + tid], source = sources[-m0 - tid];
+            const PageSlot to = page_slot(hole, v.page_size, v.magic);
+            const PageSlot from = page_slot(source, v.page_size, v.magic);
+            const int to_page = v.page_of(s, to.page), from_page = v.page_of(s, from.page);
+            const bool both = to_page >= 0 && from_page >= 0;
+            from_at[tid] = both ? v.row_at(from_page, head, from.slot) : -1;
+            to_at[tid] = v.row_at(to_page, head, to.slot);
+            a.new_weights[track + hole] = v.weights[track + source];
+            a.new_positions[track + hole] = v.positions[track + source];
+            if (a.scaled && both)
+                *reinterpret_cast<uint16_t*>(v.exponents + v.exponents_at(to_page, head, to.slot)) =
+                    *reinterpret_cast<const uint16_t*>(v.exponents + v.exponents_at(from_page, head, from.slot));
+        }
+        __syncthreads();
+        for (int r0 = tid >> shift; r0 < rows; r0 += 4 * together) {
+            int64_t from[4], to[4];
+            uint4_t data[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = min(r0 + i * together, rows - 1);
+                from[i] = from_at[r];
+                to[i] = to_at[r];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) data[i] = *reinterpret_cast<const uint4_t*>(pool + max(from[i], int64_t(0)));
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (from[i] >= 0 && r0 + i * together < rows) *reinterpret_cast<uint4_t*>(pool + to[i]) = data[i];
+        }
+        __syncthreads();
+    }
 }
 
 bool apart(const void* p, const void* q, size_t bytes) {
@@ -457,15 +649,23 @@ void launch_paged_evict(const qwen_gpu_paged_cache& cache, const qwen_gpu_paged_
                       recent,      new_lengths,
                       new_weights, new_positions,
                       reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + kPagedCounterBytes),
-                      evict_room(batch, keep),
+                      std::min(keep, batch.max_length - keep),
                       cache.head_dim * (cache.type == kPagedE4M3 ? 1 : 2),
                       cache.type == kPagedE4M3};
-    const size_t bytes = evict_bytes(cache, batch, a.room);
-    if (bytes) {
+    const size_t bytes = paged_moves_bytes(cache, batch, a.room);
+    if (a.room) {
         device.check(workspace, "workspace", 16);
         require(workspace_bytes >= kPagedCounterBytes + bytes, "Workspace is too small");
     }
-    paged_evict_kernel<<<batch.sequences * cache.kv_heads, kEvictThreads, 0, stream>>>(v, a);
+    const unsigned units = unsigned(batch.sequences) * cache.kv_heads;
+    if (a.room <= kEvictFew) {
+        paged_evict_kernel<true><<<units, kEvictThreads, 0, stream>>>(v, a);
+    } else {
+        paged_evict_kernel<false><<<units, kEvictThreads, 0, stream>>>(v, a);
+        const int64_t most = (a.room + kMoveRows - 1) / kMoveRows;
+        const unsigned share = unsigned(std::min<int64_t>(most, std::max(1u, 8192 / units)));
+        paged_move_kernel<<<dim3(units, share), 256, 0, stream>>>(v, a);
+    }
 }
 
 }  // namespace qwen_hip

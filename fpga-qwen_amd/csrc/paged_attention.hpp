@@ -1,0 +1,721 @@
+// Attention of new rows over a paged key-value cache: the kernel and its launch,
+// included by one source for each type of cache (they compile side by side).
+#pragma once
+#include <algorithm>
+#include <type_traits>
+
+#include "decode_dev.hpp"
+#include "paged_dev.hpp"
+
+namespace qwen_hip {
+
+constexpr int kTile = 32;                       // positions of a wave's step
+constexpr int kWaves = 4;                       // of a workgroup
+constexpr int kBlock = kTile * kWaves;          // positions of a workgroup's step
+constexpr int kShares = 512;                    // workgroups that the positions are dealt to
+constexpr int kLeast = 2;                       // blocks of a part of a unit, at least
+constexpr int kStream = 4 * kShares;            // blocks from which on workgroups cross units
+constexpr int kRuns = 512;                      // workgroups that do
+constexpr int kCounterStep = 16;                // ints: a counter has a line of its own
+constexpr float kInf = __builtin_huge_valf();
+static_assert(kRuns < kStream && std::max(kShares, kRuns) * kCounterStep * sizeof(int) <= kPagedCounterBytes, "counters");
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float float4_t __attribute__((ext_vector_type(4)));
+typedef short short4_t __attribute__((ext_vector_type(4)));
+
+struct AttentionArgs {
+    const float* queries;
+    int64_t query_stride;
+    float* out;
+    int64_t out_stride;
+    int group;
+    float scale;        // times log2(e)
+    float* partials;    // [workgroups][rows of a tile][DIM + 4]: output, reference, sum
+    int* counters;      // [kShares][kCounterStep], 0 between launches
+    float2* states;     // tracked: [sequences * kv_heads][rows * group]: reference, 1 / sum
+    float* scores;      // tracked: the same, times score_stride
+    int64_t score_stride;
+};
+
+// How the positions are dealt. A unit is a sequence, a KV head and a tile of
+// its query rows; it has `blocks` blocks of 128 positions (one at least, so
+// that rows without positions are written too). Workgroups find their shares
+// from the lengths on the device, every wave by itself, so the host needs no
+// lengths and a captured launch follows them. With up to kStream blocks in
+// all, a workgroup has one part of one unit: units with more blocks than the
+// mean of kShares workgroups (and than kLeast) are split evenly. With more,
+// kShares workgroups (two for each CU, all there at once) take equal runs of
+// blocks in the order of the units, across their borders: with parts of units
+// the last round of workgroups left CUs idle (64 sequences of 1 to 4096
+// positions took 131 us, now 125).
+struct Deal {
+    int length, n, first, tiles, blocks;  // of a sequence: positions, new rows, the first of them, units a head
+};
+struct Share {
+    Deal d;
+    int s, tile, head;
+    int from, to;             // blocks of the unit
+    int parts;                // of the unit; part p's sums lie at part0 (p = 0), part1 + (p - 1) * step
+    int part0, part1, step;
+    int mine;                 // where this one's lie
+    int counter;
+};
+template <int ROWS>
+__device__ __forceinline__ Deal deal_one(const PagedView& v, int group, int s) {
+    Deal d;
+    d.length = v.length(s);
+    d.n = v.new_rows(s, d.first);
+    d.tiles = (group * d.n + ROWS - 1) / ROWS;
+    d.blocks = max(1, (d.length + kBlock - 1) / kBlock);
+    return d;
+}
+__device__ __forceinline__ Deal deal_of_lane(const Deal& d, int lane) {
+    return {__builtin_amdgcn_readlane(d.length, lane), __builtin_amdgcn_readlane(d.n, lane),
+            __builtin_amdgcn_readlane(d.first, lane), __builtin_amdgcn_readlane(d.tiles, lane),
+            __builtin_amdgcn_readlane(d.blocks, lane)};
+}
+// The host has checked that all units' blocks together fit 31 bits.
+template <int ROWS>
+struct Dealer {
+    const PagedView& v;
+    const int group, lane;
+    Deal own;    // of sequence `lane`, which is all there is to know up to 64 of them
+    int total;   // blocks of all units
+    int at, end; // blocks of this workgroup's run (in order of the units)
+    bool streams;
+
+    __device__ __forceinline__ Dealer(const PagedView& view, int g)
+        : v(view), group(g), lane(threadIdx.x & 63), own{} {
+        int part = 0;
+        for (int s = lane; s < v.sequences; s += 64) {
+            own = deal_one<ROWS>(v, group, s);
+            part += own.blocks * own.tiles;
+        }
+        total = __builtin_amdgcn_readlane(scan_lanes(part), 63) * v.kv_heads;
+        streams = total > kStream;
+        at = start(blockIdx.x);
+        end = start(blockIdx.x + 1);
+    }
+    __device__ __forceinline__ int start(int w) const {
+        return w >= kRuns ? total : w * (total / kRuns) + min(w, total % kRuns);
+    }
+    __device__ __forceinline__ int owner(int block) const {
+        const int even = total / kRuns, more = total % kRuns, longer = more * (even + 1);
+        return block < longer ? block / (even + 1) : more + (block - longer) / even;
+    }
+    // This workgroup's next share, if it has one.
+    __device__ __forceinline__ bool next(Share& share) {
+        if (streams && at >= end) return false;
+        const int most = max(kLeast, (total + kShares - 1) / kShares), w = blockIdx.x;
+        const int wanted = streams ? at : w;
+        int before = 0, extra = 0;  // blocks or workgroups of the sequences before, and workgroups beyond one a unit
+        for (int begin = 0; begin < v.sequences; begin += 64) {
+            Deal d = own;
+            if (v.sequences > 64 && begin + lane < v.sequences) d = deal_one<ROWS>(v, group, begin + lane);
+            const int units = begin + lane < v.sequences ? d.tiles * v.kv_heads : 0;
+            const int splits = streams ? d.blocks : (d.blocks + most - 1) / most;
+            const int count = splits * units, upto = scan_lanes(count), more = scan_lanes(count - units);
+            const unsigned long long hit = __ballot(before + upto > wanted);
+            if (hit) {
+                const int from = __ffsll(hit) - 1;
+                share.s = begin + from;
+                share.d = d = deal_of_lane(d, from);
+                const int offset = before + __builtin_amdgcn_readlane(upto - count, from);
+                const int parts = __builtin_amdgcn_readlane(splits, from);
+                const int within = wanted - offset;
+                if (streams) {
+                    const int unit = within / d.blocks;
+                    share.tile = unit / v.kv_heads;
+                    share.head = unit - share.tile * v.kv_heads;
+                    share.from = within - unit * d.blocks;
+                    share.to = min(d.blocks, share.from + end - at);
+                    const int first = owner(at - share.from), last = owner(at - share.from + d.blocks - 1);
+                    share.parts = last - first + 1;
+                    share.part0 = 2 * first + 1;  // a run's last share; its first one is the end of another unit
+                    share.part1 = 2 * (first + 1);
+                    share.step = 2;
+                    share.mine = share.from == 0 ? 2 * w + 1 : 2 * w;
+                    share.counter = first;  // no other unit both starts in that run and ends behind it
+                    at += share.to - share.from;
+                } else {
+                    // Tiles of one head's rows are a multiple of the KV heads apart: on one XCD where that is one of
+                    // eight, so that the second reads the first one's keys and values from its L2.
+                    const int of_tile = v.kv_heads * parts, rest = within % of_tile, split = rest / v.kv_heads;
+                    share.tile = within / of_tile;
+                    share.head = rest - split * v.kv_heads;
+                    const int even = d.blocks / parts, longer = d.blocks - even * parts;
+                    share.from = split * even + min(split, longer);
+                    share.to = share.from + even + (split < longer ? 1 : 0);
+                    share.parts = parts;
+                    share.part0 = w - split * v.kv_heads;
+                    share.part1 = share.part0 + v.kv_heads;
+                    share.step = v.kv_heads;
+                    share.mine = w;
+                    share.counter = extra + __builtin_amdgcn_readlane(more - count + units, from) +
+                                    (share.tile * v.kv_heads + share.head) * (parts - 1);
+                }
+                return true;
+            }
+            before += __builtin_amdgcn_readlane(upto, 63);
+            extra += __builtin_amdgcn_readlane(more, 63);
+        }
+        return false;
+    }
+};
+
+// Values that other workgroups of the launch read, on other XCDs too: stores
+// and loads that pass by the caches of one XCD.
+__device__ __forceinline__ void post(float* p, float a, float b) {
+    const uint64_t w = __builtin_bit_cast(unsigned, a) | uint64_t(__builtin_bit_cast(unsigned, b)) << 32;
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void posted_stores_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ float2 posted(const float* p) {
+    const uint64_t w = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return float2{__builtin_bit_cast(float, unsigned(w)), __builtin_bit_cast(float, unsigned(w >> 32))};
+}
+
+// ds_read_b64_tr_b16: within each 16-lane group, lane 4a + b receives element
+// b of the 8-byte chunks addressed by lanes a, a + 4, a + 8 and a + 12.
+__device__ __forceinline__ short4_t read_transposed(const char* p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    typedef __attribute__((address_space(3))) short4_t lds_short4;
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(__attribute__((address_space(3))) char*)(p));
+#else
+    (void)p;
+    return short4_t{};
+#endif
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+__device__ __forceinline__ float4_t multiply(uint4_t a, uint4_t b, float4_t c, std::integral_constant<int, kPagedF16>) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+}
+template <int TYPE>
+__device__ __forceinline__ float4_t multiply(uint4_t a, uint4_t b, float4_t c, std::integral_constant<int, TYPE>) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                   0);
+}
+
+// FP32 values as sums of 16-bit ones, for products on the matrix cores: two
+// FP16 terms hold 22 bits, three BF16 terms 24 (two, 2^-17 off, would lose ten
+// times what the sums do). A product has 16 columns. Up to 8 query rows are
+// packed: columns 0-7 take the first term and 8-15 the second, the halves of
+// the result are added, and a third term takes a second product with empty columns 8-15. More
+// rows take a column each and a product for every term, added by the matrix cores.
+// E4M3 rows become BF16 as they are read, with their power of two: exact.
+template <int TYPE, bool PACKED>
+struct Terms {
+    static constexpr int kTerms = TYPE == kPagedF16 ? 2 : 3, kProducts = PACKED ? kTerms - 1 : kTerms;
+    // Two values; `second`: this lane's column is one of 8-15.
+    static __device__ __forceinline__ void split(float a, float b, bool second, unsigned (&out)[kProducts]) {
+        unsigned term[kTerms];
+        if constexpr (TYPE == kPagedF16) {
+            _Float16 ha, la, hb, lb;
+            split_half(a, ha, la);
+            split_half(b, hb, lb);
+            if constexpr (PACKED) {
+                const _Float16 x = second ? la : ha, y = second ? lb : hb;
+                out[0] = __builtin_bit_cast(uint16_t, x) | unsigned(__builtin_bit_cast(uint16_t, y)) << 16;
+                return;
+            }
+            term[0] = __builtin_bit_cast(uint16_t, ha) | unsigned(__builtin_bit_cast(uint16_t, hb)) << 16;
+            term[1] = __builtin_bit_cast(uint16_t, la) | unsigned(__builtin_bit_cast(uint16_t, lb)) << 16;
+        } else {
+#pragma unroll
+            for (int t = 0; t < 3; ++t) {
+                a = fp32_fixed(a);
+                b = fp32_fixed(b);
+                term[t] = pack_bf16(a, b);
+                a -= __builtin_bit_cast(float, term[t] << 16);
+                b -= __builtin_bit_cast(float, term[t] & 0xffff0000u);
+            }
+        }
+        if constexpr (PACKED) {
+            out[0] = second ? term[1] : term[0];
+            if constexpr (kProducts == 2) out[1] = second ? 0u : term[2];
+        } else {
+#pragma unroll
+            for (int t = 0; t < kTerms; ++t) out[t] = term[t];
+        }
+    }
+};
+
+// 16 bytes of a stored row as 16-bit operands: one of 8, or two (E4M3).
+template <int TYPE>
+__device__ __forceinline__ void widen(uint4_t raw, float up, uint4_t (&out)[TYPE == kPagedE4M3 ? 2 : 1]) {
+    if constexpr (TYPE != kPagedE4M3) {
+        out[0] = raw;
+    } else {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            out[w / 2][2 * (w % 2)] =
+                __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw[w], up, false));
+            out[w / 2][2 * (w % 2) + 1] =
+                __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(raw[w], up, true));
+        }
+    }
+}
+
+template <int TYPE>
+__device__ __forceinline__ float stored(const char* row, int i, float up) {
+    if constexpr (TYPE == kPagedF16) {
+        return float(reinterpret_cast<const _Float16*>(row)[i]);
+    } else if constexpr (TYPE == kPagedBF16) {
+        return __builtin_bit_cast(float, unsigned(reinterpret_cast<const uint16_t*>(row)[i]) << 16);
+    } else {
+        return float(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(reinterpret_cast<const uint8_t*>(row)[i], up, false)[0]);
+    }
+}
+
+// Lanes l and l ^ 8 of each 16: the sum of both halves in both.
+__device__ __forceinline__ float add_halves(float x) {
+    const int other = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x128, 0xF, 0xF, true);  // row_ror:8
+    return x + __builtin_bit_cast(float, other);
+}
+
+// S^T = K Q^T and O^T = V^T P^T on the matrix cores, 32 positions a step, each
+// wave with its own online softmax over every fourth step of the workgroup's
+// positions; the waves are added at the end. A lane holds row l % 16 of each
+// 16 positions, pieces l / 16, l / 16 + 4, ... of 16 bytes: the A operand of
+// S^T as it comes from memory. S^T leaves lane l with column l % 16 and
+// positions 4 (l / 16) .. + 3 of each 16, which is the B operand of O^T when
+// V^T's columns are taken in that order, so weights never change lanes. V
+// goes through LDS (each wave its own 32 rows) and comes back transposed;
+// rows are 32 bytes apart from a multiple of 256 so that the 16 rows of a
+// read fall on all banks twice.
+//
+// Memory is what bounds it (two products of 16 x 16 x 32 per 1 KiB of keys
+// take a tenth of the time that HBM needs for them), so the loads of the next step
+// are always in flight: keys are loaded again as soon as the scores have
+// been multiplied, values as soon as they are in LDS, and the table entries
+// of a step ahead of the values before it, so that no wait for one covers the other.
+template <int TYPE, int DIM, bool PACKED, bool TRACK>
+__global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attention_kernel(PagedView v, AttentionArgs a) {
+    constexpr int kSize = TYPE == kPagedE4M3 ? 1 : 2, kLoads = DIM * kSize / 64, kSteps = DIM / 32, kOut = DIM / 16;
+    constexpr int kPer = kSteps / kLoads;         // products per load: 1, or 2 for E4M3
+    constexpr int kRows = PACKED ? 8 : 16, kProducts = Terms<TYPE, PACKED>::kProducts;
+    constexpr int kPitch = DIM * 2 + 32;          // bytes of a value row in LDS
+    constexpr float kHead = TYPE == kPagedF16 ? 6.f : 0.f;  // FP16 weights are kept up to 2^14, far from subnormals
+    constexpr float kGrow = 8.f;                  // a reference is moved once a score passes it by 2^8
+    constexpr std::integral_constant<int, TYPE> kType{};
+    __shared__ __attribute__((aligned(16))) char lds[kWaves][kTile * kPitch];
+    __shared__ float2 wave_state[kWaves][kRows];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int column = lane & 15, part = lane >> 4;
+    const bool second = PACKED && column >= 8;
+    const int row_of_lane = PACKED ? column & 7 : column;
+
+    Dealer<kRows> dealer(v, a.group);
+    Share share;
+    while (dealer.next(share)) {
+        const Deal& d = share.d;
+        const int head = share.head, begin = kBlock * share.from;
+        const int query_rows = a.group * d.n, row0 = share.tile * kRows;
+        // Positions from shared_end on are seen by some of the tile's new rows only, from `end` on by none.
+        const int shared_end = d.length - d.n + row0 / a.group + 1;
+        const int seen_end = d.length - d.n + min(d.n - 1, (row0 + kRows - 1) / a.group) + 1;
+        const int end = min(seen_end, kBlock * share.to);
+        const int32_t* const table = v.table + int64_t(share.s) * v.table_stride;
+
+        float4_t acc[kOut];
+        float reference = -kInf, sum = 0.f;
+#pragma unroll
+        for (int o = 0; o < kOut; ++o) acc[o] = float4_t{0.f, 0.f, 0.f, 0.f};
+
+        // A step's rows: page entries, then offsets, then 16-byte pieces.
+        int pages[2], slots[2];
+        int64_t at[2];
+        bool there[2];
+        uint4_t keys[2][kLoads], values[2][kLoads];
+        unsigned bytes[2] = {0, 0};
+        auto find = [&](int base) {  // entries; positions past the end take the last one's
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const PageSlot where = page_slot(max(0, min(base + 16 * u + column, end - 1)), v.page_size, v.magic);
+                slots[u] = where.slot;
+                pages[u] = table[where.page];
+            }
+        };
+        auto place = [&](int base) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const bool known = pages[u] >= 0 && pages[u] < v.pages;
+                there[u] = known && base + 16 * u + column < end;
+                const int page = known ? pages[u] : 0;
+                at[u] = v.row_at(page, head, slots[u]) + 16 * part;
+                if constexpr (TYPE == kPagedE4M3)
+                    bytes[u] = *reinterpret_cast<const uint16_t*>(v.exponents + v.exponents_at(page, head, slots[u]));
+            }
+        };
+        auto load = [&](const char* pool, uint4_t (&to)[2][kLoads]) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) to[u][i] = *reinterpret_cast<const uint4_t*>(pool + at[u] + 64 * i);
+        };
+        char* const mine = lds[wave];
+        const char* const transposed = mine + (4 * part + (column >> 2)) * kPitch + (column & 3) * 8;
+
+        // The table's entries first, queries next, keys and values behind them.
+        int base = begin + kTile * wave;
+        if (base < end) find(base);
+        // Queries: row r of the tile is head r % group of new row r / group.
+        uint4_t query[kSteps][kProducts];
+        float x[kSteps][8];
+        const int query_row = row0 + row_of_lane, new_row = query_row / a.group;
+        const int64_t row = int64_t(d.first) + new_row;
+        const bool live = query_row < query_rows && row >= 0 && row < v.total_rows;
+        const int sees = live ? d.length - d.n + new_row + 1 : 0;  // positions the lane's row attends
+        {
+            const float* const from =
+                a.queries + (live ? row * a.query_stride + (head * a.group + query_row - new_row * a.group) * DIM : 0);
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+                // The channels that this lane's part of a stored row holds in step k.
+                const int from_channel = kPer == 1 ? 32 * k + 8 * part : 64 * (k / 2) + 16 * part + 8 * (k % 2);
+                const float4_a4 lo = *reinterpret_cast<const float4_a4*>(from + from_channel);
+                const float4_a4 hi = *reinterpret_cast<const float4_a4*>(from + from_channel + 4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[k][e] = live ? lo[e] : 0.f, x[k][4 + e] = live ? hi[e] : 0.f;
+            }
+        }
+        if (base < end) {
+            place(base);
+            load(v.keys, keys);
+            if (base + kBlock < end) find(base + kBlock);
+            load(v.values, values);
+        }
+        float to_score = a.scale;  // what a product's sum is multiplied by
+        if constexpr (TYPE == kPagedF16) {
+            // An exact power of two brings a row's largest query to [2^14, 2^15), so
+            // that neither term leaves FP16's range. 2^-100 is far below any query that a score depends on;
+            // non-finite ones stay so.
+            float top = 0.f;
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = fmaxf(top, __builtin_fabsf(x[k][e]));
+            top = fmaxf(top, dev::xor_lanes<16>(top));
+            top = fmaxf(top, dev::xor_lanes<32>(top));
+            const int up = 14 - max(int(__builtin_bit_cast(unsigned, top) >> 23) - 127, -100);
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[k][e] *= pow2(up);
+            to_score *= pow2(-up);
+        }
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                unsigned words[kProducts];
+                Terms<TYPE, PACKED>::split(x[k][2 * e], x[k][2 * e + 1], second, words);
+#pragma unroll
+                for (int p = 0; p < kProducts; ++p) query[k][p][e] = words[p];
+            }
+
+        for (; base < end; base += kBlock) {
+            float4_t s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) {
+                    uint4_t k[kPer];
+                    widen<TYPE>(keys[u][i], byte_pow2(bytes[u] & 255), k);
+#pragma unroll
+                    for (int j = 0; j < kPer; ++j)
+#pragma unroll
+                        for (int p = 0; p < kProducts; ++p) s[u] = multiply(k[j], query[kPer * i + j][p], s[u], kType);
+                }
+            // What the rest of this step needs of its rows, before the next one's take their place.
+            const bool was[2] = {there[0], there[1]};
+            const int64_t row_at[2] = {at[0] - 16 * part, at[1] - 16 * part};
+            const float value_up[2] = {byte_pow2(bytes[0] >> 8), byte_pow2(bytes[1] >> 8)};
+            const unsigned exist = (unsigned(__ballot(was[0])) & 0xffffu) | unsigned(__ballot(was[1])) << 16;
+            const bool more_steps = base + kBlock < end;
+            if (more_steps) {
+                place(base + kBlock);
+                load(v.keys, keys);
+            }
+            const bool whole = exist == 0xffffffffu && base + kTile <= shared_end;
+
+            float scores[2][4], weights[2][4], high = -kInf;
+            unsigned hidden = 0;  // bit 4 u + r
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    scores[u][r] = PACKED ? add_halves(s[u][r]) : s[u][r];
+                    high = fmaxf(high, scores[u][r] * to_score);
+                }
+            if (!whole) {
+                high = -kInf;
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int j = 16 * u + 4 * part + r;
+                        if (!(exist >> j & 1) || base + j >= sees)
+                            hidden |= 1u << (4 * u + r);
+                        else
+                            high = fmaxf(high, scores[u][r] * to_score);
+                    }
+            }
+            if (__any(high > reference + (kHead + kGrow))) {
+                high = fmaxf(high, dev::xor_lanes<16>(high));
+                high = fmaxf(high, dev::xor_lanes<32>(high));
+                const float moved = fmaxf(reference, high - kHead);
+                const float shrink = reference == moved ? 1.f : exp2_fast(reference - moved);
+                reference = moved;
+                sum *= shrink;
+#pragma unroll
+                for (int o = 0; o < kOut; ++o) acc[o] *= shrink;
+            }
+            {
+                const float from = reference == -kInf ? 0.f : reference;
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float p = exp2_fast(__builtin_fmaf(scores[u][r], to_score, -from));
+                        if (!whole && (hidden >> (4 * u + r) & 1)) p = 0.f;
+                        weights[u][r] = p;
+                        sum += p;
+                    }
+            }
+            if constexpr (TRACK) {
+                if (!second && query_row < query_rows) {
+                    float* const to = a.scores + base + 4 * part +
+                                      ((int64_t(share.s) * v.kv_heads + head) * (int64_t(v.rows) * a.group) + query_row) *
+                                          a.score_stride;
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        float4_t w;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            w[e] = !whole && (hidden >> (4 * u + e) & 1) ? -kInf : scores[u][e] * to_score;
+                        *reinterpret_cast<float4_t*>(to + 16 * u) = w;
+                    }
+                }
+            }
+            uint4_t weight[kProducts];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                unsigned words[kProducts];
+                Terms<TYPE, PACKED>::split(weights[e / 2][2 * (e % 2)], weights[e / 2][2 * (e % 2) + 1], second, words);
+#pragma unroll
+                for (int p = 0; p < kProducts; ++p) weight[p][e] = words[p];
+            }
+
+            // Values into LDS. What is not there, or not seen by all rows, is 0 here:
+            // a weight of 0 would not keep its infinities and NaN out.
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const bool clean = whole || (was[u] && base + 16 * u + column < shared_end);
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) {
+                    uint4_t w[kPer];
+                    widen<TYPE>(values[u][i], value_up[u], w);
+#pragma unroll
+                    for (int j = 0; j < kPer; ++j) {
+                        if (!whole && !clean) w[j] = uint4_t{0u, 0u, 0u, 0u};
+                        *reinterpret_cast<uint4_t*>(mine + (16 * u + column) * kPitch + 64 * kPer * i + 16 * kPer * part +
+                                                    16 * j) = w[j];
+                    }
+                }
+            }
+            if (more_steps) {
+                if (base + 2 * kBlock < end) find(base + 2 * kBlock);
+                load(v.values, values);
+            }
+#pragma unroll
+            for (int o = 0; o < kOut; ++o) {
+                const short4_t low = read_transposed(transposed + 32 * o);
+                const short4_t high = read_transposed(transposed + 16 * kPitch + 32 * o);
+                const uint4_t w = {__builtin_bit_cast(u32x2, low)[0], __builtin_bit_cast(u32x2, low)[1],
+                                   __builtin_bit_cast(u32x2, high)[0], __builtin_bit_cast(u32x2, high)[1]};
+#pragma unroll
+                for (int p = 0; p < kProducts; ++p) acc[o] = multiply(w, weight[p], acc[o], kType);
+            }
+
+            // The last rows of a sequence with several new ones, one at a time.
+            if (base + kTile > shared_end) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        for (int q = 0; q < 4; ++q) {
+                            const int j = 16 * u + 4 * q + r;
+                            if (base + j < shared_end || !(exist >> j & 1)) continue;
+                            const int64_t from = __shfl(row_at[u], 4 * q + r);
+                            const float up = __shfl(value_up[u], 4 * q + r);
+                            const float p = __shfl(weights[u][r], 16 * q + column);
+                            if (second || base + j >= sees) continue;
+#pragma unroll
+                            for (int o = 0; o < kOut; ++o)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    acc[o][e] = __builtin_fmaf(p, stored<TYPE>(v.values + from, 16 * o + 4 * part + e, up),
+                                                               acc[o][e]);
+                        }
+            }
+        }
+
+        // The four waves' sums, brought to their largest reference.
+        __syncthreads();
+        float* const sums = reinterpret_cast<float*>(lds);  // [kWaves][kRows][DIM]
+        sum += dev::xor_lanes<16>(sum);
+        sum += dev::xor_lanes<32>(sum);
+        if (lane < kRows) wave_state[wave][lane] = float2{reference, sum};
+#pragma unroll
+        for (int o = 0; o < kOut; ++o) {
+            float4_t w = acc[o];
+            if constexpr (PACKED)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = add_halves(acc[o][e]);
+            if (!second) *reinterpret_cast<float4_t*>(sums + (wave * kRows + row_of_lane) * DIM + 16 * o + 4 * part) = w;
+        }
+        __syncthreads();
+        auto finish = [&](int local, int channel, float4_t o, float top, float all) {
+            const int r = row0 + local, i = r / a.group;
+            const int64_t to = int64_t(d.first) + i;
+            if (r >= query_rows || to < 0 || to >= v.total_rows) return;
+            if (all == 0.f) o = float4_t{0.f, 0.f, 0.f, 0.f};
+            const float by = all == 0.f ? 0.f : 1.f / all;
+            *reinterpret_cast<float4_a4*>(a.out + to * a.out_stride + (head * a.group + r - i * a.group) * DIM + channel) =
+                o * by;
+            if (TRACK && channel == 0)
+                a.states[(int64_t(share.s) * v.kv_heads + head) * (int64_t(v.rows) * a.group) + r] =
+                    float2{top == -kInf ? 0.f : top, by};
+        };
+        for (int item = threadIdx.x; item < kRows * DIM / 4; item += kWaves * 64) {
+            const int local = item / (DIM / 4), channel = 4 * (item - local * (DIM / 4));
+            float top = -kInf, all = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) top = fmaxf(top, wave_state[w][local].x);
+            float4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                const float2 state = wave_state[w][local];
+                const float shrink = state.x == top ? 1.f : exp2_fast(state.x - top);
+                all = __builtin_fmaf(state.y, shrink, all);
+                const float4_t x = *reinterpret_cast<const float4_t*>(sums + (w * kRows + local) * DIM + channel);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(x[e], shrink, o[e]);
+            }
+            if (share.parts > 1) {
+                float* const partial = a.partials + (int64_t(share.mine) * kRows + local) * (DIM + 4);
+                post(partial + channel, o[0], o[1]);
+                post(partial + channel + 2, o[2], o[3]);
+                if (channel == 0) post(partial + DIM, top, all);
+            } else {
+                finish(local, channel, o, top, all);
+            }
+        }
+        if (share.parts > 1) {
+            // The last of the unit's workgroups to get here adds their parts, in the
+            // order of the positions. Posted values have reached memory once their
+            // stores are done, and are read past the caches, so no fence of the
+            // device's scope is needed: with one in every workgroup (it writes back
+            // and drops a whole L2) eight sequences of 2048 took 42 us instead of 16.
+            posted_stores_done();
+            __syncthreads();
+            int* const last = reinterpret_cast<int*>(wave_state);
+            int* const counter = a.counters + share.counter * kCounterStep;
+            if (threadIdx.x == 0) {
+                const int done = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (done == share.parts - 1) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                *last = done == share.parts - 1;
+            }
+            __syncthreads();
+            if (*last) {
+                for (int item = threadIdx.x; item < kRows * DIM / 4; item += kWaves * 64) {
+                    const int local = item / (DIM / 4), channel = 4 * (item - local * (DIM / 4));
+                    if (row0 + local >= query_rows) continue;
+                    float top = -kInf, all = 0.f;
+                    float4_t o = {0.f, 0.f, 0.f, 0.f};
+                    for (int p0 = 0; p0 < share.parts; p0 += 8) {  // eight parts' loads in flight
+                        float2 state[8], low[8], high[8];
+#pragma unroll
+                        for (int p = 0; p < 8; ++p) {
+                            const int q = min(p0 + p, share.parts - 1);
+                            const int64_t slot = q == 0 ? share.part0 : share.part1 + (q - 1) * share.step;
+                            const float* const from = a.partials + (slot * kRows + local) * (DIM + 4);
+                            state[p] = posted(from + DIM);
+                            low[p] = posted(from + channel);
+                            high[p] = posted(from + channel + 2);
+                        }
+                        float grown = top;
+#pragma unroll
+                        for (int p = 0; p < 8; ++p) grown = fmaxf(grown, state[p].x);
+                        const float shrink = top == grown ? 1.f : exp2_fast(top - grown);
+                        top = grown;
+                        all *= shrink;
+                        o *= shrink;
+#pragma unroll
+                        for (int p = 0; p < 8; ++p) {
+                            if (p0 + p >= share.parts) break;
+                            const float by = state[p].x == top ? 1.f : exp2_fast(state[p].x - top);
+                            all = __builtin_fmaf(state[p].y, by, all);
+                            o[0] = __builtin_fmaf(low[p].x, by, o[0]);
+                            o[1] = __builtin_fmaf(low[p].y, by, o[1]);
+                            o[2] = __builtin_fmaf(high[p].x, by, o[2]);
+                            o[3] = __builtin_fmaf(high[p].y, by, o[3]);
+                        }
+                    }
+                    finish(local, channel, o, top, all);
+                }
+            }
+        }
+        if (!dealer.streams) return;
+        __syncthreads();  // LDS is written anew
+    }
+}
+
+// Sizes of a call: the grid, and what its workspace holds.
+struct AttentionPlan {
+    bool packed;
+    int64_t blocks, groups, score_stride, score_rows;
+    size_t partial_bytes, state_bytes, score_bytes;
+    AttentionPlan(const qwen_gpu_paged_cache& c, const qwen_gpu_paged_batch& b, int query_heads) {
+        const int64_t rows = int64_t(query_heads / c.kv_heads) * b.rows;
+        packed = rows <= 8;
+        const int64_t tile_rows = packed ? 8 : 16;
+        const int64_t units = int64_t(b.sequences) * c.kv_heads * ((rows + tile_rows - 1) / tile_rows);
+        blocks = units * ((b.max_length + kBlock - 1) / kBlock);
+        groups = std::min(blocks, units + kShares);
+        if (blocks > kStream) groups = std::max<int64_t>(groups, kRuns);
+        const int64_t parts = blocks > kStream ? std::max<int64_t>(groups, 2 * kRuns) : groups;
+        partial_bytes = size_t(parts) * tile_rows * (c.head_dim + 4) * 4;
+        score_stride = (b.max_length + kTile - 1) / kTile * kTile;
+        score_rows = int64_t(b.sequences) * c.kv_heads * rows;
+        state_bytes = b.weights ? (size_t(score_rows) * 8 + 15) / 16 * 16 : 0;
+        score_bytes = b.weights ? size_t(score_rows) * score_stride * 4 : 0;
+    }
+    size_t bytes() const { return kPagedCounterBytes + partial_bytes + state_bytes + score_bytes; }
+};
+
+template <int TYPE, int DIM, bool PACKED>
+void attention_run(const PagedView& v, const AttentionArgs& a, const AttentionPlan& plan, hipStream_t stream) {
+    const dim3 grid{unsigned(plan.groups)}, block{kWaves * 64};
+    if (v.weights)
+        paged_attention_kernel<TYPE, DIM, PACKED, true><<<grid, block, 0, stream>>>(v, a);
+    else
+        paged_attention_kernel<TYPE, DIM, PACKED, false><<<grid, block, 0, stream>>>(v, a);
+}
+
+template <int TYPE>
+void attention_launch(int dim, const PagedView& v, const AttentionArgs& a, const AttentionPlan& plan, hipStream_t stream) {
+    auto run = [&](auto packed) {
+        if (dim == 64) return attention_run<TYPE, 64, packed.value>(v, a, plan, stream);
+        if (dim == 128) return attention_run<TYPE, 128, packed.value>(v, a, plan, stream);
+        attention_run<TYPE, 256, packed.value>(v, a, plan, stream);
+    };
+    plan.packed ? run(std::true_type{}) : run(std::false_type{});
+}
+
+}  // namespace qwen_hip

@@ -13,7 +13,7 @@ namespace qwen_hip {
 constexpr int kPagedF16 = QWEN_GPU_PAGED_F16, kPagedBF16 = QWEN_GPU_PAGED_BF16, kPagedE4M3 = QWEN_GPU_PAGED_E4M3;
 constexpr int kPagedMaxLength = 1 << 24;
 // The front of a workspace, zero between calls; the rest is any call's own.
-constexpr size_t kPagedCounterBytes = 0;
+constexpr size_t kPagedCounterBytes = 131072;
 
 // Slot j of a sequence is slot j % page_size of its page j / page_size. With
 // magic = floor((2^32 - 1) / page_size) the upper half of j * magic is the
@@ -88,9 +88,23 @@ __device__ __forceinline__ unsigned pack_half(float a, float b) {
     return to_half_bits(a) | unsigned(to_half_bits(b)) << 16;
 }
 
+// Sum of the lanes up to this one, through DPP row shifts and broadcasts.
+__device__ __forceinline__ int scan_lanes(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);   // row_shr:1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
+    return x;
+}
+
 // Host side: checks (std::runtime_error), the view, the device.
 PagedView paged_view(const qwen_gpu_paged_cache& cache, const qwen_gpu_paged_batch& batch);
 void paged_check_rows(const qwen_gpu_paged_batch& batch);
+
+// Workspace of an eviction that moves at most `room` rows of a head.
+size_t paged_moves_bytes(const qwen_gpu_paged_cache& cache, const qwen_gpu_paged_batch& batch, int64_t room);
 
 // Makes the device that holds the cache current for the rest of the scope.
 // Every pointer given is refused unless a kernel on that device can use it.
