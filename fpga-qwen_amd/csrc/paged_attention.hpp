@@ -18,7 +18,9 @@ constexpr int kStream = 4 * kShares;            // blocks from which on workgrou
 constexpr int kRuns = 512;                      // workgroups that do
 constexpr int kCounterStep = 16;                // ints: a counter has a line of its own
 constexpr float kInf = __builtin_huge_valf();
-static_assert(kRuns < kStream && std::max(kShares, kRuns) * kCounterStep * sizeof(int) <= kPagedCounterBytes, "counters");
+constexpr int kMostHeads = 1024;                // KV heads of a cache
+static_assert(std::max(kShares, kRuns) + kMostHeads <= int(kPagedCounterBytes / (kCounterStep * sizeof(int))),
+              "counters");
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -30,32 +32,37 @@ struct AttentionArgs {
     int64_t query_stride;
     float* out;
     int64_t out_stride;
-    int group;
+    int group;          // query heads of a KV head
+    unsigned magic;     // of the group, as page_slot takes it
+    int extra;          // counters of a KV head
     float scale;        // times log2(e)
-    float* partials;    // [workgroups][rows of a tile][DIM + 4]: output, reference, sum
-    int* counters;      // [kShares][kCounterStep], 0 between launches
+    float* partials;    // [parts][rows of a tile][DIM + 4]: output, reference, sum
+    int* counters;      // kCounterStep apart, 0 between launches
     float2* states;     // tracked: [sequences * kv_heads][rows * group]: reference, 1 / sum
     float* scores;      // tracked: the same, times score_stride
     int64_t score_stride;
+
+    // Of a KV head's query row, the new row that it belongs to.
+    __device__ __forceinline__ int new_row(int r) const { return page_slot(r, group, magic).page; }
 };
 
-// How the positions are dealt. A unit is a sequence, a KV head and a tile of
-// its query rows; it has `blocks` blocks of 128 positions (one at least, so
-// that rows without positions are written too). Workgroups find their shares
-// from the lengths on the device, every wave by itself, so the host needs no
-// lengths and a captured launch follows them. With up to kStream blocks in
-// all, a workgroup has one part of one unit: units with more blocks than the
-// mean of kShares workgroups (and than kLeast) are split evenly. With more,
-// kShares workgroups (two for each CU, all there at once) take equal runs of
-// blocks in the order of the units, across their borders: with parts of units
-// the last round of workgroups left CUs idle (64 sequences of 1 to 4096
-// positions took 131 us, now 125).
+// How the positions are dealt. A unit is a sequence, a KV head (blockIdx.y)
+// and a tile of its query rows; it has `blocks` blocks of 128 positions (one
+// at least, so that rows without positions are written too). Workgroups find
+// their shares from the lengths on the device, every wave by itself, so the
+// host needs no lengths and a captured launch follows them. With up to kStream
+// blocks in all, a workgroup has one part of one unit, of 1, 2 or 4 blocks,
+// whichever spreads all over about kShares workgroups. With more, kRuns
+// workgroups (two for each CU, all there at once) take equal runs of blocks in
+// the order of a head's units, across their borders: with parts of units the last
+// round of workgroups left CUs idle (64 sequences of 1 to 4096 positions took
+// 131 us, now 125).
 struct Deal {
     int length, n, first, tiles, blocks;  // of a sequence: positions, new rows, the first of them, units a head
 };
 struct Share {
     Deal d;
-    int s, tile, head;
+    int s, tile;
     int from, to;             // blocks of the unit
     int parts;                // of the unit; part p's sums lie at part0 (p = 0), part1 + (p - 1) * step
     int part0, part1, step;
@@ -76,90 +83,100 @@ __device__ __forceinline__ Deal deal_of_lane(const Deal& d, int lane) {
             __builtin_amdgcn_readlane(d.first, lane), __builtin_amdgcn_readlane(d.tiles, lane),
             __builtin_amdgcn_readlane(d.blocks, lane)};
 }
+// Runs of a KV head.
+__host__ __device__ __forceinline__ int runs_of_head(int kv_heads) { return kRuns > kv_heads ? kRuns / kv_heads : 1; }
+
 // The host has checked that all units' blocks together fit 31 bits.
 template <int ROWS>
 struct Dealer {
     const PagedView& v;
-    const int group, lane;
-    Deal own;    // of sequence `lane`, which is all there is to know up to 64 of them
-    int total;   // blocks of all units
-    int at, end; // blocks of this workgroup's run (in order of the units)
+    const AttentionArgs& a;
+    const int lane, w;
+    Deal own;     // of sequence `lane`, which is all there is to know up to 64 of them
+    int total;    // blocks of the head's units
+    int shift;    // parts have 2^shift blocks
+    int at, end;  // blocks of this workgroup's run
     bool streams;
 
-    __device__ __forceinline__ Dealer(const PagedView& view, int g)
-        : v(view), group(g), lane(threadIdx.x & 63), own{} {
+    __device__ __forceinline__ Dealer(const PagedView& view, const AttentionArgs& args)
+        : v(view), a(args), lane(threadIdx.x & 63), w(blockIdx.x), own{} {
         int part = 0;
         for (int s = lane; s < v.sequences; s += 64) {
-            own = deal_one<ROWS>(v, group, s);
+            own = deal_one<ROWS>(v, a.group, s);
             part += own.blocks * own.tiles;
         }
-        total = __builtin_amdgcn_readlane(scan_lanes(part), 63) * v.kv_heads;
-        streams = total > kStream;
-        at = start(blockIdx.x);
-        end = start(blockIdx.x + 1);
+        total = __builtin_amdgcn_readlane(scan_lanes(part), 63);
+        const int all = total * v.kv_heads;
+        streams = all > kStream;
+        shift = all <= kShares ? 0 : all <= 2 * kShares ? 1 : 2;
+        static_assert(kStream == 4 * kShares, "parts of 1, 2 or 4 blocks");
+        at = end = 0;
+        if (streams) {
+            at = start(w);
+            end = start(w + 1);
+        }
     }
-    __device__ __forceinline__ int start(int w) const {
-        return w >= kRuns ? total : w * (total / kRuns) + min(w, total % kRuns);
+    __device__ __forceinline__ int start(int run) const {
+        const int runs = runs_of_head(v.kv_heads), even = total / runs;
+        return run >= runs ? total : run * even + min(run, total - runs * even);
     }
     __device__ __forceinline__ int owner(int block) const {
-        const int even = total / kRuns, more = total % kRuns, longer = more * (even + 1);
+        const int runs = runs_of_head(v.kv_heads), even = total / runs, more = total - runs * even;
+        const int longer = more * (even + 1);
         return block < longer ? block / (even + 1) : more + (block - longer) / even;
     }
     // This workgroup's next share, if it has one.
     __device__ __forceinline__ bool next(Share& share) {
         if (streams && at >= end) return false;
-        const int most = max(kLeast, (total + kShares - 1) / kShares), w = blockIdx.x;
-        const int wanted = streams ? at : w;
+        const int wanted = streams ? at : w, head = blockIdx.y;
         int before = 0, extra = 0;  // blocks or workgroups of the sequences before, and workgroups beyond one a unit
         for (int begin = 0; begin < v.sequences; begin += 64) {
             Deal d = own;
-            if (v.sequences > 64 && begin + lane < v.sequences) d = deal_one<ROWS>(v, group, begin + lane);
-            const int units = begin + lane < v.sequences ? d.tiles * v.kv_heads : 0;
-            const int splits = streams ? d.blocks : (d.blocks + most - 1) / most;
-            const int count = splits * units, upto = scan_lanes(count), more = scan_lanes(count - units);
+            if (v.sequences > 64 && begin + lane < v.sequences) d = deal_one<ROWS>(v, a.group, begin + lane);
+            if (begin + lane >= v.sequences) d.tiles = 0;
+            const int splits = streams ? d.blocks : (d.blocks + (1 << shift) - 1) >> shift;
+            const int count = splits * d.tiles, upto = scan_lanes(count), beyond = scan_lanes(count - d.tiles);
             const unsigned long long hit = __ballot(before + upto > wanted);
             if (hit) {
                 const int from = __ffsll(hit) - 1;
                 share.s = begin + from;
                 share.d = d = deal_of_lane(d, from);
-                const int offset = before + __builtin_amdgcn_readlane(upto - count, from);
-                const int parts = __builtin_amdgcn_readlane(splits, from);
-                const int within = wanted - offset;
+                const int within = wanted - before - __builtin_amdgcn_readlane(upto - count, from);
+                extra += __builtin_amdgcn_readlane(beyond - count, from);
                 if (streams) {
-                    const int unit = within / d.blocks;
-                    share.tile = unit / v.kv_heads;
-                    share.head = unit - share.tile * v.kv_heads;
-                    share.from = within - unit * d.blocks;
+                    const int runs = runs_of_head(v.kv_heads);
+                    share.tile = within / d.blocks;
+                    share.from = within - share.tile * d.blocks;
                     share.to = min(d.blocks, share.from + end - at);
                     const int first = owner(at - share.from), last = owner(at - share.from + d.blocks - 1);
                     share.parts = last - first + 1;
-                    share.part0 = 2 * first + 1;  // a run's last share; its first one is the end of another unit
-                    share.part1 = 2 * (first + 1);
+                    // A run's last share comes second; its first one is the end of another unit.
+                    share.part0 = 2 * (head * runs + first) + 1;
+                    share.part1 = 2 * (head * runs + first + 1);
                     share.step = 2;
-                    share.mine = share.from == 0 ? 2 * w + 1 : 2 * w;
-                    share.counter = first;  // no other unit both starts in that run and ends behind it
+                    share.mine = 2 * (head * runs + w) + (share.from == 0 ? 1 : 0);
+                    // No other unit both starts in that run and ends behind it.
+                    share.counter = head * runs + first;
                     at += share.to - share.from;
                 } else {
-                    // Tiles of one head's rows are a multiple of the KV heads apart: on one XCD where that is one of
-                    // eight, so that the second reads the first one's keys and values from its L2.
-                    const int of_tile = v.kv_heads * parts, rest = within % of_tile, split = rest / v.kv_heads;
-                    share.tile = within / of_tile;
-                    share.head = rest - split * v.kv_heads;
-                    const int even = d.blocks / parts, longer = d.blocks - even * parts;
-                    share.from = split * even + min(split, longer);
-                    share.to = share.from + even + (split < longer ? 1 : 0);
+                    const int parts = __builtin_amdgcn_readlane(splits, from);
+                    share.tile = d.tiles == 1 ? 0 : within / parts;
+                    const int split = within - share.tile * parts;
+                    share.from = split << shift;
+                    share.to = min(d.blocks, (split + 1) << shift);
                     share.parts = parts;
-                    share.part0 = w - split * v.kv_heads;
-                    share.part1 = share.part0 + v.kv_heads;
-                    share.step = v.kv_heads;
-                    share.mine = w;
-                    share.counter = extra + __builtin_amdgcn_readlane(more - count + units, from) +
-                                    (share.tile * v.kv_heads + share.head) * (parts - 1);
+                    share.mine = head * gridDim.x + w;
+                    share.part0 = share.mine - split;
+                    share.part1 = share.part0 + 1;
+                    share.step = 1;
+                    // A head's units have fewer than kShares / kv_heads parts beyond one each, so
+                    // how many of these come before is a number of the unit's own.
+                    share.counter = head * a.extra + extra + d.tiles + share.tile * (parts - 1);
                 }
                 return true;
             }
             before += __builtin_amdgcn_readlane(upto, 63);
-            extra += __builtin_amdgcn_readlane(more, 63);
+            extra += __builtin_amdgcn_readlane(beyond, 63);
         }
         return false;
     }
@@ -309,15 +326,15 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
     const bool second = PACKED && column >= 8;
     const int row_of_lane = PACKED ? column & 7 : column;
 
-    Dealer<kRows> dealer(v, a.group);
+    Dealer<kRows> dealer(v, a);
     Share share;
     while (dealer.next(share)) {
         const Deal& d = share.d;
-        const int head = share.head, begin = kBlock * share.from;
+        const int head = blockIdx.y, begin = kBlock * share.from;
         const int query_rows = a.group * d.n, row0 = share.tile * kRows;
         // Positions from shared_end on are seen by some of the tile's new rows only, from `end` on by none.
-        const int shared_end = d.length - d.n + row0 / a.group + 1;
-        const int seen_end = d.length - d.n + min(d.n - 1, (row0 + kRows - 1) / a.group) + 1;
+        const int shared_end = d.length - d.n + a.new_row(row0) + 1;
+        const int seen_end = d.length - d.n + min(d.n - 1, a.new_row(row0 + kRows - 1)) + 1;
         const int end = min(seen_end, kBlock * share.to);
         const int32_t* const table = v.table + int64_t(share.s) * v.table_stride;
 
@@ -366,7 +383,7 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
         // Queries: row r of the tile is head r % group of new row r / group.
         uint4_t query[kSteps][kProducts];
         float x[kSteps][8];
-        const int query_row = row0 + row_of_lane, new_row = query_row / a.group;
+        const int query_row = row0 + row_of_lane, new_row = a.new_row(query_row);
         const int64_t row = int64_t(d.first) + new_row;
         const bool live = query_row < query_rows && row >= 0 && row < v.total_rows;
         const int sees = live ? d.length - d.n + new_row + 1 : 0;  // positions the lane's row attends
@@ -581,7 +598,7 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
         }
         __syncthreads();
         auto finish = [&](int local, int channel, float4_t o, float top, float all) {
-            const int r = row0 + local, i = r / a.group;
+            const int r = row0 + local, i = a.new_row(r);
             const int64_t to = int64_t(d.first) + i;
             if (r >= query_rows || to < 0 || to >= v.total_rows) return;
             if (all == 0.f) o = float4_t{0.f, 0.f, 0.f, 0.f};
@@ -608,6 +625,7 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
                 for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(x[e], shrink, o[e]);
             }
             if (share.parts > 1) {
+                if (row0 + local >= query_rows) continue;
                 float* const partial = a.partials + (int64_t(share.mine) * kRows + local) * (DIM + 4);
                 post(partial + channel, o[0], o[1]);
                 post(partial + channel + 2, o[2], o[3]);
@@ -638,10 +656,11 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
                     if (row0 + local >= query_rows) continue;
                     float top = -kInf, all = 0.f;
                     float4_t o = {0.f, 0.f, 0.f, 0.f};
-                    for (int p0 = 0; p0 < share.parts; p0 += 8) {  // eight parts' loads in flight
-                        float2 state[8], low[8], high[8];
+                    constexpr int kJoin = 16;
+                for (int p0 = 0; p0 < share.parts; p0 += kJoin) {  // that many parts' loads in flight
+                        float2 state[kJoin], low[kJoin], high[kJoin];
 #pragma unroll
-                        for (int p = 0; p < 8; ++p) {
+                        for (int p = 0; p < kJoin; ++p) {
                             const int q = min(p0 + p, share.parts - 1);
                             const int64_t slot = q == 0 ? share.part0 : share.part1 + (q - 1) * share.step;
                             const float* const from = a.partials + (slot * kRows + local) * (DIM + 4);
@@ -651,20 +670,21 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
                         }
                         float grown = top;
 #pragma unroll
-                        for (int p = 0; p < 8; ++p) grown = fmaxf(grown, state[p].x);
+                        for (int p = 0; p < kJoin; ++p) grown = fmaxf(grown, state[p].x);
                         const float shrink = top == grown ? 1.f : exp2_fast(top - grown);
                         top = grown;
                         all *= shrink;
                         o *= shrink;
 #pragma unroll
-                        for (int p = 0; p < 8; ++p) {
-                            if (p0 + p >= share.parts) break;
+                        for (int p = 0; p < kJoin; ++p) {
                             const float by = state[p].x == top ? 1.f : exp2_fast(state[p].x - top);
-                            all = __builtin_fmaf(state[p].y, by, all);
-                            o[0] = __builtin_fmaf(low[p].x, by, o[0]);
-                            o[1] = __builtin_fmaf(low[p].y, by, o[1]);
-                            o[2] = __builtin_fmaf(high[p].x, by, o[2]);
-                            o[3] = __builtin_fmaf(high[p].y, by, o[3]);
+                            if (p0 + p < share.parts) {
+                                all = __builtin_fmaf(state[p].y, by, all);
+                                o[0] = __builtin_fmaf(low[p].x, by, o[0]);
+                                o[1] = __builtin_fmaf(low[p].y, by, o[1]);
+                                o[2] = __builtin_fmaf(high[p].x, by, o[2]);
+                                o[3] = __builtin_fmaf(high[p].y, by, o[3]);
+                            }
                         }
                     }
                     finish(local, channel, o, top, all);
@@ -679,18 +699,18 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
 // Sizes of a call: the grid, and what its workspace holds.
 struct AttentionPlan {
     bool packed;
-    int64_t blocks, groups, score_stride, score_rows;
+    int64_t blocks, columns, score_stride, score_rows;  // columns: workgroups of a KV head
     size_t partial_bytes, state_bytes, score_bytes;
     AttentionPlan(const qwen_gpu_paged_cache& c, const qwen_gpu_paged_batch& b, int query_heads) {
         const int64_t rows = int64_t(query_heads / c.kv_heads) * b.rows;
         packed = rows <= 8;
-        const int64_t tile_rows = packed ? 8 : 16;
-        const int64_t units = int64_t(b.sequences) * c.kv_heads * ((rows + tile_rows - 1) / tile_rows);
-        blocks = units * ((b.max_length + kBlock - 1) / kBlock);
-        groups = std::min(blocks, units + kShares);
-        if (blocks > kStream) groups = std::max<int64_t>(groups, kRuns);
-        const int64_t parts = blocks > kStream ? std::max<int64_t>(groups, 2 * kRuns) : groups;
-        partial_bytes = size_t(parts) * tile_rows * (c.head_dim + 4) * 4;
+        const int64_t tile_rows = packed ? 8 : 16, units = b.sequences * ((rows + tile_rows - 1) / tile_rows);
+        const int64_t head_blocks = units * ((b.max_length + kBlock - 1) / kBlock);
+        blocks = head_blocks * c.kv_heads;
+        columns = std::min(head_blocks, units + kShares / c.kv_heads);
+        if (blocks > kStream) columns = std::max<int64_t>(columns, runs_of_head(c.kv_heads));
+        const int64_t parts = std::max<int64_t>(columns, blocks > kStream ? 2 * runs_of_head(c.kv_heads) : 0);
+        partial_bytes = size_t(parts) * c.kv_heads * tile_rows * (c.head_dim + 4) * 4;
         score_stride = (b.max_length + kTile - 1) / kTile * kTile;
         score_rows = int64_t(b.sequences) * c.kv_heads * rows;
         state_bytes = b.weights ? (size_t(score_rows) * 8 + 15) / 16 * 16 : 0;
@@ -701,7 +721,7 @@ struct AttentionPlan {
 
 template <int TYPE, int DIM, bool PACKED>
 void attention_run(const PagedView& v, const AttentionArgs& a, const AttentionPlan& plan, hipStream_t stream) {
-    const dim3 grid{unsigned(plan.groups)}, block{kWaves * 64};
+    const dim3 grid{unsigned(plan.columns), unsigned(v.kv_heads)}, block{kWaves * 64};
     if (v.weights)
         paged_attention_kernel<TYPE, DIM, PACKED, true><<<grid, block, 0, stream>>>(v, a);
     else
