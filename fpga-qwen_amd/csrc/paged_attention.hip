@@ -100,6 +100,7 @@ void launch_paged_attention(const qwen_gpu_paged_cache& cache, const qwen_gpu_pa
                           scale * 1.44269504088896340736f,
                           reinterpret_cast<float*>(space),
                           static_cast<int*>(workspace),
+                          plan.adds,
                           reinterpret_cast<float2*>(space + plan.partial_bytes),
                           reinterpret_cast<float*>(space + plan.partial_bytes + plan.state_bytes),
                           plan.score_stride};
@@ -109,7 +110,7 @@ void launch_paged_attention(const qwen_gpu_paged_cache& cache, const qwen_gpu_pa
         attention_launch<kPagedBF16>(cache.head_dim, v, a, plan, stream);
     else
         attention_launch<kPagedE4M3>(cache.head_dim, v, a, plan, stream);
-    if (!v.weights) return;
+    if (!v.weights || plan.adds) return;
     // Enough workgroups for the positions of few units.
     const unsigned units = unsigned(v.sequences) * v.kv_heads;
     const unsigned share = unsigned(std::max(1, std::min((v.max_length + 255) / 256, int(1024 / units) + 1)));

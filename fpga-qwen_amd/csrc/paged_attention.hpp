@@ -16,6 +16,7 @@ constexpr int kShares = 512;                    // workgroups that the positions
 constexpr int kLeast = 2;                       // blocks of a part of a unit, at least
 constexpr int kStream = 4 * kShares;            // blocks from which on workgroups cross units
 constexpr int kRuns = 512;                      // workgroups that do
+constexpr int kAdds = 2;                        // turns that a unit's last workgroup takes to add to the weights
 constexpr int kCounterStep = 16;                // ints: a counter has a line of its own
 constexpr float kInf = __builtin_huge_valf();
 constexpr int kMostHeads = 1024;                // KV heads of a cache
@@ -38,8 +39,9 @@ struct AttentionArgs {
     float scale;        // times log2(e)
     float* partials;    // [parts][rows of a tile][DIM + 4]: output, reference, sum
     int* counters;      // kCounterStep apart, 0 between launches
-    float2* states;     // tracked: [sequences * kv_heads][rows * group]: reference, 1 / sum
-    float* scores;      // tracked: the same, times score_stride
+    bool adds;          // tracked: the attention adds to the weights itself
+    float2* states;     // tracked, not so: [sequences * kv_heads][rows * group]: reference, 1 / sum
+    float* scores;      // tracked: [sequences * kv_heads][rows * group][score_stride]
     int64_t score_stride;
 
     // Of a KV head's query row, the new row that it belongs to.
@@ -277,6 +279,14 @@ __device__ __forceinline__ void widen(uint4_t raw, float up, uint4_t (&out)[TYPE
     }
 }
 
+// Nonzero if one of the word's stored values is infinite or NaN.
+template <int TYPE>
+__device__ __forceinline__ unsigned not_finite(unsigned w) {
+    if constexpr (TYPE == kPagedF16) return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+    if constexpr (TYPE == kPagedBF16) return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+    return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+}
+
 template <int TYPE>
 __device__ __forceinline__ float stored(const char* row, int i, float up) {
     if constexpr (TYPE == kPagedF16) {
@@ -320,7 +330,7 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
     constexpr float kGrow = 8.f;                  // a reference is moved once a score passes it by 2^8
     constexpr std::integral_constant<int, TYPE> kType{};
     __shared__ __attribute__((aligned(16))) char lds[kWaves][kTile * kPitch];
-    __shared__ float2 wave_state[kWaves][kRows];
+    __shared__ float2 wave_state[kWaves][kRows], row_state[TRACK ? kRows : 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int column = lane & 15, part = lane >> 4;
     const bool second = PACKED && column >= 8;
@@ -515,7 +525,12 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
                             w[e] = !whole && (hidden >> (4 * u + e) & 1) ? -kInf : scores[u][e] * to_score;
-                        *reinterpret_cast<float4_t*>(to + 16 * u) = w;
+                        if (a.adds) {
+                            post(to + 16 * u, w[0], w[1]);
+                            post(to + 16 * u + 2, w[2], w[3]);
+                        } else {
+                            *reinterpret_cast<float4_t*>(to + 16 * u) = w;
+                        }
                     }
                 }
             }
@@ -528,18 +543,35 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
                 for (int p = 0; p < kProducts; ++p) weight[p][e] = words[p];
             }
 
-            // Values into LDS. What is not there, or not seen by all rows, is 0 here:
-            // a weight of 0 would not keep its infinities and NaN out.
+            // Values into LDS, 0 for those that are not there. A weight of 0 does not keep infinities and NaN
+            // out, so those in rows that only some new rows see are 0 here as well, and added below.
+            bool spoilt = false;
+            if (base + kTile > shared_end) {
+                unsigned bits = 0;
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int i = 0; i < kLoads; ++i)
+#pragma unroll
+                        for (int w = 0; w < 4; ++w)
+                            bits |= was[u] && base + 16 * u + column >= shared_end ? not_finite<TYPE>(values[u][i][w]) : 0u;
+                spoilt = __any(bits != 0);
+            }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const bool clean = whole || (was[u] && base + 16 * u + column < shared_end);
+                const bool partly = base + 16 * u + column >= shared_end;
 #pragma unroll
                 for (int i = 0; i < kLoads; ++i) {
                     uint4_t w[kPer];
                     widen<TYPE>(values[u][i], value_up[u], w);
 #pragma unroll
                     for (int j = 0; j < kPer; ++j) {
-                        if (!whole && !clean) w[j] = uint4_t{0u, 0u, 0u, 0u};
+                        if (!whole && !was[u]) w[j] = uint4_t{0u, 0u, 0u, 0u};
+                        if (spoilt && partly)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                w[j][e] &= ~((not_finite<TYPE == kPagedF16 ? kPagedF16 : kPagedBF16>(w[j][e]) >> 15) *
+                                             0xffffu);
                         *reinterpret_cast<uint4_t*>(mine + (16 * u + column) * kPitch + 64 * kPer * i + 16 * kPer * part +
                                                     16 * j) = w[j];
                     }
@@ -559,8 +591,8 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
                 for (int p = 0; p < kProducts; ++p) acc[o] = multiply(w, weight[p], acc[o], kType);
             }
 
-            // The last rows of a sequence with several new ones, one at a time.
-            if (base + kTile > shared_end) {
+            // One row at a time, for the new rows that see it.
+            if (spoilt) {
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -575,9 +607,10 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
 #pragma unroll
                             for (int o = 0; o < kOut; ++o)
 #pragma unroll
-                                for (int e = 0; e < 4; ++e)
-                                    acc[o][e] = __builtin_fmaf(p, stored<TYPE>(v.values + from, 16 * o + 4 * part + e, up),
-                                                               acc[o][e]);
+                                for (int e = 0; e < 4; ++e) {
+                                    const float x = stored<TYPE>(v.values + from, 16 * o + 4 * part + e, up);
+                                    if (x - x != 0.f) acc[o][e] = __builtin_fmaf(p, x, acc[o][e]);
+                                }
                         }
             }
         }
@@ -597,6 +630,7 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
             if (!second) *reinterpret_cast<float4_t*>(sums + (wave * kRows + row_of_lane) * DIM + 16 * o + 4 * part) = w;
         }
         __syncthreads();
+        if (TRACK && int(threadIdx.x) < kRows) row_state[threadIdx.x] = float2{0.f, 0.f};
         auto finish = [&](int local, int channel, float4_t o, float top, float all) {
             const int r = row0 + local, i = a.new_row(r);
             const int64_t to = int64_t(d.first) + i;
@@ -605,9 +639,13 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
             const float by = all == 0.f ? 0.f : 1.f / all;
             *reinterpret_cast<float4_a4*>(a.out + to * a.out_stride + (head * a.group + r - i * a.group) * DIM + channel) =
                 o * by;
-            if (TRACK && channel == 0)
-                a.states[(int64_t(share.s) * v.kv_heads + head) * (int64_t(v.rows) * a.group) + r] =
-                    float2{top == -kInf ? 0.f : top, by};
+            if (TRACK && channel == 0) {
+                const float2 state = {top == -kInf ? 0.f : top, by};
+                if (a.adds)
+                    row_state[local] = state;
+                else
+                    a.states[(int64_t(share.s) * v.kv_heads + head) * (int64_t(v.rows) * a.group) + r] = state;
+            }
         };
         for (int item = threadIdx.x; item < kRows * DIM / 4; item += kWaves * 64) {
             const int local = item / (DIM / 4), channel = 4 * (item - local * (DIM / 4));
@@ -634,6 +672,7 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
                 finish(local, channel, o, top, all);
             }
         }
+        bool ends = share.parts == 1;  // this is the workgroup that completes the unit
         if (share.parts > 1) {
             // The last of the unit's workgroups to get here adds their parts, in the
             // order of the positions. Posted values have reached memory once their
@@ -650,7 +689,8 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
                 *last = done == share.parts - 1;
             }
             __syncthreads();
-            if (*last) {
+            ends = *last;
+            if (ends) {
                 for (int item = threadIdx.x; item < kRows * DIM / 4; item += kWaves * 64) {
                     const int local = item / (DIM / 4), channel = 4 * (item - local * (DIM / 4));
                     if (row0 + local >= query_rows) continue;
@@ -691,6 +731,40 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
                 }
             }
         }
+        if (TRACK && a.adds && ends) {
+            // The unit, which has all of the head's query rows, is done, and all its scores are posted: its slots'
+            // weights grow by the rows' softmax, summed in the rows' order.
+            if (share.parts == 1) posted_stores_done();
+            __syncthreads();
+            float* const slots = v.weights + v.track_at(share.s, head);
+            const float* const unit = a.scores + (int64_t(share.s) * v.kv_heads + head) *
+                                                     (int64_t(v.rows) * a.group) * a.score_stride;
+            for (int j = 4 * int(threadIdx.x); j < d.length; j += 4 * kWaves * 64) {
+                float4_t grown = {0.f, 0.f, 0.f, 0.f};
+                for (int r0 = 0; r0 < query_rows; r0 += 4) {
+                    float2 low[4], high[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const float* const from = unit + min(r0 + q, query_rows - 1) * a.score_stride + j;
+                        low[q] = posted(from);
+                        high[q] = posted(from + 2);
+                    }
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        if (r0 + q >= query_rows) continue;
+                        const float2 state = row_state[r0 + q];
+                        const int seen = state.y == 0.f ? 0 : d.length - d.n + a.new_row(r0 + q) + 1 - j;
+                        if (seen > 0) grown[0] += exp2_fast(low[q].x - state.x) * state.y;
+                        if (seen > 1) grown[1] += exp2_fast(low[q].y - state.x) * state.y;
+                        if (seen > 2) grown[2] += exp2_fast(high[q].x - state.x) * state.y;
+                        if (seen > 3) grown[3] += exp2_fast(high[q].y - state.x) * state.y;
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (j + e < d.length) slots[j + e] += grown[e];
+            }
+        }
         if (!dealer.streams) return;
         __syncthreads();  // LDS is written anew
     }
@@ -698,7 +772,7 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
 
 // Sizes of a call: the grid, and what its workspace holds.
 struct AttentionPlan {
-    bool packed;
+    bool packed, adds;
     int64_t blocks, columns, score_stride, score_rows;  // columns: workgroups of a KV head
     size_t partial_bytes, state_bytes, score_bytes;
     AttentionPlan(const qwen_gpu_paged_cache& c, const qwen_gpu_paged_batch& b, int query_heads) {
@@ -713,6 +787,9 @@ struct AttentionPlan {
         partial_bytes = size_t(parts) * c.kv_heads * tile_rows * (c.head_dim + 4) * 4;
         score_stride = (b.max_length + kTile - 1) / kTile * kTile;
         score_rows = int64_t(b.sequences) * c.kv_heads * rows;
+        // The workgroup that completes a unit adds to the weights, four positions a thread and four rows at a time,
+        // while that takes it a few turns; beyond, and where several units share the weights, another kernel does (@@).
+        adds = rows <= tile_rows && (b.max_length + 1023) / 1024 * ((rows + 3) / 4) <= kAdds;
         state_bytes = b.weights ? (size_t(score_rows) * 8 + 15) / 16 * 16 : 0;
         score_bytes = b.weights ? size_t(score_rows) * score_stride * 4 : 0;
     }
@@ -721,6 +798,8 @@ struct AttentionPlan {
 
 template <int TYPE, int DIM, bool PACKED>
 void attention_run(const PagedView& v, const AttentionArgs& a, const AttentionPlan& plan, hipStream_t stream) {
+    // Heads vary slowest: with heads of one position on the eight XCDs at once, 64 ragged sequences in pages of
+    // [slot][head] took 120 us, so 112.
     const dim3 grid{unsigned(plan.columns), unsigned(v.kv_heads)}, block{kWaves * 64};
     if (v.weights)
         paged_attention_kernel<TYPE, DIM, PACKED, true><<<grid, block, 0, stream>>>(v, a);
