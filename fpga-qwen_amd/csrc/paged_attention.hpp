@@ -798,8 +798,9 @@ struct AttentionPlan {
 
 template <int TYPE, int DIM, bool PACKED>
 void attention_run(const PagedView& v, const AttentionArgs& a, const AttentionPlan& plan, hipStream_t stream) {
-    // Heads vary slowest: with heads of one position on the eight XCDs at once, 64 ragged sequences in pages of
-    // [slot][head] took 120 us, so 112.
+    // Heads vary slowest, and each head's workgroups that find no work come behind its others, so that the heads
+    // start one after the other: 64 sequences of 2048 in pages of [slot][head] took 109 us with all heads at once
+    // (heads fastest, or no idle workgroups between them), so 100; in pages of [head][slot] 96 and 97.
     const dim3 grid{unsigned(plan.columns), unsigned(v.kv_heads)}, block{kWaves * 64};
     if (v.weights)
         paged_attention_kernel<TYPE, DIM, PACKED, true><<<grid, block, 0, stream>>>(v, a);
