@@ -131,20 +131,21 @@ struct Dealer {
     __device__ __forceinline__ bool next(Share& share) {
         if (streams && at >= end) return false;
         const int wanted = streams ? at : w, head = blockIdx.y;
-        int before = 0, extra = 0;  // blocks or workgroups of the sequences before, and workgroups beyond one a unit
+        int before = 0, known = 0;  // blocks or workgroups, and units, of the sequences before
         for (int begin = 0; begin < v.sequences; begin += 64) {
             Deal d = own;
             if (v.sequences > 64 && begin + lane < v.sequences) d = deal_one<ROWS>(v, a.group, begin + lane);
             if (begin + lane >= v.sequences) d.tiles = 0;
             const int splits = streams ? d.blocks : (d.blocks + (1 << shift) - 1) >> shift;
-            const int count = splits * d.tiles, upto = scan_lanes(count), beyond = scan_lanes(count - d.tiles);
+            const int count = splits * d.tiles, upto = scan_lanes(count);
             const unsigned long long hit = __ballot(before + upto > wanted);
+            // Units before the sequence (of one tile count all where every sequence has the same new rows).
+            const int units = v.offsets ? scan_lanes(d.tiles) : 0;
             if (hit) {
                 const int from = __ffsll(hit) - 1;
                 share.s = begin + from;
                 share.d = d = deal_of_lane(d, from);
                 const int within = wanted - before - __builtin_amdgcn_readlane(upto - count, from);
-                extra += __builtin_amdgcn_readlane(beyond - count, from);
                 if (streams) {
                     const int runs = runs_of_head(v.kv_heads);
                     share.tile = within / d.blocks;
@@ -171,14 +172,16 @@ struct Dealer {
                     share.part0 = share.mine - split;
                     share.part1 = share.part0 + 1;
                     share.step = 1;
-                    // A head's units have fewer than kShares / kv_heads parts beyond one each, so
-                    // how many of these come before is a number of the unit's own.
-                    share.counter = head * a.extra + extra + d.tiles + share.tile * (parts - 1);
+                    // A head's units have fewer than kShares / kv_heads parts beyond one each, so how many of
+                    // these come before is a number of the unit's own.
+                    const int unit = v.offsets ? known + __builtin_amdgcn_readlane(units, from) - d.tiles
+                                               : share.s * d.tiles;
+                    share.counter = head * a.extra + w - split - (unit + share.tile);
                 }
                 return true;
             }
             before += __builtin_amdgcn_readlane(upto, 63);
-            extra += __builtin_amdgcn_readlane(beyond, 63);
+            if (v.offsets) known += __builtin_amdgcn_readlane(units, 63);
         }
         return false;
     }
