@@ -48,7 +48,8 @@ PagedView paged_view(const qwen_gpu_paged_cache& c, const qwen_gpu_paged_batch& 
         span += a.stride * (a.count - 1);
         require(span <= (int64_t(1) << 44), "Paged strides let rows overlap or run too far");
     }
-    require(b.sequences >= 1 && b.sequences <= 65536, "Paged sequences must be in 1..65536");
+    require(b.sequences >= 1 && b.sequences <= 4096, "Paged sequences must be in 1..4096");
+    require(b.sequences * c.kv_heads < 1 << 21, "Too many sequences for that many KV heads");
     require(b.table_stride >= 1, "A paged table needs entries");
     require(b.max_length >= 1 && b.max_length <= kPagedMaxLength &&
                 b.max_length <= int64_t(b.table_stride) * c.page_size,
@@ -265,7 +266,7 @@ void launch_paged_append(const qwen_gpu_paged_cache& cache, const qwen_gpu_paged
     const int64_t row = int64_t(cache.kv_heads) * cache.head_dim;
     require(key_stride >= row && value_stride >= row, "Paged rows overlap: stride below kv_heads * head_dim");
     require(key_stride <= (int64_t(1) << 32) && value_stride <= (int64_t(1) << 32), "Paged row stride is too large");
-    require(int64_t(batch.total_rows) * ((row + 511) / 512) < (int64_t(1) << 32), "Too many new rows for one call");
+    require(int64_t(batch.total_rows) * ((row + 511) / 512) < (int64_t(1) << 26), "Too many new rows for one call");
     const PagedDevice device(cache, batch, stream);
     device.check(keys, "new keys");
     device.check(values, "new values");

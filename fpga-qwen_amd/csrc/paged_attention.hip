@@ -2,6 +2,7 @@
 // weights' part of it.
 #include "paged_attention.hpp"
 
+#include <cmath>
 #include <string>
 
 #include "paged.hpp"
@@ -76,6 +77,7 @@ void launch_paged_attention(const qwen_gpu_paged_cache& cache, const qwen_gpu_pa
     require(queries, "Null argument: queries");
     require(out, "Null argument: out");
     check_heads(cache, query_heads);
+    require(std::isfinite(scale), "The scale must be finite");
     const int64_t row = int64_t(query_heads) * cache.head_dim;
     require(query_stride >= row && out_stride >= row, "Paged rows overlap: stride below query_heads * head_dim");
     require(query_stride <= (int64_t(1) << 32) && out_stride <= (int64_t(1) << 32), "Paged row stride is too large");

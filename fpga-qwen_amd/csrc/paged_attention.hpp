@@ -13,7 +13,6 @@ constexpr int kTile = 32;                       // positions of a wave's step
 constexpr int kWaves = 4;                       // of a workgroup
 constexpr int kBlock = kTile * kWaves;          // positions of a workgroup's step
 constexpr int kShares = 512;                    // workgroups that the positions are dealt to
-constexpr int kLeast = 2;                       // blocks of a part of a unit, at least
 constexpr int kStream = 4 * kShares;            // blocks from which on workgroups cross units
 constexpr int kRuns = 512;                      // workgroups that do
 constexpr int kAdds = 2;                        // turns that a unit's last workgroup takes to add to the weights
@@ -88,26 +87,58 @@ __device__ __forceinline__ Deal deal_of_lane(const Deal& d, int lane) {
 // Runs of a KV head.
 __host__ __device__ __forceinline__ int runs_of_head(int kv_heads) { return kRuns > kv_heads ? kRuns / kv_heads : 1; }
 
+// Of 64 sequences: workgroups that they take in parts of 1, 2 and 4 blocks (the
+// first are their blocks as well), and units.
+struct ChunkSums {
+    int of[4][64];
+};
+
 // The host has checked that all units' blocks together fit 31 bits.
 template <int ROWS>
 struct Dealer {
     const PagedView& v;
     const AttentionArgs& a;
+    const ChunkSums& chunks;
     const int lane, w;
-    Deal own;     // of sequence `lane`, which is all there is to know up to 64 of them
+    Deal own;     // up to 64 sequences: of sequence `lane`
     int total;    // blocks of the head's units
     int shift;    // parts have 2^shift blocks
     int at, end;  // blocks of this workgroup's run
     bool streams;
 
-    __device__ __forceinline__ Dealer(const PagedView& view, const AttentionArgs& args)
-        : v(view), a(args), lane(threadIdx.x & 63), w(blockIdx.x), own{} {
-        int part = 0;
-        for (int s = lane; s < v.sequences; s += 64) {
-            own = deal_one<ROWS>(v, a.group, s);
-            part += own.blocks * own.tiles;
+    static __device__ __forceinline__ int parts_of(int blocks, int shift) { return (blocks + (1 << shift) - 1) >> shift; }
+
+    __device__ __forceinline__ Dealer(const PagedView& view, const AttentionArgs& args, ChunkSums& shared)
+        : v(view), a(args), chunks(shared), lane(threadIdx.x & 63), w(blockIdx.x), own{} {
+        if (v.sequences <= 64) {
+            if (lane < v.sequences) own = deal_one<ROWS>(v, a.group, lane);
+            total = __builtin_amdgcn_readlane(scan_lanes(own.blocks * own.tiles), 63);
+        } else {
+            // The waves sum 64 sequences each in turn, with four turns' loads in flight.
+            for (int c0 = threadIdx.x >> 6; c0 < 64; c0 += 4 * kWaves) {
+                Deal d[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int s = (c0 + i * kWaves) * 64 + lane;
+                    d[i] = deal_one<ROWS>(v, a.group, min(s, v.sequences - 1));
+                    if (s >= v.sequences) d[i].tiles = 0;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int sum = scan_lanes(k < 3 ? parts_of(d[i].blocks, k) * d[i].tiles : d[i].tiles);
+                        if (lane == 63) shared.of[k][c0 + i * kWaves] = sum;
+                    }
+                if ((c0 + 4 * kWaves) * 64 >= v.sequences) {  // the rest of the wave's sums are 0
+                    for (int c = c0 + 4 * kWaves + kWaves * lane; c < 64; c += 64 * kWaves)
+                        for (int k = 0; k < 4; ++k) shared.of[k][c] = 0;
+                    break;
+                }
+            }
+            __syncthreads();
+            total = __builtin_amdgcn_readlane(scan_lanes(chunks.of[0][lane]), 63);
         }
-        total = __builtin_amdgcn_readlane(scan_lanes(part), 63);
         const int all = total * v.kv_heads;
         streams = all > kStream;
         shift = all <= kShares ? 0 : all <= 2 * kShares ? 1 : 2;
@@ -130,60 +161,60 @@ struct Dealer {
     // This workgroup's next share, if it has one.
     __device__ __forceinline__ bool next(Share& share) {
         if (streams && at >= end) return false;
-        const int wanted = streams ? at : w, head = blockIdx.y;
-        int before = 0, known = 0;  // blocks or workgroups, and units, of the sequences before
-        for (int begin = 0; begin < v.sequences; begin += 64) {
-            Deal d = own;
-            if (v.sequences > 64 && begin + lane < v.sequences) d = deal_one<ROWS>(v, a.group, begin + lane);
+        const int wanted = streams ? at : w, head = blockIdx.y, split_shift = streams ? 0 : shift;
+        int begin = 0, before = 0, known = 0;  // sequences, blocks or workgroups, and units, of the chunks before
+        Deal d = own;
+        if (v.sequences > 64) {
+            const int count = chunks.of[split_shift][lane], upto = scan_lanes(count);
+            const unsigned long long hit = __ballot(upto > wanted);
+            if (!hit) return false;
+            const int chunk = __ffsll(hit) - 1, units = chunks.of[3][lane];
+            begin = 64 * chunk;
+            before = __builtin_amdgcn_readlane(upto - count, chunk);
+            known = __builtin_amdgcn_readlane(scan_lanes(units) - units, chunk);
+            d = deal_one<ROWS>(v, a.group, min(begin + lane, v.sequences - 1));
             if (begin + lane >= v.sequences) d.tiles = 0;
-            const int splits = streams ? d.blocks : (d.blocks + (1 << shift) - 1) >> shift;
-            const int count = splits * d.tiles, upto = scan_lanes(count);
-            const unsigned long long hit = __ballot(before + upto > wanted);
-            // Units before the sequence (of one tile count all where every sequence has the same new rows).
-            const int units = v.offsets ? scan_lanes(d.tiles) : 0;
-            if (hit) {
-                const int from = __ffsll(hit) - 1;
-                share.s = begin + from;
-                share.d = d = deal_of_lane(d, from);
-                const int within = wanted - before - __builtin_amdgcn_readlane(upto - count, from);
-                if (streams) {
-                    const int runs = runs_of_head(v.kv_heads);
-                    share.tile = within / d.blocks;
-                    share.from = within - share.tile * d.blocks;
-                    share.to = min(d.blocks, share.from + end - at);
-                    const int first = owner(at - share.from), last = owner(at - share.from + d.blocks - 1);
-                    share.parts = last - first + 1;
-                    // A run's last share comes second; its first one is the end of another unit.
-                    share.part0 = 2 * (head * runs + first) + 1;
-                    share.part1 = 2 * (head * runs + first + 1);
-                    share.step = 2;
-                    share.mine = 2 * (head * runs + w) + (share.from == 0 ? 1 : 0);
-                    // No other unit both starts in that run and ends behind it.
-                    share.counter = head * runs + first;
-                    at += share.to - share.from;
-                } else {
-                    const int parts = __builtin_amdgcn_readlane(splits, from);
-                    share.tile = d.tiles == 1 ? 0 : within / parts;
-                    const int split = within - share.tile * parts;
-                    share.from = split << shift;
-                    share.to = min(d.blocks, (split + 1) << shift);
-                    share.parts = parts;
-                    share.mine = head * gridDim.x + w;
-                    share.part0 = share.mine - split;
-                    share.part1 = share.part0 + 1;
-                    share.step = 1;
-                    // A head's units have fewer than kShares / kv_heads parts beyond one each, so how many of
-                    // these come before is a number of the unit's own.
-                    const int unit = v.offsets ? known + __builtin_amdgcn_readlane(units, from) - d.tiles
-                                               : share.s * d.tiles;
-                    share.counter = head * a.extra + w - split - (unit + share.tile);
-                }
-                return true;
-            }
-            before += __builtin_amdgcn_readlane(upto, 63);
-            if (v.offsets) known += __builtin_amdgcn_readlane(units, 63);
         }
-        return false;
+        const int splits = parts_of(d.blocks, split_shift), count = splits * d.tiles, upto = scan_lanes(count);
+        const unsigned long long hit = __ballot(before + upto > wanted);
+        if (!hit) return false;
+        const int from = __ffsll(hit) - 1;
+        // Units before the sequence; no sum where every sequence has the same new rows.
+        const int units = v.offsets ? known + __builtin_amdgcn_readlane(scan_lanes(d.tiles) - d.tiles, from) : -1;
+        share.s = begin + from;
+        share.d = d = deal_of_lane(d, from);
+        const int within = wanted - before - __builtin_amdgcn_readlane(upto - count, from);
+        if (streams) {
+            const int runs = runs_of_head(v.kv_heads);
+            share.tile = within / d.blocks;
+            share.from = within - share.tile * d.blocks;
+            share.to = min(d.blocks, share.from + end - at);
+            const int first = owner(at - share.from), last = owner(at - share.from + d.blocks - 1);
+            share.parts = last - first + 1;
+            // A run's last share comes second; its first one is the end of another unit.
+            share.part0 = 2 * (head * runs + first) + 1;
+            share.part1 = 2 * (head * runs + first + 1);
+            share.step = 2;
+            share.mine = 2 * (head * runs + w) + (share.from == 0 ? 1 : 0);
+            // No other unit both starts in that run and ends behind it.
+            share.counter = head * runs + first;
+            at += share.to - share.from;
+        } else {
+            const int parts = __builtin_amdgcn_readlane(splits, from);
+            share.tile = d.tiles == 1 ? 0 : within / parts;
+            const int split = within - share.tile * parts;
+            share.from = split << shift;
+            share.to = min(d.blocks, (split + 1) << shift);
+            share.parts = parts;
+            share.mine = head * gridDim.x + w;
+            share.part0 = share.mine - split;
+            share.part1 = share.part0 + 1;
+            share.step = 1;
+            // A head's units have fewer than kShares / kv_heads parts beyond one each, so how many of these come
+            // before is a number of the unit's own.
+            share.counter = head * a.extra + w - split - ((v.offsets ? units : share.s * d.tiles) + share.tile);
+        }
+        return true;
     }
 };
 
@@ -330,16 +361,18 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
     constexpr int kRows = PACKED ? 8 : 16, kProducts = Terms<TYPE, PACKED>::kProducts;
     constexpr int kPitch = DIM * 2 + 32;          // bytes of a value row in LDS
     constexpr float kHead = TYPE == kPagedF16 ? 6.f : 0.f;  // FP16 weights are kept up to 2^14, far from subnormals
+    constexpr int kJoin = 16;                     // parts added at a time
     constexpr float kGrow = 8.f;                  // a reference is moved once a score passes it by 2^8
     constexpr std::integral_constant<int, TYPE> kType{};
     __shared__ __attribute__((aligned(16))) char lds[kWaves][kTile * kPitch];
     __shared__ float2 wave_state[kWaves][kRows], row_state[TRACK ? kRows : 1];
+    __shared__ ChunkSums chunks;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int column = lane & 15, part = lane >> 4;
     const bool second = PACKED && column >= 8;
     const int row_of_lane = PACKED ? column & 7 : column;
 
-    Dealer<kRows> dealer(v, a);
+    Dealer<kRows> dealer(v, a, chunks);
     Share share;
     while (dealer.next(share)) {
         const Deal& d = share.d;
@@ -632,8 +665,8 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
                 for (int e = 0; e < 4; ++e) w[e] = add_halves(acc[o][e]);
             if (!second) *reinterpret_cast<float4_t*>(sums + (wave * kRows + row_of_lane) * DIM + 16 * o + 4 * part) = w;
         }
-        __syncthreads();
         if (TRACK && int(threadIdx.x) < kRows) row_state[threadIdx.x] = float2{0.f, 0.f};
+        __syncthreads();
         auto finish = [&](int local, int channel, float4_t o, float top, float all) {
             const int r = row0 + local, i = a.new_row(r);
             const int64_t to = int64_t(d.first) + i;
@@ -699,8 +732,7 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
                     if (row0 + local >= query_rows) continue;
                     float top = -kInf, all = 0.f;
                     float4_t o = {0.f, 0.f, 0.f, 0.f};
-                    constexpr int kJoin = 16;
-                for (int p0 = 0; p0 < share.parts; p0 += kJoin) {  // that many parts' loads in flight
+                    for (int p0 = 0; p0 < share.parts; p0 += kJoin) {  // that many parts' loads in flight
                         float2 state[kJoin], low[kJoin], high[kJoin];
 #pragma unroll
                         for (int p = 0; p < kJoin; ++p) {
@@ -791,7 +823,9 @@ struct AttentionPlan {
         score_stride = (b.max_length + kTile - 1) / kTile * kTile;
         score_rows = int64_t(b.sequences) * c.kv_heads * rows;
         // The workgroup that completes a unit adds to the weights, four positions a thread and four rows at a time,
-        // while that takes it a few turns; beyond, and where several units share the weights, another kernel does (@@).
+        // while that takes it a few turns: 14.2 us against 12.2 with another kernel for 300 positions, 20.6 and 19.5 for
+        // eight sequences of 1025, 32.9 and 37.2 for eight of 4096. Where several units share the weights, that kernel
+        // adds to them always.
         adds = rows <= tile_rows && (b.max_length + 1023) / 1024 * ((rows + 3) / 4) <= kAdds;
         state_bytes = b.weights ? (size_t(score_rows) * 8 + 15) / 16 * 16 : 0;
         score_bytes = b.weights ? size_t(score_rows) * score_stride * 4 : 0;

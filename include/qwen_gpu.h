@@ -295,7 +295,7 @@ int qwen_gpu_op_copy(const void* src, void* dst, size_t bytes, void* stream);
  * max_length; a slot whose page is not in 0 .. pages - 1 is neither written
  * nor attended; rows outside 0 .. total_rows - 1 are neither read nor
  * written; offsets must not fall (where they do, which of its rows a sequence
- * gets is open). */
+ * gets is open). None of them may change while a call runs. */
 #define QWEN_GPU_PAGED_F16 0
 #define QWEN_GPU_PAGED_BF16 1
 #define QWEN_GPU_PAGED_E4M3 2   /* rows of e4m3 * 2^(exponent byte - 127) */
@@ -323,7 +323,7 @@ typedef struct qwen_gpu_paged_batch {
     float* weights;             /* [sequences][kv_heads][track_stride], or NULL: not tracked */
     int32_t* positions;         /* the same */
     int64_t track_stride;       /* at least max_length where one of them is given */
-    int sequences;              /* 1..65536 */
+    int sequences;              /* 1..4096 */
     int table_stride;           /* pages in a row of the table */
     int max_length;             /* 1..table_stride * page_size, at most 2^24 */
     int rows;                   /* 1..max_length: most new rows of a sequence */

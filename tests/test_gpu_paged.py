@@ -380,6 +380,81 @@ def test_attention_shared_pages_and_repeated_runs(qpkg):
         assert np.allclose(call.get('weights', weights[:1]), runs[0][1][s:s + 1], rtol=0, atol=2e-6)
 
 
+@pytest.mark.parametrize('kind,kv,group,dim,rows', [('f16', 16, 1, 64, 1), ('bf16', 16, 2, 64, 2),
+                                                    ('e4m3', 12, 9, 64, 2), ('f16', 3, 2, 128, 1)])
+@pytest.mark.parametrize('tracked', [False, True])
+def test_attention_runs_across_units(qpkg, kind, kv, group, dim, rows, tracked):
+    """More blocks of 128 positions than workgroups get one by one: they take
+    runs that begin and end inside units and hold whole ones, of one tile of query
+    rows and of several, and of sequences without positions."""
+    rng = np.random.default_rng(67)
+    count = 2600 // kv // (3 if group == 9 else 1)
+    lengths = [int(x) for x in rng.integers(0, 300 if kv > 3 else 140, count)]
+    lengths[3], lengths[5:8] = 1500, [0, 0, 128]
+    table, pages = make_table(rng, lengths, 32)
+    cache = ref.Cache(kind, pages, 32, kv, dim, rng=rng)
+    weights = rng.random((count, kv, 1500)).astype(np.float32) if tracked else None
+    attend(qpkg, cache, table, lengths, rows, kv * group, rng=rng, weights=weights, max_length=1500)
+
+
+@pytest.mark.parametrize('count', [64, 65, 130, 700, 1100])
+@pytest.mark.parametrize('ragged', [False, True])
+def test_attention_many_sequences(qpkg, count, ragged):
+    rng = np.random.default_rng(71)
+    lengths = [int(x) for x in rng.integers(0, 40, count)]
+    lengths[count // 2], lengths[-1] = 700, 300
+    counts = [int(x) for x in rng.integers(0, 3, count)] if ragged else [1] * count
+    offsets = np.concatenate(([0], np.cumsum(counts))) if ragged else None
+    table, pages = make_table(rng, lengths, 16)
+    cache = ref.Cache('f16', pages, 16, 2, 64, rng=rng)
+    attend(qpkg, cache, table, lengths, 2 if ragged else 1, 4, offsets=offsets, total=sum(counts), rng=rng)
+
+
+def test_workspace_serves_calls_of_different_shapes(qpkg):
+    """One workspace, zeroed once, for calls that split differently, with an eviction in between: the
+    same bits as with fresh ones, and its counters are 0 again after each."""
+    rng = np.random.default_rng(73)
+    shapes = [([4000], 2, 4, 1), ([100] * 20, 2, 4, 2), ([900, 3, 2000], 8, 16, 1), ([4000], 2, 4, 1)]
+    shapes.append(([300] * 60, 16, 16, 1))
+    calls = []
+    for lengths, kv, heads, rows in shapes:
+        table, pages = make_table(rng, lengths, 16)
+        cache = ref.Cache('f16', pages, 16, kv, 64, rng=rng)
+        tracked = (len(lengths), kv, max(lengths))
+        weights, positions = rng.random(tracked).astype(np.float32), np.zeros(tracked, np.int32)
+        calls.append((Call(qpkg, cache, table, lengths, rows, weights=weights, positions=positions), heads))
+    space = max((call.workspace(heads) for call, heads in calls), key=lambda x: x.nbytes)
+    for call, heads in calls:
+        queries = rng.standard_normal((call.total, heads * 64)).astype(np.float32)
+        fresh = call.attention(queries, heads, 0.125, np.zeros_like(queries))
+        shared = call.attention(queries, heads, 0.125, np.zeros_like(queries), space)
+        assert np.array_equal(fresh, shared)
+        assert not space.to_array(np.uint8, 98304).any()
+        n = qpkg.DeviceBuffer(4 * len(call.lengths))
+        keep = max(1, int(call.lengths.max()) // 2)
+        call.check(call.lib.qwen_gpu_op_paged_evict(ctypes.byref(call.c), ctypes.byref(call.b), keep, 0, 1, n.ptr,
+                                                    call.b.weights, call.b.positions, space.ptr, space.nbytes, None))
+        qpkg.synchronize()
+        assert not space.to_array(np.uint8, 98304).any()
+
+
+def test_attention_in_place_of_its_queries(qpkg):
+    """out may be the queries' own memory."""
+    rng = np.random.default_rng(79)
+    lengths, heads, dim = [1000, 5, 300], 24, 64
+    table, pages = make_table(rng, lengths, 16)
+    cache = ref.Cache('bf16', pages, 16, 2, dim, rng=rng)
+    queries = rng.standard_normal((6, heads * dim)).astype(np.float32)
+    call = Call(qpkg, cache, table, lengths, 2)
+    want = call.attention(queries, heads, 0.125, np.zeros_like(queries))
+    both = qpkg.DeviceBuffer.from_array(queries)
+    call.check(call.lib.qwen_gpu_op_paged_attention(ctypes.byref(call.c), ctypes.byref(call.b), both.ptr, heads * dim,
+                                                    heads, 0.125, both.ptr, heads * dim, call.space.ptr,
+                                                    call.space.nbytes, None))
+    qpkg.synchronize()
+    assert np.array_equal(both.to_array(np.float32, queries.size).reshape(queries.shape), want)
+
+
 # ---- eviction ----
 
 @pytest.mark.parametrize('kind,heads,dim,page,layout', [('f16', 8, 128, 16, 'head'), ('bf16', 3, 64, 5, 'slot'),

@@ -98,6 +98,26 @@ def test_calls_refused(qpkg, op, message, call):
     refused(qpkg, message, op=op, **call)
 
 
+@pytest.mark.parametrize('scale', [np.inf, -np.inf, np.nan])
+def test_scale_refused(qpkg, scale):
+    status = qpkg.load_library().qwen_gpu_op_paged_attention(cache(qpkg), batch(qpkg), AT, 2048, 16, scale, AT, 2048, AT,
+                                                             1 << 30, None)
+    assert status == 1 and 'scale must be finite' in qpkg.load_library().qwen_gpu_last_error().decode()
+
+
+def test_sizes_refused_that_no_launch_holds(qpkg):
+    """Grids and indices would pass 32 bits."""
+    wide = dict(sequences=4096, total_rows=4096)
+    heads = cache(qpkg, kv_heads=1024, page_stride=1024 * 16 * 128)
+    for op in ('append', 'attention', 'evict'):
+        refused(qpkg, 'Too many sequences', heads, batch(qpkg, **wide), op=op, k_stride=1 << 20, v_stride=1 << 20,
+                q_stride=1 << 20, out_stride=1 << 20, heads=1024)
+    long = dict(table_stride=1 << 20, max_length=1 << 24, track_stride=1 << 24, sequences=4096, total_rows=4096)
+    refused(qpkg, 'Too many new rows or positions', b=batch(qpkg, **long), op='attention')
+    refused(qpkg, 'Too many new rows', cache(qpkg, kv_heads=64, page_stride=64 * 16 * 128),
+            batch(qpkg, offsets=AT, total_rows=1 << 23), op='append', k_stride=1 << 13, v_stride=1 << 13)
+
+
 def test_evict_needs_what_it_goes_by(qpkg):
     refused(qpkg, 'Null argument: weights', b=batch(qpkg, weights=None), op='evict')
     refused(qpkg, 'Null argument: positions', b=batch(qpkg, positions=None), op='evict')
