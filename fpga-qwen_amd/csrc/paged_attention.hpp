@@ -36,7 +36,7 @@ struct AttentionArgs {
     unsigned magic;     // of the group, as page_slot takes it
     int extra;          // counters of a KV head
     float scale;        // times log2(e)
-    float* partials;    // [parts][rows of a tile][DIM + 4]: output, reference, sum
+    float* partials;    // [parts][rows of a tile][DIM + 4]: output, reference, sum, the same of a group of parts
     int* counters;      // kCounterStep apart, 0 between launches
     bool adds;          // tracked: the attention adds to the weights itself
     float2* states;     // tracked, not so: [sequences * kv_heads][rows * group]: reference, 1 / sum
@@ -65,10 +65,11 @@ struct Share {
     Deal d;
     int s, tile;
     int from, to;             // blocks of the unit
-    int parts;                // of the unit; part p's sums lie at part0 (p = 0), part1 + (p - 1) * step
+    int parts, part;          // of the unit; part p's sums lie at part0 (p = 0), part1 + (p - 1) * step
     int part0, part1, step;
-    int mine;                 // where this one's lie
-    int counter;
+    int counter;              // the first of parts - 1 that are the unit's own
+
+    __device__ __forceinline__ int64_t slot(int p) const { return p == 0 ? part0 : part1 + (p - 1) * step; }
 };
 template <int ROWS>
 __device__ __forceinline__ Deal deal_one(const PagedView& v, int group, int s) {
@@ -195,8 +196,8 @@ struct Dealer {
             share.part0 = 2 * (head * runs + first) + 1;
             share.part1 = 2 * (head * runs + first + 1);
             share.step = 2;
-            share.mine = 2 * (head * runs + w) + (share.from == 0 ? 1 : 0);
-            // No other unit both starts in that run and ends behind it.
+            share.part = w - first;
+            // No other unit starts in these runs, but for the last, and ends behind its own first.
             share.counter = head * runs + first;
             at += share.to - share.from;
         } else {
@@ -206,12 +207,11 @@ struct Dealer {
             share.from = split << shift;
             share.to = min(d.blocks, (split + 1) << shift);
             share.parts = parts;
-            share.mine = head * gridDim.x + w;
-            share.part0 = share.mine - split;
+            share.part = split;
+            share.part0 = head * gridDim.x + w - split;
             share.part1 = share.part0 + 1;
             share.step = 1;
-            // A head's units have fewer than kShares / kv_heads parts beyond one each, so how many of these come
-            // before is a number of the unit's own.
+            // A head's units have fewer than kShares / kv_heads parts beyond one each: these are counted.
             share.counter = head * a.extra + w - split - ((v.offsets ? units : share.s * d.tiles) + share.tile);
         }
         return true;
@@ -361,7 +361,8 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
     constexpr int kRows = PACKED ? 8 : 16, kProducts = Terms<TYPE, PACKED>::kProducts;
     constexpr int kPitch = DIM * 2 + 32;          // bytes of a value row in LDS
     constexpr float kHead = TYPE == kPagedF16 ? 6.f : 0.f;  // FP16 weights are kept up to 2^14, far from subnormals
-    constexpr int kJoin = 16;                     // parts added at a time
+    constexpr int kJoin = PACKED ? 16 : 8;        // parts whose sums are loaded at a time, as registers allow
+    constexpr int kGroup = 16, kFlat = 32;        // parts that are added as a group, and at most without groups
     constexpr float kGrow = 8.f;                  // a reference is moved once a score passes it by 2^8
     constexpr std::integral_constant<int, TYPE> kType{};
     __shared__ __attribute__((aligned(16))) char lds[kWaves][kTile * kPitch];
@@ -700,7 +701,7 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
             }
             if (share.parts > 1) {
                 if (row0 + local >= query_rows) continue;
-                float* const partial = a.partials + (int64_t(share.mine) * kRows + local) * (DIM + 4);
+                float* const partial = a.partials + (share.slot(share.part) * kRows + local) * (DIM + 4);
                 post(partial + channel, o[0], o[1]);
                 post(partial + channel + 2, o[2], o[3]);
                 if (channel == 0) post(partial + DIM, top, all);
@@ -710,36 +711,41 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
         }
         bool ends = share.parts == 1;  // this is the workgroup that completes the unit
         if (share.parts > 1) {
-            // The last of the unit's workgroups to get here adds their parts, in the
-            // order of the positions. Posted values have reached memory once their
-            // stores are done, and are read past the caches, so no fence of the
-            // device's scope is needed: with one in every workgroup (it writes back
-            // and drops a whole L2) eight sequences of 2048 took 42 us instead of 16.
-            posted_stores_done();
-            __syncthreads();
-            int* const last = reinterpret_cast<int*>(wave_state);
-            int* const counter = a.counters + share.counter * kCounterStep;
-            if (threadIdx.x == 0) {
-                const int done = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                if (done == share.parts - 1) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                *last = done == share.parts - 1;
-            }
-            __syncthreads();
-            ends = *last;
-            if (ends) {
+            // The last of the unit's workgroups to get here adds their parts, in the order of the positions; of more
+            // than kFlat parts the last of each kGroup adds those, and the last of these the groups (115 parts of 16
+            // rows by one workgroup took 40 us). Posted values have reached memory once their stores are done, and
+            // are read past the caches, so no fence of the device's scope is needed: with one in every workgroup (it
+            // writes back and drops a whole L2) eight sequences of 2048 took 42 us instead of 16.
+            int* const flag = reinterpret_cast<int*>(wave_state);
+            auto last_of = [&](int index, int count) {
+                posted_stores_done();
+                __syncthreads();
+                if (threadIdx.x == 0) {
+                    int* const counter = a.counters + (share.counter + index) * kCounterStep;
+                    const int done = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    if (done == count - 1) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    *flag = done == count - 1;
+                }
+                __syncthreads();
+                return *flag != 0;
+            };
+            // f(row, channel, sums, reference, sum) of parts first, first + every, ...; their references and sums lie
+            // `beside` their sums.
+            auto join = [&](int first, int count, int every, int beside, auto f) {
+#pragma unroll 1
                 for (int item = threadIdx.x; item < kRows * DIM / 4; item += kWaves * 64) {
                     const int local = item / (DIM / 4), channel = 4 * (item - local * (DIM / 4));
                     if (row0 + local >= query_rows) continue;
                     float top = -kInf, all = 0.f;
                     float4_t o = {0.f, 0.f, 0.f, 0.f};
-                    for (int p0 = 0; p0 < share.parts; p0 += kJoin) {  // that many parts' loads in flight
+                    for (int p0 = 0; p0 < count; p0 += kJoin) {  // that many parts' loads in flight
                         float2 state[kJoin], low[kJoin], high[kJoin];
 #pragma unroll
                         for (int p = 0; p < kJoin; ++p) {
-                            const int q = min(p0 + p, share.parts - 1);
-                            const int64_t slot = q == 0 ? share.part0 : share.part1 + (q - 1) * share.step;
-                            const float* const from = a.partials + (slot * kRows + local) * (DIM + 4);
-                            state[p] = posted(from + DIM);
+                            const float* const from =
+                                a.partials +
+                                (share.slot(first + min(p0 + p, count - 1) * every) * kRows + local) * (DIM + 4);
+                            state[p] = posted(from + beside);
                             low[p] = posted(from + channel);
                             high[p] = posted(from + channel + 2);
                         }
@@ -753,7 +759,7 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
 #pragma unroll
                         for (int p = 0; p < kJoin; ++p) {
                             const float by = state[p].x == top ? 1.f : exp2_fast(state[p].x - top);
-                            if (p0 + p < share.parts) {
+                            if (p0 + p < count) {
                                 all = __builtin_fmaf(state[p].y, by, all);
                                 o[0] = __builtin_fmaf(low[p].x, by, o[0]);
                                 o[1] = __builtin_fmaf(low[p].y, by, o[1]);
@@ -762,7 +768,27 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
                             }
                         }
                     }
-                    finish(local, channel, o, top, all);
+                    f(local, channel, o, top, all);
+                }
+            };
+            if (share.parts <= kFlat) {
+                ends = last_of(0, share.parts);
+                if (ends) join(0, share.parts, 1, DIM, finish);
+            } else {
+                const int group = share.part / kGroup, first = group * kGroup;
+                const int of_group = min(kGroup, share.parts - first), groups = (share.parts + kGroup - 1) / kGroup;
+                ends = last_of(1 + group, of_group);
+                if (ends) {
+                    // The group's sums take the place of its first part's, which nobody else reads any more; its
+                    // reference and sum, which all threads of a row have still to read, go beside those.
+                    join(first, of_group, 1, DIM, [&](int local, int channel, float4_t o, float top, float all) {
+                        float* const partial = a.partials + (share.slot(first) * kRows + local) * (DIM + 4);
+                        post(partial + channel, o[0], o[1]);
+                        post(partial + channel + 2, o[2], o[3]);
+                        if (channel == 0) post(partial + DIM + 2, top, all);
+                    });
+                    ends = last_of(0, groups);
+                    if (ends) join(0, groups, kGroup, DIM + 2, finish);
                 }
             }
         }
