@@ -82,7 +82,7 @@ void launch_paged_attention(const qwen_gpu_paged_cache& cache, const qwen_gpu_pa
     require(query_stride >= row && out_stride >= row, "Paged rows overlap: stride below query_heads * head_dim");
     require(query_stride <= (int64_t(1) << 32) && out_stride <= (int64_t(1) << 32), "Paged row stride is too large");
     const AttentionPlan plan(cache, batch, query_heads);
-    require(plan.blocks < (int64_t(1) << 31) && plan.columns < (int64_t(1) << 24) &&
+    require(plan.blocks < (int64_t(1) << 31) && plan.columns < (int64_t(1) << 23) && plan.grid_rows <= 65535 &&
                 plan.score_rows < (int64_t(1) << 31),
             "Too many new rows or positions for one call");
     const PagedDevice device(cache, batch, stream);
@@ -98,7 +98,8 @@ void launch_paged_attention(const qwen_gpu_paged_cache& cache, const qwen_gpu_pa
                           out_stride,
                           query_heads / cache.kv_heads,
                           0xffffffffu / unsigned(query_heads / cache.kv_heads),
-                          kShares / cache.kv_heads + 1,
+                          int(kShares / plan.grid_rows) + 1,
+                          int(plan.tiles),
                           scale * 1.44269504088896340736f,
                           reinterpret_cast<float*>(space),
                           static_cast<int*>(workspace),

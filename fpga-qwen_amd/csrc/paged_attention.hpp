@@ -18,9 +18,8 @@ constexpr int kRuns = 512;                      // workgroups that do
 constexpr int kAdds = 2;                        // turns that a unit's last workgroup takes to add to the weights
 constexpr int kCounterStep = 16;                // ints: a counter has a line of its own
 constexpr float kInf = __builtin_huge_valf();
-constexpr int kMostHeads = 1024;                // KV heads of a cache
-static_assert(std::max(kShares, kRuns) + kMostHeads <= int(kPagedCounterBytes / (kCounterStep * sizeof(int))),
-              "counters");
+// More than kShares rows of the grid split no unit, up to there a row has kShares / rows + 1 counters.
+static_assert(std::max(kRuns, 2 * kShares) * kCounterStep * sizeof(int) <= kPagedCounterBytes, "counters");
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -34,7 +33,8 @@ struct AttentionArgs {
     int64_t out_stride;
     int group;          // query heads of a KV head
     unsigned magic;     // of the group, as page_slot takes it
-    int extra;          // counters of a KV head
+    int extra;          // counters of a row of the grid
+    int tiles;          // of a KV head's query rows: grid row y has head y / tiles, tile y % tiles
     float scale;        // times log2(e)
     float* partials;    // [parts][rows of a tile][DIM + 4]: output, reference, sum, the same of a group of parts
     int* counters;      // kCounterStep apart, 0 between launches
@@ -47,23 +47,25 @@ struct AttentionArgs {
     __device__ __forceinline__ int new_row(int r) const { return page_slot(r, group, magic).page; }
 };
 
-// How the positions are dealt. A unit is a sequence, a KV head (blockIdx.y)
-// and a tile of its query rows; it has `blocks` blocks of 128 positions (one
-// at least, so that rows without positions are written too). Workgroups find
-// their shares from the lengths on the device, every wave by itself, so the
-// host needs no lengths and a captured launch follows them. With up to kStream
-// blocks in all, a workgroup has one part of one unit, of 1, 2 or 4 blocks,
-// whichever spreads all over about kShares workgroups. With more, kRuns
-// workgroups (two for each CU, all there at once) take equal runs of blocks in
-// the order of a head's units, across their borders: with parts of units the last
-// round of workgroups left CUs idle (64 sequences of 1 to 4096 positions took
-// 131 us, now 125).
+// How the positions are dealt. A unit is a sequence, a KV head and a tile of its
+// query rows; it has `blocks` blocks of 128 positions (one at least, so that
+// rows without positions are written too). Row blockIdx.y of the grid has a head
+// and a tile, so the tiles of a head's rows take the same positions at the same
+// time. Workgroups find their shares from the lengths on the device, every wave
+// by itself, so the host needs no lengths and a captured launch follows them.
+// With up to kStream blocks in all, a workgroup has one part of one unit, of 1,
+// 2 or 4 blocks, whichever spreads all over about kShares workgroups. With more,
+// kRuns workgroups (two for each CU, all there at once) take equal runs of blocks
+// in the order of a grid row's units, across their borders: with parts of units
+// the last round of workgroups left CUs idle (64 sequences of 1 to 4096
+// positions took 131 us, in runs 125); 768, 1024 and 1536 runs took 130, 124 and
+// 125 us, and for 64 equal sequences 120, 103 and 116 us where 512 take 95.
 struct Deal {
-    int length, n, first, tiles, blocks;  // of a sequence: positions, new rows, the first of them, units a head
+    int length, n, first, blocks;  // of a sequence: positions, new rows, the first of them, blocks (0: no unit)
 };
 struct Share {
     Deal d;
-    int s, tile;
+    int s;
     int from, to;             // blocks of the unit
     int parts, part;          // of the unit; part p's sums lie at part0 (p = 0), part1 + (p - 1) * step
     int part0, part1, step;
@@ -72,24 +74,22 @@ struct Share {
     __device__ __forceinline__ int64_t slot(int p) const { return p == 0 ? part0 : part1 + (p - 1) * step; }
 };
 template <int ROWS>
-__device__ __forceinline__ Deal deal_one(const PagedView& v, int group, int s) {
+__device__ __forceinline__ Deal deal_one(const PagedView& v, int group, int tile, int s) {
     Deal d;
     d.length = v.length(s);
     d.n = v.new_rows(s, d.first);
-    d.tiles = (group * d.n + ROWS - 1) / ROWS;
-    d.blocks = max(1, (d.length + kBlock - 1) / kBlock);
+    d.blocks = tile * ROWS < group * d.n ? max(1, (d.length + kBlock - 1) / kBlock) : 0;
     return d;
 }
 __device__ __forceinline__ Deal deal_of_lane(const Deal& d, int lane) {
     return {__builtin_amdgcn_readlane(d.length, lane), __builtin_amdgcn_readlane(d.n, lane),
-            __builtin_amdgcn_readlane(d.first, lane), __builtin_amdgcn_readlane(d.tiles, lane),
-            __builtin_amdgcn_readlane(d.blocks, lane)};
+            __builtin_amdgcn_readlane(d.first, lane), __builtin_amdgcn_readlane(d.blocks, lane)};
 }
-// Runs of a KV head.
-__host__ __device__ __forceinline__ int runs_of_head(int kv_heads) { return kRuns > kv_heads ? kRuns / kv_heads : 1; }
+// Runs of a row of the grid.
+__host__ __device__ __forceinline__ int runs_of_row(int grid_rows) { return kRuns > grid_rows ? kRuns / grid_rows : 1; }
 
-// Of 64 sequences: workgroups that they take in parts of 1, 2 and 4 blocks (the
-// first are their blocks as well), and units.
+// Of 64 sequences' units in a row of the grid: their parts of 1, 2 and 4 blocks
+// (the first are their blocks as well), and their number.
 struct ChunkSums {
     int of[4][64];
 };
@@ -100,20 +100,25 @@ struct Dealer {
     const PagedView& v;
     const AttentionArgs& a;
     const ChunkSums& chunks;
-    const int lane, w;
+    const int lane, w, tile;
     Deal own;     // up to 64 sequences: of sequence `lane`
-    int total;    // blocks of the head's units
+    int total;    // blocks of the grid row's units
+    int runs;     // of the grid row
     int shift;    // parts have 2^shift blocks
     int at, end;  // blocks of this workgroup's run
     bool streams;
 
-    static __device__ __forceinline__ int parts_of(int blocks, int shift) { return (blocks + (1 << shift) - 1) >> shift; }
+    static __device__ __forceinline__ int parts_of(int blocks, int shift) {
+        return (blocks + (1 << shift) - 1) >> shift;
+    }
 
-    __device__ __forceinline__ Dealer(const PagedView& view, const AttentionArgs& args, ChunkSums& shared)
-        : v(view), a(args), chunks(shared), lane(threadIdx.x & 63), w(blockIdx.x), own{} {
+    __device__ __forceinline__ Dealer(const PagedView& view, const AttentionArgs& args, ChunkSums& shared,
+                                      int rows_tile)
+        : v(view), a(args), chunks(shared), lane(threadIdx.x & 63), w(blockIdx.z * gridDim.x + blockIdx.x),
+          tile(rows_tile), own{}, runs(runs_of_row(gridDim.y)) {
         if (v.sequences <= 64) {
-            if (lane < v.sequences) own = deal_one<ROWS>(v, a.group, lane);
-            total = __builtin_amdgcn_readlane(scan_lanes(own.blocks * own.tiles), 63);
+            if (lane < v.sequences) own = deal_one<ROWS>(v, a.group, tile, lane);
+            total = __builtin_amdgcn_readlane(scan_lanes(own.blocks), 63);
         } else {
             // The waves sum 64 sequences each in turn, with four turns' loads in flight.
             for (int c0 = threadIdx.x >> 6; c0 < 64; c0 += 4 * kWaves) {
@@ -121,14 +126,14 @@ struct Dealer {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int s = (c0 + i * kWaves) * 64 + lane;
-                    d[i] = deal_one<ROWS>(v, a.group, min(s, v.sequences - 1));
-                    if (s >= v.sequences) d[i].tiles = 0;
+                    d[i] = deal_one<ROWS>(v, a.group, tile, min(s, v.sequences - 1));
+                    if (s >= v.sequences) d[i].blocks = 0;
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        const int sum = scan_lanes(k < 3 ? parts_of(d[i].blocks, k) * d[i].tiles : d[i].tiles);
+                        const int sum = scan_lanes(k < 3 ? parts_of(d[i].blocks, k) : d[i].blocks > 0);
                         if (lane == 63) shared.of[k][c0 + i * kWaves] = sum;
                     }
                 if ((c0 + 4 * kWaves) * 64 >= v.sequences) {  // the rest of the wave's sums are 0
@@ -140,7 +145,7 @@ struct Dealer {
             __syncthreads();
             total = __builtin_amdgcn_readlane(scan_lanes(chunks.of[0][lane]), 63);
         }
-        const int all = total * v.kv_heads;
+        const int all = total * int(gridDim.y);
         streams = all > kStream;
         shift = all <= kShares ? 0 : all <= 2 * kShares ? 1 : 2;
         static_assert(kStream == 4 * kShares, "parts of 1, 2 or 4 blocks");
@@ -151,18 +156,18 @@ struct Dealer {
         }
     }
     __device__ __forceinline__ int start(int run) const {
-        const int runs = runs_of_head(v.kv_heads), even = total / runs;
+        const int even = total / runs;
         return run >= runs ? total : run * even + min(run, total - runs * even);
     }
     __device__ __forceinline__ int owner(int block) const {
-        const int runs = runs_of_head(v.kv_heads), even = total / runs, more = total - runs * even;
+        const int even = total / runs, more = total - runs * even;
         const int longer = more * (even + 1);
         return block < longer ? block / (even + 1) : more + (block - longer) / even;
     }
     // This workgroup's next share, if it has one.
     __device__ __forceinline__ bool next(Share& share) {
         if (streams && at >= end) return false;
-        const int wanted = streams ? at : w, head = blockIdx.y, split_shift = streams ? 0 : shift;
+        const int wanted = streams ? at : w, row = blockIdx.y, split_shift = streams ? 0 : shift;
         int begin = 0, before = 0, known = 0;  // sequences, blocks or workgroups, and units, of the chunks before
         Deal d = own;
         if (v.sequences > 64) {
@@ -173,46 +178,42 @@ struct Dealer {
             begin = 64 * chunk;
             before = __builtin_amdgcn_readlane(upto - count, chunk);
             known = __builtin_amdgcn_readlane(scan_lanes(units) - units, chunk);
-            d = deal_one<ROWS>(v, a.group, min(begin + lane, v.sequences - 1));
-            if (begin + lane >= v.sequences) d.tiles = 0;
+            d = deal_one<ROWS>(v, a.group, tile, min(begin + lane, v.sequences - 1));
+            if (begin + lane >= v.sequences) d.blocks = 0;
         }
-        const int splits = parts_of(d.blocks, split_shift), count = splits * d.tiles, upto = scan_lanes(count);
+        const int count = parts_of(d.blocks, split_shift), upto = scan_lanes(count);
         const unsigned long long hit = __ballot(before + upto > wanted);
         if (!hit) return false;
         const int from = __ffsll(hit) - 1;
-        // Units before the sequence; no sum where every sequence has the same new rows.
-        const int units = v.offsets ? known + __builtin_amdgcn_readlane(scan_lanes(d.tiles) - d.tiles, from) : -1;
+        // Units before the sequence's: all sequences where each has the same new rows.
+        const int units =
+            v.offsets ? known + __popcll(__ballot(d.blocks > 0) & ((1ull << from) - 1)) : begin + from;
         share.s = begin + from;
         share.d = d = deal_of_lane(d, from);
         const int within = wanted - before - __builtin_amdgcn_readlane(upto - count, from);
         if (streams) {
-            const int runs = runs_of_head(v.kv_heads);
-            share.tile = within / d.blocks;
-            share.from = within - share.tile * d.blocks;
+            share.from = within;
             share.to = min(d.blocks, share.from + end - at);
             const int first = owner(at - share.from), last = owner(at - share.from + d.blocks - 1);
             share.parts = last - first + 1;
             // A run's last share comes second; its first one is the end of another unit.
-            share.part0 = 2 * (head * runs + first) + 1;
-            share.part1 = 2 * (head * runs + first + 1);
+            share.part0 = 2 * (row * runs + first) + 1;
+            share.part1 = 2 * (row * runs + first + 1);
             share.step = 2;
             share.part = w - first;
             // No other unit starts in these runs, but for the last, and ends behind its own first.
-            share.counter = head * runs + first;
+            share.counter = row * runs + first;
             at += share.to - share.from;
         } else {
-            const int parts = __builtin_amdgcn_readlane(splits, from);
-            share.tile = d.tiles == 1 ? 0 : within / parts;
-            const int split = within - share.tile * parts;
-            share.from = split << shift;
-            share.to = min(d.blocks, (split + 1) << shift);
-            share.parts = parts;
-            share.part = split;
-            share.part0 = head * gridDim.x + w - split;
+            share.from = within << shift;
+            share.to = min(d.blocks, (within + 1) << shift);
+            share.parts = __builtin_amdgcn_readlane(count, from);
+            share.part = within;
+            share.part0 = row * int(gridDim.x * gridDim.z) + w - within;
             share.part1 = share.part0 + 1;
             share.step = 1;
-            // A head's units have fewer than kShares / kv_heads parts beyond one each: these are counted.
-            share.counter = head * a.extra + w - split - ((v.offsets ? units : share.s * d.tiles) + share.tile);
+            // A grid row's units have fewer than kShares / rows parts beyond one each: these are counted.
+            share.counter = row * a.extra + w - within - units;
         }
         return true;
     }
@@ -226,7 +227,8 @@ __device__ __forceinline__ void post(float* p, float a, float b) {
 }
 __device__ __forceinline__ void posted_stores_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ float2 posted(const float* p) {
-    const uint64_t w = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const uint64_t w =
+        __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     return float2{__builtin_bit_cast(float, unsigned(w)), __builtin_bit_cast(float, unsigned(w >> 32))};
 }
 
@@ -245,21 +247,24 @@ __device__ __forceinline__ short4_t read_transposed(const char* p) {
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 __device__ __forceinline__ float4_t multiply(uint4_t a, uint4_t b, float4_t c, std::integral_constant<int, kPagedF16>) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0,
+                                                  0);
 }
 template <int TYPE>
 __device__ __forceinline__ float4_t multiply(uint4_t a, uint4_t b, float4_t c, std::integral_constant<int, TYPE>) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
-                                                   0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                   0, 0);
 }
 
 // FP32 values as sums of 16-bit ones, for products on the matrix cores: two
 // FP16 terms hold 22 bits, three BF16 terms 24 (two, 2^-17 off, would lose ten
 // times what the sums do). A product has 16 columns. Up to 8 query rows are
 // packed: columns 0-7 take the first term and 8-15 the second, the halves of
-// the result are added, and a third term takes a second product with empty columns 8-15. More
-// rows take a column each and a product for every term, added by the matrix cores.
-// E4M3 rows become BF16 as they are read, with their power of two: exact.
+// the result are added, and a third term takes a second product with columns
+// 8-15 empty. More rows take a column each and a product for every term (16
+// rows as two packed tiles took 132 us for 16 sequences of 8192, so 105; BF16
+// 172 and 105). E4M3 rows become BF16 as they are read, with their power of
+// two: exact.
 template <int TYPE, bool PACKED>
 struct Terms {
     static constexpr int kTerms = TYPE == kPagedF16 ? 2 : 3, kProducts = PACKED ? kTerms - 1 : kTerms;
@@ -345,24 +350,31 @@ __device__ __forceinline__ float add_halves(float x) {
 // S^T as it comes from memory. S^T leaves lane l with column l % 16 and
 // positions 4 (l / 16) .. + 3 of each 16, which is the B operand of O^T when
 // V^T's columns are taken in that order, so weights never change lanes. V
-// goes through LDS (each wave its own 32 rows) and comes back transposed;
-// rows are 32 bytes apart from a multiple of 256 so that the 16 rows of a
-// read fall on all banks twice.
+// goes through LDS (each wave its own 32 rows) and comes back transposed; a
+// row's pitch is 32 bytes more than its values, so that the 16 rows of a read
+// fall on all banks twice.
 //
-// Memory is what bounds it (two products of 16 x 16 x 32 per 1 KiB of keys
-// take a tenth of the time that HBM needs for them), so the loads of the next step
-// are always in flight: keys are loaded again as soon as the scores have
-// been multiplied, values as soon as they are in LDS, and the table entries
-// of a step ahead of the values before it, so that no wait for one covers the other.
+// Memory bounds long calls (a step's products take a tenth of the time in which
+// HBM delivers its 16 KiB), so the loads of the next step are in flight all the
+// time: keys are loaded again as soon as the scores have been multiplied, values
+// as soon as they are in LDS, and a step's table entries ahead of the values
+// before it, so that no wait for one covers the other. 64 sequences of 2048
+// positions (FP16, 537 MB) take 97 us, 5.5 TB/s, where a copy of 1 GiB runs at
+// 5.1; 200 VGPRs and more leave two waves a SIMD (three, with 47 to 94 spilled
+// registers, took 157 us and more for 64 ragged sequences instead of 119).
+// Latency bounds short ones: 300 positions take 9 us in the kernel, 1.3 to find
+// the share, 2.2 for the table and the first rows behind it, 1.2 for a step, 1.7
+// for the waves' sums, 2 for the last workgroup to add the parts.
 template <int TYPE, int DIM, bool PACKED, bool TRACK>
-__global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attention_kernel(PagedView v, AttentionArgs a) {
+__global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attention_kernel(PagedView v,
+                                                                                          AttentionArgs a) {
     constexpr int kSize = TYPE == kPagedE4M3 ? 1 : 2, kLoads = DIM * kSize / 64, kSteps = DIM / 32, kOut = DIM / 16;
     constexpr int kPer = kSteps / kLoads;         // products per load: 1, or 2 for E4M3
     constexpr int kRows = PACKED ? 8 : 16, kProducts = Terms<TYPE, PACKED>::kProducts;
     constexpr int kPitch = DIM * 2 + 32;          // bytes of a value row in LDS
     constexpr float kHead = TYPE == kPagedF16 ? 6.f : 0.f;  // FP16 weights are kept up to 2^14, far from subnormals
     constexpr int kJoin = PACKED ? 16 : 8;        // parts whose sums are loaded at a time, as registers allow
-    constexpr int kGroup = 16, kFlat = 32;        // parts that are added as a group, and at most without groups
+    constexpr int kFlat = PACKED ? 32 : 16;       // parts that are added at once, beyond in groups of kJoin
     constexpr float kGrow = 8.f;                  // a reference is moved once a score passes it by 2^8
     constexpr std::integral_constant<int, TYPE> kType{};
     __shared__ __attribute__((aligned(16))) char lds[kWaves][kTile * kPitch];
@@ -373,12 +385,13 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
     const bool second = PACKED && column >= 8;
     const int row_of_lane = PACKED ? column & 7 : column;
 
-    Dealer<kRows> dealer(v, a, chunks);
+    const int head = a.tiles == 1 ? blockIdx.y : blockIdx.y / unsigned(a.tiles), tile = blockIdx.y - head * a.tiles;
+    const int row0 = tile * kRows;
+    Dealer<kRows> dealer(v, a, chunks, tile);
     Share share;
     while (dealer.next(share)) {
         const Deal& d = share.d;
-        const int head = blockIdx.y, begin = kBlock * share.from;
-        const int query_rows = a.group * d.n, row0 = share.tile * kRows;
+        const int begin = kBlock * share.from, query_rows = a.group * d.n;
         // Positions from shared_end on are seen by some of the tile's new rows only, from `end` on by none.
         const int shared_end = d.length - d.n + a.new_row(row0) + 1;
         const int seen_end = d.length - d.n + min(d.n - 1, a.new_row(row0 + kRows - 1)) + 1;
@@ -553,9 +566,8 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
             }
             if constexpr (TRACK) {
                 if (!second && query_row < query_rows) {
-                    float* const to = a.scores + base + 4 * part +
-                                      ((int64_t(share.s) * v.kv_heads + head) * (int64_t(v.rows) * a.group) + query_row) *
-                                          a.score_stride;
+                    const int64_t unit_rows = (int64_t(share.s) * v.kv_heads + head) * (int64_t(v.rows) * a.group);
+                    float* const to = a.scores + (unit_rows + query_row) * a.score_stride + base + 4 * part;
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         float4_t w;
@@ -586,12 +598,13 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
             if (base + kTile > shared_end) {
                 unsigned bits = 0;
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                for (int u = 0; u < 2; ++u) {
+                    const bool partly = was[u] && base + 16 * u + column >= shared_end;
 #pragma unroll
                     for (int i = 0; i < kLoads; ++i)
 #pragma unroll
-                        for (int w = 0; w < 4; ++w)
-                            bits |= was[u] && base + 16 * u + column >= shared_end ? not_finite<TYPE>(values[u][i][w]) : 0u;
+                        for (int w = 0; w < 4; ++w) bits |= partly ? not_finite<TYPE>(values[u][i][w]) : 0u;
+                }
                 spoilt = __any(bits != 0);
             }
 #pragma unroll
@@ -609,8 +622,8 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
                             for (int e = 0; e < 4; ++e)
                                 w[j][e] &= ~((not_finite<TYPE == kPagedF16 ? kPagedF16 : kPagedBF16>(w[j][e]) >> 15) *
                                              0xffffu);
-                        *reinterpret_cast<uint4_t*>(mine + (16 * u + column) * kPitch + 64 * kPer * i + 16 * kPer * part +
-                                                    16 * j) = w[j];
+                        char* const to = mine + (16 * u + column) * kPitch + 64 * kPer * i + 16 * kPer * part + 16 * j;
+                        *reinterpret_cast<uint4_t*>(to) = w[j];
                     }
                 }
             }
@@ -664,7 +677,8 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
             if constexpr (PACKED)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) w[e] = add_halves(acc[o][e]);
-            if (!second) *reinterpret_cast<float4_t*>(sums + (wave * kRows + row_of_lane) * DIM + 16 * o + 4 * part) = w;
+            float* const to = sums + (wave * kRows + row_of_lane) * DIM + 16 * o + 4 * part;
+            if (!second) *reinterpret_cast<float4_t*>(to) = w;
         }
         if (TRACK && int(threadIdx.x) < kRows) row_state[threadIdx.x] = float2{0.f, 0.f};
         __syncthreads();
@@ -674,8 +688,8 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
             if (r >= query_rows || to < 0 || to >= v.total_rows) return;
             if (all == 0.f) o = float4_t{0.f, 0.f, 0.f, 0.f};
             const float by = all == 0.f ? 0.f : 1.f / all;
-            *reinterpret_cast<float4_a4*>(a.out + to * a.out_stride + (head * a.group + r - i * a.group) * DIM + channel) =
-                o * by;
+            const int64_t at = to * a.out_stride + (head * a.group + r - i * a.group) * DIM + channel;
+            *reinterpret_cast<float4_a4*>(a.out + at) = o * by;
             if (TRACK && channel == 0) {
                 const float2 state = {top == -kInf ? 0.f : top, by};
                 if (a.adds)
@@ -712,7 +726,7 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
         bool ends = share.parts == 1;  // this is the workgroup that completes the unit
         if (share.parts > 1) {
             // The last of the unit's workgroups to get here adds their parts, in the order of the positions; of more
-            // than kFlat parts the last of each kGroup adds those, and the last of these the groups (115 parts of 16
+            // than kFlat parts the last of each kJoin adds those, and the last of these the groups (115 parts of 16
             // rows by one workgroup took 40 us). Posted values have reached memory once their stores are done, and
             // are read past the caches, so no fence of the device's scope is needed: with one in every workgroup (it
             // writes back and drops a whole L2) eight sequences of 2048 took 42 us instead of 16.
@@ -775,8 +789,8 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
                 ends = last_of(0, share.parts);
                 if (ends) join(0, share.parts, 1, DIM, finish);
             } else {
-                const int group = share.part / kGroup, first = group * kGroup;
-                const int of_group = min(kGroup, share.parts - first), groups = (share.parts + kGroup - 1) / kGroup;
+                const int group = share.part / kJoin, first = group * kJoin;
+                const int of_group = min(kJoin, share.parts - first), groups = (share.parts + kJoin - 1) / kJoin;
                 ends = last_of(1 + group, of_group);
                 if (ends) {
                     // The group's sums take the place of its first part's, which nobody else reads any more; its
@@ -788,7 +802,7 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
                         if (channel == 0) post(partial + DIM + 2, top, all);
                     });
                     ends = last_of(0, groups);
-                    if (ends) join(0, groups, kGroup, DIM + 2, finish);
+                    if (ends) join(0, groups, kJoin, DIM + 2, finish);
                 }
             }
         }
@@ -834,25 +848,31 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
 // Sizes of a call: the grid, and what its workspace holds.
 struct AttentionPlan {
     bool packed, adds;
-    int64_t blocks, columns, score_stride, score_rows;  // columns: workgroups of a KV head
+    int64_t tiles, grid_rows, blocks, columns, first, score_stride, score_rows;  // columns: workgroups of a grid row
     size_t partial_bytes, state_bytes, score_bytes;
     AttentionPlan(const qwen_gpu_paged_cache& c, const qwen_gpu_paged_batch& b, int query_heads) {
         const int64_t rows = int64_t(query_heads / c.kv_heads) * b.rows;
         packed = rows <= 8;
-        const int64_t tile_rows = packed ? 8 : 16, units = b.sequences * ((rows + tile_rows - 1) / tile_rows);
-        const int64_t head_blocks = units * ((b.max_length + kBlock - 1) / kBlock);
-        blocks = head_blocks * c.kv_heads;
-        columns = std::min(head_blocks, units + kShares / c.kv_heads);
-        if (blocks > kStream) columns = std::max<int64_t>(columns, runs_of_head(c.kv_heads));
-        const int64_t parts = std::max<int64_t>(columns, blocks > kStream ? 2 * runs_of_head(c.kv_heads) : 0);
-        partial_bytes = size_t(parts) * c.kv_heads * tile_rows * (c.head_dim + 4) * 4;
+        const int64_t tile_rows = packed ? 8 : 16, most = (b.max_length + kBlock - 1) / kBlock;
+        const int64_t row_blocks = b.sequences * most;
+        tiles = (rows + tile_rows - 1) / tile_rows;
+        grid_rows = tiles * c.kv_heads;
+        blocks = row_blocks * grid_rows;
+        const int64_t runs = kRuns > grid_rows ? kRuns / grid_rows : 1;
+        columns = std::min(row_blocks, b.sequences + kShares / grid_rows);
+        if (blocks > kStream) columns = std::max(columns, runs);
+        // Every sequence with new rows has a block, so beyond that many they are dealt in runs.
+        if (!b.offsets && b.sequences * c.kv_heads > kStream) columns = runs;
+        first = std::min(columns, 2 * runs);
+        const int64_t parts = std::max((columns + first - 1) / first * first, blocks > kStream ? 2 * runs : 0);
+        partial_bytes = size_t(parts) * grid_rows * tile_rows * (c.head_dim + 4) * 4;
         score_stride = (b.max_length + kTile - 1) / kTile * kTile;
         score_rows = int64_t(b.sequences) * c.kv_heads * rows;
         // The workgroup that completes a unit adds to the weights, four positions a thread and four rows at a time,
-        // while that takes it a few turns: 14.2 us against 12.2 with another kernel for 300 positions, 20.6 and 19.5 for
-        // eight sequences of 1025, 32.9 and 37.2 for eight of 4096. Where several units share the weights, that kernel
-        // adds to them always.
-        adds = rows <= tile_rows && (b.max_length + 1023) / 1024 * ((rows + 3) / 4) <= kAdds;
+        // while that takes it a few turns: 12.2 us for 300 positions against 14.2 with a kernel for it, 19.5 and
+        // 20.6 for eight sequences of 1025, but 37.2 and 32.9 for eight of 4096. Where several units share the
+        // weights, that kernel adds to them.
+        adds = tiles == 1 && (b.max_length + 1023) / 1024 * ((rows + 3) / 4) <= kAdds;
         state_bytes = b.weights ? (size_t(score_rows) * 8 + 15) / 16 * 16 : 0;
         score_bytes = b.weights ? size_t(score_rows) * score_stride * 4 : 0;
     }
@@ -861,10 +881,13 @@ struct AttentionPlan {
 
 template <int TYPE, int DIM, bool PACKED>
 void attention_run(const PagedView& v, const AttentionArgs& a, const AttentionPlan& plan, hipStream_t stream) {
-    // Heads vary slowest, and each head's workgroups that find no work come behind its others, so that the heads
-    // start one after the other: 64 sequences of 2048 in pages of [slot][head] took 109 us with all heads at once
-    // (heads fastest, or no idle workgroups between them), so 100; in pages of [head][slot] 96 and 97.
-    const dim3 grid{unsigned(plan.columns), unsigned(v.kv_heads)}, block{kWaves * 64};
+    // Heads vary slowest, and some of each head's workgroups that find no work come behind its others (the rest
+    // behind all), so that the heads start one after the other: 64 sequences of 2048 in pages of [slot][head] took
+    // 109 us with all heads at once (heads fastest, or no idle workgroups between them), so 100; in pages of
+    // [head][slot] 96 and 97.
+    const unsigned layers = unsigned((plan.columns + plan.first - 1) / plan.first);
+    const dim3 grid{unsigned(plan.first), unsigned(plan.grid_rows), layers};
+    const dim3 block{kWaves * 64};
     if (v.weights)
         paged_attention_kernel<TYPE, DIM, PACKED, true><<<grid, block, 0, stream>>>(v, a);
     else
@@ -872,7 +895,8 @@ void attention_run(const PagedView& v, const AttentionArgs& a, const AttentionPl
 }
 
 template <int TYPE>
-void attention_launch(int dim, const PagedView& v, const AttentionArgs& a, const AttentionPlan& plan, hipStream_t stream) {
+void attention_launch(int dim, const PagedView& v, const AttentionArgs& a, const AttentionPlan& plan,
+                      hipStream_t stream) {
     auto run = [&](auto packed) {
         if (dim == 64) return attention_run<TYPE, 64, packed.value>(v, a, plan, stream);
         if (dim == 128) return attention_run<TYPE, 128, packed.value>(v, a, plan, stream);

@@ -117,7 +117,8 @@ class Cache:
         for j in range(n):
             at = self.place(table, s, j)
             if at:
-                keys[j], values[j] = self.row(self.keys, 0, at[0], head, at[1]), self.row(self.values, 1, at[0], head, at[1])
+                keys[j] = self.row(self.keys, 0, at[0], head, at[1])
+                values[j] = self.row(self.values, 1, at[0], head, at[1])
                 there[j] = True
         return keys, values, there
 

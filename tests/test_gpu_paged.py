@@ -438,6 +438,16 @@ def test_workspace_serves_calls_of_different_shapes(qpkg):
         assert not space.to_array(np.uint8, 98304).any()
 
 
+@pytest.mark.parametrize('lengths,kv,heads,rows', [([5000, 40], 2, 16, 2), ([4300], 1, 1, 1),
+                                                   ([17000] + [100] * 2000, 1, 3, 1), ([17000] + [100] * 2000, 1, 9, 1)])
+def test_attention_joined_in_groups(qpkg, lengths, kv, heads, rows):
+    """Units of more parts than one workgroup adds, dealt in parts and in runs, 8 and 16 rows a tile."""
+    rng = np.random.default_rng(83)
+    table, pages = make_table(rng, lengths, 64)
+    cache = ref.Cache('f16', pages, 64, kv, 64, rng=rng)
+    attend(qpkg, cache, table, lengths, rows, heads, rng=rng)
+
+
 def test_attention_in_place_of_its_queries(qpkg):
     """out may be the queries' own memory."""
     rng = np.random.default_rng(79)
