@@ -84,7 +84,7 @@ PagedView paged_view(const qwen_gpu_paged_cache& c, const qwen_gpu_paged_batch& 
 }
 
 void paged_check_rows(const qwen_gpu_paged_batch& b) {
-    require(b.rows >= 1 && b.rows <= b.max_length, "Paged rows must be in 1..max_length");
+    require(b.rows >= 1 && b.rows <= kPagedMaxLength, "Paged rows must be in 1..2^24");
     require(b.total_rows >= 0 && b.total_rows <= kPagedMaxLength, "Paged total_rows must be in 0..2^24");
     require(b.offsets || int64_t(b.sequences) * b.rows == b.total_rows,
             "Paged total_rows must be sequences * rows without offsets");

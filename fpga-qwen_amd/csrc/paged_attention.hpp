@@ -12,14 +12,15 @@ namespace qwen_hip {
 constexpr int kTile = 32;                       // positions of a wave's step
 constexpr int kWaves = 4;                       // of a workgroup
 constexpr int kBlock = kTile * kWaves;          // positions of a workgroup's step
-constexpr int kShares = 512;                    // workgroups that the positions are dealt to
-constexpr int kStream = 4 * kShares;            // blocks from which on workgroups cross units
-constexpr int kRuns = 512;                      // workgroups that do
+// Workgroups that the positions are dealt to: as many as the GPU holds at once, two for each CU, one where heads of
+// 256 take the registers of two.
+__host__ __device__ constexpr int shares_of(int dim) { return dim == 256 ? 256 : 512; }
+constexpr int kStream = 4;                      // blocks a share from which on workgroups cross units
 constexpr int kAdds = 2;                        // turns that a unit's last workgroup takes to add to the weights
 constexpr int kCounterStep = 16;                // ints: a counter has a line of its own
 constexpr float kInf = __builtin_huge_valf();
-// More than kShares rows of the grid split no unit, up to there a row has kShares / rows + 1 counters.
-static_assert(std::max(kRuns, 2 * kShares) * kCounterStep * sizeof(int) <= kPagedCounterBytes, "counters");
+// More grid rows than shares split no unit, up to there a row has shares / rows + 1 counters.
+static_assert(2 * shares_of(64) * kCounterStep * sizeof(int) <= kPagedCounterBytes, "counters");
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -53,9 +54,9 @@ struct AttentionArgs {
 // and a tile, so the tiles of a head's rows take the same positions at the same
 // time. Workgroups find their shares from the lengths on the device, every wave
 // by itself, so the host needs no lengths and a captured launch follows them.
-// With up to kStream blocks in all, a workgroup has one part of one unit, of 1,
-// 2 or 4 blocks, whichever spreads all over about kShares workgroups. With more,
-// kRuns workgroups (two for each CU, all there at once) take equal runs of blocks
+// With up to 4 blocks a share, a workgroup has one part of one unit, of 1, 2 or
+// 4 blocks, whichever spreads all over as many workgroups as the GPU holds at
+// once. With more, that many workgroups take equal runs of blocks
 // in the order of a grid row's units, across their borders: with parts of units
 // the last round of workgroups left CUs idle (64 sequences of 1 to 4096
 // positions took 131 us, in runs 125); 768, 1024 and 1536 runs took 130, 124 and
@@ -86,7 +87,9 @@ __device__ __forceinline__ Deal deal_of_lane(const Deal& d, int lane) {
             __builtin_amdgcn_readlane(d.first, lane), __builtin_amdgcn_readlane(d.blocks, lane)};
 }
 // Runs of a row of the grid.
-__host__ __device__ __forceinline__ int runs_of_row(int grid_rows) { return kRuns > grid_rows ? kRuns / grid_rows : 1; }
+__host__ __device__ __forceinline__ int runs_of_row(int shares, int grid_rows) {
+    return shares > grid_rows ? shares / grid_rows : 1;
+}
 
 // Of 64 sequences' units in a row of the grid: their parts of 1, 2 and 4 blocks
 // (the first are their blocks as well), and their number.
@@ -95,7 +98,7 @@ struct ChunkSums {
 };
 
 // The host has checked that all units' blocks together fit 31 bits.
-template <int ROWS>
+template <int ROWS, int SHARES>
 struct Dealer {
     const PagedView& v;
     const AttentionArgs& a;
@@ -115,7 +118,7 @@ struct Dealer {
     __device__ __forceinline__ Dealer(const PagedView& view, const AttentionArgs& args, ChunkSums& shared,
                                       int rows_tile)
         : v(view), a(args), chunks(shared), lane(threadIdx.x & 63), w(blockIdx.z * gridDim.x + blockIdx.x),
-          tile(rows_tile), own{}, runs(runs_of_row(gridDim.y)) {
+          tile(rows_tile), own{}, runs(runs_of_row(SHARES, gridDim.y)) {
         if (v.sequences <= 64) {
             if (lane < v.sequences) own = deal_one<ROWS>(v, a.group, tile, lane);
             total = __builtin_amdgcn_readlane(scan_lanes(own.blocks), 63);
@@ -146,9 +149,9 @@ struct Dealer {
             total = __builtin_amdgcn_readlane(scan_lanes(chunks.of[0][lane]), 63);
         }
         const int all = total * int(gridDim.y);
-        streams = all > kStream;
-        shift = all <= kShares ? 0 : all <= 2 * kShares ? 1 : 2;
-        static_assert(kStream == 4 * kShares, "parts of 1, 2 or 4 blocks");
+        streams = all > kStream * SHARES;
+        shift = all <= SHARES ? 0 : all <= 2 * SHARES ? 1 : 2;
+        static_assert(kStream == 4, "parts of 1, 2 or 4 blocks");
         at = end = 0;
         if (streams) {
             at = start(w);
@@ -212,7 +215,7 @@ struct Dealer {
             share.part0 = row * int(gridDim.x * gridDim.z) + w - within;
             share.part1 = share.part0 + 1;
             share.step = 1;
-            // A grid row's units have fewer than kShares / rows parts beyond one each: these are counted.
+            // A grid row's units have fewer than shares / rows parts beyond one each: these are counted.
             share.counter = row * a.extra + w - within - units;
         }
         return true;
@@ -387,7 +390,7 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
 
     const int head = a.tiles == 1 ? blockIdx.y : blockIdx.y / unsigned(a.tiles), tile = blockIdx.y - head * a.tiles;
     const int row0 = tile * kRows;
-    Dealer<kRows> dealer(v, a, chunks, tile);
+    Dealer<kRows, shares_of(DIM)> dealer(v, a, chunks, tile);
     Share share;
     while (dealer.next(share)) {
         const Deal& d = share.d;
@@ -858,13 +861,13 @@ struct AttentionPlan {
         tiles = (rows + tile_rows - 1) / tile_rows;
         grid_rows = tiles * c.kv_heads;
         blocks = row_blocks * grid_rows;
-        const int64_t runs = kRuns > grid_rows ? kRuns / grid_rows : 1;
-        columns = std::min(row_blocks, b.sequences + kShares / grid_rows);
-        if (blocks > kStream) columns = std::max(columns, runs);
+        const int64_t shares = shares_of(c.head_dim), runs = shares > grid_rows ? shares / grid_rows : 1;
+        columns = std::min(row_blocks, b.sequences + shares / grid_rows);
+        if (blocks > kStream * shares) columns = std::max(columns, runs);
         // Every sequence with new rows has a block, so beyond that many they are dealt in runs.
-        if (!b.offsets && b.sequences * c.kv_heads > kStream) columns = runs;
+        if (!b.offsets && b.sequences * c.kv_heads > kStream * shares) columns = runs;
         first = std::min(columns, 2 * runs);
-        const int64_t parts = std::max((columns + first - 1) / first * first, blocks > kStream ? 2 * runs : 0);
+        const int64_t parts = std::max((columns + first - 1) / first * first, blocks > kStream * shares ? 2 * runs : 0);
         partial_bytes = size_t(parts) * grid_rows * tile_rows * (c.head_dim + 4) * 4;
         score_stride = (b.max_length + kTile - 1) / kTile * kTile;
         score_rows = int64_t(b.sequences) * c.kv_heads * rows;

@@ -326,7 +326,7 @@ typedef struct qwen_gpu_paged_batch {
     int sequences;              /* 1..4096 */
     int table_stride;           /* pages in a row of the table */
     int max_length;             /* 1..table_stride * page_size, at most 2^24 */
-    int rows;                   /* 1..max_length: most new rows of a sequence */
+    int rows;                   /* 1..2^24: most new rows of a sequence */
     int total_rows;             /* new rows of all sequences; sequences * rows where offsets is NULL */
 } qwen_gpu_paged_batch;
 

@@ -438,6 +438,20 @@ def test_workspace_serves_calls_of_different_shapes(qpkg):
         assert not space.to_array(np.uint8, 98304).any()
 
 
+def test_more_new_rows_than_any_sequence_holds(qpkg):
+    """Of eight new rows the last two are cached and see anything."""
+    rng = np.random.default_rng(89)
+    table, pages = make_table(rng, [2, 1], 16)
+    cache = ref.Cache('f16', pages, 16, 2, 64, fill=0)
+    call = Call(qpkg, cache, table, [2, 1], 8, max_length=2)
+    keys, values = (rng.standard_normal((16, 128)).astype(np.float32) for _ in range(2))
+    call.append(keys, values)
+    ref.append(cache, table, [2, 1], 8, None, keys.reshape(16, 2, 64), values.reshape(16, 2, 64))
+    call.expect_pools(cache)
+    call, result = attend(qpkg, cache, table, [2, 1], 8, 4, rng=rng, max_length=2)
+    assert not result[:6].any() and result[6:8].any(axis=(1, 2)).all()
+
+
 @pytest.mark.parametrize('lengths,kv,heads,rows', [([5000, 40], 2, 16, 2), ([4300], 1, 1, 1),
                                                    ([17000] + [100] * 2000, 1, 3, 1), ([17000] + [100] * 2000, 1, 9, 1)])
 def test_attention_joined_in_groups(qpkg, lengths, kv, heads, rows):

@@ -74,7 +74,7 @@ def test_batches_refused(qpkg, op, message, fields):
 
 @pytest.mark.parametrize('op', ['append', 'attention'])
 @pytest.mark.parametrize('message,fields', [
-    ('rows must be', dict(rows=0)), ('rows must be', dict(rows=65)), ('total_rows must be', dict(total_rows=3)),
+    ('rows must be', dict(rows=0)), ('rows must be', dict(rows=(1 << 24) + 1)), ('total_rows must be', dict(total_rows=3)),
     ('total_rows must be', dict(total_rows=-1, offsets=AT)),
     ('total_rows must be', dict(total_rows=(1 << 24) + 1, offsets=AT))])
 def test_new_rows_refused(qpkg, op, message, fields):
