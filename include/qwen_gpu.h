@@ -303,7 +303,8 @@ int qwen_gpu_op_copy(const void* src, void* dst, size_t bytes, void* stream);
 typedef struct qwen_gpu_paged_cache {
     void* keys;
     void* values;
-    uint8_t* exponents;         /* E4M3: [pages][kv_heads][page_size][2], of the key row and of the value row */
+    uint8_t* exponents;         /* E4M3: [pages][kv_heads][page_size][2], of the key row and of the value row,
+                                 * bytes 1..254 */
     int64_t page_stride;
     int64_t head_stride;
     int64_t slot_stride;
@@ -330,20 +331,21 @@ typedef struct qwen_gpu_paged_batch {
     int total_rows;             /* new rows of all sequences; sequences * rows where offsets is NULL */
 } qwen_gpu_paged_batch;
 
-/* Bytes of workspace (device memory, aligned to 16) that the attention and the eviction of
- * this cache and batch need at most. The caller zeroes it once; every call
- * leaves it ready for the next, of whatever shape it suffices for. Calls
- * that may overlap need workspaces of their own. */
+/* Bytes of workspace (device memory, aligned to 16) that the attention and
+ * the eviction of this cache and batch need at most. The caller zeroes it
+ * once; every call leaves it ready for the next, of whatever shape it
+ * suffices for. Calls that may overlap need workspaces of their own, and so
+ * do captured graphs that may. */
 int qwen_gpu_op_paged_workspace(const qwen_gpu_paged_cache* cache, const qwen_gpu_paged_batch* batch, int query_heads,
                                 size_t* bytes);
 /* The new rows' keys and values, FP32, rounded to the cache's type (to
  * nearest, ties to even) in their slots: row i of sequence s's n goes to slot
  * lengths[s] - n + i, a negative one nowhere. Head h of row r lies at keys +
  * r * key_stride + h * head_dim, so a projection's rows are read where they
- * are. E4M3: the exponent is the smallest (of -126 .. 127) that brings the row's largest
- * finite magnitude to 448 or below; infinities and NaN become NaN. Where tracked,
- * the slots' weights are set to 0 and their positions to seen[s] - n + i.
- * No two rows of a call may go to one slot. */
+ * are. E4M3: the exponent is the smallest of -126 .. 127 that brings the
+ * row's largest finite magnitude to 448 or below; infinities and NaN become
+ * NaN. Where tracked, the slots' weights are set to 0 and their positions to
+ * seen[s] - n + i. No two rows of a call may go to one slot. */
 int qwen_gpu_op_paged_append(const qwen_gpu_paged_cache* cache, const qwen_gpu_paged_batch* batch, const float* keys,
                              int64_t key_stride, const float* values, int64_t value_stride, void* stream);
 /* Attention of the new rows over the cached ones, which hold the new ones
@@ -353,8 +355,10 @@ int qwen_gpu_op_paged_append(const qwen_gpu_paged_cache* cache, const qwen_gpu_p
  * q . k); a row that has none gives zeros. out is laid out like queries, with
  * out_stride. With weights, weights[s][h][j] grows by the sum of slot j's
  * softmax weights over h's query heads and s's new rows. Sums are FP32, in
- * an order that depends on the call's shapes and lengths alone. Keys and values that a row attends are finite; those it
- * does not attend may be anything. */
+ * an order that depends on the call's shapes and lengths alone. Keys and
+ * values that a row attends are finite (else its output may be NaN); those
+ * that it does not attend may be anything. out may be queries themselves,
+ * with one stride. query_heads is at most 1024 * kv_heads, scale finite. */
 int qwen_gpu_op_paged_attention(const qwen_gpu_paged_cache* cache, const qwen_gpu_paged_batch* batch,
                                 const float* queries, int64_t query_stride, int query_heads, float scale, float* out,
                                 int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
