@@ -91,6 +91,10 @@ void paged_check_rows(const qwen_gpu_paged_batch& b) {
 }
 
 PagedDevice::PagedDevice(const qwen_gpu_paged_cache& c, const qwen_gpu_paged_batch& b, hipStream_t stream) {
+    // The runtime's handles 1 and 2 stand for streams and point to none: asked for the device of 1, it ends the
+    // process.
+    require(stream != hipStreamLegacy && stream != hipStreamPerThread,
+            "The stream must be NULL or a stream that was created");
     hipPointerAttribute_t a{};
     if (hipPointerGetAttributes(&a, c.keys) != hipSuccess || a.type == hipMemoryTypeUnregistered) {
         (void)hipGetLastError();

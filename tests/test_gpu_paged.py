@@ -438,6 +438,42 @@ def test_workspace_serves_calls_of_different_shapes(qpkg):
         assert not space.to_array(np.uint8, 98304).any()
 
 
+def test_attention_most_sequences(qpkg):
+    rng = np.random.default_rng(97)
+    lengths = [int(x) for x in rng.integers(0, 6, 4096)]
+    lengths[4095], lengths[2222] = 400, 90
+    counts = [int(x) for x in rng.integers(0, 2, 4096)]
+    offsets = np.concatenate(([0], np.cumsum(counts)))
+    table, pages = make_table(rng, lengths, 4)
+    cache = ref.Cache('f16', pages, 4, 1, 64, rng=rng)
+    attend(qpkg, cache, table, lengths, 1, 2, offsets=offsets, total=sum(counts), rng=rng)
+
+
+def test_calls_on_streams(qpkg):
+    """Two sequences of calls in flight at once, on streams and workspaces of their own."""
+    hip, rng = Hip(), np.random.default_rng(101)
+    lengths, heads, dim = [3000, 100], 4, 64
+    table, pages = make_table(rng, lengths, 16)
+    cache = ref.Cache('f16', pages, 16, 2, dim, rng=rng)
+    sides = []
+    for side in range(2):
+        call = Call(qpkg, cache, table, lengths)
+        queries = rng.standard_normal((2, heads * dim)).astype(np.float32)
+        want = call.attention(queries, heads, 0.125, np.zeros_like(queries))
+        stream = ctypes.c_void_p()
+        hip.hipStreamCreate(ctypes.byref(stream))
+        sides.append((call, want, stream, qpkg.DeviceBuffer(want.nbytes)))
+    for _ in range(20):
+        for call, want, stream, out in sides:
+            call.check(call.lib.qwen_gpu_op_paged_attention(
+                ctypes.byref(call.c), ctypes.byref(call.b), call.qd.ptr, heads * dim, heads, 0.125, out.ptr, heads * dim,
+                call.space.ptr, call.space.nbytes, stream))
+    qpkg.synchronize()
+    for call, want, stream, out in sides:
+        assert np.array_equal(out.to_array(np.float32, want.size).reshape(want.shape), want)
+        hip.hipStreamDestroy(stream)
+
+
 def test_more_new_rows_than_any_sequence_holds(qpkg):
     """Of eight new rows the last two are cached and see anything."""
     rng = np.random.default_rng(89)

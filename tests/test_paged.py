@@ -131,6 +131,16 @@ def test_host_memory_refused(qpkg, op):
     refused(qpkg, 'Not device memory: keys', cache(qpkg, keys=at, values=at), op=op)
 
 
+@pytest.mark.parametrize('handle', [1, 2])
+def test_stand_in_streams_refused(qpkg, handle):
+    """Handles that name the legacy and the per-thread stream are no streams to the runtime's queries."""
+    lib, c, b = qpkg.load_library(), cache(qpkg), batch(qpkg)
+    for status in (lib.qwen_gpu_op_paged_append(c, b, AT, 1024, AT, 1024, handle),
+                   lib.qwen_gpu_op_paged_attention(c, b, AT, 2048, 16, 0.1, AT, 2048, AT, 1 << 30, handle),
+                   lib.qwen_gpu_op_paged_evict(c, b, 8, 0, 0, 2 * AT, AT, AT, AT, 1 << 30, handle)):
+        assert status == 1 and 'must be NULL or a stream' in lib.qwen_gpu_last_error().decode()
+
+
 def test_null_descriptions_refused(qpkg):
     lib, c, b = qpkg.load_library(), cache(qpkg), batch(qpkg)
     size = ctypes.c_size_t()
