@@ -20,7 +20,9 @@ extern template void attention_launch<kPagedE4M3>(int, const PagedView&, const A
 namespace {
 
 // The weights of a sequence and KV head grow by the softmax of the scores that
-// the attention left, summed over its query rows in their order.
+// the attention left, summed over its query rows in their order: a thread a
+// slot, as scores of a row are read in one piece. 8 x 1025 positions of two
+// rows take 4 us, a launch behind another.
 __global__ __launch_bounds__(256) void paged_track_kernel(PagedView v, AttentionArgs a) {
     constexpr int kStates = 64;
     __shared__ float2 states[kStates];
