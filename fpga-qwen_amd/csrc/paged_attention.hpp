@@ -121,7 +121,8 @@ struct Dealer {
           tile(rows_tile), own{}, runs(runs_of_row(SHARES, gridDim.y)) {
         if (v.sequences <= 64) {
             if (lane < v.sequences) own = deal_one<ROWS>(v, a.group, tile, lane);
-            total = __builtin_amdgcn_readlane(scan_lanes(own.blocks), 63);
+            total = v.sequences == 1 ? __builtin_amdgcn_readfirstlane(own.blocks)
+                                     : __builtin_amdgcn_readlane(scan_lanes(own.blocks), 63);
         } else {
             // The waves sum 64 sequences each in turn, with four turns' loads in flight.
             for (int c0 = threadIdx.x >> 6; c0 < 64; c0 += 4 * kWaves) {
@@ -184,7 +185,7 @@ struct Dealer {
             d = deal_one<ROWS>(v, a.group, tile, min(begin + lane, v.sequences - 1));
             if (begin + lane >= v.sequences) d.blocks = 0;
         }
-        const int count = parts_of(d.blocks, split_shift), upto = scan_lanes(count);
+        const int count = parts_of(d.blocks, split_shift), upto = v.sequences == 1 ? count : scan_lanes(count);
         const unsigned long long hit = __ballot(before + upto > wanted);
         if (!hit) return false;
         const int from = __ffsll(hit) - 1;
@@ -688,7 +689,7 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
         auto finish = [&](int local, int channel, float4_t o, float top, float all) {
             const int r = row0 + local, i = a.new_row(r);
             const int64_t to = int64_t(d.first) + i;
-            if (r >= query_rows || to < 0 || to >= v.total_rows) return;
+            if (to < 0 || to >= v.total_rows) return;
             if (all == 0.f) o = float4_t{0.f, 0.f, 0.f, 0.f};
             const float by = all == 0.f ? 0.f : 1.f / all;
             const int64_t at = to * a.out_stride + (head * a.group + r - i * a.group) * DIM + channel;
@@ -703,6 +704,7 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
         };
         for (int item = threadIdx.x; item < kRows * DIM / 4; item += kWaves * 64) {
             const int local = item / (DIM / 4), channel = 4 * (item - local * (DIM / 4));
+            if (row0 + local >= query_rows) continue;
             float top = -kInf, all = 0.f;
 #pragma unroll
             for (int w = 0; w < kWaves; ++w) top = fmaxf(top, wave_state[w][local].x);
@@ -717,7 +719,6 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
                 for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(x[e], shrink, o[e]);
             }
             if (share.parts > 1) {
-                if (row0 + local >= query_rows) continue;
                 float* const partial = a.partials + (share.slot(share.part) * kRows + local) * (DIM + 4);
                 post(partial + channel, o[0], o[1]);
                 post(partial + channel + 2, o[2], o[3]);
