@@ -101,6 +101,7 @@ void launch_paged_attention(const qwen_gpu_paged_cache& cache, const qwen_gpu_pa
                           query_heads / cache.kv_heads,
                           0xffffffffu / unsigned(query_heads / cache.kv_heads),
                           int(shares_of(cache.head_dim) / plan.grid_rows) + 1,
+                          int(plan.pitch),
                           int(plan.tiles),
                           scale * 1.44269504088896340736f,
                           reinterpret_cast<float*>(space),

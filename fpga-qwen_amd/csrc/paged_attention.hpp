@@ -34,7 +34,7 @@ struct AttentionArgs {
     int64_t out_stride;
     int group;          // query heads of a KV head
     unsigned magic;     // of the group, as page_slot takes it
-    int extra;          // counters of a row of the grid
+    int extra, pitch;   // counters and partials of a row of the grid
     int tiles;          // of a KV head's query rows: grid row y has head y / tiles, tile y % tiles
     float scale;        // times log2(e)
     float* partials;    // [parts][rows of a tile][DIM + 4]: output, reference, sum, the same of a group of parts
@@ -61,6 +61,9 @@ struct AttentionArgs {
 // the last round of workgroups left CUs idle (64 sequences of 1 to 4096
 // positions took 131 us, in runs 125); 768, 1024 and 1536 runs took 130, 124 and
 // 125 us, and for 64 equal sequences 120, 103 and 116 us where 512 take 95.
+// Ragged new rows leave a head's later tiles fewer units, so that some rows of a
+// grid may take runs and others parts: a row's counters and partials lie at the
+// same place for both.
 struct Deal {
     int length, n, first, blocks;  // of a sequence: positions, new rows, the first of them, blocks (0: no unit)
 };
@@ -201,19 +204,19 @@ struct Dealer {
             const int first = owner(at - share.from), last = owner(at - share.from + d.blocks - 1);
             share.parts = last - first + 1;
             // A run's last share comes second; its first one is the end of another unit.
-            share.part0 = 2 * (row * runs + first) + 1;
-            share.part1 = 2 * (row * runs + first + 1);
+            share.part0 = row * a.pitch + 2 * first + 1;
+            share.part1 = row * a.pitch + 2 * (first + 1);
             share.step = 2;
             share.part = w - first;
             // No other unit starts in these runs, but for the last, and ends behind its own first.
-            share.counter = row * runs + first;
+            share.counter = row * a.extra + first;
             at += share.to - share.from;
         } else {
             share.from = within << shift;
             share.to = min(d.blocks, (within + 1) << shift);
             share.parts = __builtin_amdgcn_readlane(count, from);
             share.part = within;
-            share.part0 = row * int(gridDim.x * gridDim.z) + w - within;
+            share.part0 = row * a.pitch + w - within;
             share.part1 = share.part0 + 1;
             share.step = 1;
             // A grid row's units have fewer than shares / rows parts beyond one each: these are counted.
@@ -852,7 +855,8 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
 // Sizes of a call: the grid, and what its workspace holds.
 struct AttentionPlan {
     bool packed, adds;
-    int64_t tiles, grid_rows, blocks, columns, first, score_stride, score_rows;  // columns: workgroups of a grid row
+    int64_t tiles, grid_rows, blocks, score_stride, score_rows;
+    int64_t columns, first, pitch;  // of a grid row: workgroups, those of the first layer, partials
     size_t partial_bytes, state_bytes, score_bytes;
     AttentionPlan(const qwen_gpu_paged_cache& c, const qwen_gpu_paged_batch& b, int query_heads) {
         const int64_t rows = int64_t(query_heads / c.kv_heads) * b.rows;
@@ -868,8 +872,8 @@ struct AttentionPlan {
         // Every sequence with new rows has a block, so beyond that many they are dealt in runs.
         if (!b.offsets && b.sequences * c.kv_heads > kStream * shares) columns = runs;
         first = std::min(columns, 2 * runs);
-        const int64_t parts = std::max((columns + first - 1) / first * first, blocks > kStream * shares ? 2 * runs : 0);
-        partial_bytes = size_t(parts) * grid_rows * tile_rows * (c.head_dim + 4) * 4;
+        pitch = std::max((columns + first - 1) / first * first, blocks > kStream * shares ? 2 * runs : 0);
+        partial_bytes = size_t(pitch) * grid_rows * tile_rows * (c.head_dim + 4) * 4;
         score_stride = (b.max_length + kTile - 1) / kTile * kTile;
         score_rows = int64_t(b.sequences) * c.kv_heads * rows;
         // The workgroup that completes a unit adds to the weights, four positions a thread and four rows at a time,

@@ -397,6 +397,31 @@ def test_attention_runs_across_units(qpkg, kind, kv, group, dim, rows, tracked):
     attend(qpkg, cache, table, lengths, rows, kv * group, rng=rng, weights=weights, max_length=1500)
 
 
+@pytest.mark.parametrize('lengths,counts,kv,group', [
+    ([10599, 6551, 2503, 9053, 5005], [8, 7, 6, 5, 3], 1, 16),
+    ([2600, 5100, 9800, 9800, 6000], [1, 1, 4, 1, 1], 2, 16),
+    ([9000, 9000, 9000, 9000], [1, 2, 2, 4], 4, 8),
+    ([520] * 280 + [3000], [1] * 200 + [4, 0] * 40 + [3], 1, 8)])
+@pytest.mark.parametrize('kind,tracked', [('f16', False), ('bf16', True)])
+def test_attention_runs_and_parts_in_one_call(qpkg, kind, tracked, lengths, counts, kv, group):
+    """A head's first tile of query rows has more than 4 blocks a share and is dealt in runs, later tiles, whose
+    rows only some sequences have, in parts; the same again with the workspace as the first call left it."""
+    rng = np.random.default_rng(113)
+    rows, offsets = max(counts), np.concatenate(([0], np.cumsum(counts)))
+    tiles = -(-rows * group // 16)
+    blocks = [sum(-(-n // 128) for n, c in zip(lengths, counts) if c * group > 16 * t) * tiles * kv
+              for t in range(tiles)]
+    assert blocks[0] > 4 * 512 >= blocks[-1]
+    table, pages = make_table(rng, lengths, 32)
+    cache = ref.Cache(kind, pages, 32, kv, 64, rng=rng)
+    weights = rng.random((len(lengths), kv, max(lengths))).astype(np.float32) if tracked else None
+    call, result = attend(qpkg, cache, table, lengths, rows, kv * group, offsets=offsets, total=sum(counts), rng=rng,
+                          weights=weights, max_length=max(lengths))
+    queries = call.qd.to_array(np.float32, (sum(counts) + 2) * kv * group * 64).reshape(-1, kv * group * 64)
+    again = call.attention(queries, kv * group, 0.125, np.full_like(queries, 7.5), space=call.space)
+    assert np.array_equal(again[:sum(counts)].reshape(result.shape), result)
+
+
 @pytest.mark.parametrize('count', [64, 65, 130, 700, 1100])
 @pytest.mark.parametrize('ragged', [False, True])
 def test_attention_many_sequences(qpkg, count, ragged):
