@@ -208,9 +208,10 @@ def _plan(state):
                                max_length=max(1, state['longest']), rows=case['rows'], total_rows=state['total'])
     bytes_ = ctypes.c_size_t()
     query_heads = case['kv_heads'] * case['group']
-    if library.qwen_gpu_op_paged_workspace(ctypes.byref(cache), ctypes.byref(batch), query_heads,
-                                           ctypes.byref(bytes_)):
-        raise RuntimeError(library.qwen_gpu_last_error().decode())
+    if case['op'] != 'append':  # which takes none
+        if library.qwen_gpu_op_paged_workspace(ctypes.byref(cache), ctypes.byref(batch), query_heads,
+                                               ctypes.byref(bytes_)):
+            raise RuntimeError(library.qwen_gpu_last_error().decode())
     state['workspace'] = torch.zeros(bytes_.value, dtype=torch.uint8, device='cuda')
     state['plan'] = library, cache, batch, ctypes.byref(cache), ctypes.byref(batch), query_heads
     return state['plan']
