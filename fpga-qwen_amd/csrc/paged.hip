@@ -45,8 +45,8 @@ PagedView paged_view(const qwen_gpu_paged_cache& c, const qwen_gpu_paged_batch& 
         if (a.count == 1) continue;  // its stride is never taken
         require(a.stride >= span && a.stride <= (int64_t(1) << 40), "Paged strides let rows overlap or run too far");
         require(a.stride * size % 16 == 0, "Paged strides must be multiples of 16 bytes");
+        require(a.count - 1 <= ((int64_t(1) << 44) - span) / a.stride, "Paged strides let rows overlap or run too far");
         span += a.stride * (a.count - 1);
-        require(span <= (int64_t(1) << 44), "Paged strides let rows overlap or run too far");
     }
     require(b.sequences >= 1 && b.sequences <= 4096, "Paged sequences must be in 1..4096");
     require(b.sequences * c.kv_heads < 1 << 21, "Too many sequences for that many KV heads");

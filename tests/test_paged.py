@@ -62,6 +62,17 @@ def test_caches_refused(qpkg, op, message, fields):
 
 
 @pytest.mark.parametrize('op', ['append', 'attention', 'evict'])
+@pytest.mark.parametrize('fields', [
+    dict(page_stride=1 << 34, pages=1 << 30), dict(page_stride=1 << 40, pages=1 << 24),
+    dict(page_stride=1 << 34, pages=(1 << 30) + 1, head_stride=1 << 36),
+    dict(page_stride=1 << 40, pages=(1 << 24) + 1, kv_heads=2, head_stride=1 << 40),
+    dict(page_stride=1 << 24, pages=(1 << 20) + 1)])
+def test_pools_past_64_bits_refused(qpkg, op, fields):
+    """Rows further apart than any memory, the products of stride and count that pass 64 bits among them."""
+    refused(qpkg, 'let rows overlap or run too far', cache(qpkg, **fields), op=op)
+
+
+@pytest.mark.parametrize('op', ['append', 'attention', 'evict'])
 @pytest.mark.parametrize('message,fields', [
     ('Null argument: table', dict(table=None)), ('Null argument: lengths', dict(lengths=None)),
     ('sequences must be', dict(sequences=0)), ('sequences must be', dict(sequences=65537)),
