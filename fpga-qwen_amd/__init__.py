@@ -689,7 +689,7 @@ class PagedKV:
         """New rows [total, kv_heads, head_dim] behind the sequences' cached
         ones: counts[s] rows of sequence s, one after the other (None: one
         each). Their pages must be in the table."""
-        counts = np.ones(self.lengths.size, np.int32) if counts is None else np.asarray(counts, np.int32)
+        counts = np.ones(self.lengths.size, np.int32) if counts is None else np.array(counts, np.int32)
         keys, values = np.ascontiguousarray(keys, np.float32), np.ascontiguousarray(values, np.float32)
         shape = (int(counts.sum()), self.kv_heads, self.head_dim)
         if counts.shape != self.lengths.shape or (counts < 0).any():

@@ -201,3 +201,71 @@ def test_wrapper_checks_arguments(qpkg):
         qpkg.PagedKV(1, 1, 1, type='f32')
     with pytest.raises(ValueError, match='needs sequences'):
         qpkg.PagedKV(0, 1, 1)
+
+
+class Memory:
+    """Stands for DeviceBuffer where no device is: host arrays."""
+
+    def __init__(self, nbytes):
+        self.nbytes, self.array = int(nbytes), np.zeros(int(nbytes), np.uint8)
+        self.ptr = ctypes.c_void_p(self.array.ctypes.data)
+
+    @classmethod
+    def from_array(cls, array):
+        array = np.ascontiguousarray(array)
+        made = cls(array.nbytes)
+        made.array[:] = array.reshape(-1).view(np.uint8)
+        return made
+
+    def to_array(self, dtype, count):
+        return self.array.view(dtype)[:count].copy()
+
+
+class Library:
+    """Stands for the library: keeps each call's name and batch, and fails where told to."""
+
+    def __init__(self):
+        self.calls, self.fails = [], False
+
+    def __getattr__(self, name):
+        def call(cache, batch, *rest):
+            b = batch._obj
+            self.calls.append((name, b.rows, b.total_rows, b.max_length,
+                               np.ctypeslib.as_array(ctypes.cast(b.offsets, ctypes.POINTER(ctypes.c_int32)),
+                                                     (b.sequences + 1,)).copy(),
+                               np.ctypeslib.as_array(ctypes.cast(b.lengths, ctypes.POINTER(ctypes.c_int32)),
+                                                     (b.sequences,)).copy()))
+            return int(self.fails)
+        return call
+
+    def qwen_gpu_last_error(self):
+        return b'it fails'
+
+
+@pytest.fixture
+def paged(qpkg, monkeypatch):
+    """A PagedKV of two sequences over stand-ins for memory and library."""
+    qpkg.load_library()
+    library = Library()
+    monkeypatch.setattr(qpkg, 'DeviceBuffer', Memory)
+    monkeypatch.setattr(qpkg, '_LIB', library)
+    monkeypatch.setattr(qpkg, 'synchronize', lambda: None)
+    made = qpkg.PagedKV(2, 8, 4, 16, 2, 64, track=True)
+    made.table[:] = np.arange(8).reshape(2, 4)
+    return made, library
+
+
+def new(count):
+    return np.zeros((count, 2, 64), np.float32)
+
+
+def test_wrapper_keeps_its_own_counts(paged):
+    """The array of counts is the caller's, who may use it again before the attention."""
+    cache, library = paged
+    counts = np.array([3, 1], np.int32)
+    cache.append(new(4), new(4), counts)
+    counts[:] = 0
+    cache.attention(np.zeros((4, 2, 64), np.float32))
+    name, rows, total, _, offsets, lengths = library.calls[-1]
+    assert name == 'qwen_gpu_op_paged_attention' and (rows, total) == (3, 4)
+    assert offsets.tolist() == [0, 3, 4] and lengths.tolist() == [3, 1]
