@@ -664,16 +664,16 @@ class PagedKV:
                                  kv_heads, head_dim, PAGED_TYPES[type])
         self._slots = slots
 
-    def _batch(self, rows, total):
+    def _batch(self, lengths, seen, counts, rows, total):
         """The batch's description and the device arrays that it points to."""
-        if self.table.shape[1] * self.page_size != self._slots or self.table.shape[0] != self.lengths.size:
+        if self.table.shape[1] * self.page_size != self._slots or self.table.shape[0] != lengths.size:
             raise ValueError('table must keep its shape')
-        offsets = np.concatenate(([0], np.cumsum(self._counts))).astype(np.int32)
+        offsets = np.concatenate(([0], np.cumsum(counts))).astype(np.int32)
         held = [DeviceBuffer.from_array(np.ascontiguousarray(x, np.int32))
-                for x in (self.table, self.lengths, offsets, self.seen)]
+                for x in (self.table, lengths, offsets, seen)]
         batch = PagedBatch(held[0].ptr, held[1].ptr, held[2].ptr, held[3].ptr,
                            self._weights.ptr if self._weights else None,
-                           self._positions.ptr if self._positions else None, self._slots, self.lengths.size,
+                           self._positions.ptr if self._positions else None, self._slots, lengths.size,
                            self.table.shape[1], self._slots, rows, total)
         return batch, held
 
@@ -698,17 +698,16 @@ class PagedKV:
             raise ValueError(f'keys and values must both be {shape}, got {keys.shape} and {values.shape}')
         if (self.lengths + counts > self._slots).any():
             raise ValueError(f'a sequence has more than {self._slots} rows')
-        self._counts = counts
-        self.lengths, self.seen = self.lengths + counts, self.seen + counts
-        if not shape[0]:
-            return
-        batch, held = self._batch(int(counts.max()), shape[0])
-        k, v = DeviceBuffer.from_array(keys), DeviceBuffer.from_array(values)
-        stride = self.kv_heads * self.head_dim
-        _check(_LIB.qwen_gpu_op_paged_append(ctypes.byref(self._cache), ctypes.byref(batch), k.ptr, stride, v.ptr,
-                                             stride, None))
-        synchronize()
-        del held
+        lengths, seen = self.lengths + counts, self.seen + counts
+        if shape[0]:
+            batch, held = self._batch(lengths, seen, counts, int(counts.max()), shape[0])
+            k, v = DeviceBuffer.from_array(keys), DeviceBuffer.from_array(values)
+            stride = self.kv_heads * self.head_dim
+            _check(_LIB.qwen_gpu_op_paged_append(ctypes.byref(self._cache), ctypes.byref(batch), k.ptr, stride, v.ptr,
+                                                 stride, None))
+            synchronize()
+            del held
+        self.lengths, self.seen, self._counts = lengths, seen, counts  # only now that the rows are there
 
     def attention(self, queries, scale=None):
         """Attention of the rows appended last: queries [total, query_heads,
@@ -720,7 +719,7 @@ class PagedKV:
         if not total:
             return np.zeros_like(queries)
         heads = queries.shape[1]
-        batch, held = self._batch(int(self._counts.max()), total)
+        batch, held = self._batch(self.lengths, self.seen, self._counts, int(self._counts.max()), total)
         space, q, out = self._space(batch, heads), DeviceBuffer.from_array(queries), DeviceBuffer(queries.nbytes)
         stride = heads * self.head_dim
         _check(_LIB.qwen_gpu_op_paged_attention(ctypes.byref(self._cache), ctypes.byref(batch), q.ptr, stride, heads,
@@ -734,7 +733,7 @@ class PagedKV:
         """Cuts every sequence to at most `keep` rows of each KV head (weights
         and positions are changed in place). Pages behind the new lengths are
         the caller's again."""
-        batch, held = self._batch(1, 0)
+        batch, held = self._batch(self.lengths, self.seen, self._counts, 1, 0)
         space, lengths = self._space(batch, self.kv_heads), DeviceBuffer(self.lengths.nbytes)
         _check(_LIB.qwen_gpu_op_paged_evict(ctypes.byref(self._cache), ctypes.byref(batch), keep, sinks, recent,
                                             lengths.ptr, batch.weights, batch.positions, space.ptr, space.nbytes,

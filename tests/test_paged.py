@@ -269,3 +269,33 @@ def test_wrapper_keeps_its_own_counts(paged):
     name, rows, total, _, offsets, lengths = library.calls[-1]
     assert name == 'qwen_gpu_op_paged_attention' and (rows, total) == (3, 4)
     assert offsets.tolist() == [0, 3, 4] and lengths.tolist() == [3, 1]
+
+
+@pytest.mark.parametrize('fault', ['library', 'memory', 'synchronize', 'table'])
+def test_wrapper_stays_as_it_was_where_an_append_fails(qpkg, paged, monkeypatch, fault):
+    """No sequence is longer by rows that were not written, and the next append goes where the failed one would have."""
+    cache, library = paged
+    cache.append(new(5), new(5), [4, 1])
+
+    def fail(*_):
+        raise RuntimeError('it fails')
+
+    with monkeypatch.context() as broken:
+        if fault == 'library':
+            library.fails = True
+        elif fault == 'memory':
+            broken.setattr(Memory, 'from_array', fail)
+        elif fault == 'synchronize':
+            broken.setattr(qpkg, 'synchronize', fail)
+        else:
+            broken.setattr(cache, 'table', cache.table[:1])
+        with pytest.raises((RuntimeError, ValueError)):
+            cache.append(new(3), new(3), [1, 2])
+    library.fails = False
+    assert cache.lengths.tolist() == cache.seen.tolist() == [4, 1]
+    cache.attention(np.zeros((5, 2, 64), np.float32))
+    assert library.calls[-1][1:3] == (4, 5)
+    cache.append(new(3), new(3), [1, 2])
+    assert library.calls[-1][5].tolist() == cache.lengths.tolist() == [5, 3]
+    cache.append(new(0), new(0), [0, 0])
+    assert cache.lengths.tolist() == [5, 3] and cache.attention(np.zeros((0, 2, 64), np.float32)).shape == (0, 2, 64)
