@@ -79,7 +79,8 @@ void launch_paged_attention(const qwen_gpu_paged_cache& cache, const qwen_gpu_pa
     require(queries, "Null argument: queries");
     require(out, "Null argument: out");
     check_heads(cache, query_heads);
-    require(std::isfinite(scale), "The scale must be finite");
+    const float scale_of_2 = scale * 1.44269504088896340736f;  // the kernels' exponentials are powers of 2
+    require(std::isfinite(scale_of_2), "The scale must be finite, times log2(e) too");
     const int64_t row = int64_t(query_heads) * cache.head_dim;
     require(query_stride >= row && out_stride >= row, "Paged rows overlap: stride below query_heads * head_dim");
     require(query_stride <= (int64_t(1) << 32) && out_stride <= (int64_t(1) << 32), "Paged row stride is too large");
@@ -103,7 +104,7 @@ void launch_paged_attention(const qwen_gpu_paged_cache& cache, const qwen_gpu_pa
                           int(shares_of(cache.head_dim) / plan.grid_rows) + 1,
                           int(plan.pitch),
                           int(plan.tiles),
-                          scale * 1.44269504088896340736f,
+                          scale_of_2,
                           reinterpret_cast<float*>(space),
                           static_cast<int*>(workspace),
                           plan.adds,

@@ -116,6 +116,14 @@ def test_scale_refused(qpkg, scale):
     assert status == 1 and 'scale must be finite' in qpkg.load_library().qwen_gpu_last_error().decode()
 
 
+@pytest.mark.parametrize('scale', [2.4e38, -3.4e38])
+def test_scales_refused_whose_power_of_2_overflows(qpkg, scale):
+    """Finite, but not times log2(e): a score of 0 would become NaN."""
+    lib = qpkg.load_library()
+    status = lib.qwen_gpu_op_paged_attention(cache(qpkg), batch(qpkg), AT, 2048, 16, scale, AT, 2048, AT, 1 << 30, None)
+    assert status == 1 and 'scale must be finite, times' in lib.qwen_gpu_last_error().decode()
+
+
 def test_sizes_refused_that_no_launch_holds(qpkg):
     """Grids and indices would pass 32 bits."""
     wide = dict(sequences=4096, total_rows=4096)
