@@ -650,6 +650,7 @@ void launch_paged_evict(const qwen_gpu_paged_cache& cache, const qwen_gpu_paged_
             "Need 0 <= sinks, 0 <= recent and sinks + recent <= keep");
     const size_t tracked = size_t(batch.sequences) * cache.kv_heads * batch.track_stride * 4;
     require(apart(new_lengths, batch.lengths, size_t(batch.sequences) * 4), "new_lengths overlaps lengths");
+    require(!batch.seen || apart(new_lengths, batch.seen, size_t(batch.sequences) * 4), "new_lengths overlaps seen");
     require(new_weights == batch.weights || apart(new_weights, batch.weights, tracked), "new_weights overlaps weights");
     require(new_positions == batch.positions || apart(new_positions, batch.positions, tracked),
             "new_positions overlaps positions");

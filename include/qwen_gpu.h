@@ -372,7 +372,7 @@ int qwen_gpu_op_paged_attention(const qwen_gpu_paged_cache* cache, const qwen_gp
  * in slots from keep on move, in their order, into the holes before it, so
  * the rows no longer lie in the order of their positions: attention of the
  * rows that are appended next does not depend on it. new_lengths[s] =
- * min(lengths[s], keep), not the array `lengths`; new_weights and
+ * min(lengths[s], keep), not the array `lengths` or `seen`; new_weights and
  * new_positions receive the first new_lengths[s] entries and may be the
  * batch's own arrays (else they must not overlap them). weights and
  * positions are needed; offsets, rows and total_rows are not used. The

@@ -142,6 +142,12 @@ def test_evict_needs_what_it_goes_by(qpkg):
     refused(qpkg, 'Null argument: positions', b=batch(qpkg, positions=None), op='evict')
 
 
+@pytest.mark.parametrize('shift', [-4, 0, 4])
+def test_evict_refuses_new_lengths_among_the_seen(qpkg, shift):
+    """Each head of a sequence reads seen[s] while the first one writes new_lengths[s]."""
+    refused(qpkg, 'new_lengths overlaps seen', b=batch(qpkg, seen=2 * AT + shift), op='evict')
+
+
 @pytest.mark.parametrize('op', ['append', 'attention', 'evict'])
 def test_host_memory_refused(qpkg, op):
     """Pointers that no kernel could read end in an error, not in a fault."""
