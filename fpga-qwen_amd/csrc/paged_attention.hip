@@ -3,6 +3,7 @@
 #include "paged_attention.hpp"
 
 #include <cmath>
+#include <cstdlib>
 #include <string>
 
 #include "paged.hpp"
@@ -59,6 +60,17 @@ void check_heads(const qwen_gpu_paged_cache& cache, int query_heads) {
             "query_heads must be a multiple of kv_heads, at most 1024 times");
 }
 
+// Rows of `out` lie on their own queries or apart from all (between them, for one): a workgroup's output would
+// otherwise be another's queries.
+bool rows_apart(const float* queries, int64_t query_stride, const float* out, int64_t out_stride, int64_t row,
+                int64_t total) {
+    if (!total || (out == queries && out_stride == query_stride)) return true;
+    const int64_t ahead = reinterpret_cast<intptr_t>(out) - reinterpret_cast<intptr_t>(queries), bytes = row * 4;
+    if (ahead >= ((total - 1) * query_stride + row) * 4 || -ahead >= ((total - 1) * out_stride + row) * 4) return true;
+    const int64_t stride = query_stride * 4, off = std::abs(ahead) % stride;
+    return query_stride == out_stride && off >= bytes && stride - off >= bytes;
+}
+
 }  // namespace
 
 size_t paged_workspace_bytes(const qwen_gpu_paged_cache& cache, const qwen_gpu_paged_batch& batch, int query_heads) {
@@ -84,6 +96,7 @@ void launch_paged_attention(const qwen_gpu_paged_cache& cache, const qwen_gpu_pa
     const int64_t row = int64_t(query_heads) * cache.head_dim;
     require(query_stride >= row && out_stride >= row, "Paged rows overlap: stride below query_heads * head_dim");
     require(query_stride <= (int64_t(1) << 32) && out_stride <= (int64_t(1) << 32), "Paged row stride is too large");
+    require(rows_apart(queries, query_stride, out, out_stride, row, batch.total_rows), "out overlaps other rows' queries");
     const AttentionPlan plan(cache, batch, query_heads);
     require(plan.blocks < (int64_t(1) << 31) && plan.columns < (int64_t(1) << 23) && plan.grid_rows <= 65535 &&
                 plan.score_rows < (int64_t(1) << 31),

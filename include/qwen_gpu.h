@@ -360,7 +360,7 @@ int qwen_gpu_op_paged_append(const qwen_gpu_paged_cache* cache, const qwen_gpu_p
  * an order that depends on the call's shapes and lengths alone. Keys and
  * values that a row attends are finite (else its output may be NaN); those
  * that it does not attend may be anything. out may be queries themselves,
- * with one stride. query_heads is at most 1024 * kv_heads; scale, and scale
+ * with one stride, and lies apart from them otherwise. query_heads is at most 1024 * kv_heads; scale, and scale
  * times log2(e), are finite. */
 int qwen_gpu_op_paged_attention(const qwen_gpu_paged_cache* cache, const qwen_gpu_paged_batch* batch,
                                 const float* queries, int64_t query_stride, int query_heads, float scale, float* out,

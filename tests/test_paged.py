@@ -124,6 +124,19 @@ def test_scales_refused_whose_power_of_2_overflows(qpkg, scale):
     assert status == 1 and 'scale must be finite, times' in lib.qwen_gpu_last_error().decode()
 
 
+@pytest.mark.parametrize('refuses,out,stride,out_stride', [
+    (True, 0, 4096, 4097), (True, 0, 4096, 2048), (True, 4, 4096, 4096), (True, -4, 4096, 4096),
+    (True, 4096, 4096, 4096), (True, 2047, 4096, 4096), (True, 2049, 4096, 4096), (True, -4096, 4096, 4096),
+    (True, 2 * 4096 + 2047, 4096, 4096), (True, 2048, 4096, 2048), (True, 2 * 4096, 4096, 4096),
+    (False, 0, 4096, 4096), (False, 2048, 4096, 4096), (False, -2048, 4096, 4096), (False, 2 * 4096 + 2048, 4096, 2048),
+    (False, 3 * 4096, 4096, 4096), (False, -2 * 2048 - 2048, 4096, 2048), (False, 4096 + 2048, 4096, 4096)])
+def test_attention_refuses_outputs_over_other_queries(qpkg, refuses, out, stride, out_stride):
+    """Three rows of 2048: other rows and heads of the call may still read what is written there."""
+    given = dict(q=AT, q_stride=stride, out=AT + 4 * out, out_stride=out_stride, op='attention')
+    message = 'out overlaps' if refuses else 'Not device memory: keys'
+    refused(qpkg, message, b=batch(qpkg, sequences=3, total_rows=3), **given)
+
+
 def test_sizes_refused_that_no_launch_holds(qpkg):
     """Grids and indices would pass 32 bits."""
     wide = dict(sequences=4096, total_rows=4096)
