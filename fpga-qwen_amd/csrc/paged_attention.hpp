@@ -856,7 +856,7 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
 struct AttentionPlan {
     bool packed, adds;
     int64_t tiles, grid_rows, blocks, score_stride, score_rows;
-    int64_t columns, first, pitch;  // of a grid row: workgroups, those of the first layer, partials
+    int64_t columns, first, pitch;  // of a grid row: workgroups, those of the first layer, places for partials
     size_t partial_bytes, state_bytes, score_bytes;
     AttentionPlan(const qwen_gpu_paged_cache& c, const qwen_gpu_paged_batch& b, int query_heads) {
         const int64_t rows = int64_t(query_heads / c.kv_heads) * b.rows;
@@ -872,7 +872,12 @@ struct AttentionPlan {
         // Every sequence with new rows has a block, so beyond that many they are dealt in runs.
         if (!b.offsets && b.sequences * c.kv_heads > kStream * shares) columns = runs;
         first = std::min(columns, 2 * runs);
-        pitch = std::max((columns + first - 1) / first * first, blocks > kStream * shares ? 2 * runs : 0);
+        // Dealt in runs, a grid row has two places for each; dealt in parts, one for each part, and no more parts
+        // than blocks, which are then kStream * shares / grid_rows at most. With a share or less for a grid row
+        // every unit is one part, which takes none.
+        pitch = std::max(columns, blocks > kStream * shares ? 2 * runs : 0);
+        pitch = grid_rows < shares ? std::min(pitch, kStream * shares / grid_rows) : 0;
+        static_assert(kStream >= 2, "room for two places a run");
         partial_bytes = size_t(pitch) * grid_rows * tile_rows * (c.head_dim + 4) * 4;
         score_stride = (b.max_length + kTile - 1) / kTile * kTile;
         score_rows = int64_t(b.sequences) * c.kv_heads * rows;

@@ -326,3 +326,21 @@ def test_wrapper_stays_as_it_was_where_an_append_fails(qpkg, paged, monkeypatch,
     assert library.calls[-1][5].tolist() == cache.lengths.tolist() == [5, 3]
     cache.append(new(0), new(0), [0, 0])
     assert cache.lengths.tolist() == [5, 3] and cache.attention(np.zeros((0, 2, 64), np.float32)).shape == (0, 2, 64)
+
+
+@pytest.mark.parametrize('rows,sequences', [(4096, 64), (4096, 256), (2000, 64), (500, 64), (100, 512), (8, 4096),
+                                            (1, 4096), (1, 1)])
+@pytest.mark.parametrize('dim', [64, 128, 256])
+def test_workspace_holds_the_parts_of_split_units_alone(qpkg, rows, sequences, dim):
+    """Untracked, whatever the number of new rows: four shares' tiles of sums for each of the 512 workgroups (256 with
+    heads of 256) at most, none where there are as many tiles as workgroups; and the eviction's lists."""
+    lib, size = qpkg.load_library(), ctypes.c_size_t()
+    c = cache(qpkg, head_dim=dim, page_stride=8 * 16 * dim, head_stride=16 * dim, slot_stride=dim)
+    b = batch(qpkg, weights=None, positions=None, offsets=AT, sequences=sequences, rows=rows,
+              total_rows=min(1 << 24, sequences * rows), table_stride=256, max_length=4096)
+    assert lib.qwen_gpu_op_paged_workspace(c, b, 16, ctypes.byref(size)) == 0
+    fixed, lists, shares = 131072 + 16, sequences * 8 * (4096 + 4) * 4, 256 if dim == 256 else 512
+    tile = 8 if rows * 2 <= 8 else 16
+    tiles = 8 * -(-rows * 2 // tile)
+    partials = 0 if tiles >= shares else 4 * shares * tile * (dim + 4) * 4
+    assert size.value <= fixed + max(lists, partials)
