@@ -325,12 +325,11 @@ __device__ __forceinline__ void widen(uint4_t raw, float up, uint4_t (&out)[TYPE
     }
 }
 
-// Nonzero if one of the word's stored values is infinite or NaN.
-template <int TYPE>
+// The sign bits of those of a word's two 16-bit values that are infinite or NaN.
+template <bool HALF>
 __device__ __forceinline__ unsigned not_finite(unsigned w) {
-    if constexpr (TYPE == kPagedF16) return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
-    if constexpr (TYPE == kPagedBF16) return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
-    return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+    if constexpr (HALF) return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+    return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
 }
 
 template <int TYPE>
@@ -600,23 +599,13 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
             }
 
             // Values into LDS, 0 for those that are not there. A weight of 0 does not keep infinities and NaN
-            // out, so those in rows that only some new rows see are 0 here as well, and added below.
-            bool spoilt = false;
-            if (base + kTile > shared_end) {
-                unsigned bits = 0;
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const bool partly = was[u] && base + 16 * u + column >= shared_end;
-#pragma unroll
-                    for (int i = 0; i < kLoads; ++i)
-#pragma unroll
-                        for (int w = 0; w < 4; ++w) bits |= partly ? not_finite<TYPE>(values[u][i][w]) : 0u;
-                }
-                spoilt = __any(bits != 0);
-            }
+            // out, so those in rows that only some new rows see are 0 here as well, and added below. They are found
+            // in the 16-bit words: an E4M3 row's power of two may carry finite codes past what these hold.
+            const bool triangle = base + kTile > shared_end;
+            unsigned spoilt_bits = 0;
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const bool partly = base + 16 * u + column >= shared_end;
+                const unsigned partly = base + 16 * u + column >= shared_end ? ~0u : 0u;
 #pragma unroll
                 for (int i = 0; i < kLoads; ++i) {
                     uint4_t w[kPer];
@@ -624,16 +613,19 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
 #pragma unroll
                     for (int j = 0; j < kPer; ++j) {
                         if (!whole && !was[u]) w[j] = uint4_t{0u, 0u, 0u, 0u};
-                        if (spoilt && partly)
+                        if (triangle)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                w[j][e] &= ~((not_finite<TYPE == kPagedF16 ? kPagedF16 : kPagedBF16>(w[j][e]) >> 15) *
-                                             0xffffu);
+                            for (int e = 0; e < 4; ++e) {
+                                const unsigned bad = not_finite<TYPE == kPagedF16>(w[j][e]) & partly;
+                                spoilt_bits |= bad;
+                                w[j][e] &= ~((bad >> 15) * 0xffffu);
+                            }
                         char* const to = mine + (16 * u + column) * kPitch + 64 * kPer * i + 16 * kPer * part + 16 * j;
                         *reinterpret_cast<uint4_t*>(to) = w[j];
                     }
                 }
             }
+            const bool spoilt = triangle && __any(spoilt_bits != 0);
             if (more_steps) {
                 if (base + 2 * kBlock < end) find(base + 2 * kBlock);
                 load(v.values, values);

@@ -304,6 +304,31 @@ def test_attention_takes_nothing_from_what_it_does_not_attend(qpkg, kind):
         assert not np.isfinite(results[1][3 * s + 2]).any()
 
 
+@pytest.mark.parametrize('byte', [0, 1, 245, 246, 247, 248, 254, 255])
+@pytest.mark.parametrize('heads,dim', [(4, 64), (2, 256), (20, 128)])
+def test_attention_takes_nothing_from_exponents_it_does_not_attend(qpkg, byte, heads, dim):
+    """Finite codes that their row's exponent carries past what a float holds, and exponents that no row is written
+    with, where the test above has codes that are NaN."""
+    rng = np.random.default_rng(127)
+    lengths, rows, page, kv = [37, 130, 3], 3, 16, 2
+    table, pages = make_table(rng, lengths, page)
+    clean = ref.Cache('e4m3', pages, page, kv, dim, rng=rng)
+    dirty = clean.copy()
+    used = {(int(table[s, j // page]), j % page) for s, n in enumerate(lengths) for j in range(n - 1)}
+    for p in range(pages):
+        for slot in range(page):
+            if (p, slot) not in used:
+                dirty.exponents[p, :, slot] = byte
+                for h in range(kv):
+                    dirty.values[dirty.where(p, h, slot)][slot % dim] = 0x7e - 128 * -(slot % 2)  # 448 or -448
+    queries = rng.standard_normal((9, heads * dim)).astype(np.float32)
+    out = np.zeros_like(queries)
+    results = [Call(qpkg, c, table, lengths, rows).attention(queries, heads, 0.125, out) for c in (clean, dirty)]
+    for s in range(3):  # the last row of a sequence sees its own key and value
+        assert np.isfinite(results[1][3 * s:3 * s + 2]).all()
+        assert np.array_equal(results[0][3 * s:3 * s + 2], results[1][3 * s:3 * s + 2])
+
+
 def test_attention_bounds_what_the_device_holds(qpkg):
     """Slots without a page are not attended (all of them: 0), rows that do not
     exist are left alone, lengths beyond max_length are taken as that."""
