@@ -30,26 +30,25 @@ __global__ __launch_bounds__(256) void paged_track_kernel(PagedView v, Attention
     __shared__ int sees[kStates];
     const int heads = v.kv_heads, s = blockIdx.x / heads, head = blockIdx.x - s * heads;
     int first;
-    const int n = v.new_rows(s, first), length = v.length(s), query_rows = a.group * n;
+    const int n = v.new_rows(s, first), length = v.length(s);
+    int from_row, to_row;
+    v.existing(first, n, from_row, to_row);
     float* const weights = v.weights + v.track_at(s, head);
-    const int64_t unit = int64_t(blockIdx.x) * (int64_t(v.rows) * a.group);
-    const float* const scores = a.scores + unit * a.score_stride;
-    for (int r0 = 0; r0 < query_rows; r0 += kStates) {
-        const int count = min(kStates, query_rows - r0);
+    const int64_t unit = a.tracked(v, head, first);
+    for (int r0 = from_row * a.group; r0 < to_row * a.group; r0 += kStates) {
+        const int count = min(kStates, to_row * a.group - r0);
+        const float* const scores = a.scores + (unit + r0) * a.score_stride;
         __syncthreads();
         if (int(threadIdx.x) < count) {
-            const int i = (r0 + int(threadIdx.x)) / a.group;
-            const int64_t row = int64_t(first) + i;
-            const bool live = row >= 0 && row < v.total_rows;
-            states[threadIdx.x] = live ? a.states[unit + r0 + threadIdx.x] : float2{0.f, 0.f};
-            sees[threadIdx.x] = live ? length - n + i + 1 : 0;
+            states[threadIdx.x] = a.states[unit + r0 + threadIdx.x];
+            sees[threadIdx.x] = length - n + (r0 + int(threadIdx.x)) / a.group + 1;
         }
         __syncthreads();
         for (int j = blockIdx.y * 256 + threadIdx.x; j < length; j += int(gridDim.y) * 256) {
             float w = 0.f;
             for (int q = 0; q < count; ++q)
                 if (j < sees[q])
-                    w += exp2_fast(scores[(r0 + q) * a.score_stride + j] - states[q].x) * states[q].y;
+                    w += exp2_fast(scores[q * a.score_stride + j] - states[q].x) * states[q].y;
             weights[j] += w;
         }
     }

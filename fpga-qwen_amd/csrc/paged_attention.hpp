@@ -40,12 +40,17 @@ struct AttentionArgs {
     float* partials;    // [parts][rows of a tile][DIM + 4]: output, reference, sum, the same of a group of parts
     int* counters;      // kCounterStep apart, 0 between launches
     bool adds;          // tracked: the attention adds to the weights itself
-    float2* states;     // tracked, not so: [sequences * kv_heads][rows * group]: reference, 1 / sum
-    float* scores;      // tracked: [sequences * kv_heads][rows * group][score_stride]
+    float2* states;     // tracked, not so: [kv_heads][total_rows * group]: reference, 1 / sum
+    float* scores;      // tracked: [kv_heads][total_rows * group][score_stride]
     int64_t score_stride;
 
     // Of a KV head's query row, the new row that it belongs to.
     __device__ __forceinline__ int new_row(int r) const { return page_slot(r, group, magic).page; }
+    // Where query row 0 of a KV head and a sequence whose new rows begin at `first` has its state and scores. They
+    // lie by new rows, not by sequences: those of a batch may have very different numbers of them.
+    __device__ __forceinline__ int64_t tracked(const PagedView& v, int head, int first) const {
+        return (int64_t(head) * v.total_rows + first) * group;
+    }
 };
 
 // How the positions are dealt. A unit is a sequence, a KV head and a tile of its
@@ -571,9 +576,9 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
                     }
             }
             if constexpr (TRACK) {
-                if (!second && query_row < query_rows) {
-                    const int64_t unit_rows = (int64_t(share.s) * v.kv_heads + head) * (int64_t(v.rows) * a.group);
-                    float* const to = a.scores + (unit_rows + query_row) * a.score_stride + base + 4 * part;
+                if (!second && live) {
+                    const int64_t at_row = a.tracked(v, head, d.first) + query_row;
+                    float* const to = a.scores + at_row * a.score_stride + base + 4 * part;
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         float4_t w;
@@ -694,7 +699,7 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
                 if (a.adds)
                     row_state[local] = state;
                 else
-                    a.states[(int64_t(share.s) * v.kv_heads + head) * (int64_t(v.rows) * a.group) + r] = state;
+                    a.states[a.tracked(v, head, d.first) + r] = state;
             }
         };
         for (int item = threadIdx.x; item < kRows * DIM / 4; item += kWaves * 64) {
@@ -811,21 +816,23 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void paged_attenti
             if (share.parts == 1) posted_stores_done();
             __syncthreads();
             float* const slots = v.weights + v.track_at(share.s, head);
-            const float* const unit = a.scores + (int64_t(share.s) * v.kv_heads + head) *
-                                                     (int64_t(v.rows) * a.group) * a.score_stride;
+            const int64_t unit = a.tracked(v, head, d.first);
+            int from_row, to_row;
+            v.existing(d.first, d.n, from_row, to_row);
+            from_row *= a.group, to_row *= a.group;
             for (int j = 4 * int(threadIdx.x); j < d.length; j += 4 * kWaves * 64) {
                 float4_t grown = {0.f, 0.f, 0.f, 0.f};
-                for (int r0 = 0; r0 < query_rows; r0 += 4) {
+                for (int r0 = from_row; r0 < to_row; r0 += 4) {
                     float2 low[4], high[4];
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        const float* const from = unit + min(r0 + q, query_rows - 1) * a.score_stride + j;
+                        const float* const from = a.scores + (unit + min(r0 + q, to_row - 1)) * a.score_stride + j;
                         low[q] = posted(from);
                         high[q] = posted(from + 2);
                     }
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        if (r0 + q >= query_rows) continue;
+                        if (r0 + q >= to_row) continue;
                         const float2 state = row_state[r0 + q];
                         const int seen = state.y == 0.f ? 0 : d.length - d.n + a.new_row(r0 + q) + 1 - j;
                         if (seen > 0) grown[0] += exp2_fast(low[q].x - state.x) * state.y;
@@ -872,7 +879,7 @@ struct AttentionPlan {
         static_assert(kStream >= 2, "room for two places a run");
         partial_bytes = size_t(pitch) * grid_rows * tile_rows * (c.head_dim + 4) * 4;
         score_stride = (b.max_length + kTile - 1) / kTile * kTile;
-        score_rows = int64_t(b.sequences) * c.kv_heads * rows;
+        score_rows = int64_t(b.total_rows) * query_heads;
         // The workgroup that completes a unit adds to the weights, four positions a thread and four rows at a time,
         // while that takes it a few turns: 12.2 us for 300 positions against 14.2 with a kernel for it, 19.5 and
         // 20.6 for eight sequences of 1025, but 37.2 and 32.9 for eight of 4096. Where several units share the

@@ -56,6 +56,11 @@ struct PagedView {
         const int64_t n = int64_t(offsets[s + 1]) - first;
         return n < 0 ? 0 : n > rows ? rows : int(n);
     }
+    // Which of a sequence's n new rows exist: from .. to - 1 (0 .. n - 1 unless offsets pass total_rows).
+    __device__ void existing(int first, int n, int& from, int& to) const {
+        to = int(max(int64_t(0), min(int64_t(n), int64_t(total_rows) - first)));
+        from = int(min(int64_t(to), max(int64_t(0), -int64_t(first))));
+    }
     // Page of the table's entry, -1 where it holds none.
     __device__ int page_of(int s, int entry) const {
         const int page = table[int64_t(s) * table_stride + entry];

@@ -295,7 +295,7 @@ int qwen_gpu_op_copy(const void* src, void* dst, size_t bytes, void* stream);
  * max_length; a slot whose page is not in 0 .. pages - 1 is neither written
  * nor attended; rows outside 0 .. total_rows - 1 are neither read nor
  * written; offsets must not fall (where they do, which of its rows a sequence
- * gets is open). None of them may change while a call runs. `stream` is NULL
+ * gets and what its weights grow by are open). None of them may change while a call runs. `stream` is NULL
  * (the default stream of the cache's device) or a created stream of that
  * device; the current device does not matter. */
 #define QWEN_GPU_PAGED_F16 0

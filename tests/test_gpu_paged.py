@@ -329,6 +329,30 @@ def test_attention_takes_nothing_from_exponents_it_does_not_attend(qpkg, byte, h
         assert np.array_equal(results[0][3 * s:3 * s + 2], results[1][3 * s:3 * s + 2])
 
 
+@pytest.mark.parametrize('kind,kv,group,dim', [('f16', 2, 2, 64), ('bf16', 1, 4, 128), ('e4m3', 2, 1, 256)])
+@pytest.mark.parametrize('lengths,offsets,total', [
+    ([300, 40, 700, 0, 9], [-1, 1, 2, 4, 4, 7], 6),              # few rows, the first and the last of which do not exist
+    ([2500, 40, 2900, 0, 60], [-1, 1, 2, 4, 4, 6], 5),           # behind many positions
+    ([1100, 60, 70, 300, 5], [-2, 43, 44, 45, 45, 60], 50),      # a prompt among sequences with a row or none
+    ([80, 60, 1, 300, 5], [0, 1, 2, 3, 39, 39], 30)])
+def test_tracked_rows_lie_by_their_number(qpkg, kind, kv, group, dim, lengths, offsets, total):
+    """Weights of batches whose sequences have very different numbers of new rows, some of which do not exist."""
+    rng = np.random.default_rng(131)
+    table, pages = make_table(rng, lengths, 16)
+    cache = ref.Cache(kind, pages, 16, kv, dim, rng=rng)
+    weights = rng.random((len(lengths), kv, max(lengths) + 5)).astype(np.float32)
+    rows, heads, scale = int(max(np.diff(offsets))), kv * group, float(np.float32(dim ** -0.5))
+    queries = rng.standard_normal((total, heads * dim)).astype(np.float32)
+    out = np.full_like(queries, 2.5)
+    call = Call(qpkg, cache, table, lengths, rows, np.array(offsets), total, weights=weights)
+    got = call.attention(queries, heads, scale, out)
+    want, tolerance, new_weights, weight_tolerance = ref.attention(
+        cache, table, lengths, rows, np.array(offsets), queries.reshape(total, heads, dim), scale,
+        out.reshape(total, heads, dim), weights)
+    assert (np.abs(got.reshape(want.shape) - want) <= tolerance).all()
+    assert (np.abs(call.get('weights', weights) - new_weights) <= weight_tolerance).all()
+
+
 def test_attention_bounds_what_the_device_holds(qpkg):
     """Slots without a page are not attended (all of them: 0), rows that do not
     exist are left alone, lengths beyond max_length are taken as that."""

@@ -344,3 +344,16 @@ def test_workspace_holds_the_parts_of_split_units_alone(qpkg, rows, sequences, d
     tiles = 8 * -(-rows * 2 // tile)
     partials = 0 if tiles >= shares else 4 * shares * tile * (dim + 4) * 4
     assert size.value <= fixed + max(lists, partials)
+
+
+@pytest.mark.parametrize('sequences,rows,total', [(64, 512, 575), (256, 2000, 2255), (8, 512, 512), (64, 1, 64), (1, 4001, 4001)])
+def test_workspace_of_tracked_calls_goes_by_the_new_rows(qpkg, sequences, rows, total):
+    """A score for each new row, query head and position: one prompt among sequences with a row each takes what the
+    rows do, not as if each sequence had a prompt."""
+    lib, size = qpkg.load_library(), ctypes.c_size_t()
+    b = batch(qpkg, offsets=AT, sequences=sequences, rows=rows, total_rows=total, table_stride=256, max_length=4001,
+              track_stride=4096)
+    assert lib.qwen_gpu_op_paged_workspace(cache(qpkg), b, 16, ctypes.byref(size)) == 0
+    fixed, lists, partials = 131072 + 32, sequences * 8 * (4001 + 4) * 4, 4 * 512 * 16 * (128 + 4) * 4
+    scores = total * 16 * (4032 * 4 + 8)
+    assert scores < size.value <= fixed + max(lists, partials + scores)
