@@ -59,6 +59,18 @@ void check_heads(const qwen_gpu_paged_cache& cache, int query_heads) {
             "query_heads must be a multiple of kv_heads, at most 1024 times");
 }
 
+// The sizes of a call that a launch and 32-bit indices hold. A head's tiles have at most 16 query rows, so the first
+// check refuses no more than the second one would, and keeps the plan's products within 64 bits.
+AttentionPlan plan_of(const qwen_gpu_paged_cache& cache, const qwen_gpu_paged_batch& batch, int query_heads) {
+    const char* const too_many = "Too many new rows or positions for one call";
+    require(int64_t(query_heads) * batch.rows <= 65535 * 16, too_many);
+    const AttentionPlan plan(cache, batch, query_heads);
+    require(plan.grid_rows <= 65535 && plan.blocks < (int64_t(1) << 31) && plan.columns < (int64_t(1) << 23) &&
+                plan.score_rows < (int64_t(1) << 31),
+            too_many);
+    return plan;
+}
+
 // Rows of `out` lie on their own queries or apart from all (between them, for one): a workgroup's output would
 // otherwise be another's queries.
 bool rows_apart(const float* queries, int64_t query_stride, const float* out, int64_t out_stride, int64_t row,
@@ -76,7 +88,7 @@ size_t paged_workspace_bytes(const qwen_gpu_paged_cache& cache, const qwen_gpu_p
     (void)paged_view(cache, batch);
     check_heads(cache, query_heads);
     paged_check_rows(batch);
-    const AttentionPlan plan(cache, batch, query_heads);
+    const AttentionPlan plan = plan_of(cache, batch, query_heads);
     // Eviction: at most half of the longest sequence moves.
     const size_t lists = paged_moves_bytes(cache, batch, batch.max_length / 2);
     return std::max(plan.bytes(), kPagedCounterBytes + lists) + 16;
@@ -96,10 +108,7 @@ void launch_paged_attention(const qwen_gpu_paged_cache& cache, const qwen_gpu_pa
     require(query_stride >= row && out_stride >= row, "Paged rows overlap: stride below query_heads * head_dim");
     require(query_stride <= (int64_t(1) << 32) && out_stride <= (int64_t(1) << 32), "Paged row stride is too large");
     require(rows_apart(queries, query_stride, out, out_stride, row, batch.total_rows), "out overlaps other rows' queries");
-    const AttentionPlan plan(cache, batch, query_heads);
-    require(plan.blocks < (int64_t(1) << 31) && plan.columns < (int64_t(1) << 23) && plan.grid_rows <= 65535 &&
-                plan.score_rows < (int64_t(1) << 31),
-            "Too many new rows or positions for one call");
+    const AttentionPlan plan = plan_of(cache, batch, query_heads);
     const PagedDevice device(cache, batch, stream);
     device.check(queries, "queries");
     device.check(out, "out");

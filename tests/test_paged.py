@@ -150,6 +150,18 @@ def test_sizes_refused_that_no_launch_holds(qpkg):
             batch(qpkg, offsets=AT, total_rows=1 << 23), op='append', k_stride=1 << 13, v_stride=1 << 13)
 
 
+def test_workspace_of_calls_that_no_launch_holds(qpkg):
+    """The size of a call that would be refused is an error as well, and no number that has wrapped around."""
+    lib, size = qpkg.load_library(), ctypes.c_size_t()
+    long = dict(table_stride=1 << 20, max_length=1 << 24, track_stride=1 << 24)
+    for c, b, heads in ((cache(qpkg), batch(qpkg, sequences=4096, total_rows=4096, **long), 16),
+                        (cache(qpkg), batch(qpkg, sequences=1, rows=1 << 24, total_rows=1 << 24, **long), 8192),
+                        (cache(qpkg, kv_heads=1024, page_stride=1024 * 16 * 128),
+                         batch(qpkg, sequences=1, rows=1 << 24, total_rows=1 << 24, **long), 1 << 20)):
+        assert lib.qwen_gpu_op_paged_workspace(c, b, heads, ctypes.byref(size)) == 1
+        assert 'Too many new rows or positions' in lib.qwen_gpu_last_error().decode() and size.value == 0
+
+
 def test_evict_needs_what_it_goes_by(qpkg):
     refused(qpkg, 'Null argument: weights', b=batch(qpkg, weights=None), op='evict')
     refused(qpkg, 'Null argument: positions', b=batch(qpkg, positions=None), op='evict')
