@@ -734,7 +734,7 @@ class PagedKV:
         and positions are changed in place). Pages behind the new lengths are
         the caller's again."""
         batch, held = self._batch(self.lengths, self.seen, self._counts, 1, 0)
-        space, lengths = self._space(batch, self.kv_heads), DeviceBuffer(self.lengths.nbytes)
+        space, lengths = self._space(batch, 0), DeviceBuffer(self.lengths.nbytes)
         _check(_LIB.qwen_gpu_op_paged_evict(ctypes.byref(self._cache), ctypes.byref(batch), keep, sinks, recent,
                                             lengths.ptr, batch.weights, batch.positions, space.ptr, space.nbytes,
                                             None))

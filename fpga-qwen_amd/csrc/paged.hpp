@@ -19,7 +19,7 @@ void launch_paged_attention(const qwen_gpu_paged_cache& cache, const qwen_gpu_pa
 void launch_paged_evict(const qwen_gpu_paged_cache& cache, const qwen_gpu_paged_batch& batch, int keep, int sinks,
                         int recent, int32_t* new_lengths, float* new_weights, int32_t* new_positions, void* workspace,
                         size_t workspace_bytes, hipStream_t stream);
-// Bytes of workspace that serve both the attention and the eviction.
+// Bytes of workspace that serve both the attention and the eviction, without query heads the eviction alone.
 size_t paged_workspace_bytes(const qwen_gpu_paged_cache& cache, const qwen_gpu_paged_batch& batch, int query_heads);
 
 }  // namespace qwen_hip

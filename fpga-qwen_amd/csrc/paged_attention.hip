@@ -86,12 +86,12 @@ bool rows_apart(const float* queries, int64_t query_stride, const float* out, in
 
 size_t paged_workspace_bytes(const qwen_gpu_paged_cache& cache, const qwen_gpu_paged_batch& batch, int query_heads) {
     (void)paged_view(cache, batch);
+    // Eviction: at most half of the longest sequence moves.
+    const size_t lists = kPagedCounterBytes + paged_moves_bytes(cache, batch, batch.max_length / 2) + 16;
+    if (!query_heads) return lists;
     check_heads(cache, query_heads);
     paged_check_rows(batch);
-    const AttentionPlan plan = plan_of(cache, batch, query_heads);
-    // Eviction: at most half of the longest sequence moves.
-    const size_t lists = paged_moves_bytes(cache, batch, batch.max_length / 2);
-    return std::max(plan.bytes(), kPagedCounterBytes + lists) + 16;
+    return std::max(plan_of(cache, batch, query_heads).bytes() + 16, lists);
 }
 
 void launch_paged_attention(const qwen_gpu_paged_cache& cache, const qwen_gpu_paged_batch& batch, const float* queries,

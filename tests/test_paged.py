@@ -150,6 +150,16 @@ def test_sizes_refused_that_no_launch_holds(qpkg):
             batch(qpkg, offsets=AT, total_rows=1 << 23), op='append', k_stride=1 << 13, v_stride=1 << 13)
 
 
+def test_workspace_of_the_eviction_alone(qpkg):
+    """Without query heads: no scores of rows that are not attended, and no rows needed."""
+    lib, size = qpkg.load_library(), ctypes.c_size_t()
+    evicts = dict(sequences=64, rows=0, total_rows=0, table_stride=512, max_length=8192, track_stride=8192)
+    assert lib.qwen_gpu_op_paged_workspace(cache(qpkg), batch(qpkg, **evicts), 0, ctypes.byref(size)) == 0
+    assert size.value == 131072 + 64 * 8 * (2 * 4096 + 4) * 4 + 16
+    assert lib.qwen_gpu_op_paged_workspace(cache(qpkg), batch(qpkg, **evicts), 16, ctypes.byref(size)) == 1
+    assert 'rows must be' in lib.qwen_gpu_last_error().decode()
+
+
 def test_workspace_of_calls_that_no_launch_holds(qpkg):
     """The size of a call that would be refused is an error as well, and no number that has wrapped around."""
     lib, size = qpkg.load_library(), ctypes.c_size_t()
