@@ -674,7 +674,7 @@ class PagedKV:
         batch = PagedBatch(held[0].ptr, held[1].ptr, held[2].ptr, held[3].ptr,
                            self._weights.ptr if self._weights else None,
                            self._positions.ptr if self._positions else None, self._slots, lengths.size,
-                           self.table.shape[1], self._slots, rows, total)
+                           self.table.shape[1], min(self._slots, max(1, int(lengths.max()))), rows, total)
         return batch, held
 
     def _space(self, batch, query_heads):

@@ -379,3 +379,17 @@ def test_workspace_of_tracked_calls_goes_by_the_new_rows(qpkg, sequences, rows, 
     fixed, lists, partials = 131072 + 32, sequences * 8 * (4001 + 4) * 4, 4 * 512 * 16 * (128 + 4) * 4
     scores = total * 16 * (4032 * 4 + 8)
     assert scores < size.value <= fixed + max(lists, partials + scores)
+
+
+def test_wrapper_calls_go_by_the_lengths(paged):
+    """The workspace grows with the longest sequence, not with what the table has room for (64 slots)."""
+    cache, library = paged
+    cache.append(new(5), new(5), [4, 1])
+    cache.attention(np.zeros((5, 2, 64), np.float32))
+    cache.evict(3)
+    assert {name for name, *_ in library.calls} == {'qwen_gpu_op_paged_append', 'qwen_gpu_op_paged_workspace',
+                                                    'qwen_gpu_op_paged_attention', 'qwen_gpu_op_paged_evict'}
+    assert [call[3] for call in library.calls] == [4] * 5
+    cache.lengths = np.array([0, 0], np.int32)
+    cache.evict(3)
+    assert library.calls[-1][3] == 1
