@@ -52,6 +52,7 @@ class PagedBatch(ctypes.Structure):
 
 
 PAGED_TYPES = {'f16': 0, 'bf16': 1, 'e4m3': 2}
+PAGED_COUNTER_BYTES = 131072
 
 SIGNATURES = {
     'qwen_gpu_last_error': (ctypes.c_char_p, []),
@@ -682,7 +683,10 @@ class PagedKV:
         _check(_LIB.qwen_gpu_op_paged_workspace(ctypes.byref(self._cache), ctypes.byref(batch), query_heads,
                                                 ctypes.byref(need)))
         if self._workspace is None or self._workspace.nbytes < need.value:
-            self._workspace = DeviceBuffer.from_array(np.zeros(need.value, np.uint8))
+            self._workspace = None
+            space, front = DeviceBuffer(need.value), np.zeros(PAGED_COUNTER_BYTES, np.uint8)
+            _check(_LIB.qwen_gpu_memcpy_to_device(space.ptr, front.ctypes.data, front.nbytes))
+            self._workspace = space
         return self._workspace
 
     def append(self, keys, values, counts=None):

@@ -13,7 +13,7 @@ namespace qwen_hip {
 constexpr int kPagedF16 = QWEN_GPU_PAGED_F16, kPagedBF16 = QWEN_GPU_PAGED_BF16, kPagedE4M3 = QWEN_GPU_PAGED_E4M3;
 constexpr int kPagedMaxLength = 1 << 24;
 // The front of a workspace, zero between calls; the rest is any call's own.
-constexpr size_t kPagedCounterBytes = 131072;
+constexpr size_t kPagedCounterBytes = QWEN_GPU_PAGED_COUNTER_BYTES;
 
 // Slot j of a sequence is slot j % page_size of its page j / page_size. With
 // magic = floor((2^32 - 1) / page_size) the upper half of j * magic is the

@@ -334,11 +334,12 @@ typedef struct qwen_gpu_paged_batch {
 } qwen_gpu_paged_batch;
 
 /* Bytes of workspace (device memory, aligned to 16) that the attention and
- * the eviction of this cache and batch need at most. The caller zeroes it
- * once; every call leaves it ready for the next, of whatever shape it
- * suffices for. Calls that may overlap need workspaces of their own, and so
+ * the eviction of this cache and batch need at most. The caller zeroes its
+ * first QWEN_GPU_PAGED_COUNTER_BYTES once; every call leaves it ready for the
+ * next, of whatever shape it suffices for. Calls that may overlap need workspaces of their own, and so
  * do captured graphs that may. query_heads 0: what the eviction alone needs,
  * which does not use offsets, rows and total_rows. */
+#define QWEN_GPU_PAGED_COUNTER_BYTES 131072
 int qwen_gpu_op_paged_workspace(const qwen_gpu_paged_cache* cache, const qwen_gpu_paged_batch* batch, int query_heads,
                                 size_t* bytes);
 /* The new rows' keys and values, FP32, rounded to the cache's type (to

@@ -512,6 +512,34 @@ def test_workspace_serves_calls_of_different_shapes(qpkg):
         assert not space.to_array(np.uint8, 98304).any()
 
 
+def test_workspace_needs_its_counters_zeroed_and_nothing_else(qpkg):
+    """The rest may hold anything, and after each call all of the counters are 0."""
+    rng = np.random.default_rng(137)
+    for lengths, kv, heads, rows, dim in (([4000, 3], 2, 4, 1, 64), ([700] * 3, 1, 12, 40, 128), ([300] * 90, 16, 16, 1, 256),
+                                          ([17000] + [100] * 600, 1, 9, 1, 64)):
+        table, pages = make_table(rng, lengths, 16)
+        cache = ref.Cache('f16', pages, 16, kv, dim, rng=rng)
+        tracked = (len(lengths), kv, max(lengths))
+        weights, positions = rng.random(tracked).astype(np.float32), np.zeros(tracked, np.int32)
+        results = []
+        for fill in (0, 255):
+            call = Call(qpkg, cache, table, lengths, rows, weights=weights, positions=positions)
+            held = np.full(call.workspace(heads).nbytes, fill, np.uint8)
+            held[:qpkg.PAGED_COUNTER_BYTES] = 0
+            space = qpkg.DeviceBuffer.from_array(held)
+            queries = np.random.default_rng(139).standard_normal((call.total, heads * dim)).astype(np.float32)
+            results.append((call.attention(queries, heads, 0.125, np.zeros_like(queries), space),
+                            call.get('weights', weights)))
+            assert not space.to_array(np.uint8, qpkg.PAGED_COUNTER_BYTES).any()
+            n = qpkg.DeviceBuffer(4 * len(lengths))
+            call.check(call.lib.qwen_gpu_op_paged_evict(ctypes.byref(call.c), ctypes.byref(call.b), 100, 0, 1, n.ptr,
+                                                        call.b.weights, call.b.positions, space.ptr, space.nbytes, None))
+            qpkg.synchronize()
+            assert not space.to_array(np.uint8, qpkg.PAGED_COUNTER_BYTES).any()
+        for a, b in zip(*results):
+            assert np.isfinite(a).all() and np.array_equal(a, b)
+
+
 def test_attention_most_sequences(qpkg):
     rng = np.random.default_rng(97)
     lengths = [int(x) for x in rng.integers(0, 6, 4096)]

@@ -287,6 +287,10 @@ class Library:
             return int(self.fails)
         return call
 
+    def qwen_gpu_memcpy_to_device(self, to, host, nbytes):
+        self.copied = nbytes
+        return 0
+
     def qwen_gpu_last_error(self):
         return b'it fails'
 
@@ -393,3 +397,14 @@ def test_wrapper_calls_go_by_the_lengths(paged):
     cache.lengths = np.array([0, 0], np.int32)
     cache.evict(3)
     assert library.calls[-1][3] == 1
+
+
+def test_wrapper_zeroes_the_counters_alone(paged, qpkg):
+    """Not gigabytes of scores on the host."""
+    cache, library = paged
+    cache.append(new(5), new(5), [4, 1])
+    library.copied = 0
+    cache.attention(np.zeros((5, 2, 64), np.float32))
+    assert library.copied == qpkg.PAGED_COUNTER_BYTES
+    header = (Path(__file__).resolve().parents[1] / 'include' / 'qwen_gpu.h').read_text()
+    assert f'#define QWEN_GPU_PAGED_COUNTER_BYTES {qpkg.PAGED_COUNTER_BYTES}\n' in header
