@@ -600,6 +600,44 @@ def test_attention_joined_in_groups(qpkg, lengths, kv, heads, rows):
     attend(qpkg, cache, table, lengths, rows, heads, rng=rng)
 
 
+@pytest.mark.parametrize('kind', ['bf16', 'e4m3'])
+@pytest.mark.parametrize('lengths,kv,heads,rows', [([5000, 40], 2, 16, 2), ([4300], 1, 1, 1),
+                                                   ([17000] + [100] * 2000, 1, 9, 1)])
+def test_attention_of_other_types_joined_in_groups(qpkg, kind, lengths, kv, heads, rows):
+    rng = np.random.default_rng(83)
+    table, pages = make_table(rng, lengths, 64)
+    cache = ref.Cache(kind, pages, 64, kv, 64, rng=rng)
+    attend(qpkg, cache, table, lengths, rows, heads, rng=rng)
+
+
+@pytest.mark.parametrize('kind', ['f16', 'bf16', 'e4m3'])
+@pytest.mark.parametrize('tracked', [False, True])
+@pytest.mark.parametrize('dealt,lengths,counts,kv,group', [
+    ('1', [5000, 40], [1, 1], 1, 2),                             # 40 parts, joined in groups, tiles of 8 rows
+    ('1', [2600, 300], [2, 1], 1, 8),                            # 21 parts, tiles of 16 rows
+    ('1', [2600, 300], [2, 1], 1, 9),                            # two tiles
+    ('2', [9000, 7000, 50], [1, 2, 1], 3, 2),
+    ('4', [9000, 7000, 6000], [1, 1, 1], 5, 3),
+    ('runs', [2000, 0, 0, 128] + [17 * i % 290 for i in range(130)], [1] * 134, 8, 1),
+    ('runs', [17000] + [100] * 1000, [1] * 1001, 1, 2),          # a unit of many runs, joined in groups
+    ('both', [5300, 3300, 1300, 4500, 2500], [8, 7, 6, 5, 3], 1, 16)])
+def test_attention_deals_heads_of_256(qpkg, kind, tracked, dealt, lengths, counts, kv, group):
+    """Half as many workgroups as with smaller heads: parts of 1, 2 and 4 blocks, runs, and both in one call."""
+    rows, offsets = max(counts), np.concatenate(([0], np.cumsum(counts)))
+    tile = 8 if rows * group <= 8 else 16
+    tiles = -(-rows * group // tile)
+    blocks = [sum(max(1, -(-n // 128)) for n, c in zip(lengths, counts) if c * group > tile * t) * tiles * kv
+              for t in range(tiles)]
+    ways = ['1' if n <= 256 else '2' if n <= 512 else '4' if n <= 1024 else 'runs' for n in blocks]
+    assert ways[0] == dealt or (dealt == 'both' and ways[0] == 'runs' != ways[-1])
+    rng = np.random.default_rng(149)
+    table, pages = make_table(rng, lengths, 32)
+    cache = ref.Cache(kind, pages, 32, kv, 256, rng=rng)
+    weights = rng.random((len(lengths), kv, max(lengths))).astype(np.float32) if tracked else None
+    attend(qpkg, cache, table, lengths, rows, kv * group, offsets=offsets, total=sum(counts), rng=rng, weights=weights,
+           max_length=max(lengths))
+
+
 def test_attention_in_place_of_its_queries(qpkg):
     """out may be the queries' own memory."""
     rng = np.random.default_rng(79)
