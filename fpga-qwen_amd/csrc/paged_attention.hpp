@@ -63,9 +63,10 @@ struct AttentionArgs {
 // 4 blocks, whichever spreads all over as many workgroups as the GPU holds at
 // once. With more, that many workgroups take equal runs of blocks
 // in the order of a grid row's units, across their borders: with parts of units
-// the last round of workgroups left CUs idle (64 sequences of 1 to 4096
-// positions took 131 us, in runs 125); 768, 1024 and 1536 runs took 130, 124 and
-// 125 us, and for 64 equal sequences 120, 103 and 116 us where 512 take 95.
+// the last round of workgroups left CUs idle (5% for 64 sequences of 1 to 4096
+// positions, BF16). With 768, 1024 and 1536 runs these take 120, 114 and 116 us
+// where 512 take 110, and 64 equal ones of 2048 (FP16) 118, 104 and 111 where
+// 512 take 96.
 // Ragged new rows leave a head's later tiles fewer units, so that some rows of a
 // grid may take runs and others parts: a row's counters and partials lie at the
 // same place for both.
@@ -268,15 +269,17 @@ __device__ __forceinline__ float4_t multiply(uint4_t a, uint4_t b, float4_t c, s
                                                    0, 0);
 }
 
-// FP32 values as sums of 16-bit ones, for products on the matrix cores: two
-// FP16 terms hold 22 bits, three BF16 terms 24 (two, 2^-17 off, would lose ten
-// times what the sums do). A product has 16 columns. Up to 8 query rows are
+// FP32 values as sums of 16-bit ones, for products on the matrix cores: three
+// BF16 terms hold them (two, 2^-17 off, would lose ten times what the sums do),
+// two FP16 terms all but a quarter of them, which are one unit of FP32's last
+// place off, as after one addition (with a third one 8 sequences of 2048 are as
+// far from 64 bits, 4.6e-7, and take 18.4 us instead of 17.8). A product has 16 columns. Up to 8 query rows are
 // packed: columns 0-7 take the first term and 8-15 the second, the halves of
 // the result are added, and a third term takes a second product with columns
 // 8-15 empty. More rows take a column each and a product for every term (16
 // rows as two packed tiles took 132 us for 16 sequences of 8192, so 105; BF16
 // 172 and 105). E4M3 rows become BF16 as they are read, with their power of
-// two: exact.
+// two: exact, but that of what lies below 2^-126 multiples of 2^-133 are left.
 template <int TYPE, bool PACKED>
 struct Terms {
     static constexpr int kTerms = TYPE == kPagedF16 ? 2 : 3, kProducts = PACKED ? kTerms - 1 : kTerms;
@@ -370,9 +373,9 @@ __device__ __forceinline__ float add_halves(float x) {
 // time: keys are loaded again as soon as the scores have been multiplied, values
 // as soon as they are in LDS, and a step's table entries ahead of the values
 // before it, so that no wait for one covers the other. 64 sequences of 2048
-// positions (FP16, 537 MB) take 97 us, 5.5 TB/s, where a copy of 1 GiB runs at
-// 5.1; 200 VGPRs and more leave two waves a SIMD (three, with 47 to 94 spilled
-// registers, took 157 us and more for 64 ragged sequences instead of 119).
+// positions (FP16, 537 MB) take 96 us, 5.6 TB/s, where a copy of 1 GiB runs at
+// 5.1; 200 VGPRs and more leave two waves a SIMD (three, with 107 spilled
+// registers and 768 runs, take 201 us for 64 ragged BF16 sequences instead of 110).
 // Latency bounds short ones: 300 positions take 9 us in the kernel, 1.3 to find
 // the share, 2.2 for the table and the first rows behind it, 1.2 for a step, 1.7
 // for the waves' sums, 2 for the last workgroup to add the parts.

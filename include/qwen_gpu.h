@@ -336,9 +336,12 @@ typedef struct qwen_gpu_paged_batch {
 /* Bytes of workspace (device memory, aligned to 16) that the attention and
  * the eviction of this cache and batch need at most. The caller zeroes its
  * first QWEN_GPU_PAGED_COUNTER_BYTES once; every call leaves it ready for the
- * next, of whatever shape it suffices for. Calls that may overlap need workspaces of their own, and so
- * do captured graphs that may. query_heads 0: what the eviction alone needs,
- * which does not use offsets, rows and total_rows. */
+ * next, of whatever shape it suffices for. Calls that may overlap need
+ * workspaces of their own, and so do captured graphs that may. query_heads 0:
+ * what the eviction alone needs, which does not use offsets, rows and
+ * total_rows. Of the attention of tracked weights it holds 4 bytes for each
+ * new row, query head and position up to max_length: long prompts are best
+ * given in parts, whose weights add up. */
 #define QWEN_GPU_PAGED_COUNTER_BYTES 131072
 int qwen_gpu_op_paged_workspace(const qwen_gpu_paged_cache* cache, const qwen_gpu_paged_batch* batch, int query_heads,
                                 size_t* bytes);
@@ -348,8 +351,11 @@ int qwen_gpu_op_paged_workspace(const qwen_gpu_paged_cache* cache, const qwen_gp
  * r * key_stride + h * head_dim, so a projection's rows are read where they
  * are. E4M3: the exponent is the smallest of -126 .. 127 that brings the
  * row's largest finite magnitude to 448 or below; infinities and NaN become
- * NaN. Where tracked, the slots' weights are set to 0 and their positions to
- * seen[s] - n + i. No two rows of a call may go to one slot. */
+ * NaN. As any rounding may, that of the largest numbers can pass the type's
+ * (FP16 from 65520 on) or FP32's (248 * 2^120 and more in E4M3 become 2^128):
+ * attention takes such elements as infinite. Where tracked, the slots'
+ * weights are set to 0 and their positions to seen[s] - n + i. No two rows of
+ * a call may go to one slot. */
 int qwen_gpu_op_paged_append(const qwen_gpu_paged_cache* cache, const qwen_gpu_paged_batch* batch, const float* keys,
                              int64_t key_stride, const float* values, int64_t value_stride, void* stream);
 /* Attention of the new rows over the cached ones, which hold the new ones
@@ -361,9 +367,11 @@ int qwen_gpu_op_paged_append(const qwen_gpu_paged_cache* cache, const qwen_gpu_p
  * softmax weights over h's query heads and s's new rows. Sums are FP32, in
  * an order that depends on the call's shapes and lengths alone. Keys and
  * values that a row attends are finite (else its output may be NaN); those
- * that it does not attend may be anything. out may be queries themselves,
- * with one stride, and lies apart from them otherwise. query_heads is at most 1024 * kv_heads; scale, and scale
- * times log2(e), are finite. */
+ * that it does not attend may be anything. q . k, with and without the scale,
+ * and 256 times the sum of the attended values' magnitudes stay below 2^128
+ * (an FP16 cache's values do). out may be queries themselves, with one
+ * stride, and lies apart from them otherwise. query_heads is at most 1024 *
+ * kv_heads; scale, and scale times log2(e), are finite. */
 int qwen_gpu_op_paged_attention(const qwen_gpu_paged_cache* cache, const qwen_gpu_paged_batch* batch,
                                 const float* queries, int64_t query_stride, int query_heads, float scale, float* out,
                                 int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
