@@ -51,8 +51,50 @@ class PagedBatch(ctypes.Structure):
                 ('max_length', ctypes.c_int), ('rows', ctypes.c_int), ('total_rows', ctypes.c_int)]
 
 
+class PagedPool(ctypes.Structure):
+    """qwen_gpu_paged_pool: the pages of a cache's sequences, and the free ones."""
+    _fields_ = [('table', ctypes.c_void_p), ('free_pages', ctypes.c_void_p), ('held', ctypes.c_void_p),
+                ('free_count', ctypes.c_void_p), ('shared', ctypes.c_void_p), ('pages', ctypes.c_int),
+                ('page_size', ctypes.c_int), ('sequences', ctypes.c_int), ('table_stride', ctypes.c_int)]
+
+
+class PagedGrowth(ctypes.Structure):
+    """qwen_gpu_paged_growth: what a step adds to a cache's sequences and takes from them."""
+    _fields_ = [('lengths', ctypes.c_void_p), ('seen', ctypes.c_void_p), ('changes', ctypes.c_void_p),
+                ('new_lengths', ctypes.c_void_p), ('new_seen', ctypes.c_void_p), ('new_held', ctypes.c_void_p),
+                ('new_free_count', ctypes.c_void_p), ('offsets', ctypes.c_void_p),
+                ('row_sequences', ctypes.c_void_p), ('row_positions', ctypes.c_void_p),
+                ('row_slots', ctypes.c_void_p), ('total_rows', ctypes.c_int)]
+
+
+class Rotary(ctypes.Structure):
+    """qwen_gpu_rotary: how heads are normed and turned."""
+    _fields_ = [('frequencies', ctypes.c_void_p), ('dims', ctypes.c_int), ('layout', ctypes.c_int),
+                ('head_dim', ctypes.c_int), ('type', ctypes.c_int), ('magnitude', ctypes.c_float),
+                ('epsilon', ctypes.c_float)]
+
+
+class RotaryHeads(ctypes.Structure):
+    """qwen_gpu_rotary_heads: where a call's heads lie (strides in elements)."""
+    _fields_ = [('rows', ctypes.c_void_p), ('out', ctypes.c_void_p), ('norm', ctypes.c_void_p),
+                ('row_stride', ctypes.c_int64), ('head_stride', ctypes.c_int64), ('out_row_stride', ctypes.c_int64),
+                ('out_head_stride', ctypes.c_int64), ('heads', ctypes.c_int)]
+
+
+class Draft(ctypes.Structure):
+    """qwen_gpu_draft: drafted tokens and the logits that judge them."""
+    _fields_ = [('logits', ctypes.c_void_p), ('draft', ctypes.c_void_p), ('tokens', ctypes.c_void_p),
+                ('offsets', ctypes.c_void_p), ('temperature', ctypes.c_void_p), ('accept', ctypes.c_void_p),
+                ('sample', ctypes.c_void_p), ('logit_stride', ctypes.c_int64), ('draft_stride', ctypes.c_int64),
+                ('type', ctypes.c_int), ('vocabulary', ctypes.c_int), ('sequences', ctypes.c_int),
+                ('rows', ctypes.c_int), ('total_rows', ctypes.c_int)]
+
+
 PAGED_TYPES = {'f16': 0, 'bf16': 1, 'e4m3': 2}
 PAGED_COUNTER_BYTES = 131072
+TYPES = {'f32': 0, 'f16': 1, 'bf16': 2}
+ROTARY_LAYOUTS = {'halves': 0, 'interleaved': 1}
+ROTARY_SCALINGS = {'plain': 0, 'linear': 1, 'base': 2, 'ramp': 3}
 
 SIGNATURES = {
     'qwen_gpu_last_error': (ctypes.c_char_p, []),
@@ -128,6 +170,16 @@ SIGNATURES = {
     'qwen_gpu_op_paged_evict': (ctypes.c_int, [ctypes.POINTER(PagedCache), ctypes.POINTER(PagedBatch), ctypes.c_int,
                                                ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p,
                                                ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    'qwen_gpu_op_paged_reserve': (ctypes.c_int, [ctypes.POINTER(PagedPool), ctypes.POINTER(PagedGrowth),
+                                                 ctypes.c_void_p]),
+    'qwen_gpu_rotary_frequencies': (ctypes.c_int, [ctypes.c_int, ctypes.c_int] + [ctypes.c_double] * 5 +
+                                    [ctypes.POINTER(ctypes.c_double), _c_float_p]),
+    'qwen_gpu_op_rotate': (ctypes.c_int, [ctypes.POINTER(Rotary), ctypes.POINTER(RotaryHeads),
+                                          ctypes.POINTER(RotaryHeads), ctypes.c_void_p, ctypes.c_int,
+                                          ctypes.c_void_p]),
+    'qwen_gpu_op_verify_workspace': (ctypes.c_int, [ctypes.POINTER(Draft), _c_size_p]),
+    'qwen_gpu_op_verify_draft': (ctypes.c_int, [ctypes.POINTER(Draft), ctypes.c_void_p, ctypes.c_void_p,
+                                                ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     'qwen_gpu_time_kernel': (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, _c_float_p]),
 }
 
@@ -759,3 +811,148 @@ class PagedKV:
 
     def positions(self):
         return self._tracked(self._positions, np.int32)
+
+
+# ---- what a step needs around a paged cache, NumPy in and out ----
+
+def _ints(values, shape, name):
+    values = np.ascontiguousarray(values, np.int32)
+    if values.shape != shape:
+        raise ValueError(f'{name} must have shape {shape}, got {values.shape}')
+    return values
+
+
+def _optional(array):
+    return DeviceBuffer.from_array(array) if array is not None else None
+
+
+def _at(buffer):
+    return buffer.ptr if buffer is not None else None
+
+
+def paged_reserve(table, held, free, lengths, changes, page_size, pages, room, seen=None, shared=None):
+    """One step's pages and rows (qwen_gpu_op_paged_reserve): table [sequences,
+    max_pages], held, lengths, changes [sequences], free: the free pages, the
+    next one last, of `pages` in all; room: most new rows of the call. Returns
+    a dictionary of table, held, free, lengths, seen, offsets, and of the rows
+    granted sequences, positions and slots [room] (-1 behind the last)."""
+    table = np.ascontiguousarray(table, np.int32)
+    if table.ndim != 2 or not table.size:
+        raise ValueError(f'table must be [sequences, max_pages], got {table.shape}')
+    n = table.shape[0]
+    free = np.ascontiguousarray(free, np.int32)
+    if free.ndim != 1 or free.size > pages:
+        raise ValueError(f'free must hold at most {pages} pages, got {free.shape}')
+    if room < 0:
+        raise ValueError('room must not be below 0')
+    stack = np.full(max(1, pages), -1, np.int32)
+    stack[:free.size] = free
+    arrays = {'table': table, 'stack': stack, 'held': _ints(held, (n,), 'held'),
+              'count': np.asarray([free.size], np.int32), 'lengths': _ints(lengths, (n,), 'lengths'),
+              'changes': _ints(changes, (n,), 'changes'), 'offsets': np.zeros(n + 1, np.int32)}
+    if seen is not None:
+        arrays['seen'] = _ints(seen, (n,), 'seen')
+    if shared is not None:
+        arrays['shared'] = _ints(shared, (n,), 'shared')
+    if room:
+        arrays.update(sequences=np.full(room, -1, np.int32), positions=np.full(room, -1, np.int32),
+                      slots=np.full(room, -1, np.int64))
+    on = {name: DeviceBuffer.from_array(array) for name, array in arrays.items()}
+    at = {name: _at(on.get(name)) for name in ('table', 'stack', 'held', 'count', 'shared', 'lengths', 'seen', 'changes',
+                                               'offsets', 'sequences', 'positions', 'slots')}
+    pool = PagedPool(at['table'], at['stack'], at['held'], at['count'], at['shared'], pages, page_size, n, table.shape[1])
+    growth = PagedGrowth(at['lengths'], at['seen'], at['changes'], at['lengths'], at['seen'], at['held'], at['count'],
+                         at['offsets'], at['sequences'], at['positions'], at['slots'], room)
+    _check(_LIB.qwen_gpu_op_paged_reserve(ctypes.byref(pool), ctypes.byref(growth), None))
+    synchronize()
+    result = {name: on[name].to_array(arrays[name].dtype, arrays[name].size).reshape(arrays[name].shape)
+              for name in arrays if name not in ('changes', 'shared')}
+    result['free'] = result.pop('stack')[:int(result.pop('count')[0])]
+    result.setdefault('seen', result['lengths'])
+    for name in ('sequences', 'positions', 'slots'):
+        result.setdefault(name, np.zeros(0, np.int64 if name == 'slots' else np.int32))
+    return result
+
+
+def rotary_frequencies(dims, base=1e6, scaling='plain', factor=1.0, trained=0.0, slow=1.0, fast=32.0):
+    """(frequencies [dims / 2] in radians a position, magnitude) of a rotation
+    (qwen_gpu_rotary_frequencies): 'plain', 'linear', 'base' or 'ramp'."""
+    if scaling not in ROTARY_SCALINGS:
+        raise ValueError(f'scaling must be one of {", ".join(ROTARY_SCALINGS)}, got {scaling!r}')
+    frequencies, magnitude = np.zeros(max(0, int(dims)) // 2 + 1, np.float64), ctypes.c_float()
+    _check(_LIB.qwen_gpu_rotary_frequencies(ROTARY_SCALINGS[scaling], int(dims), float(base), float(factor),
+                                            float(trained), float(slow), float(fast),
+                                            frequencies.ctypes.data_as(ctypes.POINTER(ctypes.c_double)),
+                                            ctypes.byref(magnitude)))
+    return frequencies[:-1].copy(), magnitude.value
+
+
+def rotate(queries, keys, positions, frequencies, layout='halves', magnitude=1.0, query_norm=None, key_norm=None,
+           epsilon=1e-6):
+    """Heads of queries [rows, heads, head_dim] and keys (or None), FP32,
+    normed where norms [head_dim] are given and their first 2 *
+    len(frequencies) channels turned by position * frequency
+    (qwen_gpu_op_rotate). Rows of negative positions stay as they are."""
+    if layout not in ROTARY_LAYOUTS:
+        raise ValueError(f'layout must be one of {", ".join(ROTARY_LAYOUTS)}, got {layout!r}')
+    sides = [np.ascontiguousarray(x, np.float32) for x in (queries, keys) if x is not None]
+    if any(x.ndim != 3 or x.shape[0] != sides[0].shape[0] or x.shape[2] != sides[0].shape[2] or not x.shape[1]
+           for x in sides):
+        raise ValueError(f'queries and keys must be [rows, heads, head_dim], got {[x.shape for x in sides]}')
+    rows, _, dim = sides[0].shape
+    positions = _ints(positions, (rows,), 'positions')
+    frequencies = np.ascontiguousarray(frequencies, np.float64)
+    if frequencies.ndim != 1:
+        raise ValueError(f'frequencies must be a vector, got {frequencies.shape}')
+    norms = [_vector(x, dim, 'norm') if x is not None else None for x in (query_norm, key_norm)]
+    if not rows:
+        return sides[0], sides[1] if keys is not None else None
+    on, at, turns = [DeviceBuffer.from_array(x) for x in sides], DeviceBuffer.from_array(positions), None
+    if frequencies.size:
+        turns = DeviceBuffer.from_array(frequencies)
+    rotary = Rotary(_at(turns), 2 * frequencies.size, ROTARY_LAYOUTS[layout], dim, TYPES['f32'], magnitude, epsilon)
+    heads = [RotaryHeads(b.ptr, b.ptr, _at(norm), x.shape[1] * dim, dim, x.shape[1] * dim, dim, x.shape[1])
+             for b, x, norm in zip(on, sides, norms)]
+    _check(_LIB.qwen_gpu_op_rotate(ctypes.byref(rotary), ctypes.byref(heads[0]),
+                                   ctypes.byref(heads[1]) if keys is not None else None, at.ptr, rows, None))
+    synchronize()
+    out = [b.to_array(np.float32, x.size).reshape(x.shape) for b, x in zip(on, sides)]
+    return out[0], out[1] if keys is not None else None
+
+
+def verify_draft(logits, tokens, accept, sample, draft=None, counts=None, temperature=None):
+    """Drafted tokens against the target's probabilities
+    (qwen_gpu_op_verify_draft): logits FP32 [rows, vocabulary], tokens and
+    accept [rows], sample [sequences], draft [rows, vocabulary] or None;
+    counts: rows of each sequence (None: the same of all). Returns (accepted,
+    next), [sequences] each."""
+    logits = np.ascontiguousarray(logits, np.float32)
+    sample = np.ascontiguousarray(sample, np.float32)
+    if logits.ndim != 2 or not logits.size or sample.ndim != 1 or not sample.size:
+        raise ValueError(f'need logits [rows, vocabulary] and sample [sequences], got {logits.shape} and {sample.shape}')
+    total, n = logits.shape[0], sample.size
+    tokens, offsets = _ints(tokens, (total,), 'tokens'), None
+    if counts is not None:
+        counts = _ints(counts, (n,), 'counts')
+        if (counts < 0).any() or int(counts.sum()) != total:
+            raise ValueError(f'counts must add up to {total} rows')
+        offsets = np.concatenate(([0], np.cumsum(counts))).astype(np.int32)
+    elif total % n:
+        raise ValueError(f'{total} rows are no equal parts of {n} sequences')
+    rows = max(1, int(counts.max())) if counts is not None else total // n
+    if draft is not None:
+        draft = np.ascontiguousarray(draft, np.float32)
+        if draft.shape != logits.shape:
+            raise ValueError(f'draft must have shape {logits.shape}, got {draft.shape}')
+    on = [DeviceBuffer.from_array(logits), _optional(draft), DeviceBuffer.from_array(tokens), _optional(offsets),
+          _vector(temperature, n, 'temperature') if temperature is not None else None, _vector(accept, total, 'accept'),
+          DeviceBuffer.from_array(sample)]
+    width = logits.shape[1]
+    batch = Draft(*map(_at, on), width, width, TYPES['f32'], width, n, rows, total)
+    need = ctypes.c_size_t()
+    _check(_LIB.qwen_gpu_op_verify_workspace(ctypes.byref(batch), ctypes.byref(need)))
+    space, accepted, following = DeviceBuffer(need.value), DeviceBuffer(4 * n), DeviceBuffer(4 * n)
+    _check(_LIB.qwen_gpu_op_verify_draft(ctypes.byref(batch), accepted.ptr, following.ptr, None, space.ptr, space.nbytes,
+                                         None))
+    synchronize()
+    return accepted.to_array(np.int32, n), following.to_array(np.int32, n)

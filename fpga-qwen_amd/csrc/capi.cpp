@@ -8,6 +8,9 @@
 #include "pack.hpp"
 #include "paged.hpp"
 #include "prefill.hpp"
+#include "reserve.hpp"
+#include "rotate.hpp"
+#include "verify.hpp"
 
 struct qwen_gpu_model {
     qwen_hip::Engine engine;
@@ -513,6 +516,51 @@ int qwen_gpu_op_paged_evict(const qwen_gpu_paged_cache* cache, const qwen_gpu_pa
         need(batch, "batch");
         qwen_hip::launch_paged_evict(*cache, *batch, keep, sinks, recent, new_lengths, new_weights, new_positions,
                                      workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+        hip_ok(hipGetLastError());
+    });
+}
+
+int qwen_gpu_op_paged_reserve(const qwen_gpu_paged_pool* pool, const qwen_gpu_paged_growth* growth, void* stream) {
+    return guarded([&] {
+        need(pool, "pool");
+        need(growth, "growth");
+        qwen_hip::launch_paged_reserve(*pool, *growth, static_cast<hipStream_t>(stream));
+        hip_ok(hipGetLastError());
+    });
+}
+
+int qwen_gpu_rotary_frequencies(int scaling, int dims, double base, double factor, double trained, double slow,
+                                double fast, double* frequencies, float* magnitude) {
+    return guarded([&] {
+        qwen_hip::rotary_frequencies(scaling, dims, base, factor, trained, slow, fast, frequencies, magnitude);
+    });
+}
+
+int qwen_gpu_op_rotate(const qwen_gpu_rotary* rotary, const qwen_gpu_rotary_heads* queries,
+                       const qwen_gpu_rotary_heads* keys, const int32_t* positions, int rows, void* stream) {
+    return guarded([&] {
+        need(rotary, "rotary");
+        need(queries, "queries");
+        qwen_hip::launch_rotate(*rotary, *queries, keys, positions, rows, static_cast<hipStream_t>(stream));
+        hip_ok(hipGetLastError());
+    });
+}
+
+int qwen_gpu_op_verify_workspace(const qwen_gpu_draft* draft, size_t* bytes) {
+    return guarded([&] {
+        need(draft, "draft");
+        need(bytes, "bytes");
+        *bytes = 0;
+        *bytes = qwen_hip::verify_workspace_bytes(*draft);
+    });
+}
+
+int qwen_gpu_op_verify_draft(const qwen_gpu_draft* draft, int32_t* accepted, int32_t* next, int32_t* back,
+                             void* workspace, size_t workspace_bytes, void* stream) {
+    return guarded([&] {
+        need(draft, "draft");
+        qwen_hip::launch_verify_draft(*draft, accepted, next, back, workspace, workspace_bytes,
+                                      static_cast<hipStream_t>(stream));
         hip_ok(hipGetLastError());
     });
 }

@@ -13,9 +13,6 @@ namespace qwen_hip {
 namespace {
 constexpr int kEvictHead = 4;  // ints of a unit's moves before its lists
 
-void hip_check(hipError_t e) {
-    if (e != hipSuccess) throw std::runtime_error(std::string("HIP error: ") + hipGetErrorString(e));
-}
 void need(const void* p, const char* what) {
     if (!p) throw std::runtime_error(std::string("Null argument: ") + what);
 }
@@ -90,17 +87,8 @@ void paged_check_rows(const qwen_gpu_paged_batch& b) {
             "Paged total_rows must be sequences * rows without offsets");
 }
 
-PagedDevice::PagedDevice(const qwen_gpu_paged_cache& c, const qwen_gpu_paged_batch& b, hipStream_t stream) {
-    // The runtime's handles 1 and 2 stand for streams and point to none: asked for the device of 1, it ends the
-    // process.
-    require(stream != hipStreamLegacy && stream != hipStreamPerThread,
-            "The stream must be NULL or a stream that was created");
-    hipPointerAttribute_t a{};
-    if (hipPointerGetAttributes(&a, c.keys) != hipSuccess || a.type == hipMemoryTypeUnregistered) {
-        (void)hipGetLastError();
-        throw std::runtime_error("Not device memory: keys");
-    }
-    device_ = a.device;
+PagedDevice::PagedDevice(const qwen_gpu_paged_cache& c, const qwen_gpu_paged_batch& b, hipStream_t stream)
+    : OpDevice(c.keys, "keys", "the cache", stream) {
     check(c.keys, "keys", 16);
     check(c.values, "values", 16);
     if (c.type == kPagedE4M3) check(c.exponents, "exponents", 2);
@@ -110,30 +98,6 @@ PagedDevice::PagedDevice(const qwen_gpu_paged_cache& c, const qwen_gpu_paged_bat
     if (b.seen) check(b.seen, "seen");
     if (b.weights) check(b.weights, "weights");
     if (b.positions) check(b.positions, "positions");
-    hip_check(hipGetDevice(&before_));
-    if (stream) {
-        hipDevice_t of = 0;
-        hip_check(hipStreamGetDevice(stream, &of));
-        require(of == device_, "The stream belongs to another device than the cache");
-    }
-    if (before_ != device_) hip_check(hipSetDevice(device_));
-}
-
-PagedDevice::~PagedDevice() {
-    if (before_ != device_) (void)hipSetDevice(before_);
-}
-
-void PagedDevice::check(const void* p, const char* what, unsigned alignment) const {
-    need(p, what);
-    require(reinterpret_cast<uintptr_t>(p) % alignment == 0,
-            std::string("Not aligned to ") + std::to_string(alignment) + " bytes: " + what);
-    hipPointerAttribute_t a{};
-    if (hipPointerGetAttributes(&a, p) != hipSuccess || a.type == hipMemoryTypeUnregistered) {
-        (void)hipGetLastError();
-        throw std::runtime_error(std::string("Not device memory: ") + what);
-    }
-    require(a.type != hipMemoryTypeDevice || a.device == device_,
-            std::string("On another device than the cache: ") + what);
 }
 
 size_t paged_moves_bytes(const qwen_gpu_paged_cache& c, const qwen_gpu_paged_batch& b, int64_t room) {

@@ -6,6 +6,7 @@
 #include <cstdint>
 
 #include "half_split.hpp"
+#include "op_device.hpp"
 #include "qwen_gpu.h"
 
 namespace qwen_hip {
@@ -111,18 +112,10 @@ void paged_check_rows(const qwen_gpu_paged_batch& batch);
 // Workspace of an eviction that moves at most `room` rows of a head.
 size_t paged_moves_bytes(const qwen_gpu_paged_cache& cache, const qwen_gpu_paged_batch& batch, int64_t room);
 
-// Makes the device that holds the cache current for the rest of the scope.
-// Every pointer given is refused unless a kernel on that device can use it.
-class PagedDevice {
+// The device that holds the cache; all of a call's arrays are checked.
+class PagedDevice : public OpDevice {
 public:
     PagedDevice(const qwen_gpu_paged_cache& cache, const qwen_gpu_paged_batch& batch, hipStream_t stream);
-    ~PagedDevice();
-    PagedDevice(const PagedDevice&) = delete;
-    PagedDevice& operator=(const PagedDevice&) = delete;
-    void check(const void* pointer, const char* what, unsigned alignment = 4) const;
-
-private:
-    int device_ = 0, before_ = 0;
 };
 
 }  // namespace qwen_hip

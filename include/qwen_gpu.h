@@ -390,6 +390,166 @@ int qwen_gpu_op_paged_attention(const qwen_gpu_paged_cache* cache, const qwen_gp
 int qwen_gpu_op_paged_evict(const qwen_gpu_paged_cache* cache, const qwen_gpu_paged_batch* batch, int keep, int sinks,
                             int recent, int32_t* new_lengths, float* new_weights, int32_t* new_positions,
                             void* workspace, size_t workspace_bytes, void* stream);
+/* ---- Pages and rows of a step (no reference counterpart) ----
+ *
+ * Which pages a sequence has, kept on the device: the sequences' tables and a
+ * stack of the free pages, free_pages[0 .. free_count[0] - 1]. */
+typedef struct qwen_gpu_paged_pool {
+    int32_t* table;             /* [sequences][table_stride]; entries from held[s] on may hold anything */
+    int32_t* free_pages;        /* [pages] */
+    const int32_t* held;        /* [sequences]: pages in a sequence's row of the table */
+    const int32_t* free_count;  /* [1] */
+    const int32_t* shared;      /* [sequences]: its first pages, which others use too and are never given back; or NULL */
+    int pages;                  /* 1..2^30 */
+    int page_size;              /* 1..65536 */
+    int sequences;              /* 1..4096 */
+    int table_stride;           /* 1..2^24 */
+} qwen_gpu_paged_pool;
+
+typedef struct qwen_gpu_paged_growth {
+    const int32_t* lengths;     /* [sequences]: cached rows */
+    const int32_t* seen;        /* [sequences]: tokens of the text, evicted ones too; NULL: lengths, and no new_seen */
+    const int32_t* changes;     /* [sequences]: new rows wished for; below zero: cached rows taken back from the end */
+    int32_t* new_lengths;       /* [sequences] */
+    int32_t* new_seen;          /* [sequences], with seen */
+    int32_t* new_held;          /* [sequences] */
+    int32_t* new_free_count;    /* [1] */
+    int32_t* offsets;           /* [sequences + 1]: as a batch's, of the rows that were granted */
+    int32_t* row_sequences;     /* [total_rows] each, or NULL: of every row granted its sequence, */
+    int32_t* row_positions;     /*   its position in the text, */
+    int64_t* row_slots;         /*   and page * page_size + slot; -1 in all three behind the last row */
+    int total_rows;             /* 0..2^24: room for rows */
+} qwen_gpu_paged_growth;
+
+/* One step's bookkeeping. First, pages behind the wished lengths are given
+ * back: they are pushed on the free stack in the order of the sequences and
+ * of their tables. A call with changes of 0 gives back what an eviction has
+ * emptied. Then sequences get their new rows, in order: one that needs pages
+ * takes them from the stack's end, until one needs more than there are, and
+ * from there on only those that need none are granted; and no sequence
+ * whose rows, with those granted before, pass total_rows, nor any with new rows behind
+ * it. One that is not granted keeps its length and has no rows in `offsets`.
+ * A wish that the table has no entries for (length + change above
+ * table_stride * page_size) counts as a change of 0; a change never takes
+ * back more than there is. The lengths, seen, held and changes of one call
+ * are read before the results are written, so new_lengths may be lengths,
+ * new_seen seen, new_held held and new_free_count free_count; otherwise the
+ * arrays must not overlap. What the arrays hold is bounded: held into 0 ..
+ * table_stride, lengths into 0 .. table_stride * page_size (at most 2^30), free_count into 0
+ * .. pages; pages given back beyond `pages` free ones are dropped. Tables and
+ * slots of pages outside 0 .. pages - 1 (which only a wrong stack can hold)
+ * get -1 as their slots. Streams as for the paged cache; the device is that
+ * of `table`. */
+int qwen_gpu_op_paged_reserve(const qwen_gpu_paged_pool* pool, const qwen_gpu_paged_growth* growth, void* stream);
+
+/* ---- Norm and rotation of heads by position (no reference counterpart) ---- */
+#define QWEN_GPU_F32 0
+#define QWEN_GPU_F16 1
+#define QWEN_GPU_BF16 2
+#define QWEN_GPU_ROTARY_HALVES 0        /* channel i turns with channel i + dims / 2 */
+#define QWEN_GPU_ROTARY_INTERLEAVED 1   /* channel 2 i turns with channel 2 i + 1 */
+#define QWEN_GPU_ROTARY_PLAIN 0
+#define QWEN_GPU_ROTARY_LINEAR 1
+#define QWEN_GPU_ROTARY_BASE 2
+#define QWEN_GPU_ROTARY_RAMP 3
+
+typedef struct qwen_gpu_rotary {
+    const double* frequencies;  /* device, [dims / 2]: radians a position of pair i; may be NULL where dims is 0 */
+    int dims;                   /* even, 0..head_dim: the first channels of a head, which turn */
+    int layout;                 /* QWEN_GPU_ROTARY_HALVES or _INTERLEAVED */
+    int head_dim;               /* even, 2..512 */
+    int type;                   /* QWEN_GPU_F32, _F16 or _BF16: of the rows, read and written */
+    float magnitude;            /* the turned channels are multiplied by it: 1, or what scaled positions ask for */
+    float epsilon;              /* of the norm, above 0 */
+} qwen_gpu_rotary;
+
+/* Heads of a call's rows: channel d of head h of row r lies at r * row_stride
+ * + h * head_stride + d (elements; any alignment that the type has). */
+typedef struct qwen_gpu_rotary_heads {
+    const void* rows;
+    void* out;                  /* may be `rows` with its strides; otherwise apart from all heads that are read */
+    const float* norm;          /* device, [head_dim]: weights of the RMS norm of each head; NULL: no norm */
+    int64_t row_stride;
+    int64_t head_stride;
+    int64_t out_row_stride;
+    int64_t out_head_stride;
+    int heads;                  /* 1..4096 */
+} qwen_gpu_rotary_heads;
+
+/* Frequencies of `dims` turned channels (host memory, [dims / 2]) and the
+ * magnitude (NULL: not wanted) of a rotation with base `base`, f_i =
+ * base^(-2 i / dims), scaled for texts `factor` (1 or more) times as long as
+ * the `trained` positions:
+ * PLAIN   f_i (factor and trained are not used);
+ * LINEAR  f_i / factor, positions squeezed;
+ * BASE    the base raised to base * factor^(dims / (dims - 2)), which leaves
+ *         the first frequency and divides the last by factor;
+ * RAMP    f_i where pair i makes `fast` turns or more within the trained
+ *         positions, f_i / factor where it makes `slow` or fewer, in between
+ *         their mean weighted by where the turns lie between the two;
+ *         magnitude 0.1 ln(factor) + 1.
+ * The magnitude of the others is 1. */
+int qwen_gpu_rotary_frequencies(int scaling, int dims, double base, double factor, double trained, double slow,
+                                double fast, double* frequencies, float* magnitude);
+/* Every head of every row, normed (x / sqrt(mean x^2 + epsilon) * norm) and
+ * its first channels turned by the angle position * frequency: queries and
+ * keys (NULL: none) of up to 2^24 rows in one launch. Row r has
+ * positions[r] (device); rows of a negative position, such as those behind
+ * the last one in a map of qwen_gpu_op_paged_reserve, are neither read nor
+ * written. Angles are FP64, the rest FP32, rounded once to the rows' type;
+ * the sum of a normed head's squares stays below 2^128.
+ * The rotation multiplies (a, b) by magnitude * (cos, sin) as a cos - b sin,
+ * b cos + a sin. Streams as for the paged cache; the device is that of
+ * queries->out. */
+int qwen_gpu_op_rotate(const qwen_gpu_rotary* rotary, const qwen_gpu_rotary_heads* queries,
+                       const qwen_gpu_rotary_heads* keys, const int32_t* positions, int rows, void* stream);
+
+/* ---- Verification of drafted tokens (no reference counterpart) ----
+ *
+ * Sequence s has n rows of logits: row i is the target's for the token behind
+ * the row's own, so that row i of the first n - 1 judges the drafted token
+ * tokens[first + i + 1] and the last one is for the token after all drafts. A
+ * sequence of one row has no drafts: a token is drawn for it. */
+typedef struct qwen_gpu_draft {
+    const void* logits;         /* [total_rows] rows of `vocabulary`, logit_stride apart */
+    const float* draft;         /* [total_rows] rows of `vocabulary`, draft_stride apart: the probabilities that row
+                                 * i's drafted token was drawn from (last rows are not read); NULL: it was certain */
+    const int32_t* tokens;      /* [total_rows]: the rows' own tokens */
+    const int32_t* offsets;     /* [sequences + 1]: as a paged batch's; NULL: `rows` rows each */
+    const float* temperature;   /* [sequences], NULL: 1 */
+    const float* accept;        /* [total_rows]: numbers of [0, 1), one for each drafted token, at its judge's row */
+    const float* sample;        /* [sequences]: numbers of [0, 1), for the token that is drawn */
+    int64_t logit_stride;       /* elements */
+    int64_t draft_stride;
+    int type;                   /* of the logits: QWEN_GPU_F32, _F16 or _BF16 */
+    int vocabulary;             /* 1..2^24 */
+    int sequences;              /* 1..4096 */
+    int rows;                   /* 1..1024: most rows of a sequence */
+    int total_rows;             /* 0..2^20; sequences * rows where offsets is NULL */
+} qwen_gpu_draft;
+
+/* Bytes of workspace (device memory, aligned to 16); it needs no zeroing and keeps nothing between calls. */
+int qwen_gpu_op_verify_workspace(const qwen_gpu_draft* draft, size_t* bytes);
+/* With p = softmax(logits / temperature) of a row and q its draft's
+ * probabilities, the drafted token t is accepted where accept * q(t) < p(t).
+ * At the first one that is not, the token is drawn from max(p - q, 0)
+ * (from p, where that is 0 throughout), and where all are accepted, from the
+ * last row's p: the lowest token up to which the weights' sum passes sample
+ * times their whole sum. So the tokens follow the target's distribution
+ * whatever the draft's is. Temperatures of 0 and below (and NaN) stand for the
+ * limit: the largest logit, of equal ones the lowest token, has all of p.
+ * accepted[s] is the number of accepted tokens, next[s] the one drawn, back[s]
+ * accepted[s] less the drafted ones, the rows that a paged cache takes back
+ * (qwen_gpu_op_paged_reserve's changes); accepted and back may be NULL. What is left out by a
+ * filter has a logit of minus infinity; NaN counts as that, an infinite logit
+ * as all of p (shared by equal ones). Where a row has no token left, its
+ * drafted one is not accepted and next is -1, as it is for a sequence without rows. A drafted
+ * token outside the vocabulary is not accepted; probabilities below 0 and NaN
+ * count as 0. Weights and sums are FP64, summed in an order that depends on the
+ * vocabulary alone. Streams as for the paged cache; the device is that of
+ * `logits`. */
+int qwen_gpu_op_verify_draft(const qwen_gpu_draft* draft, int32_t* accepted, int32_t* next, int32_t* back,
+                             void* workspace, size_t workspace_bytes, void* stream);
 /* Average milliseconds of one standalone launch of a decode kernel on the
  * model's stream, timed with HIP events (which: 0 norm+QKV, 1 attention,
  * 2 O, 3 norm+gate/up, 4 down, 5 lm_head, 6 the fused FFN kernel and 7 the
