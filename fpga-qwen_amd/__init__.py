@@ -51,6 +51,12 @@ class PagedBatch(ctypes.Structure):
                 ('max_length', ctypes.c_int), ('rows', ctypes.c_int), ('total_rows', ctypes.c_int)]
 
 
+class PagedPrefix(ctypes.Structure):
+    """qwen_gpu_paged_prefix: groups of sequences that share their first positions."""
+    _fields_ = [('lengths', ctypes.c_void_p), ('offsets', ctypes.c_void_p), ('groups', ctypes.c_int),
+                ('max_length', ctypes.c_int), ('max_rest', ctypes.c_int)]
+
+
 class PagedPool(ctypes.Structure):
     """qwen_gpu_paged_pool: the pages of a cache's sequences, and the free ones."""
     _fields_ = [('table', ctypes.c_void_p), ('free_pages', ctypes.c_void_p), ('held', ctypes.c_void_p),
@@ -170,6 +176,13 @@ SIGNATURES = {
     'qwen_gpu_op_paged_evict': (ctypes.c_int, [ctypes.POINTER(PagedCache), ctypes.POINTER(PagedBatch), ctypes.c_int,
                                                ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p,
                                                ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    'qwen_gpu_op_paged_shared_workspace': (ctypes.c_int, [ctypes.POINTER(PagedCache), ctypes.POINTER(PagedBatch),
+                                                          ctypes.POINTER(PagedPrefix), ctypes.c_int, _c_size_p]),
+    'qwen_gpu_op_paged_attention_shared': (ctypes.c_int, [ctypes.POINTER(PagedCache), ctypes.POINTER(PagedBatch),
+                                                          ctypes.POINTER(PagedPrefix), ctypes.c_void_p,
+                                                          ctypes.c_int64, ctypes.c_int, ctypes.c_float,
+                                                          ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
+                                                          ctypes.c_size_t, ctypes.c_void_p]),
     'qwen_gpu_op_paged_reserve': (ctypes.c_int, [ctypes.POINTER(PagedPool), ctypes.POINTER(PagedGrowth),
                                                  ctypes.c_void_p]),
     'qwen_gpu_rotary_frequencies': (ctypes.c_int, [ctypes.c_int, ctypes.c_int] + [ctypes.c_double] * 5 +
@@ -781,6 +794,45 @@ class PagedKV:
         _check(_LIB.qwen_gpu_op_paged_attention(ctypes.byref(self._cache), ctypes.byref(batch), q.ptr, stride, heads,
                                                 self.head_dim ** -0.5 if scale is None else scale, out.ptr, stride,
                                                 space.ptr, space.nbytes, None))
+        synchronize()
+        del held
+        return out.to_array(np.float32, queries.size).reshape(queries.shape)
+
+    def attention_shared(self, queries, lengths, counts=None, scale=None):
+        """attention() of sequences that share prefixes: the first lengths[g]
+        positions of counts[g] sequences each, one group after the other
+        (None: one group of all), read once for a group. The same results;
+        a cache that tracks has no use for it."""
+        queries = np.ascontiguousarray(queries, np.float32)
+        total = int(self._counts.sum())
+        if queries.ndim != 3 or queries.shape[0] != total or queries.shape[2] != self.head_dim:
+            raise ValueError(f'queries must be [{total}, query_heads, {self.head_dim}], got {queries.shape}')
+        lengths = np.atleast_1d(np.array(lengths, np.int32))
+        counts = np.atleast_1d(np.array(self.lengths.size if counts is None else counts, np.int32))
+        if lengths.ndim != 1 or lengths.shape != counts.shape or (counts < 0).any() or \
+                int(counts.sum()) > self.lengths.size:
+            raise ValueError(f'need a length and a count for each group, of {self.lengths.size} sequences together')
+        if (lengths < 0).any():
+            raise ValueError('lengths must not be below 0')
+        if not total:
+            return np.zeros_like(queries)
+        heads, ends = queries.shape[1], np.concatenate(([0], np.cumsum(counts))).astype(np.int32)
+        batch, held = self._batch(self.lengths, self.seen, self._counts, int(self._counts.max()), total)
+        shared = np.zeros(self.lengths.size, np.int32)
+        for g in range(lengths.size):
+            shared[ends[g]:ends[g + 1]] = lengths[g]
+        rest = max(1, int((self.lengths - np.minimum(shared, self.lengths - self._counts)).max()))
+        held += [DeviceBuffer.from_array(lengths), DeviceBuffer.from_array(ends)]
+        prefix = PagedPrefix(held[-2].ptr, held[-1].ptr, lengths.size, min(batch.max_length, int(lengths.max())),
+                             min(batch.max_length, rest))
+        need = ctypes.c_size_t()
+        given = ctypes.byref(self._cache), ctypes.byref(batch), ctypes.byref(prefix)
+        _check(_LIB.qwen_gpu_op_paged_shared_workspace(*given, heads, ctypes.byref(need)))
+        space, q, out = DeviceBuffer(need.value), DeviceBuffer.from_array(queries), DeviceBuffer(queries.nbytes)
+        stride = heads * self.head_dim
+        _check(_LIB.qwen_gpu_op_paged_attention_shared(*given, q.ptr, stride, heads,
+                                                       self.head_dim ** -0.5 if scale is None else scale, out.ptr,
+                                                       stride, space.ptr, space.nbytes, None))
         synchronize()
         del held
         return out.to_array(np.float32, queries.size).reshape(queries.shape)

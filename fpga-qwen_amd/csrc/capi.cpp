@@ -520,6 +520,33 @@ int qwen_gpu_op_paged_evict(const qwen_gpu_paged_cache* cache, const qwen_gpu_pa
     });
 }
 
+int qwen_gpu_op_paged_shared_workspace(const qwen_gpu_paged_cache* cache, const qwen_gpu_paged_batch* batch,
+                                       const qwen_gpu_paged_prefix* prefix, int query_heads, size_t* bytes) {
+    return guarded([&] {
+        need(cache, "cache");
+        need(batch, "batch");
+        need(prefix, "prefix");
+        need(bytes, "bytes");
+        *bytes = 0;
+        *bytes = qwen_hip::paged_shared_workspace_bytes(*cache, *batch, *prefix, query_heads);
+    });
+}
+
+int qwen_gpu_op_paged_attention_shared(const qwen_gpu_paged_cache* cache, const qwen_gpu_paged_batch* batch,
+                                       const qwen_gpu_paged_prefix* prefix, const float* queries, int64_t query_stride,
+                                       int query_heads, float scale, float* out, int64_t out_stride, void* workspace,
+                                       size_t workspace_bytes, void* stream) {
+    return guarded([&] {
+        need(cache, "cache");
+        need(batch, "batch");
+        need(prefix, "prefix");
+        qwen_hip::launch_paged_attention_shared(*cache, *batch, *prefix, queries, query_stride, query_heads, scale, out,
+                                                out_stride, workspace, workspace_bytes,
+                                                static_cast<hipStream_t>(stream));
+        hip_ok(hipGetLastError());
+    });
+}
+
 int qwen_gpu_op_paged_reserve(const qwen_gpu_paged_pool* pool, const qwen_gpu_paged_growth* growth, void* stream) {
     return guarded([&] {
         need(pool, "pool");

@@ -87,6 +87,11 @@ void paged_check_rows(const qwen_gpu_paged_batch& b) {
             "Paged total_rows must be sequences * rows without offsets");
 }
 
+void paged_check_heads(const qwen_gpu_paged_cache& cache, int query_heads) {
+    require(query_heads >= cache.kv_heads && query_heads % cache.kv_heads == 0 && query_heads / cache.kv_heads <= 1024,
+            "query_heads must be a multiple of kv_heads, at most 1024 times");
+}
+
 PagedDevice::PagedDevice(const qwen_gpu_paged_cache& c, const qwen_gpu_paged_batch& b, hipStream_t stream)
     : OpDevice(c.keys, "keys", "the cache", stream) {
     check(c.keys, "keys", 16);
@@ -107,27 +112,6 @@ size_t paged_moves_bytes(const qwen_gpu_paged_cache& c, const qwen_gpu_paged_bat
 // ---- append ----
 
 namespace {
-
-// Sequence of a new row, -1 where it has none: the number of offsets up to
-// `row`, less one. The lanes of a wave probe 64 of them at a time.
-__device__ int sequence_of(const PagedView& v, int row, int lane) {
-    if (!v.offsets) return row / v.rows;
-    int low = 0, high = v.sequences + 1;  // the number lies in low .. high
-    while (high > low) {
-        const int step = (high - low + 63) / 64;
-        const int at = low + lane * step;
-        const unsigned long long upto = __ballot(at < high && v.offsets[min(at, v.sequences)] <= row);
-        const int n = __popcll(upto);  // offsets rise, so these are the first lanes
-        if (n == 0) {
-            high = low;
-        } else {
-            const int last = low + (n - 1) * step;  // offsets[last] <= row
-            high = min(high, last + step);
-            low = last + 1;
-        }
-    }
-    return low - 1 < v.sequences ? low - 1 : -1;
-}
 
 // The smallest exponent byte whose power of two brings `top` to 448 = 1.75 * 2^8
 // or below, and what the row's values are multiplied by. A power of two keeps
@@ -163,7 +147,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedView v, const fl
             for (int i = 0; i < 4; ++i) x[side][i] = a[i], x[side][4 + i] = b[i];
         }
     }
-    const int s = sequence_of(v, row, lane);
+    const int s = v.sequence_of(row, lane);
     if (s < 0) return;
     int first;
     const int n = v.new_rows(s, first), rank = row - first;

@@ -54,11 +54,6 @@ __global__ __launch_bounds__(256) void paged_track_kernel(PagedView v, Attention
     }
 }
 
-void check_heads(const qwen_gpu_paged_cache& cache, int query_heads) {
-    require(query_heads >= cache.kv_heads && query_heads % cache.kv_heads == 0 && query_heads / cache.kv_heads <= 1024,
-            "query_heads must be a multiple of kv_heads, at most 1024 times");
-}
-
 // The sizes of a call that a launch and 32-bit indices hold. A head's tiles have at most 16 query rows, so the first
 // check refuses no more than the second one would, and keeps the plan's products within 64 bits.
 AttentionPlan plan_of(const qwen_gpu_paged_cache& cache, const qwen_gpu_paged_batch& batch, int query_heads) {
@@ -89,7 +84,7 @@ size_t paged_workspace_bytes(const qwen_gpu_paged_cache& cache, const qwen_gpu_p
     // Eviction: at most half of the longest sequence moves.
     const size_t lists = kPagedCounterBytes + paged_moves_bytes(cache, batch, batch.max_length / 2) + 16;
     if (!query_heads) return lists;
-    check_heads(cache, query_heads);
+    paged_check_heads(cache, query_heads);
     paged_check_rows(batch);
     return std::max(plan_of(cache, batch, query_heads).bytes() + 16, lists);
 }
@@ -101,7 +96,7 @@ void launch_paged_attention(const qwen_gpu_paged_cache& cache, const qwen_gpu_pa
     paged_check_rows(batch);
     require(queries, "Null argument: queries");
     require(out, "Null argument: out");
-    check_heads(cache, query_heads);
+    paged_check_heads(cache, query_heads);
     const float scale_of_2 = scale * 1.44269504088896340736f;  // the kernels' exponentials are powers of 2
     require(std::isfinite(scale_of_2), "The scale must be finite, times log2(e) too");
     const int64_t row = int64_t(query_heads) * cache.head_dim;

@@ -62,6 +62,26 @@ struct PagedView {
         to = int(max(int64_t(0), min(int64_t(n), int64_t(total_rows) - first)));
         from = int(min(int64_t(to), max(int64_t(0), -int64_t(first))));
     }
+    // Sequence of a new row, -1 where it has none: the number of offsets up to
+    // `row`, less one. The lanes of a wave probe 64 of them at a time.
+    __device__ int sequence_of(int row, int lane) const {
+        if (!offsets) return row / rows;
+        int low = 0, high = sequences + 1;  // the number lies in low .. high
+        while (high > low) {
+            const int step = (high - low + 63) / 64;
+            const int at = low + lane * step;
+            const unsigned long long upto = __ballot(at < high && offsets[min(at, sequences)] <= row);
+            const int n = __popcll(upto);  // offsets rise, so these are the first lanes
+            if (n == 0) {
+                high = low;
+            } else {
+                const int last = low + (n - 1) * step;  // offsets[last] <= row
+                high = min(high, last + step);
+                low = last + 1;
+            }
+        }
+        return low - 1 < sequences ? low - 1 : -1;
+    }
     // Page of the table's entry, -1 where it holds none.
     __device__ int page_of(int s, int entry) const {
         const int page = table[int64_t(s) * table_stride + entry];
@@ -108,6 +128,7 @@ __device__ __forceinline__ int scan_lanes(int x) {
 // Host side: checks (std::runtime_error), the view, the device.
 PagedView paged_view(const qwen_gpu_paged_cache& cache, const qwen_gpu_paged_batch& batch);
 void paged_check_rows(const qwen_gpu_paged_batch& batch);
+void paged_check_heads(const qwen_gpu_paged_cache& cache, int query_heads);
 
 // Workspace of an eviction that moves at most `room` rows of a head.
 size_t paged_moves_bytes(const qwen_gpu_paged_cache& cache, const qwen_gpu_paged_batch& batch, int64_t room);

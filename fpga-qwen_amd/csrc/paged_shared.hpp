@@ -1,0 +1,607 @@
+// Attention of new rows over a paged key-value cache whose sequences share
+// prefixes: the kernel and its launch, included by one source for each type of
+// cache (they compile side by side).
+#pragma once
+#include <algorithm>
+
+#include "paged_attention.hpp"
+
+namespace qwen_hip {
+
+struct SharedArgs {
+    const float* queries;
+    int64_t query_stride;
+    float* out;
+    int64_t out_stride;
+    int group, query_heads;
+    unsigned magic;             // of the group
+    float scale;                // times log2(e)
+    const int32_t* lengths;     // of the prefixes
+    const int32_t* offsets;     // NULL: one group of all sequences
+    int groups;
+    int tiles, rest_tiles;      // of all groups' query rows at most, of a sequence's
+    int parts, rest_parts;      // of a prefix, of what is behind it, at most
+    int part, rest_part;        // positions of each
+    int jobs;                   // workgroups of the prefixes
+    float* sums;                // [parts + rest_parts][total_rows][query_heads][DIM]
+    float2* states;             // [parts + rest_parts][total_rows][query_heads]: reference, sum
+
+    __device__ __forceinline__ int new_row(int r) const { return page_slot(r, group, magic).page; }
+    __device__ __forceinline__ int64_t place(const PagedView& v, int slot, int row, int head) const {
+        return (int64_t(slot) * v.total_rows + row) * query_heads + head;
+    }
+    // Sequences of a group.
+    __device__ __forceinline__ int first_of(const PagedView& v, int g) const {
+        return offsets ? min(max(offsets[g], 0), v.sequences) : g ? v.sequences : 0;
+    }
+    // First new row of a sequence, which is the end of the one before.
+    __device__ __forceinline__ int row_of(const PagedView& v, int s) const {
+        return v.offsets ? min(max(v.offsets[s], 0), v.total_rows) : s * v.rows;
+    }
+    // Query rows of a KV head in a group.
+    __device__ __forceinline__ int rows_of(const PagedView& v, int g) const {
+        const int from = first_of(v, g), to = first_of(v, g + 1);
+        return to > from ? max(0, row_of(v, to) - row_of(v, from)) * group : 0;
+    }
+    // Group of a sequence, -1 where it has none; the same in all lanes.
+    __device__ __forceinline__ int group_of(const PagedView& v, int s, int lane) const {
+        if (!offsets) return 0;
+        int low = 0, high = groups;  // the number of groups that begin at s or before lies in low .. high
+        while (high > low) {
+            const int step = (high - low + 63) / 64, at = low + lane * step;
+            const int n = __popcll(__ballot(at < high && offsets[min(at, groups)] <= s));
+            if (n == 0) {
+                high = low;
+            } else {
+                const int last = low + (n - 1) * step;
+                high = min(high, last + step);
+                low = last + 1;
+            }
+        }
+        return low > 0 && s < offsets[low] ? low - 1 : -1;
+    }
+    // Positions that a group's sequences share, no more than any of them has before its new rows, and its first
+    // sequence with new rows, through whose table they are read.
+    __device__ __forceinline__ int prefix_of(const PagedView& v, int g, int lane, int& reads) const {
+        if (g < 0 || !jobs) return 0;  // no group, or none that has workgroups
+        const int from = first_of(v, g), to = first_of(v, g + 1);
+        int least = lengths[g];
+        reads = to;
+        for (int s = from + lane; s < to; s += 64) {
+            int first;
+            const int n = v.new_rows(s, first);
+            if (n > 0) least = min(least, v.length(s) - n), reads = min(reads, s);
+        }
+        for (int off = 1; off < 64; off *= 2) {
+            least = min(least, __shfl_xor(least, off));
+            reads = min(reads, __shfl_xor(reads, off));
+        }
+        reads = __builtin_amdgcn_readfirstlane(reads);
+        return max(0, __builtin_amdgcn_readfirstlane(least));
+    }
+    __device__ __forceinline__ static int parts_of(int positions, int part, int most) {
+        return min(most, (positions + part - 1) / part);
+    }
+};
+
+// Tiles of a wave behind the prefixes, where query rows are those of one sequence.
+__host__ __device__ constexpr int rest_tiles_of(int tiles) { return tiles < 2 ? tiles : 2; }
+
+// What a workgroup does: a tile of query rows of a KV head against a range of
+// a sequence's positions.
+struct SharedJob {
+    int head, s;              // whose table
+    int first, rows;          // new row of query row 0, query rows in all
+    int row0;                 // of the tile
+    int from, to;             // positions
+    int sees;                 // behind a prefix: positions that the first new row attends, one more each row
+    int slot;                 // of its sums
+};
+
+// LDS of a workgroup: a wave's values, then its sums.
+template <int DIM>
+struct SharedSpace {
+    static constexpr int kPitch = DIM * 2 + 32;  // bytes of a value row
+    __attribute__((aligned(16))) char rows[kWaves][kTile * kPitch];
+    float2 states[kWaves][16];
+};
+
+// S^T = K Q^T and O^T = V^T P^T on the matrix cores as paged_attention_kernel
+// has them (32 positions a wave's step, FP32 queries and weights as two FP16
+// or three BF16 terms), but with up to TILES times 16 query rows in a wave:
+// keys stay in registers and values in LDS while all tiles are multiplied by
+// them. A prefix's query rows are those of all new rows of its group, so its
+// positions are read once for TILES * 16 of them. CAUSAL: positions behind a
+// prefix, which end at each new row's own.
+template <int TYPE, int DIM, int TILES, bool CAUSAL>
+__device__ __forceinline__ void shared_attend(const PagedView& v, const SharedArgs& a, const SharedJob& job,
+                                              SharedSpace<DIM>& space) {
+    constexpr int kSize = TYPE == kPagedE4M3 ? 1 : 2, kLoads = DIM * kSize / 64, kSteps = DIM / 32, kOut = DIM / 16;
+    constexpr int kPer = kSteps / kLoads;         // products per load: 1, or 2 for E4M3
+    constexpr int kRows = 16 * TILES, kProducts = Terms<TYPE, false>::kProducts;
+    constexpr int kPitch = SharedSpace<DIM>::kPitch;
+    constexpr float kHead = TYPE == kPagedF16 ? 6.f : 0.f;  // FP16 weights are kept up to 2^14, far from subnormals
+    constexpr float kGrow = 8.f;                  // a reference is moved once a score passes it by 2^8
+    constexpr std::integral_constant<int, TYPE> kType{};
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int column = lane & 15, part = lane >> 4;
+    const int begin = job.from;
+    // Positions from shared_end on are seen by some of the tile's new rows only, from `end` on by none.
+    const int last_row = min(job.rows - 1, job.row0 + kRows - 1);
+    const int shared_end = CAUSAL ? min(job.to, job.sees + a.new_row(job.row0)) : job.to;
+    const int end = CAUSAL ? min(job.to, job.sees + a.new_row(last_row)) : job.to;
+    const int live_tiles = (last_row - job.row0) / 16 + 1;
+    const int32_t* const table = v.table + int64_t(job.s) * v.table_stride;
+
+    float4_t acc[TILES][kOut];
+    float reference[TILES], sum[TILES];
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+        reference[t] = -kInf, sum[t] = 0.f;
+#pragma unroll
+        for (int o = 0; o < kOut; ++o) acc[t][o] = float4_t{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // A step's rows: page entries, then offsets, then 16-byte pieces.
+    int pages[2], slots[2];
+    int64_t at[2];
+    bool there[2];
+    uint4_t keys[2][kLoads], values[2][kLoads];
+    unsigned bytes[2] = {0, 0};
+    auto find = [&](int base) {  // entries; positions past the end take the last one's
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const PageSlot where = page_slot(max(0, min(base + 16 * u + column, end - 1)), v.page_size, v.magic);
+            slots[u] = where.slot;
+            pages[u] = table[where.page];
+        }
+    };
+    auto place = [&](int base) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const bool known = pages[u] >= 0 && pages[u] < v.pages;
+            there[u] = known && base + 16 * u + column < end;
+            const int page = known ? pages[u] : 0;
+            at[u] = v.row_at(page, job.head, slots[u]) + 16 * part;
+            if constexpr (TYPE == kPagedE4M3)
+                bytes[u] = *reinterpret_cast<const uint16_t*>(v.exponents + v.exponents_at(page, job.head, slots[u]));
+        }
+    };
+    auto load = [&](const char* pool, uint4_t (&to)[2][kLoads]) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) to[u][i] = *reinterpret_cast<const uint4_t*>(pool + at[u] + 64 * i);
+    };
+    char* const mine = space.rows[wave];
+    const char* const transposed = mine + (4 * part + (column >> 2)) * kPitch + (column & 3) * 8;
+
+    int base = begin + kTile * wave;
+    if (base < end) find(base);
+    // Queries: row r of the job is head r % group of new row r / group.
+    uint4_t query[TILES][kSteps][kProducts];
+    float to_score[TILES];  // what a product's sum is multiplied by
+    int sees[TILES];        // positions the lane's row attends
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+        if (t >= live_tiles) continue;
+        __builtin_amdgcn_sched_barrier(0);  // a tile's queries at a time, for the registers
+        const int query_row = job.row0 + 16 * t + column, new_row = a.new_row(query_row);
+        const int64_t row = int64_t(job.first) + new_row;
+        const bool live = query_row < job.rows && row >= 0 && row < v.total_rows;
+        sees[t] = !live ? 0 : CAUSAL ? job.sees + new_row : job.to;
+        const float* const from =
+            a.queries + (live ? row * a.query_stride + (job.head * a.group + query_row - new_row * a.group) * DIM : 0);
+        float x[kSteps][8], top = 0.f;
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+            // The channels that this lane's part of a stored row holds in step k.
+            const int from_channel = kPer == 1 ? 32 * k + 8 * part : 64 * (k / 2) + 16 * part + 8 * (k % 2);
+            const float4_a4 lo = *reinterpret_cast<const float4_a4*>(from + from_channel);
+            const float4_a4 hi = *reinterpret_cast<const float4_a4*>(from + from_channel + 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[k][e] = live ? lo[e] : 0.f, x[k][4 + e] = live ? hi[e] : 0.f;
+        }
+        to_score[t] = a.scale;
+        if constexpr (TYPE == kPagedF16) {
+            // An exact power of two brings a row's largest query to [2^14, 2^15), so that neither term leaves
+            // FP16's range; non-finite ones stay so.
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = fmaxf(top, __builtin_fabsf(x[k][e]));
+            top = fmaxf(top, dev::xor_lanes<16>(top));
+            top = fmaxf(top, dev::xor_lanes<32>(top));
+            const int up = 14 - max(int(__builtin_bit_cast(unsigned, top) >> 23) - 127, -100);
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[k][e] *= pow2(up);
+            to_score[t] *= pow2(-up);
+        }
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                unsigned words[kProducts];
+                Terms<TYPE, false>::split(x[k][2 * e], x[k][2 * e + 1], false, words);
+#pragma unroll
+                for (int p = 0; p < kProducts; ++p) query[t][k][p][e] = words[p];
+            }
+    }
+    if (base < end) {
+        place(base);
+        load(v.keys, keys);
+        if (base + kBlock < end) find(base + kBlock);
+        load(v.values, values);
+    }
+
+    auto each_tile = [](auto f) {
+        f(std::integral_constant<int, 0>{});
+        if constexpr (TILES > 1) f(std::integral_constant<int, 1>{});
+        if constexpr (TILES > 2) f(std::integral_constant<int, 2>{}), f(std::integral_constant<int, 3>{});
+    };
+    for (; base < end; base += kBlock) {
+        float4_t s[TILES][2];
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) s[t][0] = s[t][1] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                uint4_t k[kPer];
+                widen<TYPE>(keys[u][i], byte_pow2(bytes[u] & 255), k);
+#pragma unroll
+                for (int t = 0; t < TILES; ++t) {
+                    if (t >= live_tiles) continue;
+#pragma unroll
+                    for (int j = 0; j < kPer; ++j)
+#pragma unroll
+                        for (int p = 0; p < kProducts; ++p)
+                            s[t][u] = multiply(k[j], query[t][kPer * i + j][p], s[t][u], kType);
+                }
+            }
+        // What the rest of this step needs of its rows, before the next one's take their place.
+        const bool was[2] = {there[0], there[1]};
+        const int64_t row_at[2] = {at[0] - 16 * part, at[1] - 16 * part};
+        const float value_up[2] = {byte_pow2(bytes[0] >> 8), byte_pow2(bytes[1] >> 8)};
+        const unsigned exist = (unsigned(__ballot(was[0])) & 0xffffu) | unsigned(__ballot(was[1])) << 16;
+        const bool more_steps = base + kBlock < end;
+        if (more_steps) {
+            place(base + kBlock);
+            load(v.keys, keys);
+        }
+        const bool whole = exist == 0xffffffffu && base + kTile <= shared_end;
+
+        // Values into LDS, 0 for those that are not there. A weight of 0 does not keep infinities and NaN
+        // out, so those in rows that only some new rows see are 0 here as well, and added below. They are found
+        // in the 16-bit words: an E4M3 row's power of two may carry finite codes past what these hold.
+        const bool triangle = CAUSAL && base + kTile > shared_end;
+        unsigned spoilt_bits = 0;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const unsigned partly = base + 16 * u + column >= shared_end ? ~0u : 0u;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                uint4_t w[kPer];
+                widen<TYPE>(values[u][i], value_up[u], w);
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) {
+                    if (!whole && !was[u]) w[j] = uint4_t{0u, 0u, 0u, 0u};
+                    if (triangle)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const unsigned bad = not_finite<TYPE == kPagedF16>(w[j][e]) & partly;
+                            spoilt_bits |= bad;
+                            w[j][e] &= ~((bad >> 15) * 0xffffu);
+                        }
+                    char* const to = mine + (16 * u + column) * kPitch + 64 * kPer * i + 16 * kPer * part + 16 * j;
+                    *reinterpret_cast<uint4_t*>(to) = w[j];
+                }
+            }
+        }
+        const bool spoilt = triangle && __any(spoilt_bits != 0);
+        if (more_steps) {
+            if (base + 2 * kBlock < end) find(base + 2 * kBlock);
+            load(v.values, values);
+        }
+
+        float weights[TILES][2][4];
+        uint4_t weight[TILES][kProducts];
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+            if (t >= live_tiles) continue;
+            float high = -kInf;
+            unsigned hidden = 0;  // bit 4 u + r
+            if (whole) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) high = fmaxf(high, s[t][u][r] * to_score[t]);
+            } else {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int j = 16 * u + 4 * part + r;
+                        if (!(exist >> j & 1) || (CAUSAL && base + j >= sees[t]))
+                            hidden |= 1u << (4 * u + r);
+                        else
+                            high = fmaxf(high, s[t][u][r] * to_score[t]);
+                    }
+            }
+            if (__any(high > reference[t] + (kHead + kGrow))) {
+                high = fmaxf(high, dev::xor_lanes<16>(high));
+                high = fmaxf(high, dev::xor_lanes<32>(high));
+                const float moved = fmaxf(reference[t], high - kHead);
+                const float shrink = reference[t] == moved ? 1.f : exp2_fast(reference[t] - moved);
+                reference[t] = moved;
+                sum[t] *= shrink;
+#pragma unroll
+                for (int o = 0; o < kOut; ++o) acc[t][o] *= shrink;
+            }
+            const float from = reference[t] == -kInf ? 0.f : reference[t];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float p = exp2_fast(__builtin_fmaf(s[t][u][r], to_score[t], -from));
+                    if (!whole && (hidden >> (4 * u + r) & 1)) p = 0.f;
+                    weights[t][u][r] = p;
+                    sum[t] += p;
+                }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                unsigned words[kProducts];
+                Terms<TYPE, false>::split(weights[t][e / 2][2 * (e % 2)], weights[t][e / 2][2 * (e % 2) + 1], false, words);
+#pragma unroll
+                for (int p = 0; p < kProducts; ++p) weight[t][p][e] = words[p];
+            }
+        }
+#pragma unroll
+        for (int o = 0; o < kOut; ++o) {
+            const short4_t low = read_transposed(transposed + 32 * o);
+            const short4_t high = read_transposed(transposed + 16 * kPitch + 32 * o);
+            const uint4_t w = {__builtin_bit_cast(u32x2, low)[0], __builtin_bit_cast(u32x2, low)[1],
+                               __builtin_bit_cast(u32x2, high)[0], __builtin_bit_cast(u32x2, high)[1]};
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) {
+                if (t >= live_tiles) continue;
+#pragma unroll
+                for (int p = 0; p < kProducts; ++p) acc[t][o] = multiply(w, weight[t][p], acc[t][o], kType);
+            }
+        }
+
+        // One row at a time, for the new rows that see it; the wave's weights pass through its part of LDS, whose
+        // values have been read.
+        if (CAUSAL && spoilt) {
+            float* const passed = reinterpret_cast<float*>(mine);
+            each_tile([&](auto of) {
+                constexpr int t = decltype(of)::value;
+                if (t >= live_tiles) return;
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                    *reinterpret_cast<float4_t*>(passed + column * kTile + 16 * u + 4 * part) =
+                        float4_t{weights[t][u][0], weights[t][u][1], weights[t][u][2], weights[t][u][3]};
+                for (int j = max(0, shared_end - base); j < kTile; ++j) {
+                    if (!(exist >> j & 1)) continue;
+                    const int64_t from = __shfl(j < 16 ? row_at[0] : row_at[1], j & 15);
+                    const float up = __shfl(j < 16 ? value_up[0] : value_up[1], j & 15);
+                    const float p = passed[column * kTile + j];
+                    if (base + j >= sees[t]) continue;
+#pragma unroll
+                    for (int o = 0; o < kOut; ++o)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float x = stored<TYPE>(v.values + from, 16 * o + 4 * part + e, up);
+                            if (x - x != 0.f) acc[t][o][e] = __builtin_fmaf(p, x, acc[t][o][e]);
+                        }
+                }
+            });
+        }
+    }
+
+    // The four waves' sums, a tile at a time, brought to their largest reference.
+    float* const sums = reinterpret_cast<float*>(space.rows);  // [kWaves][16][DIM]
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+        if (t >= live_tiles) continue;
+        __syncthreads();
+        float all_of = sum[t];
+        all_of += dev::xor_lanes<16>(all_of);
+        all_of += dev::xor_lanes<32>(all_of);
+        if (lane < 16) space.states[wave][lane] = float2{reference[t], all_of};
+#pragma unroll
+        for (int o = 0; o < kOut; ++o)
+            *reinterpret_cast<float4_t*>(sums + (wave * 16 + column) * DIM + 16 * o + 4 * part) = acc[t][o];
+        __syncthreads();
+        for (int item = threadIdx.x; item < 16 * DIM / 4; item += kWaves * 64) {
+            const int local = item / (DIM / 4), channel = 4 * (item - local * (DIM / 4));
+            const int query_row = job.row0 + 16 * t + local, new_row = a.new_row(query_row);
+            const int64_t row = int64_t(job.first) + new_row;
+            if (query_row >= job.rows || row < 0 || row >= v.total_rows) continue;
+            float top = -kInf, all = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) top = fmaxf(top, space.states[w][local].x);
+            float4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                const float2 state = space.states[w][local];
+                const float shrink = state.x == top ? 1.f : exp2_fast(state.x - top);
+                all = __builtin_fmaf(state.y, shrink, all);
+                const float4_t x = *reinterpret_cast<const float4_t*>(sums + (w * 16 + local) * DIM + channel);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(x[e], shrink, o[e]);
+            }
+            const int64_t to = a.place(v, job.slot, int(row), job.head * a.group + query_row - new_row * a.group);
+            *reinterpret_cast<float4_t*>(a.sums + to * DIM + channel) = o;
+            if (channel == 0) a.states[to] = float2{top, all};
+        }
+    }
+}
+
+// Workgroups of the prefixes come first, then those of what is behind them.
+template <int TYPE, int DIM, int TILES>
+__global__ __launch_bounds__(kWaves * 64, DIM * TILES > 128 ? 1 : 2) void shared_attention_kernel(PagedView v,
+                                                                                                 SharedArgs a) {
+    constexpr int kRows = 16 * TILES, kRestTiles = rest_tiles_of(TILES), kRestRows = 16 * kRestTiles;
+    __shared__ SharedSpace<DIM> space;
+    const int lane = threadIdx.x & 63;
+    SharedJob job;
+    if (int(blockIdx.x) < a.jobs) {
+        // Tiles of one head and part are 8 workgroups apart, on one XCD, whose L2 reads its positions once for all.
+        const int of_eight = blockIdx.x / (8 * a.tiles), within = blockIdx.x - of_eight * 8 * a.tiles;
+        const int pair = of_eight * 8 + (within & 7), tile = within >> 3;
+        const int index = pair % a.parts;
+        job.head = pair / a.parts;
+        if (job.head >= v.kv_heads) return;
+        // The tile's group.
+        int before = 0, g = -1;
+        for (int g0 = 0; g0 < a.groups; g0 += 64) {
+            const int count = g0 + lane < a.groups ? (a.rows_of(v, g0 + lane) + kRows - 1) / kRows : 0;
+            const int upto = before + scan_lanes(count);
+            const unsigned long long hit = __ballot(upto > tile);
+            if (hit) {
+                const int at = __ffsll(hit) - 1;
+                g = g0 + at;
+                job.row0 = (tile - __builtin_amdgcn_readlane(upto - count, at)) * kRows;
+                break;
+            }
+            before = __builtin_amdgcn_readlane(upto, 63);
+        }
+        if (g < 0) return;
+        const int prefix = a.prefix_of(v, g, lane, job.s);
+        if (job.s >= v.sequences) return;
+        job.first = a.row_of(v, a.first_of(v, g));
+        job.rows = a.rows_of(v, g);
+        job.from = index * a.part;
+        if (job.from >= prefix) return;
+        job.to = index == a.parts - 1 ? prefix : min(prefix, job.from + a.part);
+        job.sees = 0;
+        job.slot = index;
+        shared_attend<TYPE, DIM, TILES, false>(v, a, job, space);
+    } else {
+        int at = blockIdx.x - a.jobs;
+        const int index = at % a.rest_parts;
+        at /= a.rest_parts;
+        job.row0 = at % a.rest_tiles * kRestRows;
+        at /= a.rest_tiles;
+        job.s = at % v.sequences;
+        job.head = at / v.sequences;
+        const int n = v.new_rows(job.s, job.first), length = v.length(job.s);
+        job.rows = n * a.group;
+        if (job.row0 >= job.rows) return;
+        int reads;
+        const int prefix = a.prefix_of(v, a.group_of(v, job.s, lane), lane, reads);
+        job.from = prefix + index * a.rest_part;
+        if (job.from >= length) return;
+        job.to = index == a.rest_parts - 1 ? length : min(length, job.from + a.rest_part);
+        job.sees = length - n + 1;
+        job.slot = a.parts + index;
+        shared_attend<TYPE, DIM, kRestTiles, true>(v, a, job, space);
+    }
+}
+
+// A new row's parts: those of its group's prefix, then those behind it, by
+// their references. A workgroup a row, a thread four channels of a head.
+template <int DIM>
+__global__ __launch_bounds__(256) void shared_join_kernel(PagedView v, SharedArgs a) {
+    const int row = blockIdx.x, lane = threadIdx.x & 63;
+    const int s = v.sequence_of(row, lane);
+    if (s < 0) return;
+    int first;
+    const int n = v.new_rows(s, first);
+    if (row - first >= n) return;
+    int reads;
+    const int prefix = a.prefix_of(v, a.group_of(v, s, lane), lane, reads);
+    const int shared = a.parts_of(prefix, a.part, a.parts);
+    const int count = shared + a.parts_of(max(0, v.length(s) - prefix), a.rest_part, a.rest_parts);
+    for (int item = threadIdx.x; item < a.query_heads * (DIM / 4); item += 256) {
+        const int head = item / (DIM / 4), channel = 4 * (item - head * (DIM / 4));
+        float top = -kInf, all = 0.f;
+        float4_t o = {0.f, 0.f, 0.f, 0.f};
+        for (int p0 = 0; p0 < count; p0 += 4) {  // that many parts' loads in flight
+            float2 state[4];
+            float4_t x[4];
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                const int index = min(p0 + p, count - 1);
+                const int64_t from = a.place(v, index < shared ? index : a.parts + index - shared, row, head);
+                state[p] = a.states[from];
+                x[p] = *reinterpret_cast<const float4_t*>(a.sums + from * DIM + channel);
+            }
+            float grown = top;
+#pragma unroll
+            for (int p = 0; p < 4; ++p) grown = fmaxf(grown, state[p].x);
+            const float shrink = top == grown ? 1.f : exp2_fast(top - grown);
+            top = grown;
+            all *= shrink;
+            o *= shrink;
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                if (p0 + p >= count) continue;
+                const float by = state[p].x == top ? 1.f : exp2_fast(state[p].x - top);
+                all = __builtin_fmaf(state[p].y, by, all);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(x[p][e], by, o[e]);
+            }
+        }
+        o = all == 0.f ? float4_t{0.f, 0.f, 0.f, 0.f} : o * (1.f / all);
+        *reinterpret_cast<float4_a4*>(a.out + row * a.out_stride + item * 4) = o;
+    }
+}
+
+// Sizes of a call: how its work is split, and what its workspace holds.
+struct SharedPlan {
+    int wide;  // 16 query rows this many times
+    int64_t tiles, rest_tiles, parts, rest_parts, part, rest_part, jobs, rest_jobs, slots;
+    size_t sum_bytes, state_bytes;
+    SharedPlan(const qwen_gpu_paged_cache& c, const qwen_gpu_paged_batch& b, const qwen_gpu_paged_prefix& p,
+               int query_heads) {
+        const int64_t group = query_heads / c.kv_heads, rows = group * b.total_rows;
+        const int64_t of_group = rows / p.groups;  // a group has as many of them if all have the same
+        wide = of_group <= 16 ? 1 : of_group <= 32 || c.head_dim == 256 ? 2 : 4;
+        const int64_t tile = 16 * wide;
+        tiles = p.groups + rows / tile;
+        const int64_t rest_tile = 16 * rest_tiles_of(wide);
+        rest_tiles = (group * b.rows + rest_tile - 1) / rest_tile;
+        // Parts for as many workgroups as the GPU holds at once, of 256 positions or more.
+        const int64_t held = wide * c.head_dim > 128 ? 256 : 512;
+        auto split = [&](int64_t units, int64_t positions, int64_t& count, int64_t& size) {
+            const int64_t most = std::max<int64_t>(1, (positions + 255) / 256);
+            count = std::clamp<int64_t>(held / std::max<int64_t>(1, units), 1, most);
+            size = (positions + count - 1) / count;
+            size = std::max<int64_t>(kBlock, (size + kBlock - 1) / kBlock * kBlock);
+            count = std::max<int64_t>(1, (positions + size - 1) / size);
+        };
+        split(std::max<int64_t>(1, (rows + tile - 1) / tile) * c.kv_heads, p.max_length, parts, part);
+        split(rest_tiles * b.sequences * c.kv_heads, p.max_rest, rest_parts, rest_part);
+        jobs = p.max_length ? (parts * c.kv_heads + 7) / 8 * 8 * tiles : 0;
+        rest_jobs = rest_parts * rest_tiles * b.sequences * c.kv_heads;
+        slots = parts + rest_parts;
+        state_bytes = (size_t(slots) * b.total_rows * query_heads * 8 + 15) / 16 * 16;
+        sum_bytes = size_t(slots) * b.total_rows * query_heads * c.head_dim * 4;
+    }
+    size_t bytes() const { return sum_bytes + state_bytes; }
+};
+
+template <int TYPE, int DIM, int TILES>
+void shared_run(const PagedView& v, const SharedArgs& a, const SharedPlan& plan, hipStream_t stream) {
+    shared_attention_kernel<TYPE, DIM, TILES>
+        <<<unsigned(plan.jobs + plan.rest_jobs), kWaves * 64, 0, stream>>>(v, a);
+}
+
+template <int TYPE>
+void shared_launch(int dim, const PagedView& v, const SharedArgs& a, const SharedPlan& plan, hipStream_t stream) {
+    auto run = [&](auto of_dim) {
+        constexpr int kDim = decltype(of_dim)::value;
+        if (plan.wide == 1) return shared_run<TYPE, kDim, 1>(v, a, plan, stream);
+        if (plan.wide == 2) return shared_run<TYPE, kDim, 2>(v, a, plan, stream);
+        if constexpr (kDim < 256) shared_run<TYPE, kDim, 4>(v, a, plan, stream);
+    };
+    if (dim == 64) return run(std::integral_constant<int, 64>{});
+    if (dim == 128) return run(std::integral_constant<int, 128>{});
+    run(std::integral_constant<int, 256>{});
+}
+
+}  // namespace qwen_hip

@@ -1,0 +1,6 @@
+// Attention behind shared prefixes over BF16 caches.
+#include "paged_shared.hpp"
+
+namespace qwen_hip {
+template void shared_launch<kPagedBF16>(int, const PagedView&, const SharedArgs&, const SharedPlan&, hipStream_t);
+}  // namespace qwen_hip

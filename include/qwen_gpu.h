@@ -390,6 +390,34 @@ int qwen_gpu_op_paged_attention(const qwen_gpu_paged_cache* cache, const qwen_gp
 int qwen_gpu_op_paged_evict(const qwen_gpu_paged_cache* cache, const qwen_gpu_paged_batch* batch, int keep, int sinks,
                             int recent, int32_t* new_lengths, float* new_weights, int32_t* new_positions,
                             void* workspace, size_t workspace_bytes, void* stream);
+/* Attention of the new rows, as qwen_gpu_op_paged_attention, for a batch
+ * whose sequences share the first positions of their text: each group's
+ * prefix is read once for all of its sequences. Group g has the sequences
+ * offsets[g] .. offsets[g + 1] - 1 (bounded to 0 .. sequences on the device;
+ * offsets must not fall), which hold the same keys and values in their first
+ * lengths[g] slots; those are read through the table of its first sequence
+ * with new rows. The prefix is taken no longer than the rows that each of the group's sequences
+ * with new rows cached before them, and a sequence of no group has none, so
+ * every row attends what qwen_gpu_op_paged_attention gives it. max_length
+ * and max_rest size the launch: what a sequence has beyond them is attended
+ * too, by fewer workgroups. Weights are not tracked: batch->weights and
+ * batch->positions must be NULL. The workspace (device memory, aligned to 16)
+ * needs no zeroing and keeps nothing between calls. */
+typedef struct qwen_gpu_paged_prefix {
+    const int32_t* lengths;     /* [groups] */
+    const int32_t* offsets;     /* [groups + 1]; NULL: one group of all sequences */
+    int groups;                 /* 1..sequences; 1 where offsets is NULL */
+    int max_length;             /* 0..batch->max_length: most positions of a prefix */
+    int max_rest;               /* 1..batch->max_length: most positions of a sequence behind its prefix */
+} qwen_gpu_paged_prefix;
+
+int qwen_gpu_op_paged_shared_workspace(const qwen_gpu_paged_cache* cache, const qwen_gpu_paged_batch* batch,
+                                       const qwen_gpu_paged_prefix* prefix, int query_heads, size_t* bytes);
+int qwen_gpu_op_paged_attention_shared(const qwen_gpu_paged_cache* cache, const qwen_gpu_paged_batch* batch,
+                                       const qwen_gpu_paged_prefix* prefix, const float* queries, int64_t query_stride,
+                                       int query_heads, float scale, float* out, int64_t out_stride, void* workspace,
+                                       size_t workspace_bytes, void* stream);
+
 /* ---- Pages and rows of a step (no reference counterpart) ----
  *
  * Which pages a sequence has, kept on the device: the sequences' tables and a
