@@ -84,9 +84,6 @@ struct SharedArgs {
     }
 };
 
-// Tiles of a wave behind the prefixes, where query rows are those of one sequence.
-__host__ __device__ constexpr int rest_tiles_of(int tiles) { return tiles < 2 ? tiles : 2; }
-
 // What a workgroup does: a tile of query rows of a KV head against a range of
 // a sequence's positions.
 struct SharedJob {
@@ -440,12 +437,266 @@ __device__ __forceinline__ void shared_attend(const PagedView& v, const SharedAr
     }
 }
 
-// Workgroups of the prefixes come first, then those of what is behind them.
+// LDS of a workgroup whose waves share its positions: two steps' keys and
+// values, 16-bit whatever the cache's type, and which of them exist.
+template <int DIM>
+struct WideSpace {
+    static constexpr int kPositions = DIM == 256 ? 32 : 64, kPitch = DIM * 2 + 32;
+    __attribute__((aligned(16))) char keys[2][kPositions * kPitch];
+    __attribute__((aligned(16))) char values[2][kPositions * kPitch];
+    __attribute__((aligned(16))) int there[2][kPositions];
+    __attribute__((aligned(16))) int all[2][kWaves];
+};
+
+// A prefix against more query rows: each wave has TILES times 16 rows of its
+// own and all waves go over the same positions, which the workgroup brings
+// into LDS together, a step ahead, widened to 16 bits once. A wave's part of the loads
+// takes a quarter of the registers, so that two workgroups fit a CU and one's
+// products run beside the other's exponentials.
 template <int TYPE, int DIM, int TILES>
-__global__ __launch_bounds__(kWaves * 64, DIM * TILES > 128 ? 1 : 2) void shared_attention_kernel(PagedView v,
-                                                                                                 SharedArgs a) {
-    constexpr int kRows = 16 * TILES, kRestTiles = rest_tiles_of(TILES), kRestRows = 16 * kRestTiles;
-    __shared__ SharedSpace<DIM> space;
+__device__ __forceinline__ void shared_attend_wide(const PagedView& v, const SharedArgs& a, const SharedJob& job,
+                                                   WideSpace<DIM>& space) {
+    typedef WideSpace<DIM> Space;
+    constexpr int kSize = TYPE == kPagedE4M3 ? 1 : 2, kSteps = DIM / 32, kOut = DIM / 16;
+    constexpr int kPositions = Space::kPositions, kPitch = Space::kPitch;
+    constexpr int kProducts = Terms<TYPE, false>::kProducts;
+    constexpr int kChunks = DIM * kSize / 16;     // threads of a stored row, 16 bytes each
+    constexpr int kAtOnce = kWaves * 64 / kChunks, kLoads = kPositions / kAtOnce;  // rows of a load; loads
+    constexpr int kWords = TYPE == kPagedE4M3 ? 2 : 1;
+    constexpr float kHead = TYPE == kPagedF16 ? 6.f : 0.f;  // FP16 weights are kept up to 2^14, far from subnormals
+    constexpr float kGrow = 8.f;                  // a reference is moved once a score passes it by 2^8
+    constexpr std::integral_constant<int, TYPE> kType{};
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int column = lane & 15, part = lane >> 4;
+    const int my_row = threadIdx.x / kChunks, chunk = threadIdx.x % kChunks, end = job.to;
+    const int32_t* const table = v.table + int64_t(job.s) * v.table_stride;
+
+    int pages[kLoads], slots[kLoads];
+    bool there[kLoads];
+    uint4_t keys[kLoads], values[kLoads];
+    unsigned bytes[kLoads] = {};
+    auto find = [&](int base) {  // entries; positions past the end take the last one's
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const PageSlot where = page_slot(min(base + i * kAtOnce + my_row, end - 1), v.page_size, v.magic);
+            slots[i] = where.slot;
+            pages[i] = table[where.page];
+        }
+    };
+    auto load = [&](int base) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const bool known = pages[i] >= 0 && pages[i] < v.pages;
+            there[i] = known && base + i * kAtOnce + my_row < end;
+            const int page = known ? pages[i] : 0;
+            const int64_t at = v.row_at(page, job.head, slots[i]) + 16 * chunk;
+            if constexpr (TYPE == kPagedE4M3)
+                bytes[i] = *reinterpret_cast<const uint16_t*>(v.exponents + v.exponents_at(page, job.head, slots[i]));
+            keys[i] = *reinterpret_cast<const uint4_t*>(v.keys + at);
+            values[i] = *reinterpret_cast<const uint4_t*>(v.values + at);
+        }
+    };
+    int base = job.from, buffer = 0;
+    find(base);
+
+    // Queries: row r of the job is head r % group of new row r / group.
+    const int first_row = job.row0 + wave * 16 * TILES;
+    const int live_tiles = first_row < job.rows ? min(TILES, (job.rows - first_row + 15) / 16) : 0;
+    uint4_t query[TILES][kSteps][kProducts];
+    float to_score[TILES], reference[TILES], sum[TILES];
+    float4_t acc[TILES][kOut];
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+        reference[t] = -kInf, sum[t] = 0.f;
+#pragma unroll
+        for (int o = 0; o < kOut; ++o) acc[t][o] = float4_t{0.f, 0.f, 0.f, 0.f};
+        if (t >= live_tiles) continue;
+        __builtin_amdgcn_sched_barrier(0);  // a tile's queries at a time, for the registers
+        const int query_row = first_row + 16 * t + column, new_row = a.new_row(query_row);
+        const bool live = query_row < job.rows;
+        const float* const from =
+            a.queries + (live ? int64_t(job.first + new_row) * a.query_stride +
+                                    (job.head * a.group + query_row - new_row * a.group) * DIM
+                              : 0);
+        float x[kSteps][8], top = 0.f;
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+            const float4_a4 lo = *reinterpret_cast<const float4_a4*>(from + 32 * k + 8 * part);
+            const float4_a4 hi = *reinterpret_cast<const float4_a4*>(from + 32 * k + 8 * part + 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[k][e] = live ? lo[e] : 0.f, x[k][4 + e] = live ? hi[e] : 0.f;
+        }
+        to_score[t] = a.scale;
+        if constexpr (TYPE == kPagedF16) {
+            // An exact power of two brings a row's largest query to [2^14, 2^15), so that neither term leaves
+            // FP16's range; non-finite ones stay so.
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = fmaxf(top, __builtin_fabsf(x[k][e]));
+            top = fmaxf(top, dev::xor_lanes<16>(top));
+            top = fmaxf(top, dev::xor_lanes<32>(top));
+            const int up = 14 - max(int(__builtin_bit_cast(unsigned, top) >> 23) - 127, -100);
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[k][e] *= pow2(up);
+            to_score[t] *= pow2(-up);
+        }
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                unsigned words[kProducts];
+                Terms<TYPE, false>::split(x[k][2 * e], x[k][2 * e + 1], false, words);
+#pragma unroll
+                for (int p = 0; p < kProducts; ++p) query[t][k][p][e] = words[p];
+            }
+    }
+    load(base);
+    if (base + kPositions < end) find(base + kPositions);
+
+    for (; base < end; base += kPositions, buffer ^= 1) {
+        bool whole_here = true;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            uint4_t k[kWords], w[kWords];
+            widen<TYPE>(keys[i], byte_pow2(bytes[i] & 255), k);
+            widen<TYPE>(values[i], byte_pow2(bytes[i] >> 8), w);
+            const int row = i * kAtOnce + my_row, to = row * kPitch + 16 * kWords * chunk;
+#pragma unroll
+            for (int j = 0; j < kWords; ++j) {
+                if (!there[i]) w[j] = uint4_t{0u, 0u, 0u, 0u};  // a weight of 0 does not keep NaN out
+                *reinterpret_cast<uint4_t*>(space.keys[buffer] + to + 16 * j) = k[j];
+                *reinterpret_cast<uint4_t*>(space.values[buffer] + to + 16 * j) = w[j];
+            }
+            if (chunk == 0) space.there[buffer][row] = there[i];
+            whole_here = whole_here && there[i];
+        }
+        const bool whole_wave = __all(whole_here);
+        if (lane == 0) space.all[buffer][wave] = whole_wave;
+        if (base + kPositions < end) {
+            load(base + kPositions);
+            if (base + 2 * kPositions < end) find(base + 2 * kPositions);
+        }
+        // Nobody writes a buffer again before all have passed the next barrier, and so have read it.
+        __syncthreads();
+        if (!live_tiles) continue;
+        bool whole = true;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) whole = whole && space.all[buffer][w];
+
+        // 32 positions at a time, for the registers.
+#pragma unroll 1
+        for (int h = 0; h < kPositions / 32; ++h) {
+            const char* const key = space.keys[buffer] + (32 * h + column) * kPitch + 16 * part;
+            const char* const transposed =
+                space.values[buffer] + (32 * h + 4 * part + (column >> 2)) * kPitch + (column & 3) * 8;
+            float4_t s[TILES][2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                for (int t = 0; t < TILES; ++t) s[t][u] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k) {
+                    const uint4_t x = *reinterpret_cast<const uint4_t*>(key + 16 * u * kPitch + 64 * k);
+#pragma unroll
+                    for (int t = 0; t < TILES; ++t) {
+                        if (t >= live_tiles) continue;
+#pragma unroll
+                        for (int p = 0; p < kProducts; ++p) s[t][u] = multiply(x, query[t][k][p], s[t][u], kType);
+                    }
+                }
+            }
+            unsigned hidden = 0;  // bit 4 u + r
+            if (!whole)
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (!space.there[buffer][32 * h + 16 * u + 4 * part + r]) hidden |= 1u << (4 * u + r);
+            uint4_t weight[TILES][kProducts];
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) {
+                if (t >= live_tiles) continue;
+                float high = -kInf;
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (whole || !(hidden >> (4 * u + r) & 1)) high = fmaxf(high, s[t][u][r] * to_score[t]);
+                if (__any(high > reference[t] + (kHead + kGrow))) {
+                    high = fmaxf(high, dev::xor_lanes<16>(high));
+                    high = fmaxf(high, dev::xor_lanes<32>(high));
+                    const float moved = fmaxf(reference[t], high - kHead);
+                    const float shrink = reference[t] == moved ? 1.f : exp2_fast(reference[t] - moved);
+                    reference[t] = moved;
+                    sum[t] *= shrink;
+#pragma unroll
+                    for (int o = 0; o < kOut; ++o) acc[t][o] *= shrink;
+                }
+                const float from = reference[t] == -kInf ? 0.f : reference[t];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    float p[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        p[r] = exp2_fast(__builtin_fmaf(s[t][u][r], to_score[t], -from));
+                        if (!whole && (hidden >> (4 * u + r) & 1)) p[r] = 0.f;
+                        sum[t] += p[r];
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        unsigned words[kProducts];
+                        Terms<TYPE, false>::split(p[2 * e], p[2 * e + 1], false, words);
+#pragma unroll
+                        for (int q = 0; q < kProducts; ++q) weight[t][q][2 * u + e] = words[q];
+                    }
+                }
+            }
+#pragma unroll
+            for (int o = 0; o < kOut; ++o) {
+                const short4_t low = read_transposed(transposed + 32 * o);
+                const short4_t high = read_transposed(transposed + 16 * kPitch + 32 * o);
+                const uint4_t w = {__builtin_bit_cast(u32x2, low)[0], __builtin_bit_cast(u32x2, low)[1],
+                                   __builtin_bit_cast(u32x2, high)[0], __builtin_bit_cast(u32x2, high)[1]};
+#pragma unroll
+                for (int t = 0; t < TILES; ++t) {
+                    if (t >= live_tiles) continue;
+#pragma unroll
+                    for (int p = 0; p < kProducts; ++p) acc[t][o] = multiply(w, weight[t][p], acc[t][o], kType);
+                }
+            }
+        }
+    }
+
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+        if (t >= live_tiles) continue;
+        float all = sum[t];
+        all += dev::xor_lanes<16>(all);
+        all += dev::xor_lanes<32>(all);
+        const int query_row = first_row + 16 * t + column, new_row = a.new_row(query_row);
+        if (query_row >= job.rows) continue;
+        const int64_t to = a.place(v, job.slot, job.first + new_row, job.head * a.group + query_row - new_row * a.group);
+#pragma unroll
+        for (int o = 0; o < kOut; ++o) *reinterpret_cast<float4_t*>(a.sums + to * DIM + 16 * o + 4 * part) = acc[t][o];
+        if (part == 0) a.states[to] = float2{reference[t], all};
+    }
+}
+
+// Query rows of a workgroup of the prefixes, by how wide it is: 16 that its
+// waves split the positions of, or 64 or 128 dealt to the waves.
+__host__ __device__ constexpr int rows_of_wide(int wide) { return wide ? 64 * wide : 16; }
+
+// Workgroups of the prefixes come first, then those of what is behind them.
+template <int TYPE, int DIM, int WIDE>
+__global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void shared_attention_kernel(PagedView v, SharedArgs a) {
+    constexpr int kRows = rows_of_wide(WIDE), kRestRows = 16;
+    __shared__ union Space {
+        SharedSpace<DIM> narrow;
+        WideSpace<DIM> wide;
+    } space;
     const int lane = threadIdx.x & 63;
     SharedJob job;
     if (int(blockIdx.x) < a.jobs) {
@@ -479,7 +730,10 @@ __global__ __launch_bounds__(kWaves * 64, DIM * TILES > 128 ? 1 : 2) void shared
         job.to = index == a.parts - 1 ? prefix : min(prefix, job.from + a.part);
         job.sees = 0;
         job.slot = index;
-        shared_attend<TYPE, DIM, TILES, false>(v, a, job, space);
+        if constexpr (WIDE)
+            shared_attend_wide<TYPE, DIM, WIDE>(v, a, job, space.wide);
+        else
+            shared_attend<TYPE, DIM, 1, false>(v, a, job, space.narrow);
     } else {
         int at = blockIdx.x - a.jobs;
         const int index = at % a.rest_parts;
@@ -498,7 +752,7 @@ __global__ __launch_bounds__(kWaves * 64, DIM * TILES > 128 ? 1 : 2) void shared
         job.to = index == a.rest_parts - 1 ? length : min(length, job.from + a.rest_part);
         job.sees = length - n + 1;
         job.slot = a.parts + index;
-        shared_attend<TYPE, DIM, kRestTiles, true>(v, a, job, space);
+        shared_attend<TYPE, DIM, 1, true>(v, a, job, space.narrow);
     }
 }
 
@@ -553,20 +807,19 @@ __global__ __launch_bounds__(256) void shared_join_kernel(PagedView v, SharedArg
 
 // Sizes of a call: how its work is split, and what its workspace holds.
 struct SharedPlan {
-    int wide;  // 16 query rows this many times
+    int wide;
     int64_t tiles, rest_tiles, parts, rest_parts, part, rest_part, jobs, rest_jobs, slots;
     size_t sum_bytes, state_bytes;
     SharedPlan(const qwen_gpu_paged_cache& c, const qwen_gpu_paged_batch& b, const qwen_gpu_paged_prefix& p,
                int query_heads) {
         const int64_t group = query_heads / c.kv_heads, rows = group * b.total_rows;
         const int64_t of_group = rows / p.groups;  // a group has as many of them if all have the same
-        wide = of_group <= 16 ? 1 : of_group <= 32 || c.head_dim == 256 ? 2 : 4;
-        const int64_t tile = 16 * wide;
+        wide = of_group <= 16 ? 0 : of_group <= 64 || c.head_dim == 256 ? 1 : 2;
+        const int64_t tile = rows_of_wide(wide);
         tiles = p.groups + rows / tile;
-        const int64_t rest_tile = 16 * rest_tiles_of(wide);
-        rest_tiles = (group * b.rows + rest_tile - 1) / rest_tile;
+        rest_tiles = (group * b.rows + 15) / 16;
         // Parts for as many workgroups as the GPU holds at once, of 256 positions or more.
-        const int64_t held = wide * c.head_dim > 128 ? 256 : 512;
+        const int64_t held = c.head_dim == 256 ? 256 : 512;
         auto split = [&](int64_t units, int64_t positions, int64_t& count, int64_t& size) {
             const int64_t most = std::max<int64_t>(1, (positions + 255) / 256);
             count = std::clamp<int64_t>(held / std::max<int64_t>(1, units), 1, most);
@@ -585,9 +838,9 @@ struct SharedPlan {
     size_t bytes() const { return sum_bytes + state_bytes; }
 };
 
-template <int TYPE, int DIM, int TILES>
+template <int TYPE, int DIM, int WIDE>
 void shared_run(const PagedView& v, const SharedArgs& a, const SharedPlan& plan, hipStream_t stream) {
-    shared_attention_kernel<TYPE, DIM, TILES>
+    shared_attention_kernel<TYPE, DIM, WIDE>
         <<<unsigned(plan.jobs + plan.rest_jobs), kWaves * 64, 0, stream>>>(v, a);
 }
 
@@ -595,9 +848,9 @@ template <int TYPE>
 void shared_launch(int dim, const PagedView& v, const SharedArgs& a, const SharedPlan& plan, hipStream_t stream) {
     auto run = [&](auto of_dim) {
         constexpr int kDim = decltype(of_dim)::value;
+        if (plan.wide == 0) return shared_run<TYPE, kDim, 0>(v, a, plan, stream);
         if (plan.wide == 1) return shared_run<TYPE, kDim, 1>(v, a, plan, stream);
-        if (plan.wide == 2) return shared_run<TYPE, kDim, 2>(v, a, plan, stream);
-        if constexpr (kDim < 256) shared_run<TYPE, kDim, 4>(v, a, plan, stream);
+        if constexpr (kDim < 256) shared_run<TYPE, kDim, 2>(v, a, plan, stream);
     };
     if (dim == 64) return run(std::integral_constant<int, 64>{});
     if (dim == 128) return run(std::integral_constant<int, 128>{});
