@@ -78,7 +78,6 @@ void launch_paged_attention_shared(const qwen_gpu_paged_cache& cache, const qwen
                        prefix.lengths,
                        prefix.offsets,
                        prefix.groups,
-                       int(plan.tiles),
                        int(plan.rest_tiles),
                        int(plan.parts),
                        int(plan.rest_parts),
@@ -93,7 +92,7 @@ void launch_paged_attention_shared(const qwen_gpu_paged_cache& cache, const qwen
         shared_launch<kPagedBF16>(cache.head_dim, v, a, plan, stream);
     else
         shared_launch<kPagedE4M3>(cache.head_dim, v, a, plan, stream);
-    const unsigned grid = unsigned(batch.total_rows);
+    const dim3 grid(unsigned(batch.total_rows), unsigned((row / 4 + kJoinItems - 1) / kJoinItems));
     if (cache.head_dim == 64)
         shared_join_kernel<64><<<grid, 256, 0, stream>>>(v, a);
     else if (cache.head_dim == 128)

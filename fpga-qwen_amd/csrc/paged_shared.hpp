@@ -19,7 +19,7 @@ struct SharedArgs {
     const int32_t* lengths;     // of the prefixes
     const int32_t* offsets;     // NULL: one group of all sequences
     int groups;
-    int tiles, rest_tiles;      // of all groups' query rows at most, of a sequence's
+    int rest_tiles;             // of a sequence's query rows
     int parts, rest_parts;      // of a prefix, of what is behind it, at most
     int part, rest_part;        // positions of each
     int jobs;                   // workgroups of the prefixes
@@ -441,7 +441,7 @@ __device__ __forceinline__ void shared_attend(const PagedView& v, const SharedAr
 // values, 16-bit whatever the cache's type, and which of them exist.
 template <int DIM>
 struct WideSpace {
-    static constexpr int kPositions = DIM == 256 ? 32 : 64, kPitch = DIM * 2 + 32;
+    static constexpr int kPositions = DIM == 64 ? 64 : 32, kPitch = DIM * 2 + 32;
     __attribute__((aligned(16))) char keys[2][kPositions * kPitch];
     __attribute__((aligned(16))) char values[2][kPositions * kPitch];
     __attribute__((aligned(16))) int there[2][kPositions];
@@ -700,27 +700,33 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void shared_attent
     const int lane = threadIdx.x & 63;
     SharedJob job;
     if (int(blockIdx.x) < a.jobs) {
-        // Tiles of one head and part are 8 workgroups apart, on one XCD, whose L2 reads its positions once for all.
-        const int of_eight = blockIdx.x / (8 * a.tiles), within = blockIdx.x - of_eight * 8 * a.tiles;
-        const int pair = of_eight * 8 + (within & 7), tile = within >> 3;
-        const int index = pair % a.parts;
-        job.head = pair / a.parts;
-        if (job.head >= v.kv_heads) return;
-        // The tile's group.
-        int before = 0, g = -1;
+        // Each group has its tiles for each head and part of its prefix. Those of one head and part are 8 workgroups
+        // apart, on one XCD, whose L2 reads its positions once for all; workgroups without work come behind all
+        // others (between them, they left half of the CUs with twice the work: 65000 positions took 205 us, not 110).
+        int before = 0, g = -1, tiles = 0, index = 0;
         for (int g0 = 0; g0 < a.groups; g0 += 64) {
-            const int count = g0 + lane < a.groups ? (a.rows_of(v, g0 + lane) + kRows - 1) / kRows : 0;
-            const int upto = before + scan_lanes(count);
-            const unsigned long long hit = __ballot(upto > tile);
+            const bool there = g0 + lane < a.groups;
+            const int of_lane = there ? (a.rows_of(v, g0 + lane) + kRows - 1) / kRows : 0;
+            const int most = there ? a.parts_of(max(0, min(a.lengths[g0 + lane], v.max_length)), a.part, a.parts) : 0;
+            const int count = (most * v.kv_heads + 7) / 8 * 8 * of_lane, upto = before + scan_lanes(count);
+            const unsigned long long hit = __ballot(upto > int(blockIdx.x));
             if (hit) {
                 const int at = __ffsll(hit) - 1;
                 g = g0 + at;
-                job.row0 = (tile - __builtin_amdgcn_readlane(upto - count, at)) * kRows;
+                tiles = __builtin_amdgcn_readlane(of_lane, at);
+                index = blockIdx.x - __builtin_amdgcn_readlane(upto - count, at);
+                before = __builtin_amdgcn_readlane(most, at);
                 break;
             }
             before = __builtin_amdgcn_readlane(upto, 63);
         }
         if (g < 0) return;
+        const int of_eight = index / (8 * tiles), within = index - of_eight * 8 * tiles;
+        const int pair = of_eight * 8 + (within & 7);
+        job.row0 = (within >> 3) * kRows;
+        job.head = pair / before;  // the group's parts
+        index = pair - job.head * before;
+        if (job.head >= v.kv_heads) return;
         const int prefix = a.prefix_of(v, g, lane, job.s);
         if (job.s >= v.sequences) return;
         job.first = a.row_of(v, a.first_of(v, g));
@@ -757,52 +763,71 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void shared_attent
 }
 
 // A new row's parts: those of its group's prefix, then those behind it, by
-// their references. A workgroup a row, a thread four channels of a head.
+// their references. A workgroup has 256 channels of a row, a lane four of
+// them, and each of its waves every fourth part.
+constexpr int kJoinItems = 64;  // of four channels
 template <int DIM>
-__global__ __launch_bounds__(256) void shared_join_kernel(PagedView v, SharedArgs a) {
-    const int row = blockIdx.x, lane = threadIdx.x & 63;
+__global__ __launch_bounds__(kWaves * 64) void shared_join_kernel(PagedView v, SharedArgs a) {
+    __shared__ float4_t sums[kWaves][kJoinItems];
+    __shared__ float2 states[kWaves][kJoinItems];
+    const int row = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int s = v.sequence_of(row, lane);
     if (s < 0) return;
-    int first;
+    int first, reads;
     const int n = v.new_rows(s, first);
     if (row - first >= n) return;
-    int reads;
     const int prefix = a.prefix_of(v, a.group_of(v, s, lane), lane, reads);
     const int shared = a.parts_of(prefix, a.part, a.parts);
     const int count = shared + a.parts_of(max(0, v.length(s) - prefix), a.rest_part, a.rest_parts);
-    for (int item = threadIdx.x; item < a.query_heads * (DIM / 4); item += 256) {
-        const int head = item / (DIM / 4), channel = 4 * (item - head * (DIM / 4));
-        float top = -kInf, all = 0.f;
-        float4_t o = {0.f, 0.f, 0.f, 0.f};
-        for (int p0 = 0; p0 < count; p0 += 4) {  // that many parts' loads in flight
-            float2 state[4];
-            float4_t x[4];
+    const int item = blockIdx.y * kJoinItems + lane, head = min(item / (DIM / 4), a.query_heads - 1);
+    const int channel = 4 * (item % (DIM / 4));
+    float top = -kInf, all = 0.f;
+    float4_t o = {0.f, 0.f, 0.f, 0.f};
+    constexpr int kFlight = 8;  // parts whose sums are loaded at a time
+    for (int p0 = wave; p0 < count; p0 += kFlight * kWaves) {
+        float2 state[kFlight];
+        float4_t x[kFlight];
 #pragma unroll
-            for (int p = 0; p < 4; ++p) {
-                const int index = min(p0 + p, count - 1);
-                const int64_t from = a.place(v, index < shared ? index : a.parts + index - shared, row, head);
-                state[p] = a.states[from];
-                x[p] = *reinterpret_cast<const float4_t*>(a.sums + from * DIM + channel);
-            }
-            float grown = top;
-#pragma unroll
-            for (int p = 0; p < 4; ++p) grown = fmaxf(grown, state[p].x);
-            const float shrink = top == grown ? 1.f : exp2_fast(top - grown);
-            top = grown;
-            all *= shrink;
-            o *= shrink;
-#pragma unroll
-            for (int p = 0; p < 4; ++p) {
-                if (p0 + p >= count) continue;
-                const float by = state[p].x == top ? 1.f : exp2_fast(state[p].x - top);
-                all = __builtin_fmaf(state[p].y, by, all);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(x[p][e], by, o[e]);
-            }
+        for (int p = 0; p < kFlight; ++p) {
+            const int index = min(p0 + p * kWaves, count - 1);
+            const int64_t from = a.place(v, index < shared ? index : a.parts + index - shared, row, head);
+            state[p] = a.states[from];
+            x[p] = *reinterpret_cast<const float4_t*>(a.sums + from * DIM + channel);
         }
-        o = all == 0.f ? float4_t{0.f, 0.f, 0.f, 0.f} : o * (1.f / all);
-        *reinterpret_cast<float4_a4*>(a.out + row * a.out_stride + item * 4) = o;
+        float grown = top;
+#pragma unroll
+        for (int p = 0; p < kFlight; ++p) grown = fmaxf(grown, state[p].x);
+        const float shrink = top == grown ? 1.f : exp2_fast(top - grown);
+        top = grown;
+        all *= shrink;
+        o *= shrink;
+#pragma unroll
+        for (int p = 0; p < kFlight; ++p) {
+            if (p0 + p * kWaves >= count) continue;
+            const float by = state[p].x == top ? 1.f : exp2_fast(state[p].x - top);
+            all = __builtin_fmaf(state[p].y, by, all);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(x[p][e], by, o[e]);
+        }
     }
+    states[wave][lane] = float2{top, all};
+    sums[wave][lane] = o;
+    __syncthreads();
+    if (wave || item >= a.query_heads * (DIM / 4)) return;
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, states[w][lane].x);
+    all = 0.f;
+    o = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        const float2 state = states[w][lane];
+        const float by = state.x == top ? 1.f : exp2_fast(state.x - top);
+        all = __builtin_fmaf(state.y, by, all);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(sums[w][lane][e], by, o[e]);
+    }
+    o = all == 0.f ? float4_t{0.f, 0.f, 0.f, 0.f} : o * (1.f / all);
+    *reinterpret_cast<float4_a4*>(a.out + row * a.out_stride + item * 4) = o;
 }
 
 // Sizes of a call: how its work is split, and what its workspace holds.
@@ -816,7 +841,7 @@ struct SharedPlan {
         const int64_t of_group = rows / p.groups;  // a group has as many of them if all have the same
         wide = of_group <= 16 ? 0 : of_group <= 64 || c.head_dim == 256 ? 1 : 2;
         const int64_t tile = rows_of_wide(wide);
-        tiles = p.groups + rows / tile;
+        tiles = (rows + p.groups * (tile - 1)) / tile;  // however the groups share them
         rest_tiles = (group * b.rows + 15) / 16;
         // Parts for as many workgroups as the GPU holds at once, of 256 positions or more.
         const int64_t held = c.head_dim == 256 ? 256 : 512;
