@@ -88,8 +88,8 @@ struct SharedArgs {
 // a sequence's positions.
 struct SharedJob {
     int head, s;              // whose table
-    int first, rows;          // new row of query row 0, query rows in all
-    int row0;                 // of the tile
+    int first;                // new row of query row 0
+    int row0, rows;           // query rows: the tile's first one, the end
     int from, to;             // positions
     int sees;                 // behind a prefix: positions that the first new row attends, one more each row
     int slot;                 // of its sums
@@ -127,7 +127,7 @@ __device__ __forceinline__ void shared_attend(const PagedView& v, const SharedAr
     const int last_row = min(job.rows - 1, job.row0 + kRows - 1);
     const int shared_end = CAUSAL ? min(job.to, job.sees + a.new_row(job.row0)) : job.to;
     const int end = CAUSAL ? min(job.to, job.sees + a.new_row(last_row)) : job.to;
-    const int live_tiles = (last_row - job.row0) / 16 + 1;
+    constexpr int live_tiles = TILES;
     const int32_t* const table = v.table + int64_t(job.s) * v.table_stride;
 
     float4_t acc[TILES][kOut];
@@ -500,8 +500,9 @@ __device__ __forceinline__ void shared_attend_wide(const PagedView& v, const Sha
     find(base);
 
     // Queries: row r of the job is head r % group of new row r / group.
-    const int first_row = job.row0 + wave * 16 * TILES;
-    const int live_tiles = first_row < job.rows ? min(TILES, (job.rows - first_row + 15) / 16) : 0;
+    // A wave's tiles are four apart, so that fewer than 4 * TILES of them are shared out evenly.
+    const int first_row = job.row0 + 16 * wave;
+    const int live_tiles = first_row < job.rows ? min(TILES, (job.rows - first_row + 63) / 64) : 0;
     uint4_t query[TILES][kSteps][kProducts];
     float to_score[TILES], reference[TILES], sum[TILES];
     float4_t acc[TILES][kOut];
@@ -512,7 +513,7 @@ __device__ __forceinline__ void shared_attend_wide(const PagedView& v, const Sha
         for (int o = 0; o < kOut; ++o) acc[t][o] = float4_t{0.f, 0.f, 0.f, 0.f};
         if (t >= live_tiles) continue;
         __builtin_amdgcn_sched_barrier(0);  // a tile's queries at a time, for the registers
-        const int query_row = first_row + 16 * t + column, new_row = a.new_row(query_row);
+        const int query_row = first_row + 64 * t + column, new_row = a.new_row(query_row);
         const bool live = query_row < job.rows;
         const float* const from =
             a.queries + (live ? int64_t(job.first + new_row) * a.query_stride +
@@ -526,7 +527,13 @@ __device__ __forceinline__ void shared_attend_wide(const PagedView& v, const Sha
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[k][e] = live ? lo[e] : 0.f, x[k][4 + e] = live ? hi[e] : 0.f;
         }
-        to_score[t] = a.scale;
+        // Above 0, so that minus infinity stays that: a scale's sign goes into the queries.
+        to_score[t] = fmaxf(__builtin_fabsf(a.scale), 1e-37f);
+        const float sign = a.scale == 0.f ? 0.f : __builtin_copysignf(1.f, a.scale);
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[k][e] *= sign;
         if constexpr (TYPE == kPagedF16) {
             // An exact power of two brings a row's largest query to [2^14, 2^15), so that neither term leaves
             // FP16's range; non-finite ones stay so.
@@ -541,7 +548,7 @@ __device__ __forceinline__ void shared_attend_wide(const PagedView& v, const Sha
             for (int k = 0; k < kSteps; ++k)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[k][e] *= pow2(up);
-            to_score[t] *= pow2(-up);
+            to_score[t] = fmaxf(to_score[t] * pow2(-up), 0x1p-149f);
         }
 #pragma unroll
         for (int k = 0; k < kSteps; ++k)
@@ -556,119 +563,128 @@ __device__ __forceinline__ void shared_attend_wide(const PagedView& v, const Sha
     load(base);
     if (base + kPositions < end) find(base + kPositions);
 
-    for (; base < end; base += kPositions, buffer ^= 1) {
-        bool whole_here = true;
+    // The loop has no branches around a tile's products, which would wait for every piece of LDS by itself.
+    auto go = [&](auto live) {
+        constexpr int LIVE = decltype(live)::value;
+        for (; base < end; base += kPositions, buffer ^= 1) {
+            bool whole_here = true;
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            uint4_t k[kWords], w[kWords];
-            widen<TYPE>(keys[i], byte_pow2(bytes[i] & 255), k);
-            widen<TYPE>(values[i], byte_pow2(bytes[i] >> 8), w);
-            const int row = i * kAtOnce + my_row, to = row * kPitch + 16 * kWords * chunk;
+            for (int i = 0; i < kLoads; ++i) {
+                uint4_t k[kWords], w[kWords];
+                widen<TYPE>(keys[i], byte_pow2(bytes[i] & 255), k);
+                widen<TYPE>(values[i], byte_pow2(bytes[i] >> 8), w);
+                const int row = i * kAtOnce + my_row, to = row * kPitch + 16 * kWords * chunk;
 #pragma unroll
-            for (int j = 0; j < kWords; ++j) {
-                if (!there[i]) w[j] = uint4_t{0u, 0u, 0u, 0u};  // a weight of 0 does not keep NaN out
-                *reinterpret_cast<uint4_t*>(space.keys[buffer] + to + 16 * j) = k[j];
-                *reinterpret_cast<uint4_t*>(space.values[buffer] + to + 16 * j) = w[j];
+                for (int j = 0; j < kWords; ++j) {
+                    if (!there[i]) w[j] = uint4_t{0u, 0u, 0u, 0u};  // a weight of 0 does not keep NaN out
+                    *reinterpret_cast<uint4_t*>(space.keys[buffer] + to + 16 * j) = k[j];
+                    *reinterpret_cast<uint4_t*>(space.values[buffer] + to + 16 * j) = w[j];
+                }
+                if (chunk == 0) space.there[buffer][row] = there[i];
+                whole_here = whole_here && there[i];
             }
-            if (chunk == 0) space.there[buffer][row] = there[i];
-            whole_here = whole_here && there[i];
-        }
-        const bool whole_wave = __all(whole_here);
-        if (lane == 0) space.all[buffer][wave] = whole_wave;
-        if (base + kPositions < end) {
-            load(base + kPositions);
-            if (base + 2 * kPositions < end) find(base + 2 * kPositions);
-        }
-        // Nobody writes a buffer again before all have passed the next barrier, and so have read it.
-        __syncthreads();
-        if (!live_tiles) continue;
-        bool whole = true;
+            const bool whole_wave = __all(whole_here);
+            if (lane == 0) space.all[buffer][wave] = whole_wave;
+            if (base + kPositions < end) {
+                load(base + kPositions);
+                if (base + 2 * kPositions < end) find(base + 2 * kPositions);
+            }
+            // Nobody writes a buffer again before all have passed the next barrier, and so have read it.
+            __syncthreads();
+            if constexpr (!LIVE) continue;
+            bool whole = true;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) whole = whole && space.all[buffer][w];
+            for (int w = 0; w < kWaves; ++w) whole = whole && space.all[buffer][w];
 
-        // 32 positions at a time, for the registers.
+            // 32 positions at a time, for the registers.
 #pragma unroll 1
-        for (int h = 0; h < kPositions / 32; ++h) {
-            const char* const key = space.keys[buffer] + (32 * h + column) * kPitch + 16 * part;
-            const char* const transposed =
-                space.values[buffer] + (32 * h + 4 * part + (column >> 2)) * kPitch + (column & 3) * 8;
-            float4_t s[TILES][2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-#pragma unroll
-                for (int t = 0; t < TILES; ++t) s[t][u] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int k = 0; k < kSteps; ++k) {
-                    const uint4_t x = *reinterpret_cast<const uint4_t*>(key + 16 * u * kPitch + 64 * k);
-#pragma unroll
-                    for (int t = 0; t < TILES; ++t) {
-                        if (t >= live_tiles) continue;
-#pragma unroll
-                        for (int p = 0; p < kProducts; ++p) s[t][u] = multiply(x, query[t][k][p], s[t][u], kType);
-                    }
-                }
-            }
-            unsigned hidden = 0;  // bit 4 u + r
-            if (!whole)
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (!space.there[buffer][32 * h + 16 * u + 4 * part + r]) hidden |= 1u << (4 * u + r);
-            uint4_t weight[TILES][kProducts];
-#pragma unroll
-            for (int t = 0; t < TILES; ++t) {
-                if (t >= live_tiles) continue;
-                float high = -kInf;
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (whole || !(hidden >> (4 * u + r) & 1)) high = fmaxf(high, s[t][u][r] * to_score[t]);
-                if (__any(high > reference[t] + (kHead + kGrow))) {
-                    high = fmaxf(high, dev::xor_lanes<16>(high));
-                    high = fmaxf(high, dev::xor_lanes<32>(high));
-                    const float moved = fmaxf(reference[t], high - kHead);
-                    const float shrink = reference[t] == moved ? 1.f : exp2_fast(reference[t] - moved);
-                    reference[t] = moved;
-                    sum[t] *= shrink;
-#pragma unroll
-                    for (int o = 0; o < kOut; ++o) acc[t][o] *= shrink;
-                }
-                const float from = reference[t] == -kInf ? 0.f : reference[t];
+            for (int h = 0; h < kPositions / 32; ++h) {
+                const char* const key = space.keys[buffer] + (32 * h + column) * kPitch + 16 * part;
+                const char* const transposed =
+                    space.values[buffer] + (32 * h + 4 * part + (column >> 2)) * kPitch + (column & 3) * 8;
+                float4_t s[LIVE ? LIVE : 1][2];
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    float p[4];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        p[r] = exp2_fast(__builtin_fmaf(s[t][u][r], to_score[t], -from));
-                        if (!whole && (hidden >> (4 * u + r) & 1)) p[r] = 0.f;
-                        sum[t] += p[r];
-                    }
+                    for (int t = 0; t < LIVE; ++t) s[t][u] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        unsigned words[kProducts];
-                        Terms<TYPE, false>::split(p[2 * e], p[2 * e + 1], false, words);
+                    for (int k = 0; k < kSteps; ++k) {
+                        const uint4_t x = *reinterpret_cast<const uint4_t*>(key + 16 * u * kPitch + 64 * k);
 #pragma unroll
-                        for (int q = 0; q < kProducts; ++q) weight[t][q][2 * u + e] = words[q];
+                        for (int t = 0; t < LIVE; ++t) {
+#pragma unroll
+                            for (int p = 0; p < kProducts; ++p) s[t][u] = multiply(x, query[t][k][p], s[t][u], kType);
+                        }
                     }
                 }
-            }
+                unsigned hidden = 0;  // bit 4 u + r
+                if (!whole)
 #pragma unroll
-            for (int o = 0; o < kOut; ++o) {
-                const short4_t low = read_transposed(transposed + 32 * o);
-                const short4_t high = read_transposed(transposed + 16 * kPitch + 32 * o);
-                const uint4_t w = {__builtin_bit_cast(u32x2, low)[0], __builtin_bit_cast(u32x2, low)[1],
-                                   __builtin_bit_cast(u32x2, high)[0], __builtin_bit_cast(u32x2, high)[1]};
+                    for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int t = 0; t < TILES; ++t) {
-                    if (t >= live_tiles) continue;
+                        for (int r = 0; r < 4; ++r)
+                            if (!space.there[buffer][32 * h + 16 * u + 4 * part + r]) hidden |= 1u << (4 * u + r);
+                uint4_t weight[LIVE ? LIVE : 1][kProducts];
 #pragma unroll
-                    for (int p = 0; p < kProducts; ++p) acc[t][o] = multiply(w, weight[t][p], acc[t][o], kType);
+                for (int t = 0; t < LIVE; ++t) {
+                    if (!whole)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) s[t][u][r] = hidden >> (4 * u + r) & 1 ? -kInf : s[t][u][r];
+                    float high = s[t][0][0];
+#pragma unroll
+                    for (int i = 1; i < 8; ++i) high = fmaxf(high, s[t][i / 4][i % 4]);
+                    high *= to_score[t];
+                    if (__any(high > reference[t] + (kHead + kGrow))) {
+                        high = fmaxf(high, dev::xor_lanes<16>(high));
+                        high = fmaxf(high, dev::xor_lanes<32>(high));
+                        const float moved = fmaxf(reference[t], high - kHead);
+                        const float shrink = reference[t] == moved ? 1.f : exp2_fast(reference[t] - moved);
+                        reference[t] = moved;
+                        sum[t] *= shrink;
+#pragma unroll
+                        for (int o = 0; o < kOut; ++o) acc[t][o] *= shrink;
+                    }
+                    const float from = reference[t] == -kInf ? 0.f : reference[t];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        float p[4];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            p[r] = exp2_fast(__builtin_fmaf(s[t][u][r], to_score[t], -from));
+                            sum[t] += p[r];
+                        }
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            unsigned words[kProducts];
+                            Terms<TYPE, false>::split(p[2 * e], p[2 * e + 1], false, words);
+#pragma unroll
+                            for (int q = 0; q < kProducts; ++q) weight[t][q][2 * u + e] = words[q];
+                        }
+                    }
+                }
+#pragma unroll
+                for (int o = 0; o < kOut; ++o) {
+                    const short4_t low = read_transposed(transposed + 32 * o);
+                    const short4_t high = read_transposed(transposed + 16 * kPitch + 32 * o);
+                    const uint4_t w = {__builtin_bit_cast(u32x2, low)[0], __builtin_bit_cast(u32x2, low)[1],
+                                       __builtin_bit_cast(u32x2, high)[0], __builtin_bit_cast(u32x2, high)[1]};
+#pragma unroll
+                    for (int t = 0; t < LIVE; ++t) {
+        #pragma unroll
+                        for (int p = 0; p < kProducts; ++p) acc[t][o] = multiply(w, weight[t][p], acc[t][o], kType);
+                    }
                 }
             }
         }
-    }
+    };
+    if (live_tiles == TILES)
+        go(std::integral_constant<int, TILES>{});
+    else if (TILES > 1 && live_tiles)
+        go(std::integral_constant<int, 1>{});
+    else
+        go(std::integral_constant<int, 0>{});
 
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
@@ -676,7 +692,7 @@ __device__ __forceinline__ void shared_attend_wide(const PagedView& v, const Sha
         float all = sum[t];
         all += dev::xor_lanes<16>(all);
         all += dev::xor_lanes<32>(all);
-        const int query_row = first_row + 16 * t + column, new_row = a.new_row(query_row);
+        const int query_row = first_row + 64 * t + column, new_row = a.new_row(query_row);
         if (query_row >= job.rows) continue;
         const int64_t to = a.place(v, job.slot, job.first + new_row, job.head * a.group + query_row - new_row * a.group);
 #pragma unroll
@@ -723,14 +739,17 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void shared_attent
         if (g < 0) return;
         const int of_eight = index / (8 * tiles), within = index - of_eight * 8 * tiles;
         const int pair = of_eight * 8 + (within & 7);
-        job.row0 = (within >> 3) * kRows;
+        // Tiles of equal size, of whole 16 rows.
+        const int group_rows = a.rows_of(v, g), tile_rows = (group_rows + 16 * tiles - 1) / (16 * tiles) * 16;
+        job.row0 = (within >> 3) * tile_rows;
         job.head = pair / before;  // the group's parts
         index = pair - job.head * before;
         if (job.head >= v.kv_heads) return;
         const int prefix = a.prefix_of(v, g, lane, job.s);
         if (job.s >= v.sequences) return;
         job.first = a.row_of(v, a.first_of(v, g));
-        job.rows = a.rows_of(v, g);
+        job.rows = min(group_rows, job.row0 + tile_rows);
+        if (job.row0 >= job.rows) return;
         job.from = index * a.part;
         if (job.from >= prefix) return;
         job.to = index == a.parts - 1 ? prefix : min(prefix, job.from + a.part);
