@@ -84,6 +84,8 @@ void launch_paged_attention_shared(const qwen_gpu_paged_cache& cache, const qwen
                        int(plan.part),
                        int(plan.rest_part),
                        int(plan.jobs),
+                       int(plan.rest_jobs),
+                       plan.part < 2 * plan.rest_part,
                        reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.state_bytes),
                        static_cast<float2*>(workspace)};
     if (cache.type == kPagedF16)
@@ -92,7 +94,9 @@ void launch_paged_attention_shared(const qwen_gpu_paged_cache& cache, const qwen
         shared_launch<kPagedBF16>(cache.head_dim, v, a, plan, stream);
     else
         shared_launch<kPagedE4M3>(cache.head_dim, v, a, plan, stream);
-    const dim3 grid(unsigned(batch.total_rows), unsigned((row / 4 + kJoinItems - 1) / kJoinItems));
+    // A workgroup for each piece of few rows; of many, it finds its row's parts once for several pieces.
+    const int64_t pieces = (row / 4 + kJoinItems - 1) / kJoinItems;
+    const dim3 grid(unsigned(batch.total_rows), unsigned(std::clamp<int64_t>(2048 / batch.total_rows, 1, pieces)));
     if (cache.head_dim == 64)
         shared_join_kernel<64><<<grid, 256, 0, stream>>>(v, a);
     else if (cache.head_dim == 128)

@@ -22,7 +22,8 @@ struct SharedArgs {
     int rest_tiles;             // of a sequence's query rows
     int parts, rest_parts;      // of a prefix, of what is behind it, at most
     int part, rest_part;        // positions of each
-    int jobs;                   // workgroups of the prefixes
+    int jobs, rest_jobs;        // workgroups of the prefixes (a multiple of 8), of what is behind them
+    bool in_turn;               // workgroups of both kinds
     float* sums;                // [parts + rest_parts][total_rows][query_heads][DIM]
     float2* states;             // [parts + rest_parts][total_rows][query_heads]: reference, sum
 
@@ -38,18 +39,55 @@ struct SharedArgs {
     __device__ __forceinline__ int row_of(const PagedView& v, int s) const {
         return v.offsets ? min(max(v.offsets[s], 0), v.total_rows) : s * v.rows;
     }
-    // Query rows of a KV head in a group.
-    __device__ __forceinline__ int rows_of(const PagedView& v, int g) const {
-        const int from = first_of(v, g), to = first_of(v, g + 1);
-        return to > from ? max(0, row_of(v, to) - row_of(v, from)) * group : 0;
+    __device__ __forceinline__ static int parts_of(int positions, int part, int most) {
+        return min(most, (positions + part - 1) / part);
+    }
+};
+
+// The groups, as a wave knows them: of up to 63, lane g has group g's first
+// sequence and prefix, so that a job is found in two or three loads one behind
+// the other instead of five.
+struct SharedGroups {
+    const PagedView& v;
+    const SharedArgs& a;
+    const int lane;
+    const bool few;
+    int start = 0, length = 0;
+
+    __device__ __forceinline__ SharedGroups(const PagedView& view, const SharedArgs& args)
+        : v(view), a(args), lane(threadIdx.x & 63), few(args.groups < 64) {
+        if (few) {
+            start = a.first_of(v, min(lane, a.groups));
+            length = a.lengths[min(lane, a.groups - 1)];
+        }
+    }
+    __device__ __forceinline__ int first(int g) const {
+        return few ? __builtin_amdgcn_readlane(start, g) : a.first_of(v, g);
+    }
+    // Query rows of a KV head in group g0 + lane, and the parts of its prefix at most.
+    __device__ __forceinline__ void of_lane(int g0, int& rows, int& parts) const {
+        const int g = g0 + lane;
+        const bool there = g < a.groups;
+        const int from = few ? start : a.first_of(v, min(g, a.groups));
+        const int row = a.row_of(v, from);
+        int next;
+        if (few)
+            next = __shfl_down(row, 1);
+        else
+            next = a.row_of(v, a.first_of(v, min(g + 1, a.groups)));
+        rows = there ? max(0, next - row) * a.group : 0;
+        parts = there ? a.parts_of(max(0, min(few ? length : a.lengths[g], v.max_length)), a.part, a.parts) : 0;
     }
     // Group of a sequence, -1 where it has none; the same in all lanes.
-    __device__ __forceinline__ int group_of(const PagedView& v, int s, int lane) const {
-        if (!offsets) return 0;
-        int low = 0, high = groups;  // the number of groups that begin at s or before lies in low .. high
+    __device__ __forceinline__ int of(int s) const {
+        if (few) {
+            const int n = __popcll(__ballot(lane < a.groups && start <= s));
+            return n > 0 && s < __builtin_amdgcn_readlane(start, n) ? n - 1 : -1;
+        }
+        int low = 0, high = a.groups;  // the number of groups that begin at s or before lies in low .. high
         while (high > low) {
             const int step = (high - low + 63) / 64, at = low + lane * step;
-            const int n = __popcll(__ballot(at < high && offsets[min(at, groups)] <= s));
+            const int n = __popcll(__ballot(at < high && a.offsets[min(at, a.groups)] <= s));
             if (n == 0) {
                 high = low;
             } else {
@@ -58,29 +96,32 @@ struct SharedArgs {
                 low = last + 1;
             }
         }
-        return low > 0 && s < offsets[low] ? low - 1 : -1;
+        return low > 0 && s < a.offsets[low] ? low - 1 : -1;
     }
     // Positions that a group's sequences share, no more than any of them has before its new rows, and its first
     // sequence with new rows, through whose table they are read.
-    __device__ __forceinline__ int prefix_of(const PagedView& v, int g, int lane, int& reads) const {
-        if (g < 0 || !jobs) return 0;  // no group, or none that has workgroups
-        const int from = first_of(v, g), to = first_of(v, g + 1);
-        int least = lengths[g];
+    __device__ __forceinline__ int prefix(int g, int& reads) const {
+        if (g < 0 || !a.jobs) return 0;  // no group, or none that has workgroups
+        const int from = first(g), to = first(g + 1);
+        int least = few ? __builtin_amdgcn_readlane(length, g) : a.lengths[g];
         reads = to;
         for (int s = from + lane; s < to; s += 64) {
-            int first;
-            const int n = v.new_rows(s, first);
-            if (n > 0) least = min(least, v.length(s) - n), reads = min(reads, s);
+            int row;
+            const int n = v.new_rows(s, row), positions = v.length(s);
+            if (n > 0) least = min(least, positions - n), reads = min(reads, s);
         }
-        for (int off = 1; off < 64; off *= 2) {
-            least = min(least, __shfl_xor(least, off));
-            reads = min(reads, __shfl_xor(reads, off));
-        }
+        each_half([&](auto off) {
+            constexpr int kOff = decltype(off)::value;
+            least = min(least, dev::xor_lanes<kOff>(least));
+            reads = min(reads, dev::xor_lanes<kOff>(reads));
+        });
         reads = __builtin_amdgcn_readfirstlane(reads);
         return max(0, __builtin_amdgcn_readfirstlane(least));
     }
-    __device__ __forceinline__ static int parts_of(int positions, int part, int most) {
-        return min(most, (positions + part - 1) / part);
+    template <class F>
+    static __device__ __forceinline__ void each_half(F f) {
+        f(std::integral_constant<int, 32>{}), f(std::integral_constant<int, 16>{}), f(std::integral_constant<int, 8>{});
+        f(std::integral_constant<int, 4>{}), f(std::integral_constant<int, 2>{}), f(std::integral_constant<int, 1>{});
     }
 };
 
@@ -437,6 +478,15 @@ __device__ __forceinline__ void shared_attend(const PagedView& v, const SharedAr
     }
 }
 
+// 16 E4M3 values as FP16, exact.
+__device__ __forceinline__ void widen_f16(uint4_t raw, uint4_t (&out)[2]) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        out[w / 2][2 * (w % 2)] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(raw[w], 1.f, false));
+        out[w / 2][2 * (w % 2) + 1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(raw[w], 1.f, true));
+    }
+}
+
 // LDS of a workgroup whose waves share its positions: two steps' keys and
 // values, 16-bit whatever the cache's type, and which of them exist.
 template <int DIM>
@@ -445,6 +495,7 @@ struct WideSpace {
     __attribute__((aligned(16))) char keys[2][kPositions * kPitch];
     __attribute__((aligned(16))) char values[2][kPositions * kPitch];
     __attribute__((aligned(16))) int there[2][kPositions];
+    __attribute__((aligned(16))) float powers[2][kPositions];  // E4M3: of the keys
     __attribute__((aligned(16))) int all[2][kWaves];
 };
 
@@ -459,13 +510,18 @@ __device__ __forceinline__ void shared_attend_wide(const PagedView& v, const Sha
     typedef WideSpace<DIM> Space;
     constexpr int kSize = TYPE == kPagedE4M3 ? 1 : 2, kSteps = DIM / 32, kOut = DIM / 16;
     constexpr int kPositions = Space::kPositions, kPitch = Space::kPitch;
-    constexpr int kProducts = Terms<TYPE, false>::kProducts;
+    // E4M3 keys are FP16 in LDS, which holds them all, and their rows' powers of two go to the scores: two terms
+    // of a query instead of three. Values' powers belong to the sums over positions, so values become BF16.
+    constexpr bool kScaled = TYPE == kPagedE4M3;
+    constexpr int kKeyType = kScaled ? kPagedF16 : TYPE;
+    constexpr int kProducts = Terms<TYPE, false>::kProducts, kTerms = Terms<kKeyType, false>::kProducts;
     constexpr int kChunks = DIM * kSize / 16;     // threads of a stored row, 16 bytes each
     constexpr int kAtOnce = kWaves * 64 / kChunks, kLoads = kPositions / kAtOnce;  // rows of a load; loads
     constexpr int kWords = TYPE == kPagedE4M3 ? 2 : 1;
     constexpr float kHead = TYPE == kPagedF16 ? 6.f : 0.f;  // FP16 weights are kept up to 2^14, far from subnormals
     constexpr float kGrow = 8.f;                  // a reference is moved once a score passes it by 2^8
     constexpr std::integral_constant<int, TYPE> kType{};
+    constexpr std::integral_constant<int, kKeyType> kKeys{};
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int column = lane & 15, part = lane >> 4;
     const int my_row = threadIdx.x / kChunks, chunk = threadIdx.x % kChunks, end = job.to;
@@ -503,7 +559,7 @@ __device__ __forceinline__ void shared_attend_wide(const PagedView& v, const Sha
     // A wave's tiles are four apart, so that fewer than 4 * TILES of them are shared out evenly.
     const int first_row = job.row0 + 16 * wave;
     const int live_tiles = first_row < job.rows ? min(TILES, (job.rows - first_row + 63) / 64) : 0;
-    uint4_t query[TILES][kSteps][kProducts];
+    uint4_t query[TILES][kSteps][kTerms];
     float to_score[TILES], reference[TILES], sum[TILES];
     float4_t acc[TILES][kOut];
 #pragma unroll
@@ -534,7 +590,7 @@ __device__ __forceinline__ void shared_attend_wide(const PagedView& v, const Sha
         for (int k = 0; k < kSteps; ++k)
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[k][e] *= sign;
-        if constexpr (TYPE == kPagedF16) {
+        if constexpr (kKeyType == kPagedF16) {
             // An exact power of two brings a row's largest query to [2^14, 2^15), so that neither term leaves
             // FP16's range; non-finite ones stay so.
 #pragma unroll
@@ -554,10 +610,10 @@ __device__ __forceinline__ void shared_attend_wide(const PagedView& v, const Sha
         for (int k = 0; k < kSteps; ++k)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                unsigned words[kProducts];
-                Terms<TYPE, false>::split(x[k][2 * e], x[k][2 * e + 1], false, words);
+                unsigned words[kTerms];
+                Terms<kKeyType, false>::split(x[k][2 * e], x[k][2 * e + 1], false, words);
 #pragma unroll
-                for (int p = 0; p < kProducts; ++p) query[t][k][p][e] = words[p];
+                for (int p = 0; p < kTerms; ++p) query[t][k][p][e] = words[p];
             }
     }
     load(base);
@@ -571,7 +627,10 @@ __device__ __forceinline__ void shared_attend_wide(const PagedView& v, const Sha
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
                 uint4_t k[kWords], w[kWords];
-                widen<TYPE>(keys[i], byte_pow2(bytes[i] & 255), k);
+                if constexpr (kScaled)
+                    widen_f16(keys[i], k);
+                else
+                    widen<TYPE>(keys[i], 1.f, k);
                 widen<TYPE>(values[i], byte_pow2(bytes[i] >> 8), w);
                 const int row = i * kAtOnce + my_row, to = row * kPitch + 16 * kWords * chunk;
 #pragma unroll
@@ -580,7 +639,10 @@ __device__ __forceinline__ void shared_attend_wide(const PagedView& v, const Sha
                     *reinterpret_cast<uint4_t*>(space.keys[buffer] + to + 16 * j) = k[j];
                     *reinterpret_cast<uint4_t*>(space.values[buffer] + to + 16 * j) = w[j];
                 }
-                if (chunk == 0) space.there[buffer][row] = there[i];
+                if (chunk == 0) {
+                    space.there[buffer][row] = there[i];
+                    if constexpr (kScaled) space.powers[buffer][row] = byte_pow2(bytes[i] & 255);
+                }
                 whole_here = whole_here && there[i];
             }
             const bool whole_wave = __all(whole_here);
@@ -613,10 +675,15 @@ __device__ __forceinline__ void shared_attend_wide(const PagedView& v, const Sha
 #pragma unroll
                         for (int t = 0; t < LIVE; ++t) {
 #pragma unroll
-                            for (int p = 0; p < kProducts; ++p) s[t][u] = multiply(x, query[t][k][p], s[t][u], kType);
+                            for (int p = 0; p < kTerms; ++p) s[t][u] = multiply(x, query[t][k][p], s[t][u], kKeys);
                         }
                     }
                 }
+                float4_t powers[2];
+                if constexpr (kScaled)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+                        powers[u] = *reinterpret_cast<const float4_t*>(space.powers[buffer] + 32 * h + 16 * u + 4 * part);
                 unsigned hidden = 0;  // bit 4 u + r
                 if (!whole)
 #pragma unroll
@@ -632,10 +699,20 @@ __device__ __forceinline__ void shared_attend_wide(const PagedView& v, const Sha
                         for (int u = 0; u < 2; ++u)
 #pragma unroll
                             for (int r = 0; r < 4; ++r) s[t][u][r] = hidden >> (4 * u + r) & 1 ? -kInf : s[t][u][r];
-                    float high = s[t][0][0];
+                    float high, factor[2][4];
+                    if constexpr (kScaled) {
+                        high = -kInf;
 #pragma unroll
-                    for (int i = 1; i < 8; ++i) high = fmaxf(high, s[t][i / 4][i % 4]);
-                    high *= to_score[t];
+                        for (int i = 0; i < 8; ++i) {
+                            factor[i / 4][i % 4] = fmaxf(to_score[t] * powers[i / 4][i % 4], 0x1p-149f);
+                            high = fmaxf(high, s[t][i / 4][i % 4] * factor[i / 4][i % 4]);
+                        }
+                    } else {
+                        high = s[t][0][0];
+#pragma unroll
+                        for (int i = 1; i < 8; ++i) high = fmaxf(high, s[t][i / 4][i % 4]);
+                        high *= to_score[t];
+                    }
                     if (__any(high > reference[t] + (kHead + kGrow))) {
                         high = fmaxf(high, dev::xor_lanes<16>(high));
                         high = fmaxf(high, dev::xor_lanes<32>(high));
@@ -652,7 +729,7 @@ __device__ __forceinline__ void shared_attend_wide(const PagedView& v, const Sha
                         float p[4];
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            p[r] = exp2_fast(__builtin_fmaf(s[t][u][r], to_score[t], -from));
+                            p[r] = exp2_fast(__builtin_fmaf(s[t][u][r], kScaled ? factor[u][r] : to_score[t], -from));
                             sum[t] += p[r];
                         }
 #pragma unroll
@@ -672,7 +749,7 @@ __device__ __forceinline__ void shared_attend_wide(const PagedView& v, const Sha
                                        __builtin_bit_cast(u32x2, high)[0], __builtin_bit_cast(u32x2, high)[1]};
 #pragma unroll
                     for (int t = 0; t < LIVE; ++t) {
-        #pragma unroll
+#pragma unroll
                         for (int p = 0; p < kProducts; ++p) acc[t][o] = multiply(w, weight[t][p], acc[t][o], kType);
                     }
                 }
@@ -713,25 +790,38 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void shared_attent
         SharedSpace<DIM> narrow;
         WideSpace<DIM> wide;
     } space;
-    const int lane = threadIdx.x & 63;
+    const SharedGroups groups(v, a);
+    // Both kinds in turn, 8 workgroups at a time (one an XCD) and 256 of them the other way round, so that a CU gets
+    // one of each: a prefix's products run beside the loads of what is behind it.
+    int block = blockIdx.x;
+    bool of_prefix;
+    const int both = a.in_turn ? 2 * min(a.jobs, (a.rest_jobs + 7) / 8 * 8) : 0;
+    if (block < both) {
+        of_prefix = !((block / 8 + block / 256) & 1);
+        block = block / 16 * 8 + block % 8;
+    } else {
+        of_prefix = block - both / 2 < a.jobs;
+        block -= of_prefix ? both / 2 : both ? both / 2 : a.jobs;
+    }
     SharedJob job;
-    if (int(blockIdx.x) < a.jobs) {
+    if (of_prefix) {
         // Each group has its tiles for each head and part of its prefix. Those of one head and part are 8 workgroups
         // apart, on one XCD, whose L2 reads its positions once for all; workgroups without work come behind all
         // others (between them, they left half of the CUs with twice the work: 65000 positions took 205 us, not 110).
-        int before = 0, g = -1, tiles = 0, index = 0;
+        int before = 0, g = -1, tiles = 0, index = 0, group_rows = 0, most = 0;
         for (int g0 = 0; g0 < a.groups; g0 += 64) {
-            const bool there = g0 + lane < a.groups;
-            const int of_lane = there ? (a.rows_of(v, g0 + lane) + kRows - 1) / kRows : 0;
-            const int most = there ? a.parts_of(max(0, min(a.lengths[g0 + lane], v.max_length)), a.part, a.parts) : 0;
-            const int count = (most * v.kv_heads + 7) / 8 * 8 * of_lane, upto = before + scan_lanes(count);
-            const unsigned long long hit = __ballot(upto > int(blockIdx.x));
+            int rows, parts;
+            groups.of_lane(g0, rows, parts);
+            const int of_lane = (rows + kRows - 1) / kRows;
+            const int count = (parts * v.kv_heads + 7) / 8 * 8 * of_lane, upto = before + scan_lanes(count);
+            const unsigned long long hit = __ballot(upto > block);
             if (hit) {
                 const int at = __ffsll(hit) - 1;
                 g = g0 + at;
                 tiles = __builtin_amdgcn_readlane(of_lane, at);
-                index = blockIdx.x - __builtin_amdgcn_readlane(upto - count, at);
-                before = __builtin_amdgcn_readlane(most, at);
+                index = block - __builtin_amdgcn_readlane(upto - count, at);
+                most = __builtin_amdgcn_readlane(parts, at);
+                group_rows = __builtin_amdgcn_readlane(rows, at);
                 break;
             }
             before = __builtin_amdgcn_readlane(upto, 63);
@@ -740,14 +830,14 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void shared_attent
         const int of_eight = index / (8 * tiles), within = index - of_eight * 8 * tiles;
         const int pair = of_eight * 8 + (within & 7);
         // Tiles of equal size, of whole 16 rows.
-        const int group_rows = a.rows_of(v, g), tile_rows = (group_rows + 16 * tiles - 1) / (16 * tiles) * 16;
+        const int tile_rows = (group_rows + 16 * tiles - 1) / (16 * tiles) * 16;
         job.row0 = (within >> 3) * tile_rows;
-        job.head = pair / before;  // the group's parts
-        index = pair - job.head * before;
+        job.head = pair / most;
+        index = pair - job.head * most;
         if (job.head >= v.kv_heads) return;
-        const int prefix = a.prefix_of(v, g, lane, job.s);
+        const int prefix = groups.prefix(g, job.s);
         if (job.s >= v.sequences) return;
-        job.first = a.row_of(v, a.first_of(v, g));
+        job.first = a.row_of(v, groups.first(g));
         job.rows = min(group_rows, job.row0 + tile_rows);
         if (job.row0 >= job.rows) return;
         job.from = index * a.part;
@@ -760,18 +850,20 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void shared_attent
         else
             shared_attend<TYPE, DIM, 1, false>(v, a, job, space.narrow);
     } else {
-        int at = blockIdx.x - a.jobs;
-        const int index = at % a.rest_parts;
-        at /= a.rest_parts;
+        if (block >= a.rest_jobs) return;
+        // First parts first: of ragged lengths, the last parts are those that some sequences do not have.
+        int at = block;
         job.row0 = at % a.rest_tiles * kRestRows;
         at /= a.rest_tiles;
         job.s = at % v.sequences;
-        job.head = at / v.sequences;
+        at /= v.sequences;
+        job.head = at % v.kv_heads;
+        const int index = at / v.kv_heads;
         const int n = v.new_rows(job.s, job.first), length = v.length(job.s);
         job.rows = n * a.group;
         if (job.row0 >= job.rows) return;
         int reads;
-        const int prefix = a.prefix_of(v, a.group_of(v, job.s, lane), lane, reads);
+        const int prefix = groups.prefix(groups.of(job.s), reads);
         job.from = prefix + index * a.rest_part;
         if (job.from >= length) return;
         job.to = index == a.rest_parts - 1 ? length : min(length, job.from + a.rest_part);
@@ -789,64 +881,69 @@ template <int DIM>
 __global__ __launch_bounds__(kWaves * 64) void shared_join_kernel(PagedView v, SharedArgs a) {
     __shared__ float4_t sums[kWaves][kJoinItems];
     __shared__ float2 states[kWaves][kJoinItems];
+    const SharedGroups groups(v, a);
     const int row = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int s = v.sequence_of(row, lane);
     if (s < 0) return;
     int first, reads;
     const int n = v.new_rows(s, first);
     if (row - first >= n) return;
-    const int prefix = a.prefix_of(v, a.group_of(v, s, lane), lane, reads);
+    const int prefix = groups.prefix(groups.of(s), reads);
     const int shared = a.parts_of(prefix, a.part, a.parts);
     const int count = shared + a.parts_of(max(0, v.length(s) - prefix), a.rest_part, a.rest_parts);
-    const int item = blockIdx.y * kJoinItems + lane, head = min(item / (DIM / 4), a.query_heads - 1);
-    const int channel = 4 * (item % (DIM / 4));
-    float top = -kInf, all = 0.f;
-    float4_t o = {0.f, 0.f, 0.f, 0.f};
-    constexpr int kFlight = 8;  // parts whose sums are loaded at a time
-    for (int p0 = wave; p0 < count; p0 += kFlight * kWaves) {
-        float2 state[kFlight];
-        float4_t x[kFlight];
+    for (int piece = blockIdx.y; piece * kJoinItems < a.query_heads * (DIM / 4); piece += gridDim.y) {
+        const int item = piece * kJoinItems + lane, head = min(item / (DIM / 4), a.query_heads - 1);
+        const int channel = 4 * (item % (DIM / 4));
+        float top = -kInf, all = 0.f;
+        float4_t o = {0.f, 0.f, 0.f, 0.f};
+        constexpr int kFlight = 8;  // parts whose sums are loaded at a time
+        for (int p0 = wave; p0 < count; p0 += kFlight * kWaves) {
+            float2 state[kFlight];
+            float4_t x[kFlight];
 #pragma unroll
-        for (int p = 0; p < kFlight; ++p) {
-            const int index = min(p0 + p * kWaves, count - 1);
-            const int64_t from = a.place(v, index < shared ? index : a.parts + index - shared, row, head);
-            state[p] = a.states[from];
-            x[p] = *reinterpret_cast<const float4_t*>(a.sums + from * DIM + channel);
+            for (int p = 0; p < kFlight; ++p) {
+                const int index = min(p0 + p * kWaves, count - 1);
+                const int64_t from = a.place(v, index < shared ? index : a.parts + index - shared, row, head);
+                state[p] = a.states[from];
+                x[p] = *reinterpret_cast<const float4_t*>(a.sums + from * DIM + channel);
+            }
+            float grown = top;
+#pragma unroll
+            for (int p = 0; p < kFlight; ++p) grown = fmaxf(grown, state[p].x);
+            const float shrink = top == grown ? 1.f : exp2_fast(top - grown);
+            top = grown;
+            all *= shrink;
+            o *= shrink;
+#pragma unroll
+            for (int p = 0; p < kFlight; ++p) {
+                if (p0 + p * kWaves >= count) continue;
+                const float by = state[p].x == top ? 1.f : exp2_fast(state[p].x - top);
+                all = __builtin_fmaf(state[p].y, by, all);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(x[p][e], by, o[e]);
+            }
         }
-        float grown = top;
+        states[wave][lane] = float2{top, all};
+        sums[wave][lane] = o;
+        __syncthreads();
+        if (wave == 0 && item < a.query_heads * (DIM / 4)) {
 #pragma unroll
-        for (int p = 0; p < kFlight; ++p) grown = fmaxf(grown, state[p].x);
-        const float shrink = top == grown ? 1.f : exp2_fast(top - grown);
-        top = grown;
-        all *= shrink;
-        o *= shrink;
+            for (int w = 1; w < kWaves; ++w) top = fmaxf(top, states[w][lane].x);
+            all = 0.f;
+            o = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int p = 0; p < kFlight; ++p) {
-            if (p0 + p * kWaves >= count) continue;
-            const float by = state[p].x == top ? 1.f : exp2_fast(state[p].x - top);
-            all = __builtin_fmaf(state[p].y, by, all);
+            for (int w = 0; w < kWaves; ++w) {
+                const float2 state = states[w][lane];
+                const float by = state.x == top ? 1.f : exp2_fast(state.x - top);
+                all = __builtin_fmaf(state.y, by, all);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(x[p][e], by, o[e]);
+                for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(sums[w][lane][e], by, o[e]);
+            }
+            o = all == 0.f ? float4_t{0.f, 0.f, 0.f, 0.f} : o * (1.f / all);
+            *reinterpret_cast<float4_a4*>(a.out + row * a.out_stride + item * 4) = o;
         }
+        __syncthreads();  // LDS is written anew
     }
-    states[wave][lane] = float2{top, all};
-    sums[wave][lane] = o;
-    __syncthreads();
-    if (wave || item >= a.query_heads * (DIM / 4)) return;
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, states[w][lane].x);
-    all = 0.f;
-    o = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-        const float2 state = states[w][lane];
-        const float by = state.x == top ? 1.f : exp2_fast(state.x - top);
-        all = __builtin_fmaf(state.y, by, all);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(sums[w][lane][e], by, o[e]);
-    }
-    o = all == 0.f ? float4_t{0.f, 0.f, 0.f, 0.f} : o * (1.f / all);
-    *reinterpret_cast<float4_a4*>(a.out + row * a.out_stride + item * 4) = o;
 }
 
 // Sizes of a call: how its work is split, and what its workspace holds.
@@ -885,7 +982,7 @@ struct SharedPlan {
 template <int TYPE, int DIM, int WIDE>
 void shared_run(const PagedView& v, const SharedArgs& a, const SharedPlan& plan, hipStream_t stream) {
     shared_attention_kernel<TYPE, DIM, WIDE>
-        <<<unsigned(plan.jobs + plan.rest_jobs), kWaves * 64, 0, stream>>>(v, a);
+        <<<unsigned(plan.jobs + (plan.rest_jobs + 7) / 8 * 8), kWaves * 64, 0, stream>>>(v, a);
 }
 
 template <int TYPE>
