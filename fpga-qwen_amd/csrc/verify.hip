@@ -23,8 +23,8 @@ constexpr int kThreads = 256, kWaves = kThreads / 64, kEach = 16;
 constexpr int kChunk = kThreads * kEach;  // tokens of a workgroup
 constexpr float kInf = __builtin_huge_valf();
 
-// Of a row and a chunk: its largest logit, the lowest token that has it, and
-// the sum of the weights relative to it.
+// Of a range of a row: its largest logit, the lowest token that has it (where
+// the largest wins), and the sum of the weights relative to it.
 struct Part {
     double sum;
     float top;
@@ -48,9 +48,10 @@ struct VerifyArgs {
     const float *temperature, *accept, *sample;
     int64_t logit_stride, draft_stride;
     int vocabulary, chunks, sequences, rows, total_rows;
-    Part* parts;        // [total_rows][chunks]
-    double* rest;       // [sequences][chunks]: sums of max(p - q, 0)
-    Verdict* verdicts;  // [sequences]
+    int ranges, draw_chunks;    // ranges that a row's sums are made of; chunks of a workgroup that draws
+    Part* parts;        // [total_rows][ranges]
+    double* rest;       // [sequences][chunks]: sums of the weights that a token is drawn from
+    int* done;          // [sequences]: workgroups that have added up their chunks, 0 before the second kernel
     int32_t *accepted, *next, *back;
 
     // First row of a sequence and how many of them there are.
@@ -64,19 +65,18 @@ struct VerifyArgs {
         const int64_t n = min(int64_t(offsets[s + 1]) - first, int64_t(total_rows) - first);
         return n < 0 ? 0 : int(min(n, int64_t(rows)));
     }
-    // log2(e) / T; 0: the largest logit alone counts.
+    // 64 log2(e) / T; 0: the largest logit alone counts.
     __device__ double heat(int s) const {
         const float t = temperature ? temperature[s] : 1.f;
-        return t > 0.f ? 1.44269504088896340736 / t : 0.;
+        return t > 0.f ? 64 * 1.44269504088896340736 / t : 0.;
     }
     __device__ bool greedy(int s) const { return temperature && !(temperature[s] > 0.f); }
 };
 
-// 2^z for z <= 0, 0 for NaN: the power of the nearest whole number, and the
-// exponential series of the rest (at most ln(2) / 2 from 0, where the first
-// term left out is 6e-15 of the whole).
-__device__ __forceinline__ double power(double z) {
-    z = fmax(z, -1100.);
+// 2^z for z <= 0 through the exponential series of its part behind the whole
+// number (at most ln(2) / 2 from 0, where the first term left out is 6e-15 of
+// the whole).
+__device__ __forceinline__ double series(double z) {
     const double whole = rint(z), x = (z - whole) * 0.693147180559945309417;
     double p = 1. / 39916800;
     p = __builtin_fma(p, x, 1. / 3628800);
@@ -92,12 +92,50 @@ __device__ __forceinline__ double power(double z) {
     p = __builtin_fma(p, x, 1.);
     return __builtin_amdgcn_ldexp(p, int(whole));
 }
-// Weight of a logit in a row (or chunk) whose largest is `top`. Minus
-// infinity and NaN weigh nothing; with a top of infinity only equal logits do.
-__device__ __forceinline__ double weight(float x, float top, double heat) {
-    if (top == kInf || top == -kInf) return x == kInf ? 1. : 0.;
-    return power((double(x) - double(top)) * heat);
-}
+
+// Weights of tokens. 2^z as 2^n * 2^(j / 64) * 2^r with the 64 powers in LDS
+// and |r| <= 1 / 128, where four terms of the series are 4e-14 off: the FP64
+// operations of a token bound the kernel, 13 of them here, 21 with the
+// series alone (260 rows of 151936 BF16 logits took 47 us with that).
+struct Powers {
+    double at[64];
+
+    __device__ __forceinline__ void make() {  // by all threads of a workgroup, before a barrier
+        if (threadIdx.x < 64) at[threadIdx.x] = series(threadIdx.x / 64. - 1.) * 2.;
+    }
+    // 2^(z / 64) for -64000 <= z <= 0.
+    __device__ __forceinline__ double within(double z) const {
+        constexpr double kRound = 6755399441055744.;  // 1.5 * 2^52: adding it leaves the nearest whole number in the low bits
+        constexpr double kLn = 0.693147180559945309417 / 64;
+        const double shifted = z + kRound, x = z - (shifted - kRound);
+        const int whole = int(__builtin_bit_cast(uint64_t, shifted));
+        double p = kLn * kLn * kLn * kLn / 24;
+        p = __builtin_fma(p, x, kLn * kLn * kLn / 6);
+        p = __builtin_fma(p, x, kLn * kLn / 2);
+        p = __builtin_fma(p, x, kLn);
+        p = __builtin_fma(p, x, 1.);
+        const uint64_t bits = __builtin_bit_cast(uint64_t, p * at[whole & 63]);
+        const unsigned high = unsigned(bits >> 32) + (unsigned(whole & ~63) << 14);
+        return __builtin_bit_cast(double, (bits & 0xffffffffu) | uint64_t(high) << 32);
+    }
+    // The same for z <= 0; 0 for NaN and below 2^-1000.
+    __device__ __forceinline__ double of(double z) const {
+        const bool tiny = !(z >= -64000.);
+        const double w = within(tiny ? 0. : z);
+        return tiny ? 0. : w;
+    }
+    // Of finite tops, with 2^-1000 for what weighs nothing: for sums, which it does not change.
+    __device__ __forceinline__ double summand(float x, float top, double heat) const {
+        return within(fmax((double(x) - double(top)) * heat, -64000.));
+    }
+    // Weight of a logit in a row (or chunk) whose largest is `top`, heat 64 log2(e) / T. Minus infinity and NaN weigh
+    // nothing; with a top of infinity (FINITE: it is known to be none) only equal logits do.
+    template <bool FINITE = false>
+    __device__ __forceinline__ double weight(float x, float top, double heat) const {
+        if (!FINITE && (top == kInf || top == -kInf)) return x == kInf ? 1. : 0.;
+        return of((double(x) - double(top)) * heat);
+    }
+};
 
 template <typename T>
 __device__ __forceinline__ float logit(const char* logits, int64_t at) {
@@ -105,36 +143,44 @@ __device__ __forceinline__ float logit(const char* logits, int64_t at) {
 }
 
 // A thread's 16 tokens of a chunk. `together`: 16 in a row, otherwise the
-// pieces of 16 bytes that make a wave's load one range.
+// pieces of 16 bytes that make a wave's load one range. The loads of a chunk
+// have no branches of their own, so that all are in flight at once.
 template <typename T>
 struct Tokens {
     static constexpr int kPiece = 16 / sizeof(T), kPieces = kEach / kPiece;
     typedef T piece_t __attribute__((ext_vector_type(kPiece), aligned(sizeof(T))));
-    static __device__ __forceinline__ int at(int piece, bool together) {
-        return together ? threadIdx.x * kEach + piece * kPiece : (piece * kThreads + threadIdx.x) * kPiece;
+    piece_t raw[kPieces];
+
+    static __device__ __forceinline__ int at(int i, bool together) {
+        const int piece = i / kPiece;
+        return i % kPiece + (together ? threadIdx.x * kEach + piece * kPiece : (piece * kThreads + threadIdx.x) * kPiece);
     }
-    // x[i] is token at(i / kPiece) + i % kPiece of the chunk; minus infinity behind the vocabulary and for NaN.
-    static __device__ __forceinline__ void load(const char* logits, int64_t row, int from, int vocabulary, bool together,
-                                                float (&x)[kEach]) {
-        const T* const p = reinterpret_cast<const T*>(logits) + row + from;
+    // `behind` stands for tokens past the end.
+    __device__ __forceinline__ void load(const T* row, int from, int vocabulary, bool together, T behind) {
+        if (from + kChunk <= vocabulary) {
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-            const int t = at(i, together);
-            if (from + t + kPiece <= vocabulary) {
-                const piece_t v = *reinterpret_cast<const piece_t*>(p + t);
+            for (int i = 0; i < kPieces; ++i)
+                raw[i] = *reinterpret_cast<const piece_t*>(row + from + at(i * kPiece, together));
+        } else {
 #pragma unroll
-                for (int j = 0; j < kPiece; ++j) x[i * kPiece + j] = float(v[j]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < kPiece; ++j) x[i * kPiece + j] = from + t + j < vocabulary ? float(p[t + j]) : -kInf;
+            for (int i = 0; i < kEach; ++i) {
+                const int token = from + at(i, together);
+                const T x = row[min(token, vocabulary - 1)];
+                raw[i / kPiece][i % kPiece] = token < vocabulary ? x : behind;
             }
         }
-#pragma unroll
-        for (int i = 0; i < kEach; ++i)
-            if (!(x[i] == x[i])) x[i] = -kInf;
+    }
+    __device__ __forceinline__ float value(int i) const { return float(raw[i / kPiece][i % kPiece]); }
+    // NaN counts as minus infinity.
+    __device__ __forceinline__ float logit(int i) const {
+        const float x = value(i);
+        return x == x ? x : -kInf;
     }
 };
 
+__device__ __forceinline__ float uniform(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+}
 __device__ __forceinline__ int wave_min(int x) {
     x = min(x, dev::xor_lanes<32>(x));
     x = min(x, dev::xor_lanes<16>(x));
@@ -144,16 +190,23 @@ __device__ __forceinline__ int wave_min(int x) {
     return min(x, dev::xor_lanes<1>(x));
 }
 
-// A chunk of a row: its largest logit and the sum of its weights.
+// A range of a row, of whole chunks: its largest logit and the sum of its
+// weights, each lane by itself until the end, with the next chunk's logits on
+// their way. The largest is wanted as a token where it wins.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void verify_parts_kernel(VerifyArgs a) {
+    __shared__ Powers powers;
     __shared__ double sums[kWaves];
     __shared__ float tops[kWaves];
     __shared__ int bests[kWaves];
-    const int row = blockIdx.x / a.chunks, chunk = blockIdx.x - row * a.chunks, from = chunk * kChunk;
+    const int row = blockIdx.x / a.ranges, range = blockIdx.x - row * a.ranges;
+    const int first = int(int64_t(a.chunks) * range / a.ranges), end = int(int64_t(a.chunks) * (range + 1) / a.ranges);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    float x[kEach];
-    Tokens<T>::load(a.logits, row * a.logit_stride, from, a.vocabulary, false, x);
+    const T* const logits = reinterpret_cast<const T*>(a.logits) + row * a.logit_stride;
+    Tokens<T> tokens;
+    tokens.load(logits, first * kChunk, a.vocabulary, false, T(-kInf));
+    powers.make();
+    for (int s = blockIdx.x * kThreads + threadIdx.x; s < a.sequences; s += gridDim.x * kThreads) a.done[s] = 0;
     // The row's sequence: the last one that does not start behind it.
     int s;
     if (a.offsets) {
@@ -170,43 +223,80 @@ __global__ __launch_bounds__(kThreads) void verify_parts_kernel(VerifyArgs a) {
         s = row / a.rows;
     }
     const double heat = a.heat(s);
-    float top = x[0];
-#pragma unroll
-    for (int i = 1; i < kEach; ++i) top = fmaxf(top, x[i]);
-    top = dev::wave_max(top);
-    if (lane == 0) tops[wave] = top;
+    const bool greedy = a.greedy(s);
+    // Weights below 2^-90 of a lane's largest would not change its sum: what a filter has left out costs nothing.
+    const float span = heat > 0. ? float(64 * 90 / heat) : kInf;
     __syncthreads();
-    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-    int best = a.vocabulary;
-#pragma unroll
-    for (int i = kEach - 1; i >= 0; --i)
-        if (x[i] == top) best = from + Tokens<T>::at(i / Tokens<T>::kPiece, false) + i % Tokens<T>::kPiece;
-    best = wave_min(best);
+    float top = -kInf;
     double sum = 0.;
+    int best = a.vocabulary;
+    for (int chunk = first; chunk < end; ++chunk) {
+        const int from = chunk * kChunk;
+        float x[kEach];
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) sum += weight(x[i], top, heat);
-    sum = dev::wave_sum(sum);
+        for (int i = 0; i < kEach; ++i) x[i] = tokens.value(i);
+        if (chunk + 1 < end) tokens.load(logits, from + kChunk, a.vocabulary, false, T(-kInf));
+        float high = x[0];
+#pragma unroll
+        for (int i = 1; i < kEach; ++i) high = fmaxf(high, x[i]);  // NaN is passed over
+        if (greedy) {
+            if (__any(high > top)) {
+#pragma unroll
+                for (int i = kEach - 1; i >= 0; --i)
+                    if (high > top && x[i] == high) best = from + Tokens<T>::at(i, false);
+                top = fmaxf(top, high);
+            }
+            continue;
+        }
+        if (high > top) {
+            // Infinities: all of the weight, counted below.
+            sum = high == kInf || top == -kInf ? 0. : sum * powers.weight<true>(top, high, heat);
+            top = high;
+        }
+        if (!__any(high > -kInf && high >= top - span)) continue;
+        if (__any(top == kInf)) {
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) sum += powers.weight(x[i], top, heat);
+            continue;
+        }
+#pragma unroll
+        for (int i = 0; i < kEach; i += 4)
+            if (const float four = fmaxf(fmaxf(x[i], x[i + 1]), fmaxf(x[i + 2], x[i + 3])); __any(four > -kInf && four >= top - span))
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum += powers.summand(x[i + j], top, heat);
+    }
+    // All lanes' by the largest of all (a lane without tokens has added 2^-1000 up at most); where it wins, its sum is 1 and the token the lowest that has it.
+    auto weigh = [&](float of, float whole) { return of == whole ? 1. : powers.weight(of, whole, heat); };
+    float whole = dev::wave_max(top);
+    if (lane == 0) tops[wave] = whole;
+    __syncthreads();
+    whole = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    best = wave_min(top == whole ? best : a.vocabulary);
+    sum = dev::wave_sum(top == -kInf ? 0. : sum * weigh(top, whole));
     if (lane == 0) {
         sums[wave] = sum;
         bests[wave] = best;
     }
     __syncthreads();
     if (threadIdx.x == 0)
-        a.parts[int64_t(row) * a.chunks + chunk] = {(sums[0] + sums[1]) + (sums[2] + sums[3]), top,
-                                                    min(min(bests[0], bests[1]), min(bests[2], bests[3]))};
+        a.parts[int64_t(row) * a.ranges + range] = {
+            greedy ? double(whole > -kInf) : (sums[0] + sums[1]) + (sums[2] + sums[3]), whole,
+            min(min(bests[0], bests[1]), min(bests[2], bests[3]))};
 }
 
 // A row's parts together, by a wave; the same in all lanes.
-__device__ __forceinline__ Part whole_row(const VerifyArgs& a, int row, double heat, int lane) {
-    const Part* const parts = a.parts + int64_t(row) * a.chunks;
-    float top = -kInf;
-    for (int c = lane; c < a.chunks; c += 64) top = fmaxf(top, parts[c].top);
+__device__ __forceinline__ Part whole_row(const VerifyArgs& a, const Powers& powers, int row, double heat, int lane) {
+    const Part* const parts = a.parts + int64_t(row) * a.ranges;
+    const Part none{0., -kInf, a.vocabulary};
+    const Part first = lane < a.ranges ? parts[lane] : none;
+    float top = first.top;
+    for (int c = lane + 64; c < a.ranges; c += 64) top = fmaxf(top, parts[c].top);
     top = dev::wave_max(top);
     double sum = 0.;
     int best = a.vocabulary;
-    for (int c = lane; c < a.chunks; c += 64) {
-        const Part part = parts[c];
-        sum = __builtin_fma(part.sum, part.top == top ? 1. : weight(part.top, top, heat), sum);
+    for (int c = lane; c < a.ranges; c += 64) {
+        const Part part = c == lane ? first : parts[c];
+        sum = __builtin_fma(part.sum, part.top == top ? 1. : powers.weight(part.top, top, heat), sum);
         if (part.top == top) best = min(best, part.best);
     }
     sum = dev::wave_sum(sum);
@@ -223,94 +313,49 @@ struct Drawn {
     bool judged;       // less q
     const float* q;    // of the row, or NULL: all at the token
     int token;
+    const Powers& powers;
 
-    __device__ __forceinline__ double operator()(float x, float of_q, int at) const {
-        const double p = weight(x, top, heat) * by;
-        if (!judged) return p;
-        if (!q) return at == token ? 0. : p;
-        return fmax(p - fmax(double(of_q), 0.), 0.);
-    }
     // The weights of a thread's tokens of a chunk (their places as Tokens<T> has them).
     template <typename T>
     __device__ __forceinline__ void load(const VerifyArgs& a, int row, int from, bool together, double (&w)[kEach]) const {
-        float x[kEach], of_q[kEach];
-        Tokens<T>::load(a.logits, row * a.logit_stride, from, a.vocabulary, together, x);
-#pragma unroll
-        for (int i = 0; i < Tokens<T>::kPieces; ++i) {
-            const int t = Tokens<T>::at(i, together);
-#pragma unroll
-            for (int j = 0; j < Tokens<T>::kPiece; j += 4) {
+        Tokens<T> logits;
+        logits.load(reinterpret_cast<const T*>(a.logits) + row * a.logit_stride, from, a.vocabulary, together, T(-kInf));
+        float of_q[kEach];
+        if (judged && q) {
+            if (from + kChunk <= a.vocabulary) {
                 typedef float float4_a4 __attribute__((ext_vector_type(4), aligned(4)));
-                float* const to = of_q + i * Tokens<T>::kPiece + j;
-                if (judged && q && from + t + j + 4 <= a.vocabulary) {
-                    const float4_a4 v = *reinterpret_cast<const float4_a4*>(q + from + t + j);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) to[e] = v[e];
-                } else {
+                for (int i = 0; i < kEach; i += 4) {
+                    const float4_a4 v = *reinterpret_cast<const float4_a4*>(q + from + Tokens<T>::at(i, together));
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) to[e] = judged && q && from + t + j + e < a.vocabulary ? q[from + t + j + e] : 0.f;
+                    for (int e = 0; e < 4; ++e) of_q[i + e] = v[e];
                 }
+            } else {
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) of_q[i] = q[min(from + Tokens<T>::at(i, together), a.vocabulary - 1)];
             }
         }
+        if (top < kInf && top > -kInf) {
 #pragma unroll
-        for (int i = 0; i < kEach; ++i)
-            w[i] = (*this)(x[i], of_q[i], from + Tokens<T>::at(i / Tokens<T>::kPiece, together) + i % Tokens<T>::kPiece);
+            for (int i = 0; i < kEach; ++i) w[i] = powers.weight<true>(logits.logit(i), top, heat) * by;
+        } else {
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) w[i] = powers.weight(logits.logit(i), top, heat) * by;
+        }
+        if (!judged) return;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            if (q)
+                w[i] = fmax(w[i] - fmax(double(of_q[i]), 0.), 0.);
+            else if (from + Tokens<T>::at(i, together) == token)
+                w[i] = 0.;
+        }
     }
 };
-__device__ __forceinline__ Drawn drawn_from(const VerifyArgs& a, const Verdict& v, double heat) {
+__device__ __forceinline__ Drawn drawn_from(const VerifyArgs& a, const Powers& powers, const Verdict& v, double heat) {
     const bool judged = v.accepted < v.drafted;
-    return {v.top, heat, judged ? 1. / v.z : 1., judged, judged && a.draft ? a.draft + v.row * a.draft_stride : nullptr, v.token};
-}
-
-// Every workgroup of a sequence finds, from its rows' parts, the row that the
-// token is drawn from, and sums that row's max(p - q, 0) over its own chunk.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void verify_rest_kernel(VerifyArgs a) {
-    __shared__ double sums[kWaves];
-    __shared__ Verdict of_wave[kWaves];
-    __shared__ int fits[kWaves];
-    const int s = blockIdx.x / a.chunks, chunk = blockIdx.x - s * a.chunks;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int first;
-    const int n = a.rows_of(s, first);
-    const double heat = a.heat(s);
-    const bool greedy = a.greedy(s);
-    Verdict v{0., -kInf, -1, -1, -1, 0, max(n - 1, 0)};
-    for (int i0 = 0; i0 < n && v.row < 0; i0 += kWaves) {
-        const int i = i0 + wave;
-        if (i < n) {
-            const int row = first + i, token = i + 1 < n ? a.tokens[row + 1] : -1;
-            const Part whole = whole_row(a, row, heat, lane);
-            bool fit = false;
-            if (token >= 0 && token < a.vocabulary && whole.sum > 0.) {
-                const double q = a.draft ? fmax(double(a.draft[row * a.draft_stride + token]), 0.) : 1.;
-                const float x = logit<T>(a.logits, row * a.logit_stride + token);
-                const double w = greedy ? (token == whole.best ? whole.sum : 0.) : weight(x, whole.top, heat);
-                fit = double(a.accept[row]) * q * whole.sum < w;
-            }
-            if (lane == 0) {
-                of_wave[wave] = {whole.sum, whole.top, whole.best, row, token, i, n - 1};
-                fits[wave] = fit;
-            }
-        }
-        __syncthreads();
-        for (int w = 0; w < kWaves && i0 + w < n; ++w)
-            if (!fits[w]) {
-                v = of_wave[w];
-                break;
-            }
-        __syncthreads();
-    }
-    if (chunk == 0 && threadIdx.x == 0) a.verdicts[s] = v;
-    if (v.row < 0 || greedy || !(v.z > 0.) || v.accepted == v.drafted) return;
-    double w[kEach], sum = 0.;
-    drawn_from(a, v, heat).load<T>(a, v.row, chunk * kChunk, false, w);
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) sum += w[i];
-    sum = dev::wave_sum(sum);
-    if (lane == 0) sums[wave] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) a.rest[int64_t(s) * a.chunks + chunk] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    return {uniform(v.top), heat, judged ? 1. / v.z : 1., judged, judged && a.draft ? a.draft + v.row * a.draft_stride : nullptr, v.token,
+            powers};
 }
 
 // The sum over the threads before this one, and over all.
@@ -348,49 +393,124 @@ __device__ __forceinline__ int lowest_or_last(int number, int none, int other, i
     return number < none ? number : other;
 }
 
-// One workgroup a sequence: the chunk in which the sum of the weights passes
-// sample times the whole, then the token in it. Sums of one range in two
-// orders may differ in their last place, so that a border can lie between them: the last
-// token with a weight stands for what lies behind all.
+// What a sequence's rows come to: the first row whose drafted token is not
+// accepted, or the last. A wave judges a row, so a workgroup four at a time.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs a) {
+__device__ __forceinline__ Verdict judge(const VerifyArgs& a, const Powers& powers, int s, double heat, bool greedy,
+                                         Verdict (&of_wave)[kWaves], int (&fits)[kWaves]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int first;
+    const int n = a.rows_of(s, first);
+    Verdict v{0., -kInf, -1, -1, -1, 0, max(n - 1, 0)};
+    for (int i0 = 0; i0 < n && v.row < 0; i0 += kWaves) {
+        const int i = i0 + wave;
+        if (i < n) {
+            const int row = first + i, token = i + 1 < n ? a.tokens[row + 1] : -1;
+            const bool there = token >= 0 && token < a.vocabulary;
+            // Loads that only need the token go out before the row's parts are added.
+            const float x = there ? logit<T>(a.logits, row * a.logit_stride + token) : -kInf;
+            const float of_q = there && a.draft ? a.draft[row * a.draft_stride + token] : 1.f;
+            const float number = a.accept[row];
+            const Part whole = whole_row(a, powers, row, heat, lane);
+            const double w = greedy ? (token == whole.best ? whole.sum : 0.) : powers.weight(x, whole.top, heat);
+            const bool fit = there && whole.sum > 0. && double(number) * fmax(double(of_q), 0.) * whole.sum < w;
+            if (lane == 0) {
+                of_wave[wave] = {whole.sum, whole.top, whole.best, row, token, i, n - 1};
+                fits[wave] = fit;
+            }
+        }
+        __syncthreads();
+        for (int w = 0; w < kWaves && i0 + w < n; ++w)
+            if (!fits[w]) {
+                v = of_wave[w];
+                break;
+            }
+        __syncthreads();
+    }
+    return v;
+}
+
+// Sums that other workgroups of the launch read, on other XCDs too.
+__device__ __forceinline__ void post(double* p, double x) {
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, x), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void posted_stores_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ double posted(const double* p) {
+    return __builtin_bit_cast(double, __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED,
+                                                        __HIP_MEMORY_SCOPE_AGENT));
+}
+
+// Every workgroup of a sequence judges its rows (from sums, which takes no
+// longer than to wait for another's word) and adds the weights that the token
+// is drawn from up over its own chunks; the last one to do so draws: the
+// chunk in which the sum of the weights passes sample times the whole, then
+// the token in it. Sums of one range in two orders may differ in their last
+// place, so that a border can lie between them: the last token with a weight
+// stands for what lies behind all.
+template <typename T>
+__global__ __launch_bounds__(kThreads, 4) void verify_draw_kernel(VerifyArgs a) {
+    __shared__ Powers powers;
     __shared__ double waves[kWaves], base_of;
-    __shared__ int picks[2 * kWaves];
-    const int s = blockIdx.x, tid = threadIdx.x;
-    const Verdict v = a.verdicts[s];
+    __shared__ Verdict of_wave[kWaves];
+    __shared__ int fits[kWaves], picks[2 * kWaves], last_one;
+    const int groups = (a.chunks + a.draw_chunks - 1) / a.draw_chunks;
+    const int s = blockIdx.x / groups, own = blockIdx.x - s * groups, tid = threadIdx.x;
+    powers.make();
+    __syncthreads();
     const double heat = a.heat(s);
-    int token = -1;
-    if (v.row >= 0 && v.z > 0. && a.greedy(s)) token = v.best;
-    if (v.row >= 0 && v.z > 0. && !a.greedy(s)) {
-        Drawn drawn = drawn_from(a, v, heat);
-        const Part* const parts = a.parts + int64_t(v.row) * a.chunks;
-        const double* const rest = a.rest + int64_t(s) * a.chunks;
-        const int each = (a.chunks + kThreads - 1) / kThreads, c0 = min(tid * each, a.chunks), c1 = min(c0 + each, a.chunks);
-        auto of_chunk = [&](int c) {
-            if (drawn.judged) return rest[c];
-            const Part part = parts[c];
-            return part.sum * (part.top == drawn.top ? 1. : weight(part.top, drawn.top, heat)) * drawn.by;
+    const bool greedy = a.greedy(s);
+    const Verdict v = judge<T>(a, powers, s, heat, greedy, of_wave, fits);
+    const bool draws = v.row >= 0 && v.z > 0. && !greedy;
+    int token = draws || v.row < 0 || !(v.z > 0.) ? -1 : v.best;
+    Drawn drawn = drawn_from(a, powers, v, heat);
+    double* const rest = a.rest + int64_t(s) * a.chunks;
+    if (!draws && own) return;
+    if (draws) {
+        double all = 0.;
+        // Several chunks: p - q of each; where q is p or more throughout, which the last workgroup sees, p itself.
+        auto add_up = [&](int c) {
+            double w[kEach], sum = 0., whole;
+            drawn.load<T>(a, v.row, c * kChunk, false, w);
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) sum += w[i];
+            (void)sum_before(sum, waves, whole);
+            if (tid == 0) post(rest + c, whole);
         };
-        double before = 0., all = 0.;
+        for (int c = own * a.draw_chunks; c < min((own + 1) * a.draw_chunks, a.chunks); ++c) add_up(c);
+        if (tid == 0) {
+            posted_stores_done();
+            last_one = __hip_atomic_fetch_add(a.done + s, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == groups - 1;
+        }
+        __syncthreads();
+        if (!last_one) return;
+        const int each = (a.chunks + kThreads - 1) / kThreads, c0 = min(tid * each, a.chunks), c1 = min(c0 + each, a.chunks);
+        double before = 0., only = 0.;  // only: of up to 256 chunks, the thread's
         for (;;) {
             double sum = 0.;
-            for (int c = c0; c < c1; ++c) sum += of_chunk(c);
+            for (int c = c0; c < c1; ++c) sum += only = posted(rest + c);
             before = sum_before(sum, waves, all);
             if (!drawn.judged || all > 0.) break;
-            drawn.judged = false;  // q is p or more throughout
+            drawn.judged = false;
+            drawn.by = 1.;
+            for (int c = 0; c < a.chunks; ++c) add_up(c);
+            if (tid == 0) posted_stores_done();
+            __syncthreads();
         }
         const double target = double(a.sample[s]) * all;
         int chunk = a.chunks, last = -1;
         double upto = before, base = before, last_base = before;
         for (int c = c0; c < c1; ++c) {
-            const double sum = of_chunk(c);
+            const double sum = each == 1 ? only : posted(rest + c);
             if (sum > 0.) last = c, last_base = upto;
             if (chunk == a.chunks && upto + sum > target && sum > 0.) chunk = c, base = upto;
             upto += sum;
         }
         const int found = max(0, lowest_or_last(chunk, a.chunks, last, picks));
-        if (found == chunk) base_of = base;
-        else if (found == last && found >= c0 && found < c1) base_of = last_base;
+        if (found == chunk)
+            base_of = base;
+        else if (found == last && found >= c0 && found < c1)
+            base_of = last_base;
         __syncthreads();
         double w[kEach], sum = 0.;
         drawn.load<T>(a, v.row, found * kChunk, true, w);
@@ -417,16 +537,19 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyArgs a) {
 }
 
 struct Plan {
-    int64_t chunks, units;
-    size_t parts, rest, verdicts;
+    int64_t chunks, units, ranges, draw_chunks;
+    size_t parts, rest, done;
     explicit Plan(const qwen_gpu_draft& d) {
         chunks = (d.vocabulary + kChunk - 1) / kChunk;
         units = chunks * std::max(d.total_rows, d.sequences);
-        parts = sizeof(Part) * chunks * d.total_rows;
+        // As many workgroups as the GPU holds, of a chunk at least.
+        ranges = std::clamp<int64_t>(1536 / std::max(d.total_rows, 1), 1, chunks);
+        draw_chunks = std::clamp<int64_t>((chunks * d.sequences + 639) / 640, 1, 8);
+        parts = sizeof(Part) * ranges * d.total_rows;
         rest = sizeof(double) * chunks * d.sequences;
-        verdicts = sizeof(Verdict) * d.sequences;
+        done = sizeof(int) * d.sequences;
     }
-    size_t bytes() const { return parts + rest + verdicts; }
+    size_t bytes() const { return parts + rest + done; }
 };
 
 Plan plan_of(const qwen_gpu_draft& d) {
@@ -444,9 +567,9 @@ Plan plan_of(const qwen_gpu_draft& d) {
 
 template <typename T>
 void run(const VerifyArgs& a, hipStream_t stream) {
-    if (a.total_rows) verify_parts_kernel<T><<<unsigned(a.total_rows * a.chunks), kThreads, 0, stream>>>(a);
-    verify_rest_kernel<T><<<unsigned(a.sequences * a.chunks), kThreads, 0, stream>>>(a);
-    verify_draw_kernel<T><<<unsigned(a.sequences), kThreads, 0, stream>>>(a);
+    const unsigned draws = (a.chunks + a.draw_chunks - 1) / a.draw_chunks;
+    if (a.total_rows) verify_parts_kernel<T><<<unsigned(a.total_rows * a.ranges), kThreads, 0, stream>>>(a);
+    verify_draw_kernel<T><<<a.sequences * draws, kThreads, 0, stream>>>(a);
 }
 
 }  // namespace
@@ -496,9 +619,9 @@ void launch_verify_draft(const qwen_gpu_draft& d, int32_t* accepted, int32_t* ne
     char* const space = static_cast<char*>(workspace);
     const VerifyArgs a{static_cast<const char*>(d.logits), d.draft, d.tokens, d.offsets, d.temperature, d.accept, d.sample,
                        d.total_rows > 1 ? d.logit_stride : 0, d.total_rows > 1 ? d.draft_stride : 0, d.vocabulary,
-                       int(plan.chunks), d.sequences, d.rows, d.total_rows, reinterpret_cast<Part*>(space),
+                       int(plan.chunks), d.sequences, d.rows, d.total_rows, int(plan.ranges), int(plan.draw_chunks), reinterpret_cast<Part*>(space),
                        reinterpret_cast<double*>(space + plan.parts),
-                       reinterpret_cast<Verdict*>(space + plan.parts + plan.rest), accepted, next, back};
+                       reinterpret_cast<int*>(space + plan.parts + plan.rest), accepted, next, back};
     if (d.type == QWEN_GPU_F32)
         run<float>(a, stream);
     else if (d.type == QWEN_GPU_F16)

@@ -574,7 +574,7 @@ int qwen_gpu_op_verify_workspace(const qwen_gpu_draft* draft, size_t* bytes);
  * drafted one is not accepted and next is -1, as it is for a sequence without rows. A drafted
  * token outside the vocabulary is not accepted; probabilities below 0 and NaN
  * count as 0. Weights and sums are FP64, summed in an order that depends on the
- * vocabulary alone. Streams as for the paged cache; the device is that of
+ * call's sizes alone. Streams as for the paged cache; the device is that of
  * `logits`. */
 int qwen_gpu_op_verify_draft(const qwen_gpu_draft* draft, int32_t* accepted, int32_t* next, int32_t* back,
                              void* workspace, size_t workspace_bytes, void* stream);
