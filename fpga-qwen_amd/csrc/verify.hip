@@ -20,7 +20,8 @@ namespace qwen_hip {
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64, kEach = 16;
-constexpr int kChunk = kThreads * kEach;  // tokens of a workgroup
+constexpr int kChunk = kThreads * kEach;  // tokens of a workgroup's step
+constexpr int kMostChunks = 8;            // of a workgroup that draws
 constexpr float kInf = __builtin_huge_valf();
 
 // Of a range of a row: its largest logit, the lowest token that has it (where
@@ -315,40 +316,54 @@ struct Drawn {
     int token;
     const Powers& powers;
 
-    // The weights of a thread's tokens of a chunk (their places as Tokens<T> has them).
+    // A thread's tokens of a chunk, and q of them.
     template <typename T>
-    __device__ __forceinline__ void load(const VerifyArgs& a, int row, int from, bool together, double (&w)[kEach]) const {
+    struct Chunk {
         Tokens<T> logits;
-        logits.load(reinterpret_cast<const T*>(a.logits) + row * a.logit_stride, from, a.vocabulary, together, T(-kInf));
         float of_q[kEach];
-        if (judged && q) {
-            if (from + kChunk <= a.vocabulary) {
-                typedef float float4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+    };
+    template <typename T>
+    __device__ __forceinline__ void load(const VerifyArgs& a, int row, int from, bool together, Chunk<T>& c) const {
+        c.logits.load(reinterpret_cast<const T*>(a.logits) + row * a.logit_stride, from, a.vocabulary, together, T(-kInf));
+        if (!judged || !q) return;
+        if (from + kChunk <= a.vocabulary) {
+            typedef float float4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 #pragma unroll
-                for (int i = 0; i < kEach; i += 4) {
-                    const float4_a4 v = *reinterpret_cast<const float4_a4*>(q + from + Tokens<T>::at(i, together));
+            for (int i = 0; i < kEach; i += 4) {
+                const float4_a4 v = *reinterpret_cast<const float4_a4*>(q + from + Tokens<T>::at(i, together));
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) of_q[i + e] = v[e];
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < kEach; ++i) of_q[i] = q[min(from + Tokens<T>::at(i, together), a.vocabulary - 1)];
+                for (int e = 0; e < 4; ++e) c.of_q[i + e] = v[e];
             }
-        }
-        if (top < kInf && top > -kInf) {
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) w[i] = powers.weight<true>(logits.logit(i), top, heat) * by;
         } else {
 #pragma unroll
-            for (int i = 0; i < kEach; ++i) w[i] = powers.weight(logits.logit(i), top, heat) * by;
+            for (int i = 0; i < kEach; ++i) c.of_q[i] = q[min(from + Tokens<T>::at(i, together), a.vocabulary - 1)];
         }
-        if (!judged) return;
+    }
+    // Their weights (places as Tokens<T> has them), four at a time where one of a wave's has any.
+    template <typename T>
+    __device__ __forceinline__ void weigh(const Chunk<T>& c, int from, bool together, double (&w)[kEach]) const {
+        const bool finite = top < kInf && top > -kInf;
+        const float least = heat > 0. ? float(top - 64 * 1001 / heat) : -kInf;
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            if (q)
-                w[i] = fmax(w[i] - fmax(double(of_q[i]), 0.), 0.);
-            else if (from + Tokens<T>::at(i, together) == token)
-                w[i] = 0.;
+        for (int i = 0; i < kEach; i += 4) {
+            float x[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = c.logits.logit(i + j), w[i + j] = 0.;
+            const float high = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+            if (finite && __any(high >= least && high > -kInf)) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[i + j] = powers.weight<true>(x[j], top, heat) * by;
+            } else if (!finite) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[i + j] = powers.weight(x[j], top, heat) * by;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (judged && q)
+                    w[i + j] = fmax(w[i + j] - fmax(double(c.of_q[i + j]), 0.), 0.);
+                else if (judged && from + Tokens<T>::at(i + j, together) == token)
+                    w[i + j] = 0.;
+            }
         }
     }
 };
@@ -451,7 +466,7 @@ __device__ __forceinline__ double posted(const double* p) {
 template <typename T>
 __global__ __launch_bounds__(kThreads, 4) void verify_draw_kernel(VerifyArgs a) {
     __shared__ Powers powers;
-    __shared__ double waves[kWaves], base_of;
+    __shared__ double waves[kWaves], base_of, chunk_sums[kMostChunks][kWaves];
     __shared__ Verdict of_wave[kWaves];
     __shared__ int fits[kWaves], picks[2 * kWaves], last_one;
     const int groups = (a.chunks + a.draw_chunks - 1) / a.draw_chunks;
@@ -468,20 +483,31 @@ __global__ __launch_bounds__(kThreads, 4) void verify_draw_kernel(VerifyArgs a) 
     if (!draws && own) return;
     if (draws) {
         double all = 0.;
-        // Several chunks: p - q of each; where q is p or more throughout, which the last workgroup sees, p itself.
-        auto add_up = [&](int c) {
-            double w[kEach], sum = 0., whole;
-            drawn.load<T>(a, v.row, c * kChunk, false, w);
+        // Up to 8 chunks' sums, the next one's tokens on their way; wave 0 posts them.
+        auto add_up = [&](int c0, int c1) {
+            Drawn::Chunk<T> ahead;
+            drawn.load<T>(a, v.row, c0 * kChunk, false, ahead);
+            for (int c = c0; c < c1; ++c) {
+                const Drawn::Chunk<T> here = ahead;
+                if (c + 1 < c1) drawn.load<T>(a, v.row, (c + 1) * kChunk, false, ahead);
+                double w[kEach], sum = 0.;
+                drawn.weigh<T>(here, c * kChunk, false, w);
 #pragma unroll
-            for (int i = 0; i < kEach; ++i) sum += w[i];
-            (void)sum_before(sum, waves, whole);
-            if (tid == 0) post(rest + c, whole);
+                for (int i = 0; i < kEach; ++i) sum += w[i];
+                sum = dev::wave_sum(sum);
+                if ((tid & 63) == 0) chunk_sums[c - c0][tid >> 6] = sum;
+            }
+            __syncthreads();
+            if (tid < c1 - c0) {
+                const double* const of = chunk_sums[tid];
+                post(rest + c0 + tid, (of[0] + of[1]) + (of[2] + of[3]));
+            }
+            if (tid < 64) posted_stores_done();
+            __syncthreads();
         };
-        for (int c = own * a.draw_chunks; c < min((own + 1) * a.draw_chunks, a.chunks); ++c) add_up(c);
-        if (tid == 0) {
-            posted_stores_done();
+        add_up(own * a.draw_chunks, min((own + 1) * a.draw_chunks, a.chunks));
+        if (tid == 0)
             last_one = __hip_atomic_fetch_add(a.done + s, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == groups - 1;
-        }
         __syncthreads();
         if (!last_one) return;
         const int each = (a.chunks + kThreads - 1) / kThreads, c0 = min(tid * each, a.chunks), c1 = min(c0 + each, a.chunks);
@@ -491,11 +517,9 @@ __global__ __launch_bounds__(kThreads, 4) void verify_draw_kernel(VerifyArgs a) 
             for (int c = c0; c < c1; ++c) sum += only = posted(rest + c);
             before = sum_before(sum, waves, all);
             if (!drawn.judged || all > 0.) break;
-            drawn.judged = false;
+            drawn.judged = false;  // q is p or more throughout
             drawn.by = 1.;
-            for (int c = 0; c < a.chunks; ++c) add_up(c);
-            if (tid == 0) posted_stores_done();
-            __syncthreads();
+            for (int c = 0; c < a.chunks; c += kMostChunks) add_up(c, min(c + kMostChunks, a.chunks));
         }
         const double target = double(a.sample[s]) * all;
         int chunk = a.chunks, last = -1;
@@ -513,7 +537,9 @@ __global__ __launch_bounds__(kThreads, 4) void verify_draw_kernel(VerifyArgs a) 
             base_of = last_base;
         __syncthreads();
         double w[kEach], sum = 0.;
-        drawn.load<T>(a, v.row, found * kChunk, true, w);
+        Drawn::Chunk<T> here;
+        drawn.load<T>(a, v.row, found * kChunk, true, here);
+        drawn.weigh<T>(here, found * kChunk, true, w);
 #pragma unroll
         for (int i = 0; i < kEach; ++i) sum += w[i];
         upto = base_of + sum_before(sum, waves, all);
@@ -544,7 +570,7 @@ struct Plan {
         units = chunks * std::max(d.total_rows, d.sequences);
         // As many workgroups as the GPU holds, of a chunk at least.
         ranges = std::clamp<int64_t>(1536 / std::max(d.total_rows, 1), 1, chunks);
-        draw_chunks = std::clamp<int64_t>((chunks * d.sequences + 639) / 640, 1, 8);
+        draw_chunks = std::clamp<int64_t>((chunks * d.sequences + 639) / 640, 1, kMostChunks);
         parts = sizeof(Part) * ranges * d.total_rows;
         rest = sizeof(double) * chunks * d.sequences;
         done = sizeof(int) * d.sequences;
