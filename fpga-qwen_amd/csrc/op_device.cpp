@@ -33,7 +33,7 @@ OpDevice::OpDevice(const void* anchor, const char* what, const char* owner, hipS
     if (stream) {
         hipDevice_t of = 0;
         hip_check(hipStreamGetDevice(stream, &of));
-        require(of == device_, std::string("The stream belongs to another device than ") + owner_);
+        if (of != device_) throw std::runtime_error(std::string("The stream belongs to another device than ") + owner_);
     }
     if (before_ != device_) hip_check(hipSetDevice(device_));
 }
@@ -43,12 +43,28 @@ OpDevice::~OpDevice() {
 }
 
 void OpDevice::check(const void* p, const char* what, unsigned alignment) const {
-    require(p, std::string("Null argument: ") + what);
-    require(reinterpret_cast<uintptr_t>(p) % alignment == 0,
-            std::string("Not aligned to ") + std::to_string(alignment) + " bytes: " + what);
+    // (Messages are put together where they are needed: a call has many arguments.)
+    if (!p) throw std::runtime_error(std::string("Null argument: ") + what);
+    if (reinterpret_cast<uintptr_t>(p) % alignment != 0)
+        throw std::runtime_error(std::string("Not aligned to ") + std::to_string(alignment) + " bytes: " + what);
     const hipPointerAttribute_t a = attributes(p, what);
-    require(a.type != hipMemoryTypeDevice || a.device == device_,
-            std::string("On another device than ") + owner_ + ": " + what);
+    if (a.type == hipMemoryTypeDevice && a.device != device_)
+        throw std::runtime_error(std::string("On another device than ") + owner_ + ": " + what);
+}
+
+void check_arrays(const OpArray* arrays, int count) {
+    for (int i = 0; i < count; ++i)
+        if (!arrays[i].at && arrays[i].needed) throw std::runtime_error(std::string("Null argument: ") + arrays[i].name);
+    for (int i = 0; i < count; ++i) {
+        const OpArray& a = arrays[i];
+        if (!a.written || !a.at) continue;
+        for (int j = 0; j < count; ++j) {
+            const OpArray& b = arrays[j];
+            if (j == i || !b.at || (a.at == b.at && (a.in_place_of == b.at || b.in_place_of == a.at))) continue;
+            if (!apart(a.at, a.bytes, b.at, b.bytes))
+                throw std::runtime_error(std::string(a.name) + " overlaps " + b.name);
+        }
+    }
 }
 
 bool apart(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {

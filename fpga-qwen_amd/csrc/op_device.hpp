@@ -22,6 +22,19 @@ private:
     int device_ = 0, before_ = 0;
 };
 
+// An argument of a call. Arrays that are written overlap no others, but for
+// the one whose place they may take, from its start.
+struct OpArray {
+    const char* name;
+    const void* at;
+    size_t bytes;
+    bool needed, written;
+    unsigned alignment = 4;
+    const void* in_place_of = nullptr;
+};
+// Null and overlapping arguments are refused; no device is needed.
+void check_arrays(const OpArray* arrays, int count);
+
 // Whether two arrays of `bytes` have nothing in common.
 bool apart(const void* a, size_t a_bytes, const void* b, size_t b_bytes);
 

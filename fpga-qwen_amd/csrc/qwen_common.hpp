@@ -23,6 +23,9 @@ inline constexpr int kKVDim = kKVHeads * kHeadDim;  // 1024
 inline constexpr int kQKVRows = kQDim + 2 * kKVDim; // 4096
 inline constexpr int kEosA = 151643, kEosB = 151645;
 
+inline void require(bool ok, const char* message) {  // no string is made of a message that nobody reads
+    if (!ok) throw std::runtime_error(message);
+}
 inline void require(bool ok, const std::string& message) {
     if (!ok) throw std::runtime_error(message);
 }

@@ -1,9 +1,11 @@
 // Pages and rows of a step over a paged cache.
 #include "reserve.hpp"
 
+#include <algorithm>
 #include <cstdint>
-#include <string>
+#include <iterator>
 
+#include "decode_dev.hpp"
 #include "op_device.hpp"
 #include "paged_dev.hpp"
 #include "qwen_common.hpp"
@@ -12,8 +14,9 @@ namespace qwen_hip {
 
 namespace {
 
-constexpr int kThreads = 1024, kEach = 4, kMost = kThreads * kEach;  // sequences of a thread, of a call
+constexpr int kMost = 4096;  // sequences of a call
 constexpr int kMaxRow = 1 << 30;
+constexpr int kFewRows = 1024;  // up to which they are mapped without a launch of their own
 
 struct ReserveView {
     int32_t* table;
@@ -25,27 +28,46 @@ struct ReserveView {
     unsigned magic;
 };
 
-// What a scan has to hold: pages are at most 2^24 a sequence, rows 2^30.
-__device__ __forceinline__ int64_t scan_wave(int64_t x, int lane) {
-#pragma unroll
-    for (int off = 1; off < 64; off *= 2) {
-        const int64_t other = __shfl_up(x, off);
-        if (lane >= off) x += other;
-    }
+// Sums are 32 bits and stop at a limit above all pages and rows there can be,
+// which two of them do not carry past 32 bits: nothing behind the place where a sum of pages passes
+// those there are, or a sum of rows the room, is granted whatever the sum is.
+constexpr unsigned kLimit = (1u << 30) + 1;
+__device__ __forceinline__ unsigned limited(unsigned a, unsigned b) { return min(a + b, kLimit); }
+
+// Sums of the lanes up to each, through DPP row shifts and broadcasts.
+__device__ __forceinline__ unsigned scan_wave(unsigned x) {
+    auto step = [&](int from) { x = limited(x, unsigned(from)); };
+    step(__builtin_amdgcn_update_dpp(0, int(x), 0x111, 0xF, 0xF, true));  // row_shr:1, 2, 4, 8
+    step(__builtin_amdgcn_update_dpp(0, int(x), 0x112, 0xF, 0xF, true));
+    step(__builtin_amdgcn_update_dpp(0, int(x), 0x114, 0xF, 0xF, true));
+    step(__builtin_amdgcn_update_dpp(0, int(x), 0x118, 0xF, 0xF, true));
+    step(__builtin_amdgcn_update_dpp(0, int(x), 0x142, 0xA, 0xF, false));  // row_bcast:15 into rows 1 and 3
+    step(__builtin_amdgcn_update_dpp(0, int(x), 0x143, 0xC, 0xF, false));  // row_bcast:31 into rows 2 and 3
     return x;
 }
 
-// The sum over all threads before this one; `total` of all.
-__device__ __forceinline__ int64_t scan_block(int64_t x, int64_t* waves, int64_t& total) {
+// N sums at once over the threads: `before` each thread, and `all`.
+template <int THREADS, int N>
+__device__ __forceinline__ void scan_block(const unsigned (&x)[N], unsigned (*waves)[16], unsigned (&before)[N],
+                                           unsigned (&all)[N]) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t upto = scan_wave(x, lane);
-    if (lane == 63) waves[wave] = upto;
+    unsigned upto[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        upto[i] = scan_wave(x[i]);
+        if (lane == 63) waves[i][wave] = upto[i];
+    }
     __syncthreads();
-    const int64_t of_lane = scan_wave(lane < kThreads / 64 ? waves[lane] : 0, lane);
-    total = __shfl(of_lane, kThreads / 64 - 1);
-    const int64_t before = __shfl(of_lane, max(wave - 1, 0));
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const unsigned of_lane = scan_wave(lane < THREADS / 64 ? waves[i][lane] : 0u);
+        all[i] = __builtin_amdgcn_readlane(of_lane, 63);
+        const unsigned base = wave ? __builtin_amdgcn_readlane(of_lane, __builtin_amdgcn_readfirstlane(max(wave - 1, 0))) : 0u;
+        // The sum up to the lane before, which the limit keeps from being a difference.
+        const unsigned one_less = __shfl_up(upto[i], 1);
+        before[i] = limited(base, lane ? one_less : 0u);
+    }
     __syncthreads();
-    return (wave ? before : 0) + upto - x;
 }
 
 // The first of n rising sums that is above k; the last one is.
@@ -61,149 +83,183 @@ __device__ __forceinline__ int owner(const int* upto, int n, int k) {
     return low;
 }
 
-__device__ __forceinline__ int clipped(int64_t x) { return int(min(x, int64_t(0x7fffffff))); }
+// Pages k below `count`, whose sequences' sums are `upto`: f(s, k) gives a
+// place to read and one to write. A thread has eight in a row, so it looks
+// for the first one's sequence alone, and all its loads are in flight.
+template <int THREADS, class F>
+__device__ __forceinline__ void move_pages(const int* upto, int n, int count, F f) {
+    constexpr int kRow = 8;
+    for (int k0 = kRow * threadIdx.x; k0 < count; k0 += kRow * THREADS) {
+        int s = owner(upto, n, k0), page[kRow];
+        int32_t* to[kRow];
+#pragma unroll
+        for (int j = 0; j < kRow; ++j) {
+            const int k = min(k0 + j, count - 1);
+            while (upto[s] <= k) ++s;  // ends: the last sum is `count` or more
+            const int32_t* from;
+            f(s, k, from, to[j]);
+            page[j] = *from;
+        }
+#pragma unroll
+        for (int j = 0; j < kRow; ++j)
+            if (k0 + j < count) *to[j] = page[j];
+    }
+}
 
-// One workgroup: three sums over the sequences (pages given back, pages
-// needed, rows granted), and after each the pages or rows themselves, a thread each,
-// whose sequences are found in the sums. Latency bounds it.
-__global__ __launch_bounds__(kThreads) void reserve_kernel(ReserveView v) {
-    __shared__ int64_t waves[kThreads / 64];
-    __shared__ int upto[kMost], start[kMost];
+// The maps of a row.
+__device__ __forceinline__ void map_row(const ReserveView& v, const int* upto, int all, int row) {
+    int sequence = -1, position = -1;
+    int64_t slot = -1;
+    if (row < all) {
+        sequence = owner(upto, v.sequences, row);
+        const int back = upto[sequence] - row, length = v.new_lengths[sequence];
+        position = (v.new_seen ? v.new_seen[sequence] : length) - back;
+        const PageSlot at = page_slot(unsigned(length - back), v.page_size, v.magic);
+        const int page = v.table[int64_t(sequence) * v.table_stride + at.page];
+        if (page >= 0 && page < v.pages) slot = int64_t(page) * v.page_size + at.slot;
+    }
+    if (v.row_sequences) v.row_sequences[row] = sequence;
+    if (v.row_positions) v.row_positions[row] = position;
+    if (v.row_slots) v.row_slots[row] = slot;
+}
+
+// One workgroup: sums over the sequences (pages given back and needed, then
+// rows granted), and after each the pages themselves, a thread each, whose
+// sequences are found in the sums. Few rows are mapped here too. Latency
+// bounds it: a thread has EACH sequences, one where there are few, and there
+// are no more threads than they need.
+template <int THREADS, int EACH>
+__global__ __launch_bounds__(THREADS) void reserve_kernel(ReserveView v, bool maps) {
+    __shared__ unsigned waves[2][16];
+    __shared__ int upto[THREADS * EACH], start[THREADS * EACH];
     const int tid = threadIdx.x, n = v.sequences;
     const int free_count = min(max(v.free_count[0], 0), v.pages);
-    int length[kEach], change[kEach], held[kEach], needed[kEach], keep[kEach], need[kEach];
-    int64_t surplus_sum = 0, need_sum = 0;
+    int length[EACH], change[EACH], held[EACH], needed[EACH], keep[EACH];
+    unsigned need[EACH], surplus[EACH], sums[2] = {0, 0}, before[2], all[2];
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-        const int s = kEach * tid + i;
-        length[i] = change[i] = held[i] = needed[i] = keep[i] = need[i] = 0;
-        if (s >= n) continue;
-        length[i] = min(max(v.lengths[s], 0), v.most);
-        held[i] = min(max(v.held[s], 0), v.table_stride);
-        change[i] = max(v.changes[s], -length[i]);
+    for (int i = 0; i < EACH; ++i) {  // all loads first; sequences that are not there count as empty ones
+        const int s = min(EACH * tid + i, n - 1);
+        length[i] = v.lengths[s];
+        held[i] = v.held[s];
+        change[i] = v.changes[s];
+        keep[i] = v.shared ? v.shared[s] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        const bool there = EACH * tid + i < n;
+        length[i] = there ? min(max(length[i], 0), v.most) : 0;
+        held[i] = there ? min(max(held[i], 0), v.table_stride) : 0;
+        change[i] = there ? max(change[i], -length[i]) : 0;
         if (int64_t(length[i]) + change[i] > v.most) change[i] = 0;
         const PageSlot end = page_slot(unsigned(length[i] + change[i]), v.page_size, v.magic);
         needed[i] = end.page + (end.slot > 0);
-        const int fixed = v.shared ? min(max(v.shared[s], 0), held[i]) : 0;
-        keep[i] = min(held[i], max(needed[i], fixed));
+        keep[i] = min(held[i], max(needed[i], keep[i]));
         need[i] = max(0, needed[i] - held[i]);
-        surplus_sum += held[i] - keep[i];
-        need_sum += need[i];
+        surplus[i] = held[i] - keep[i];
+        sums[0] = limited(sums[0], surplus[i]);
+        sums[1] = limited(sums[1], need[i]);
     }
-    int64_t surplus_all, need_all, rows_all;
-    int64_t surplus_before = scan_block(surplus_sum, waves, surplus_all);
-    int64_t need_before = scan_block(need_sum, waves, need_all);
-    const int available = int(min(int64_t(v.pages), free_count + surplus_all));
+    scan_block<THREADS>(sums, waves, before, all);
+    const int available = int(min(unsigned(v.pages), limited(free_count, all[0])));
 
-    if (surplus_all) {
+    if (all[0]) {
+        unsigned given = before[0];
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const int s = kEach * tid + i;
-            if (s >= n) continue;
+        for (int i = 0; i < EACH; ++i) {
+            const int s = EACH * tid + i;
             // A place k of the pages given back is entry start + k.
-            start[s] = keep[i] - clipped(surplus_before);
-            surplus_before += held[i] - keep[i];
-            upto[s] = clipped(surplus_before);
+            start[s] = keep[i] - int(given);
+            given = limited(given, surplus[i]);
+            upto[s] = int(given);
         }
         __syncthreads();
-        for (int k = tid; k < available - free_count; k += kThreads) {
-            const int s = owner(upto, n, k);
-            v.free_pages[free_count + k] = v.table[int64_t(s) * v.table_stride + start[s] + k];
-        }
+        move_pages<THREADS>(upto, n, available - free_count, [&](int s, int k, const int32_t*& from, int32_t*& to) {
+            from = v.table + (int64_t(s) * v.table_stride + start[s] + k);
+            to = v.free_pages + (free_count + k);
+        });
         __syncthreads();
     }
 
     // Rows of the sequences that have their pages.
-    int64_t rows_sum = 0, upto_need = need_before;
-    int rows[kEach];
+    unsigned rows[EACH], pages = before[1], of_rows[1] = {0}, rows_before[1], rows_all[1];
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-        upto_need += need[i];
-        rows[i] = need[i] == 0 || upto_need <= available ? max(change[i], 0) : 0;
-        rows_sum += rows[i];
+    for (int i = 0; i < EACH; ++i) {
+        pages = limited(pages, need[i]);
+        rows[i] = need[i] == 0 || pages <= unsigned(available) ? max(change[i], 0) : 0;
+        of_rows[0] = limited(of_rows[0], rows[i]);
     }
-    int64_t rows_before = scan_block(rows_sum, waves, rows_all);
+    scan_block<THREADS>(of_rows, waves, rows_before, rows_all);
     // How many pages are taken, and rows granted: the sums at the last sequence that gets any.
-    int64_t pages_taken = 0, rows_granted = 0;
-    upto_need = need_before;
+    unsigned taken = 0, granted_rows = 0, row = rows_before[0];
+    pages = before[1];
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-        const int s = kEach * tid + i;
-        upto_need += need[i];
-        rows_before += rows[i];
-        const bool granted = rows[i] > 0 && rows_before <= v.total_rows;
+    for (int i = 0; i < EACH; ++i) {
+        const int s = EACH * tid + i;
+        // A place k of the pages taken is entry start + k.
+        start[s] = held[i] - int(pages);
+        pages = limited(pages, need[i]);
+        upto[s] = int(pages);
+        row = limited(row, rows[i]);
+        const bool granted = rows[i] > 0 && row <= unsigned(v.total_rows);
         if (granted) {
-            rows_granted = rows_before;
-            if (need[i]) pages_taken = upto_need;
+            granted_rows = row;
+            if (need[i]) taken = pages;
         }
-        const bool keeps = change[i] > 0 && !granted;  // its length, for want of pages or room
         if (s < n) {
-            // A place k of the pages taken is entry start + k.
-            start[s] = held[i] - clipped(upto_need - need[i]);
-            upto[s] = clipped(upto_need);
-            const int delta = keeps ? 0 : change[i];
+            const int delta = change[i] > 0 && !granted ? 0 : change[i];
             v.new_lengths[s] = length[i] + delta;
             if (v.new_seen) v.new_seen[s] = v.seen[s] + delta;
             v.new_held[s] = granted && need[i] ? needed[i] : keep[i];
         }
     }
-    // The largest of all threads: they rise with the sequences.
-    auto largest = [&](int64_t x) {
-#pragma unroll
-        for (int off = 1; off < 64; off *= 2) x = max(x, __shfl_xor(x, off));
-        if ((tid & 63) == 0) waves[tid >> 6] = x;
-        __syncthreads();
-        int64_t all = 0;
-        for (int w = 0; w < kThreads / 64; ++w) all = max(all, waves[w]);
-        __syncthreads();
-        return all;
+    // The largest of all threads.
+    auto largest = [&](unsigned x) {
+        x = max(x, unsigned(dev::xor_lanes<1>(int(x))));
+        x = max(x, unsigned(dev::xor_lanes<2>(int(x))));
+        x = max(x, unsigned(dev::xor_lanes<4>(int(x))));
+        x = max(x, unsigned(dev::xor_lanes<8>(int(x))));
+        x = max(x, unsigned(dev::xor_lanes<16>(int(x))));
+        return max(x, unsigned(dev::xor_lanes<32>(int(x))));
     };
-    const int taken = int(largest(pages_taken)), granted_rows = int(largest(rows_granted));
+    taken = largest(taken), granted_rows = largest(granted_rows);
+    if ((tid & 63) == 0) waves[0][tid >> 6] = taken, waves[1][tid >> 6] = granted_rows;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) taken = max(taken, waves[0][w]), granted_rows = max(granted_rows, waves[1][w]);
     if (tid == 0) {
-        v.new_free_count[0] = available - taken;
+        v.new_free_count[0] = available - int(taken);
         v.offsets[0] = 0;
     }
-    for (int k = tid; k < taken; k += kThreads) {
-        const int s = owner(upto, n, k);
-        v.table[int64_t(s) * v.table_stride + start[s] + k] = v.free_pages[available - 1 - k];
-    }
-    __syncthreads();
-    rows_before -= rows_sum;
+    row = rows_before[0];
+    int offset[EACH];
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-        const int s = kEach * tid + i;
-        rows_before += rows[i];
-        if (s < n) v.offsets[s + 1] = int(min(rows_before, int64_t(granted_rows)));
+    for (int i = 0; i < EACH; ++i) {
+        const int s = EACH * tid + i;
+        row = limited(row, rows[i]);
+        offset[i] = int(min(row, granted_rows));
+        if (s < n) v.offsets[s + 1] = offset[i];
     }
+    move_pages<THREADS>(upto, n, int(taken), [&](int s, int k, const int32_t*& from, int32_t*& to) {
+        from = v.free_pages + (available - 1 - k);
+        to = v.table + (int64_t(s) * v.table_stride + start[s] + k);
+    });
+    if (!maps) return;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) upto[EACH * tid + i] = offset[i];
+    __syncthreads();
+    for (int r = tid; r < v.total_rows; r += THREADS) map_row(v, upto, int(granted_rows), r);
 }
 
-// The rows' maps, a thread a row: the sequence from the offsets, which every
-// workgroup brings into LDS first.
-constexpr int kMapThreads = 256, kMapRows = 4;
+// The maps of many rows, a thread a row; every workgroup brings the offsets into LDS first.
+constexpr int kMapThreads = 256;
 __global__ __launch_bounds__(kMapThreads) void reserve_rows_kernel(ReserveView v) {
     __shared__ int upto[kMost];
-    const int n = v.sequences;
-    for (int s = threadIdx.x; s < n; s += kMapThreads) upto[s] = v.offsets[s + 1];
+    for (int s = threadIdx.x; s < v.sequences; s += kMapThreads) upto[s] = v.offsets[s + 1];
     __syncthreads();
-    const int all = upto[n - 1];
-#pragma unroll
-    for (int i = 0; i < kMapRows; ++i) {
-        const int row = (blockIdx.x * kMapRows + i) * kMapThreads + threadIdx.x;
-        if (row >= v.total_rows) return;
-        int sequence = -1, position = -1;
-        int64_t slot = -1;
-        if (row < all) {
-            sequence = owner(upto, n, row);
-            const int back = upto[sequence] - row, length = v.new_lengths[sequence];
-            position = (v.new_seen ? v.new_seen[sequence] : length) - back;
-            const PageSlot at = page_slot(unsigned(length - back), v.page_size, v.magic);
-            const int page = v.table[int64_t(sequence) * v.table_stride + at.page];
-            if (page >= 0 && page < v.pages) slot = int64_t(page) * v.page_size + at.slot;
-        }
-        if (v.row_sequences) v.row_sequences[row] = sequence;
-        if (v.row_positions) v.row_positions[row] = position;
-        if (v.row_slots) v.row_slots[row] = slot;
-    }
+    const int all = upto[v.sequences - 1];
+    for (int row = blockIdx.x * kMapThreads + threadIdx.x; row < v.total_rows; row += gridDim.x * kMapThreads)
+        map_row(v, upto, all, row);
 }
 
 }  // namespace
@@ -216,51 +272,45 @@ void launch_paged_reserve(const qwen_gpu_paged_pool& p, const qwen_gpu_paged_gro
     require(g.total_rows >= 0 && g.total_rows <= 1 << 24, "Room for rows must be in 0..2^24");
     require(!g.seen == !g.new_seen, "seen and new_seen come together");
     const size_t n = size_t(p.sequences) * 4, room = size_t(g.total_rows) * 4;
-    struct Array {
-        const char* name;
-        const void* at;
-        size_t bytes;
-        bool needed, written;
-        const void* before;  // the array whose place it may take
-        unsigned align = 4;
+    const OpArray arrays[] = {
+        {"table", p.table, n * p.table_stride, true, true},
+        {"free_pages", p.free_pages, size_t(p.pages) * 4, true, true},
+        {"held", p.held, n, true, false},
+        {"free_count", p.free_count, 4, true, false},
+        {"shared", p.shared, n, false, false},
+        {"lengths", g.lengths, n, true, false},
+        {"seen", g.seen, n, false, false},
+        {"changes", g.changes, n, true, false},
+        {"new_lengths", g.new_lengths, n, true, true, 4, g.lengths},
+        {"new_seen", g.new_seen, n, false, true, 4, g.seen},
+        {"new_held", g.new_held, n, true, true, 4, p.held},
+        {"new_free_count", g.new_free_count, 4, true, true, 4, p.free_count},
+        {"offsets", g.offsets, n + 4, true, true},
+        {"row_sequences", g.row_sequences, room, false, true},
+        {"row_positions", g.row_positions, room, false, true},
+        {"row_slots", g.row_slots, 2 * room, false, true, 8},
     };
-    const Array arrays[] = {
-        {"table", p.table, n * p.table_stride, true, true, nullptr},
-        {"free_pages", p.free_pages, size_t(p.pages) * 4, true, true, nullptr},
-        {"held", p.held, n, true, false, nullptr},
-        {"free_count", p.free_count, 4, true, false, nullptr},
-        {"shared", p.shared, n, false, false, nullptr},
-        {"lengths", g.lengths, n, true, false, nullptr},
-        {"seen", g.seen, n, false, false, nullptr},
-        {"changes", g.changes, n, true, false, nullptr},
-        {"new_lengths", g.new_lengths, n, true, true, g.lengths},
-        {"new_seen", g.new_seen, n, false, true, g.seen},
-        {"new_held", g.new_held, n, true, true, p.held},
-        {"new_free_count", g.new_free_count, 4, true, true, p.free_count},
-        {"offsets", g.offsets, n + 4, true, true, nullptr},
-        {"row_sequences", g.row_sequences, room, false, true, nullptr},
-        {"row_positions", g.row_positions, room, false, true, nullptr},
-        {"row_slots", g.row_slots, 2 * room, false, true, nullptr, 8},
-    };
-    for (const Array& a : arrays) require(a.at || !a.needed, std::string("Null argument: ") + a.name);
-    for (const Array& a : arrays)
-        for (const Array& b : arrays)
-            if (&a != &b && a.at && b.at && a.written && !(a.before == b.at && a.at == b.at))
-                require((b.before == a.at && a.at == b.at) || apart(a.at, a.bytes, b.at, b.bytes),
-                        std::string(a.name) + " overlaps " + b.name);
+    check_arrays(arrays, std::size(arrays));
     const OpDevice device(p.table, "table", "the table", stream);
-    for (const Array& a : arrays)
-        if (a.at) device.check(a.at, a.name, a.align);
+    for (const OpArray& a : arrays)
+        if (a.at) device.check(a.at, a.name, a.alignment);
     ReserveView v{p.table,        p.free_pages,      p.held,         p.free_count,   p.shared,    g.lengths,
                   g.seen,         g.changes,         g.new_lengths,  g.new_seen,     g.new_held,  g.new_free_count,
                   g.offsets,      g.row_sequences,   g.row_positions, g.row_slots,   p.pages,     p.page_size,
                   p.sequences,    p.table_stride,    g.total_rows,   0,              0xffffffffu / unsigned(p.page_size)};
     const int64_t most = int64_t(p.table_stride) * p.page_size;
     v.most = int(most < kMaxRow ? most : kMaxRow);
-    reserve_kernel<<<1, kThreads, 0, stream>>>(v);
-    if (!g.total_rows || !(g.row_sequences || g.row_positions || g.row_slots)) return;
-    constexpr int kOf = kMapThreads * kMapRows;
-    reserve_rows_kernel<<<unsigned((g.total_rows + kOf - 1) / kOf), kMapThreads, 0, stream>>>(v);
+    const bool maps = g.total_rows && (g.row_sequences || g.row_positions || g.row_slots);
+    const bool few = g.total_rows <= kFewRows;
+    if (p.sequences <= 256)
+        reserve_kernel<256, 1><<<1, 256, 0, stream>>>(v, maps && few);
+    else if (p.sequences <= 1024)
+        reserve_kernel<1024, 1><<<1, 1024, 0, stream>>>(v, maps && few);
+    else
+        reserve_kernel<1024, 4><<<1, 1024, 0, stream>>>(v, maps && few);
+    if (!maps || few) return;
+    const int grid = std::min((g.total_rows + kMapThreads - 1) / kMapThreads, 2048);
+    reserve_rows_kernel<<<unsigned(grid), kMapThreads, 0, stream>>>(v);
 }
 
 }  // namespace qwen_hip

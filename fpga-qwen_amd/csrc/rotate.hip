@@ -256,9 +256,9 @@ bool regions_apart(const Region& a, const Region& b) {
            between(ahead, inner, a.piece, b.piece);
 }
 
-void check_side(const qwen_gpu_rotary_heads& h, const std::string& name, int head_dim, int rows) {
-    require(h.rows, "Null argument: " + name);
-    require(h.out, "Null argument: out of " + name);
+void check_side(const qwen_gpu_rotary_heads& h, const char* name, int head_dim, int rows) {
+    if (!h.rows) throw std::runtime_error(std::string("Null argument: ") + name);
+    if (!h.out) throw std::runtime_error(std::string("Null argument: out of ") + name);
     require(h.heads >= 1 && h.heads <= 4096, "Rotary heads must be in 1..4096");
     const int64_t most = int64_t(1) << 32;
     for (int64_t stride : {h.row_stride, h.head_stride, h.out_row_stride, h.out_head_stride})
@@ -306,7 +306,8 @@ void launch_rotate(const qwen_gpu_rotary& rotary, const qwen_gpu_rotary_heads& q
                     "The outs of queries and keys overlap");
         }
         auto clear = [&](const void* p, size_t bytes, const char* what) {
-            require(!p || apart(out.at, size_t(out.span()), p, bytes), std::string("out overlaps ") + what);
+            if (p && !apart(out.at, size_t(out.span()), p, bytes))
+                throw std::runtime_error(std::string("out overlaps ") + what);
         };
         clear(positions, size_t(rows) * 4, "positions");
         clear(rotary.dims ? rotary.frequencies : nullptr, size_t(rotary.dims) * 4, "frequencies");

@@ -8,8 +8,7 @@
 #include "verify.hpp"
 
 #include <algorithm>
-#include <string>
-#include <type_traits>
+#include <iterator>
 
 #include "decode_dev.hpp"
 #include "op_device.hpp"
@@ -615,33 +614,22 @@ void launch_verify_draft(const qwen_gpu_draft& d, int32_t* accepted, int32_t* ne
     auto span = [&](int64_t stride, int element) {
         return d.total_rows ? (size_t(d.total_rows - 1) * stride + d.vocabulary) * element : size_t(0);
     };
-    struct Array {
-        const char* name;
-        const void* at;
-        size_t bytes;
-        bool needed, written;
-        unsigned align = 4;
-    };
-    const Array arrays[] = {{"logits", d.logits, span(d.logit_stride, size), true, false, unsigned(size)},
-                            {"draft", d.draft, span(d.draft_stride, 4), false, false},
-                            {"tokens", d.tokens, rows, true, false},
-                            {"offsets", d.offsets, n + 4, false, false},
-                            {"temperature", d.temperature, n, false, false},
-                            {"accept", d.accept, rows, true, false},
-                            {"sample", d.sample, n, true, false},
-                            {"accepted", accepted, n, false, true},
-                            {"next", next, n, true, true},
-                            {"back", back, n, false, true},
-                            {"workspace", workspace, plan.bytes(), true, true, 16}};
-    for (const Array& a : arrays) require(a.at || !a.needed, std::string("Null argument: ") + a.name);
-    for (const Array& a : arrays)
-        for (const Array& b : arrays)
-            if (&a != &b && a.at && b.at && a.written)
-                require(apart(a.at, a.bytes, b.at, b.bytes), std::string(a.name) + " overlaps " + b.name);
+    const OpArray arrays[] = {{"logits", d.logits, span(d.logit_stride, size), true, false, unsigned(size)},
+                              {"draft", d.draft, span(d.draft_stride, 4), false, false},
+                              {"tokens", d.tokens, rows, true, false},
+                              {"offsets", d.offsets, n + 4, false, false},
+                              {"temperature", d.temperature, n, false, false},
+                              {"accept", d.accept, rows, true, false},
+                              {"sample", d.sample, n, true, false},
+                              {"accepted", accepted, n, false, true},
+                              {"next", next, n, true, true},
+                              {"back", back, n, false, true},
+                              {"workspace", workspace, plan.bytes(), true, true, 16}};
+    check_arrays(arrays, std::size(arrays));
     require(workspace_bytes >= plan.bytes(), "Workspace is too small");
     const OpDevice device(d.logits, "logits", "the logits", stream);
-    for (const Array& a : arrays)
-        if (a.at) device.check(a.at, a.name, a.align);
+    for (const OpArray& a : arrays)
+        if (a.at) device.check(a.at, a.name, a.alignment);
     char* const space = static_cast<char*>(workspace);
     const VerifyArgs a{static_cast<const char*>(d.logits), d.draft, d.tokens, d.offsets, d.temperature, d.accept, d.sample,
                        d.total_rows > 1 ? d.logit_stride : 0, d.total_rows > 1 ? d.draft_stride : 0, d.vocabulary,
