@@ -84,10 +84,19 @@ __device__ __forceinline__ int owner(const int* upto, int n, int k) {
 }
 
 // Pages k below `count`, whose sequences' sums are `upto`: f(s, k) gives a
-// place to read and one to write. A thread has eight in a row, so it looks
-// for the first one's sequence alone, and all its loads are in flight.
+// place to read and one to write. Of many, a thread has eight in a row, so it
+// looks for the first one's sequence alone, and all its loads are in flight.
 template <int THREADS, class F>
 __device__ __forceinline__ void move_pages(const int* upto, int n, int count, F f) {
+    if (count <= THREADS) {
+        const int k = threadIdx.x;
+        if (k >= count) return;
+        const int32_t* from;
+        int32_t* to;
+        f(owner(upto, n, k), k, from, to);
+        *to = *from;
+        return;
+    }
     constexpr int kRow = 8;
     for (int k0 = kRow * threadIdx.x; k0 < count; k0 += kRow * THREADS) {
         int s = owner(upto, n, k0), page[kRow];

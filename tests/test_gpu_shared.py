@@ -316,3 +316,201 @@ def test_wrapper(qpkg):
             # Twice the distance of either from 64 bits, which the tests above hold to less.
             assert np.abs(got - want).max() < 2e-5
     assert cache.attention_shared(queries, 32, scale=0.5).shape == queries.shape
+
+
+# ---- a whole step ----
+
+class Server:
+    """A cache whose sequences share a prefix and whose pages, lengths and rows never leave the device: each step's
+    drafted tokens are given pages, rotated, appended, attended and verified, and those refused are taken back."""
+
+    def __init__(self, q, rng, kind='bf16', n=5, drafts=3, page=4, prefix=18, kv=2, heads=6, dim=64, vocabulary=40):
+        self.q, self.lib, self.kv, self.heads, self.dim, self.n, self.vocabulary = q, q.load_library(), kv, heads, dim, n, vocabulary
+        self.page, self.rows, self.kind = page, drafts + 1, kind
+        self.pages, self.width, whole = 90, 14, -(-prefix // page)
+        make = lambda x, dtype=np.int32: q.DeviceBuffer.from_array(np.asarray(x, dtype))  # noqa: E731
+        # The prefix' pages belong to all; its last one is full, so that nobody appends to it.
+        prefix = whole * page
+        self.prefix, self.cache = prefix, ref.Cache(kind, self.pages, page, kv, dim, fill=0)
+        order = rng.permutation(self.pages)
+        table = np.full((n, self.width), -1, np.int32)
+        table[:, :whole] = order[:whole]
+        for name in ('keys', 'values'):
+            rows = ref.to_bits(rng.standard_normal((whole * page * kv, dim)), kind)
+            for j in range(prefix):
+                for h in range(kv):
+                    getattr(self.cache, name)[self.cache.where(order[j // page], h, j % page)] = rows[j * kv + h]
+        stack = np.full(self.pages, -1, np.int32)
+        stack[:self.pages - whole] = order[whole:]
+        self.state = dict(table=table, held=np.full(n, whole), free=order[whole:], lengths=np.full(n, prefix),
+                          page_size=page, pages=self.pages, shared=np.full(n, whole))
+        room = n * self.rows
+        self.on = {'table': make(table), 'stack': make(stack), 'held': make(np.full(n, whole)),
+                   'count': make([self.pages - whole]), 'shared': make(np.full(n, whole)), 'lengths': make(np.full(n, prefix)),
+                   'changes': make(np.zeros(n)), 'offsets': make(np.zeros(n + 1)), 'positions': make(np.zeros(room)),
+                   'keys': make(self.cache.keys, None), 'values': make(self.cache.values, None),
+                   'prefix': make([prefix]), 'qkv': make(np.zeros((room, (heads + 2 * kv) * dim)), np.float32),
+                   'norm': make(np.linspace(0.5, 1.5, dim), np.float32),
+                   'frequencies': make(1e4 ** (-np.arange(dim // 2) / (dim // 2)), np.float64),
+                   'logits': make(np.zeros((room, vocabulary)), np.float32), 'tokens': make(np.zeros(room)),
+                   'accept': make(np.zeros(room), np.float32), 'sample': make(np.zeros(n), np.float32),
+                   'accepted': make(np.zeros(n)), 'next': make(np.zeros(n)), 'back': make(np.zeros(n))}
+        at = {name: buffer.ptr.value for name, buffer in self.on.items()}
+        self.pool = q.PagedPool(at['table'], at['stack'], at['held'], at['count'], at['shared'], self.pages, page, n, self.width)
+        more = self._more(n + 1)  # the second call's offsets, which nobody reads
+        self.grow, self.shrink = (q.PagedGrowth(at['lengths'], None, at[change], at['lengths'], None, at['held'], at['count'],
+                                                offsets, None, positions, None, rows)
+                                  for change, offsets, positions, rows in (('changes', at['offsets'], at['positions'], room),
+                                                                           ('back', more, None, 0)))
+        self.c = q.PagedCache(at['keys'], at['values'], None, *self.cache.strides, self.pages, page, kv, dim, q.PAGED_TYPES[kind])
+        self.b = q.PagedBatch(at['table'], at['lengths'], at['offsets'], None, None, None, 0, n, self.width,
+                              self.width * page, self.rows, room)
+        self.p = q.PagedPrefix(at['prefix'], None, 1, prefix, self.width * page - prefix)
+        row = (heads + 2 * kv) * dim
+        self.row = row
+        self.rotary = q.Rotary(at['frequencies'], dim, 0, dim, 0, 1, 1e-6)
+        self.sides = [q.RotaryHeads(at['qkv'] + 4 * shift, at['qkv'] + 4 * shift, at['norm'], row, dim, row, dim, count)
+                      for shift, count in ((0, heads), (heads * dim, kv))]
+        self.draft = q.Draft(at['logits'], None, at['tokens'], at['offsets'], None, at['accept'], at['sample'], vocabulary, 0, 0,
+                             vocabulary, n, self.rows, room)
+        need = ctypes.c_size_t()
+        self.ok(self.lib.qwen_gpu_op_paged_shared_workspace(self.c, self.b, self.p, heads, ctypes.byref(need)))
+        self.space = make(np.full(need.value, 0x5a), np.uint8)
+        self.ok(self.lib.qwen_gpu_op_verify_workspace(self.draft, ctypes.byref(need)))
+        self.space2 = make(np.full(need.value, 0x5a), np.uint8)
+
+    def _more(self, count):
+        self.extra = self.q.DeviceBuffer.from_array(np.zeros(count, np.int32))
+        return self.extra.ptr.value
+
+    def ok(self, status):
+        if status:
+            raise RuntimeError(self.lib.qwen_gpu_last_error().decode())
+
+    def give(self, **arrays):
+        for name, array in arrays.items():
+            array = np.ascontiguousarray(array)
+            self.ok(self.lib.qwen_gpu_memcpy_to_device(self.on[name].ptr, array.ctypes.data, array.nbytes))
+
+    def get(self, name, dtype, count):
+        return self.on[name].to_array(dtype, count)
+
+    def enqueue(self, stream=None):
+        """One step; out takes the queries' place."""
+        lib, at, row, dim = self.lib, self.on['qkv'].ptr.value, self.row, self.dim
+        keys, values = at + 4 * self.heads * dim, at + 4 * (self.heads + self.kv) * dim
+        self.ok(lib.qwen_gpu_op_paged_reserve(self.pool, self.grow, stream))
+        self.ok(lib.qwen_gpu_op_rotate(self.rotary, self.sides[0], self.sides[1], self.on['positions'].ptr,
+                                       self.n * self.rows, stream))
+        self.ok(lib.qwen_gpu_op_paged_append(self.c, self.b, keys, row, values, row, stream))
+        self.ok(lib.qwen_gpu_op_paged_attention_shared(self.c, self.b, self.p, at, row, self.heads, 0.125, at, row,
+                                                       self.space.ptr, self.space.nbytes, stream))
+        self.ok(lib.qwen_gpu_op_verify_draft(self.draft, self.on['accepted'].ptr, self.on['next'].ptr, self.on['back'].ptr,
+                                             self.space2.ptr, self.space2.nbytes, stream))
+        self.ok(lib.qwen_gpu_op_paged_reserve(self.pool, self.shrink, stream))
+
+    def inputs(self, rng):
+        room = self.n * self.rows
+        counts = rng.integers(0, self.rows + 1, self.n)
+        logits = 2 * rng.standard_normal((room, self.vocabulary))
+        tokens = rng.integers(0, self.vocabulary, room)
+        tokens[1:] = np.where(rng.random(room - 1) < 0.6, logits[:-1].argmax(1), tokens[1:])
+        return dict(changes=counts.astype(np.int32), qkv=rng.standard_normal((room, self.row)).astype(np.float32),
+                    logits=logits.astype(np.float32), tokens=tokens.astype(np.int32),
+                    accept=rng.random(room).astype(np.float32), sample=rng.random(self.n).astype(np.float32))
+
+    def expect(self, given):
+        """The step's results against the oracles, which carry the state on."""
+        room, n, dim, heads, kv = self.n * self.rows, self.n, self.dim, self.heads, self.kv
+        there = steps.reserve(**self.state, changes=given['changes'], room=room)
+        total = int(there['offsets'][-1])
+        assert np.array_equal(self.get('positions', np.int32, room), there['positions'])
+        qkv = given['qkv'].reshape(room, heads + 2 * kv, dim)
+        norm = np.linspace(0.5, 1.5, dim).astype(np.float32)
+        turned, _ = steps.rotate(qkv[:total, :heads + kv], there['positions'][:total],
+                                 1e4 ** (-np.arange(dim // 2) / (dim // 2)), False, 1.0, norm, np.float32(1e-6))
+        # What the kernels wrote is within a rounding of these; the attention is held against the device's own keys.
+        pools = {name: self.get(name, np.uint16, self.cache.keys.size) for name in ('keys', 'values')}
+        expected = self.cache.copy()
+        ref.append(expected, there['table'], there['lengths'], self.rows, there['offsets'], turned[:, heads:].astype(np.float32),
+                   qkv[:total, heads + kv:])
+        assert np.array_equal(expected.values, pools['values'])
+        got, want = (ref.from_bits(x, self.kind) for x in (pools['keys'], expected.keys))
+        # 27 u of two channels, then BF16's half step: a value next to a border may go the other way.
+        assert (np.abs(got - want) <= 2.0 ** -7 * np.abs(want) + 1e-4).all()
+        self.cache.keys, self.cache.values = pools['keys'], pools['values']
+        queries = turned[:, :heads].astype(np.float32)
+        out, tolerance, _, _ = ref.attention(self.cache, there['table'], there['lengths'], self.rows, there['offsets'], queries,
+                                             0.125, queries)
+        after = self.get('qkv', np.float32, room * self.row).reshape(room, heads + 2 * kv, dim)
+        off = np.abs(after[:total, :heads] - out)
+        # Queries are off by 27 u of up to 2 * sqrt(64) * 1.5: scores by 1e-4 at most, weights and outputs by as much.
+        assert (off <= tolerance + 4e-4).all(), off.max()
+        assert np.array_equal(after[total:].view(np.uint32), qkv[total:].view(np.uint32))
+        counts = np.diff(there['offsets'])
+        accepted, following = steps.verify(given['logits'][:total], given['tokens'][:total], given['accept'][:total],
+                                           given['sample'], None, counts)
+        assert np.array_equal(self.get('accepted', np.int32, n), accepted)
+        assert np.array_equal(self.get('next', np.int32, n), following)
+        back = accepted - np.maximum(counts - 1, 0)
+        assert np.array_equal(self.get('back', np.int32, n), back)
+        done = steps.reserve(there['table'], there['held'], there['free'], there['lengths'], back, self.page, self.pages, 0,
+                             shared=self.state['shared'])
+        self.state.update({name: done[name] for name in ('table', 'held', 'free', 'lengths')})
+        for name, size in (('held', n), ('lengths', n)):
+            assert np.array_equal(self.get(name, np.int32, size), done[name]), name
+        assert np.array_equal(self.get('table', np.int32, done['table'].size).reshape(done['table'].shape), done['table'])
+        count = int(self.get('count', np.int32, 1)[0])
+        assert np.array_equal(self.get('stack', np.int32, self.pages)[:count], done['free'])
+
+
+@pytest.mark.parametrize('kind', ['f16', 'bf16'])
+def test_steps(qpkg, kind):
+    """Eight steps of a server, to where sequences run into the ends of their tables."""
+    rng = np.random.default_rng(31)
+    server = Server(qpkg, rng, kind)
+    for _ in range(8):
+        given = server.inputs(rng)
+        server.give(**given)
+        server.enqueue()
+        qpkg.synchronize()
+        server.expect(given)
+
+
+def test_captured_steps(qpkg):
+    """A step captured once and replayed, eager steps on another server between the replays; then two graphs of two
+    servers, each with workspaces of its own, in flight at once."""
+    hip, rng = Hip(), np.random.default_rng(32)
+    servers = [Server(qpkg, np.random.default_rng(33)) for _ in range(3)]
+    streams, runs, graphs = [ctypes.c_void_p() for _ in range(2)], [ctypes.c_void_p() for _ in range(2)], []
+    for stream, run, server in zip(streams, runs, servers):
+        graph = ctypes.c_void_p()
+        hip.hipStreamCreate(ctypes.byref(stream))
+        hip.hipStreamBeginCapture(stream, 0)
+        server.enqueue(stream)
+        hip.hipStreamEndCapture(stream, ctypes.byref(graph))
+        hip.hipGraphInstantiate(ctypes.byref(run), graph, None, None, 0)
+        graphs.append(graph)
+    for turn in range(6):
+        given = [server.inputs(rng) for server in servers]
+        for server, arrays in zip(servers, given):
+            server.give(**arrays)
+        if turn % 2:
+            for stream, run in zip(streams, runs):
+                hip.hipGraphLaunch(run, stream)
+            servers[2].enqueue()
+        else:
+            for stream, run in zip(streams, runs):
+                hip.hipGraphLaunch(run, stream)
+                hip.hipStreamSynchronize(stream)
+                if run is runs[0]:
+                    servers[2].enqueue()
+        for stream in streams:
+            hip.hipStreamSynchronize(stream)
+        qpkg.synchronize()
+        for server, arrays in zip(servers, given):
+            server.expect(arrays)
+    for stream, run, graph in zip(streams, runs, graphs):
+        hip.hipGraphExecDestroy(run)
+        hip.hipGraphDestroy(graph)
+        hip.hipStreamDestroy(stream)

@@ -506,3 +506,53 @@ def test_verify_repeats(qpkg):
     for _ in range(3):
         for call, want in zip(calls, first):
             assert all(np.array_equal(a, b) for a, b in zip(call(), want))
+
+
+# ---- calls at once, streams, graphs ----
+
+def test_calls_on_streams(qpkg):
+    """Every operator on a stream of its own, all in flight at once, against the same calls one after the other; the
+    runtime's stand-in handles are refused."""
+    q, hip, rng = qpkg, Hip(), np.random.default_rng(21)
+    lib, streams = q.load_library(), []
+    for _ in range(4):
+        streams.append(ctypes.c_void_p())
+        hip.hipStreamCreate(ctypes.byref(streams[-1]))
+    drafts = [Drafts(q, **random_drafts(rng, 5, 4, 9000, ragged=True)) for _ in range(2)]
+    alone = [call() for call in drafts]
+    x = [rng.standard_normal((200, 6 * 64)).astype(np.float32) for _ in range(2)]
+    frequencies, positions = 1e4 ** (-np.arange(32) / 32), rng.integers(0, 9999, 200)
+    place, turns = q.DeviceBuffer.from_array(positions.astype(np.int32)), q.DeviceBuffer.from_array(frequencies)
+    rotary = q.Rotary(turns.ptr, 64, 0, 64, 0, 1, 1e-6)
+    want = []
+    for array in x:
+        side = Heads(q, array, 6, 64, 0)
+        want.append(rotate(q, [side], [None], positions, frequencies, False, 1.0, 'f32')[0])
+    on = [q.DeviceBuffer.from_array(array) for array in x]
+    for turn in range(2):
+        for call, stream in zip(drafts, streams):
+            call.enqueue(stream)
+        for buffer, stream in zip(on, streams[2:]):
+            if turn == 0:
+                heads = q.RotaryHeads(buffer.ptr, buffer.ptr, None, 384, 64, 384, 64, 6)
+                ok(q, lib.qwen_gpu_op_rotate(rotary, heads, None, place.ptr, 200, stream))
+    for stream in streams:
+        hip.hipStreamSynchronize(stream)
+    for call, given in zip(drafts, alone):
+        assert all(np.array_equal(a, b) for a, b in zip(call.results(), given))
+    for buffer, given in zip(on, want):
+        assert np.array_equal(buffer.to_array(np.float32, given.size), given.reshape(-1))
+    for handle in (1, 2):
+        with pytest.raises(RuntimeError, match='The stream must be NULL'):
+            drafts[0].enqueue(ctypes.c_void_p(handle))
+    for stream in streams:
+        hip.hipStreamDestroy(stream)
+
+
+def test_host_memory_is_refused(qpkg):
+    """Plain host arrays, which a kernel cannot read, are found before anything is launched."""
+    call = Drafts(qpkg, **random_drafts(np.random.default_rng(22), 2, 2, 50))
+    host = np.zeros(100, np.float32)
+    call.given.sample = host.ctypes.data
+    with pytest.raises(RuntimeError, match='Not device memory: sample'):
+        call()
