@@ -144,41 +144,117 @@ struct SharedSpace {
     float2 states[kWaves][16];
 };
 
-// S^T = K Q^T and O^T = V^T P^T on the matrix cores as paged_attention_kernel
-// has them (32 positions a wave's step, FP32 queries and weights as two FP16
-// or three BF16 terms), but with up to TILES times 16 query rows in a wave:
-// keys stay in registers and values in LDS while all tiles are multiplied by
-// them. A prefix's query rows are those of all new rows of its group, so its
-// positions are read once for TILES * 16 of them. CAUSAL: positions behind a
-// prefix, which end at each new row's own.
-template <int TYPE, int DIM, int TILES, bool CAUSAL>
+// Query rows of a job as their terms: row r is head r % group of new row
+// r / group. Scores' factor is above 0, so that minus infinity stays that: a scale's
+// sign goes into the queries.
+template <int DIM>
+__device__ __forceinline__ const float* query_at(const PagedView& v, const SharedArgs& a, const SharedJob& job, int query_row,
+                                                 bool& live) {
+    const int new_row = a.new_row(query_row);
+    const int64_t row = int64_t(job.first) + new_row;
+    live = query_row < job.rows && row >= 0 && row < v.total_rows;
+    return a.queries + (live ? row * a.query_stride + (job.head * a.group + query_row - new_row * a.group) * DIM : 0);
+}
+// PER: 16-bit products of a lane's 16 bytes of a stored row, whose channels it holds.
+template <int DIM, int PER>
+__device__ __forceinline__ void load_query(const float* from, bool live, int part, float (&x)[DIM / 32][8]) {
+#pragma unroll
+    for (int k = 0; k < DIM / 32; ++k) {
+        const int channel = PER == 1 ? 32 * k + 8 * part : 64 * (k / 2) + 16 * part + 8 * (k % 2);
+        const float4_a4 lo = *reinterpret_cast<const float4_a4*>(from + channel);
+        const float4_a4 hi = *reinterpret_cast<const float4_a4*>(from + channel + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[k][e] = live ? lo[e] : 0.f, x[k][4 + e] = live ? hi[e] : 0.f;
+    }
+}
+template <int TYPE, int DIM, int TERMS>
+__device__ __forceinline__ float split_query(float (&x)[DIM / 32][8], float scale, uint4_t (&query)[DIM / 32][TERMS]) {
+    float to_score = fmaxf(__builtin_fabsf(scale), 1e-37f), times = scale == 0.f ? 0.f : __builtin_copysignf(1.f, scale);
+    if constexpr (TYPE == kPagedF16) {
+        // An exact power of two brings a row's largest query to [2^14, 2^15), so that neither term leaves
+        // FP16's range; non-finite ones stay so.
+        float top = 0.f;
+#pragma unroll
+        for (int k = 0; k < DIM / 32; ++k)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = fmaxf(top, __builtin_fabsf(x[k][e]));
+        top = fmaxf(top, dev::xor_lanes<16>(top));
+        top = fmaxf(top, dev::xor_lanes<32>(top));
+        const int up = 14 - max(int(__builtin_bit_cast(unsigned, top) >> 23) - 127, -100);
+        times *= pow2(up);
+        to_score = fmaxf(to_score * pow2(-up), 0x1p-149f);
+    }
+#pragma unroll
+    for (int k = 0; k < DIM / 32; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            unsigned words[TERMS];
+            Terms<TYPE, false>::split(x[k][2 * e] * times, x[k][2 * e + 1] * times, false, words);
+#pragma unroll
+            for (int p = 0; p < TERMS; ++p) query[k][p][e] = words[p];
+        }
+    return to_score;
+}
+
+// A step of a row's online softmax: 8 scores of a lane (minus infinity where
+// hidden) times factor(u, r) become weights relative to the row's reference,
+// which moves, and the sums so far with it, only when a score passes it by 2^8.
+template <int TYPE, int OUT, class F>
+__device__ __forceinline__ void soften(const float4_t (&s)[2], F factor, float high, float& reference, float& sum,
+                                       float4_t (&acc)[OUT], float (&weights)[2][4]) {
+    constexpr float kHead = TYPE == kPagedF16 ? 6.f : 0.f;  // FP16 weights are kept up to 2^14, far from subnormals
+    constexpr float kGrow = 8.f;
+    if (__any(high > reference + (kHead + kGrow))) {
+        high = fmaxf(high, dev::xor_lanes<16>(high));
+        high = fmaxf(high, dev::xor_lanes<32>(high));
+        const float moved = fmaxf(reference, high - kHead);
+        const float shrink = reference == moved ? 1.f : exp2_fast(reference - moved);
+        reference = moved;
+        sum *= shrink;
+#pragma unroll
+        for (int o = 0; o < OUT; ++o) acc[o] *= shrink;
+    }
+    const float from = reference == -kInf ? 0.f : reference;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            weights[u][r] = exp2_fast(__builtin_fmaf(s[u][r], factor(u, r), -from));
+            sum += weights[u][r];
+        }
+}
+template <int TYPE, int TERMS>
+__device__ __forceinline__ void split_weights(const float (&weights)[2][4], uint4_t (&terms)[TERMS]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        unsigned words[TERMS];
+        Terms<TYPE, false>::split(weights[e / 2][2 * (e % 2)], weights[e / 2][2 * (e % 2) + 1], false, words);
+#pragma unroll
+        for (int p = 0; p < TERMS; ++p) terms[p][e] = words[p];
+    }
+}
+
+// Up to 16 query rows: S^T = K Q^T and O^T = V^T P^T on the matrix cores as
+// paged_attention_kernel has them, 32 positions a wave's step, FP32 queries and
+// weights as two FP16 or three BF16 terms, each wave every fourth step, the
+// next one's loads in flight. CAUSAL: positions behind a prefix, which end at
+// each new row's own. Memory bounds it where there are many positions; a
+// workgroup spends 8 us besides (2 to find its job, 3 for the first rows, 3
+// for the waves' sums and to make place for the next).
+template <int TYPE, int DIM, bool CAUSAL>
 __device__ __forceinline__ void shared_attend(const PagedView& v, const SharedArgs& a, const SharedJob& job,
                                               SharedSpace<DIM>& space) {
     constexpr int kSize = TYPE == kPagedE4M3 ? 1 : 2, kLoads = DIM * kSize / 64, kSteps = DIM / 32, kOut = DIM / 16;
     constexpr int kPer = kSteps / kLoads;         // products per load: 1, or 2 for E4M3
-    constexpr int kRows = 16 * TILES, kProducts = Terms<TYPE, false>::kProducts;
-    constexpr int kPitch = SharedSpace<DIM>::kPitch;
-    constexpr float kHead = TYPE == kPagedF16 ? 6.f : 0.f;  // FP16 weights are kept up to 2^14, far from subnormals
-    constexpr float kGrow = 8.f;                  // a reference is moved once a score passes it by 2^8
+    constexpr int kProducts = Terms<TYPE, false>::kProducts, kPitch = SharedSpace<DIM>::kPitch;
     constexpr std::integral_constant<int, TYPE> kType{};
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int column = lane & 15, part = lane >> 4;
-    const int begin = job.from;
     // Positions from shared_end on are seen by some of the tile's new rows only, from `end` on by none.
-    const int last_row = min(job.rows - 1, job.row0 + kRows - 1);
+    const int last_row = min(job.rows, job.row0 + 16) - 1;
     const int shared_end = CAUSAL ? min(job.to, job.sees + a.new_row(job.row0)) : job.to;
     const int end = CAUSAL ? min(job.to, job.sees + a.new_row(last_row)) : job.to;
-    constexpr int live_tiles = TILES;
     const int32_t* const table = v.table + int64_t(job.s) * v.table_stride;
-
-    float4_t acc[TILES][kOut];
-    float reference[TILES], sum[TILES];
-#pragma unroll
-    for (int t = 0; t < TILES; ++t) {
-        reference[t] = -kInf, sum[t] = 0.f;
-#pragma unroll
-        for (int o = 0; o < kOut; ++o) acc[t][o] = float4_t{0.f, 0.f, 0.f, 0.f};
-    }
 
     // A step's rows: page entries, then offsets, then 16-byte pieces.
     int pages[2], slots[2];
@@ -214,75 +290,29 @@ __device__ __forceinline__ void shared_attend(const PagedView& v, const SharedAr
     char* const mine = space.rows[wave];
     const char* const transposed = mine + (4 * part + (column >> 2)) * kPitch + (column & 3) * 8;
 
-    int base = begin + kTile * wave;
+    // The table's entries first, then queries, keys and values in one flight.
+    int base = job.from + kTile * wave;
     if (base < end) find(base);
-    // Queries: row r of the job is head r % group of new row r / group.
-    uint4_t query[TILES][kSteps][kProducts];
-    float to_score[TILES];  // what a product's sum is multiplied by
-    int sees[TILES];        // positions the lane's row attends
-#pragma unroll
-    for (int t = 0; t < TILES; ++t) {
-        if (t >= live_tiles) continue;
-        __builtin_amdgcn_sched_barrier(0);  // a tile's queries at a time, for the registers
-        const int query_row = job.row0 + 16 * t + column, new_row = a.new_row(query_row);
-        const int64_t row = int64_t(job.first) + new_row;
-        const bool live = query_row < job.rows && row >= 0 && row < v.total_rows;
-        sees[t] = !live ? 0 : CAUSAL ? job.sees + new_row : job.to;
-        const float* const from =
-            a.queries + (live ? row * a.query_stride + (job.head * a.group + query_row - new_row * a.group) * DIM : 0);
-        float x[kSteps][8], top = 0.f;
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-            // The channels that this lane's part of a stored row holds in step k.
-            const int from_channel = kPer == 1 ? 32 * k + 8 * part : 64 * (k / 2) + 16 * part + 8 * (k % 2);
-            const float4_a4 lo = *reinterpret_cast<const float4_a4*>(from + from_channel);
-            const float4_a4 hi = *reinterpret_cast<const float4_a4*>(from + from_channel + 4);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[k][e] = live ? lo[e] : 0.f, x[k][4 + e] = live ? hi[e] : 0.f;
-        }
-        to_score[t] = a.scale;
-        if constexpr (TYPE == kPagedF16) {
-            // An exact power of two brings a row's largest query to [2^14, 2^15), so that neither term leaves
-            // FP16's range; non-finite ones stay so.
-#pragma unroll
-            for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) top = fmaxf(top, __builtin_fabsf(x[k][e]));
-            top = fmaxf(top, dev::xor_lanes<16>(top));
-            top = fmaxf(top, dev::xor_lanes<32>(top));
-            const int up = 14 - max(int(__builtin_bit_cast(unsigned, top) >> 23) - 127, -100);
-#pragma unroll
-            for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[k][e] *= pow2(up);
-            to_score[t] *= pow2(-up);
-        }
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                unsigned words[kProducts];
-                Terms<TYPE, false>::split(x[k][2 * e], x[k][2 * e + 1], false, words);
-#pragma unroll
-                for (int p = 0; p < kProducts; ++p) query[t][k][p][e] = words[p];
-            }
-    }
+    bool live;
+    const float* const from = query_at<DIM>(v, a, job, job.row0 + column, live);
+    const int sees = !live ? 0 : CAUSAL ? job.sees + a.new_row(job.row0 + column) : job.to;  // of the lane's row
+    float x[kSteps][8];
+    load_query<DIM, kPer>(from, live, part, x);
     if (base < end) {
         place(base);
         load(v.keys, keys);
         if (base + kBlock < end) find(base + kBlock);
         load(v.values, values);
     }
-
-    auto each_tile = [](auto f) {
-        f(std::integral_constant<int, 0>{});
-        if constexpr (TILES > 1) f(std::integral_constant<int, 1>{});
-        if constexpr (TILES > 2) f(std::integral_constant<int, 2>{}), f(std::integral_constant<int, 3>{});
-    };
-    for (; base < end; base += kBlock) {
-        float4_t s[TILES][2];
+    uint4_t query[kSteps][kProducts];
+    const float to_score = split_query<TYPE, DIM>(x, a.scale, query);
+    float4_t acc[kOut];
+    float reference = -kInf, sum = 0.f;
 #pragma unroll
-        for (int t = 0; t < TILES; ++t) s[t][0] = s[t][1] = float4_t{0.f, 0.f, 0.f, 0.f};
+    for (int o = 0; o < kOut; ++o) acc[o] = float4_t{0.f, 0.f, 0.f, 0.f};
+
+    for (; base < end; base += kBlock) {
+        float4_t s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -290,14 +320,9 @@ __device__ __forceinline__ void shared_attend(const PagedView& v, const SharedAr
                 uint4_t k[kPer];
                 widen<TYPE>(keys[u][i], byte_pow2(bytes[u] & 255), k);
 #pragma unroll
-                for (int t = 0; t < TILES; ++t) {
-                    if (t >= live_tiles) continue;
+                for (int j = 0; j < kPer; ++j)
 #pragma unroll
-                    for (int j = 0; j < kPer; ++j)
-#pragma unroll
-                        for (int p = 0; p < kProducts; ++p)
-                            s[t][u] = multiply(k[j], query[t][kPer * i + j][p], s[t][u], kType);
-                }
+                    for (int p = 0; p < kProducts; ++p) s[u] = multiply(k[j], query[kPer * i + j][p], s[u], kType);
             }
         // What the rest of this step needs of its rows, before the next one's take their place.
         const bool was[2] = {there[0], there[1]};
@@ -344,137 +369,86 @@ __device__ __forceinline__ void shared_attend(const PagedView& v, const SharedAr
             load(v.values, values);
         }
 
-        float weights[TILES][2][4];
-        uint4_t weight[TILES][kProducts];
-#pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-            if (t >= live_tiles) continue;
-            float high = -kInf;
-            unsigned hidden = 0;  // bit 4 u + r
-            if (whole) {
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) high = fmaxf(high, s[t][u][r] * to_score[t]);
-            } else {
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int j = 16 * u + 4 * part + r;
-                        if (!(exist >> j & 1) || (CAUSAL && base + j >= sees[t]))
-                            hidden |= 1u << (4 * u + r);
-                        else
-                            high = fmaxf(high, s[t][u][r] * to_score[t]);
-                    }
-            }
-            if (__any(high > reference[t] + (kHead + kGrow))) {
-                high = fmaxf(high, dev::xor_lanes<16>(high));
-                high = fmaxf(high, dev::xor_lanes<32>(high));
-                const float moved = fmaxf(reference[t], high - kHead);
-                const float shrink = reference[t] == moved ? 1.f : exp2_fast(reference[t] - moved);
-                reference[t] = moved;
-                sum[t] *= shrink;
-#pragma unroll
-                for (int o = 0; o < kOut; ++o) acc[t][o] *= shrink;
-            }
-            const float from = reference[t] == -kInf ? 0.f : reference[t];
+        if (!whole)
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    float p = exp2_fast(__builtin_fmaf(s[t][u][r], to_score[t], -from));
-                    if (!whole && (hidden >> (4 * u + r) & 1)) p = 0.f;
-                    weights[t][u][r] = p;
-                    sum[t] += p;
+                    const int j = 16 * u + 4 * part + r;
+                    if (!(exist >> j & 1) || (CAUSAL && base + j >= sees)) s[u][r] = -kInf;
                 }
+        float high = s[0][0], weights[2][4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                unsigned words[kProducts];
-                Terms<TYPE, false>::split(weights[t][e / 2][2 * (e % 2)], weights[t][e / 2][2 * (e % 2) + 1], false, words);
-#pragma unroll
-                for (int p = 0; p < kProducts; ++p) weight[t][p][e] = words[p];
-            }
-        }
+        for (int i = 1; i < 8; ++i) high = fmaxf(high, s[i / 4][i % 4]);
+        soften<TYPE>(s, [&](int, int) { return to_score; }, high * to_score, reference, sum, acc, weights);
+        uint4_t weight[kProducts];
+        split_weights<TYPE>(weights, weight);
 #pragma unroll
         for (int o = 0; o < kOut; ++o) {
             const short4_t low = read_transposed(transposed + 32 * o);
-            const short4_t high = read_transposed(transposed + 16 * kPitch + 32 * o);
+            const short4_t top = read_transposed(transposed + 16 * kPitch + 32 * o);
             const uint4_t w = {__builtin_bit_cast(u32x2, low)[0], __builtin_bit_cast(u32x2, low)[1],
-                               __builtin_bit_cast(u32x2, high)[0], __builtin_bit_cast(u32x2, high)[1]};
+                               __builtin_bit_cast(u32x2, top)[0], __builtin_bit_cast(u32x2, top)[1]};
 #pragma unroll
-            for (int t = 0; t < TILES; ++t) {
-                if (t >= live_tiles) continue;
-#pragma unroll
-                for (int p = 0; p < kProducts; ++p) acc[t][o] = multiply(w, weight[t][p], acc[t][o], kType);
-            }
+            for (int p = 0; p < kProducts; ++p) acc[o] = multiply(w, weight[p], acc[o], kType);
         }
 
         // One row at a time, for the new rows that see it; the wave's weights pass through its part of LDS, whose
         // values have been read.
         if (CAUSAL && spoilt) {
             float* const passed = reinterpret_cast<float*>(mine);
-            each_tile([&](auto of) {
-                constexpr int t = decltype(of)::value;
-                if (t >= live_tiles) return;
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
-                    *reinterpret_cast<float4_t*>(passed + column * kTile + 16 * u + 4 * part) =
-                        float4_t{weights[t][u][0], weights[t][u][1], weights[t][u][2], weights[t][u][3]};
-                for (int j = max(0, shared_end - base); j < kTile; ++j) {
-                    if (!(exist >> j & 1)) continue;
-                    const int64_t from = __shfl(j < 16 ? row_at[0] : row_at[1], j & 15);
-                    const float up = __shfl(j < 16 ? value_up[0] : value_up[1], j & 15);
-                    const float p = passed[column * kTile + j];
-                    if (base + j >= sees[t]) continue;
+            for (int u = 0; u < 2; ++u)
+                *reinterpret_cast<float4_t*>(passed + column * kTile + 16 * u + 4 * part) =
+                    float4_t{weights[u][0], weights[u][1], weights[u][2], weights[u][3]};
+            for (int j = max(0, shared_end - base); j < kTile; ++j) {
+                if (!(exist >> j & 1)) continue;
+                const int64_t row = __shfl(j < 16 ? row_at[0] : row_at[1], j & 15);
+                const float up = __shfl(j < 16 ? value_up[0] : value_up[1], j & 15);
+                const float p = passed[column * kTile + j];
+                if (base + j >= sees) continue;
 #pragma unroll
-                    for (int o = 0; o < kOut; ++o)
+                for (int o = 0; o < kOut; ++o)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float x = stored<TYPE>(v.values + from, 16 * o + 4 * part + e, up);
-                            if (x - x != 0.f) acc[t][o][e] = __builtin_fmaf(p, x, acc[t][o][e]);
-                        }
-                }
-            });
+                    for (int e = 0; e < 4; ++e) {
+                        const float value = stored<TYPE>(v.values + row, 16 * o + 4 * part + e, up);
+                        if (value - value != 0.f) acc[o][e] = __builtin_fmaf(p, value, acc[o][e]);
+                    }
+            }
         }
     }
 
-    // The four waves' sums, a tile at a time, brought to their largest reference.
+    // The four waves' sums, brought to their largest reference.
     float* const sums = reinterpret_cast<float*>(space.rows);  // [kWaves][16][DIM]
+    __syncthreads();
+    sum += dev::xor_lanes<16>(sum);
+    sum += dev::xor_lanes<32>(sum);
+    if (lane < 16) space.states[wave][lane] = float2{reference, sum};
 #pragma unroll
-    for (int t = 0; t < TILES; ++t) {
-        if (t >= live_tiles) continue;
-        __syncthreads();
-        float all_of = sum[t];
-        all_of += dev::xor_lanes<16>(all_of);
-        all_of += dev::xor_lanes<32>(all_of);
-        if (lane < 16) space.states[wave][lane] = float2{reference[t], all_of};
+    for (int o = 0; o < kOut; ++o)
+        *reinterpret_cast<float4_t*>(sums + (wave * 16 + column) * DIM + 16 * o + 4 * part) = acc[o];
+    __syncthreads();
+    for (int item = threadIdx.x; item < 16 * DIM / 4; item += kWaves * 64) {
+        const int local = item / (DIM / 4), channel = 4 * (item - local * (DIM / 4));
+        const int query_row = job.row0 + local, new_row = a.new_row(query_row);
+        const int64_t row = int64_t(job.first) + new_row;
+        if (query_row >= job.rows || row < 0 || row >= v.total_rows) continue;
+        float top = -kInf, all = 0.f;
 #pragma unroll
-        for (int o = 0; o < kOut; ++o)
-            *reinterpret_cast<float4_t*>(sums + (wave * 16 + column) * DIM + 16 * o + 4 * part) = acc[t][o];
-        __syncthreads();
-        for (int item = threadIdx.x; item < 16 * DIM / 4; item += kWaves * 64) {
-            const int local = item / (DIM / 4), channel = 4 * (item - local * (DIM / 4));
-            const int query_row = job.row0 + 16 * t + local, new_row = a.new_row(query_row);
-            const int64_t row = int64_t(job.first) + new_row;
-            if (query_row >= job.rows || row < 0 || row >= v.total_rows) continue;
-            float top = -kInf, all = 0.f;
+        for (int w = 0; w < kWaves; ++w) top = fmaxf(top, space.states[w][local].x);
+        float4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) top = fmaxf(top, space.states[w][local].x);
-            float4_t o = {0.f, 0.f, 0.f, 0.f};
+        for (int w = 0; w < kWaves; ++w) {
+            const float2 state = space.states[w][local];
+            const float shrink = state.x == top ? 1.f : exp2_fast(state.x - top);
+            all = __builtin_fmaf(state.y, shrink, all);
+            const float4_t y = *reinterpret_cast<const float4_t*>(sums + (w * 16 + local) * DIM + channel);
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
-                const float2 state = space.states[w][local];
-                const float shrink = state.x == top ? 1.f : exp2_fast(state.x - top);
-                all = __builtin_fmaf(state.y, shrink, all);
-                const float4_t x = *reinterpret_cast<const float4_t*>(sums + (w * 16 + local) * DIM + channel);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(x[e], shrink, o[e]);
-            }
-            const int64_t to = a.place(v, job.slot, int(row), job.head * a.group + query_row - new_row * a.group);
-            *reinterpret_cast<float4_t*>(a.sums + to * DIM + channel) = o;
-            if (channel == 0) a.states[to] = float2{top, all};
+            for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(y[e], shrink, o[e]);
         }
+        const int64_t to = a.place(v, job.slot, int(row), job.head * a.group + query_row - new_row * a.group);
+        *reinterpret_cast<float4_t*>(a.sums + to * DIM + channel) = o;
+        if (channel == 0) a.states[to] = float2{top, all};
     }
 }
 
@@ -518,8 +492,6 @@ __device__ __forceinline__ void shared_attend_wide(const PagedView& v, const Sha
     constexpr int kChunks = DIM * kSize / 16;     // threads of a stored row, 16 bytes each
     constexpr int kAtOnce = kWaves * 64 / kChunks, kLoads = kPositions / kAtOnce;  // rows of a load; loads
     constexpr int kWords = TYPE == kPagedE4M3 ? 2 : 1;
-    constexpr float kHead = TYPE == kPagedF16 ? 6.f : 0.f;  // FP16 weights are kept up to 2^14, far from subnormals
-    constexpr float kGrow = 8.f;                  // a reference is moved once a score passes it by 2^8
     constexpr std::integral_constant<int, TYPE> kType{};
     constexpr std::integral_constant<int, kKeyType> kKeys{};
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -555,7 +527,6 @@ __device__ __forceinline__ void shared_attend_wide(const PagedView& v, const Sha
     int base = job.from, buffer = 0;
     find(base);
 
-    // Queries: row r of the job is head r % group of new row r / group.
     // A wave's tiles are four apart, so that fewer than 4 * TILES of them are shared out evenly.
     const int first_row = job.row0 + 16 * wave;
     const int live_tiles = first_row < job.rows ? min(TILES, (job.rows - first_row + 63) / 64) : 0;
@@ -567,57 +538,19 @@ __device__ __forceinline__ void shared_attend_wide(const PagedView& v, const Sha
         reference[t] = -kInf, sum[t] = 0.f;
 #pragma unroll
         for (int o = 0; o < kOut; ++o) acc[t][o] = float4_t{0.f, 0.f, 0.f, 0.f};
-        if (t >= live_tiles) continue;
+        float x[kSteps][8];
+        if (t < live_tiles) {
+            bool live;
+            const float* const from = query_at<DIM>(v, a, job, first_row + 64 * t + column, live);
+            load_query<DIM, 1>(from, live, part, x);
+        }
+        if (t == 0) {  // in one flight with the first queries
+            load(base);
+            if (base + kPositions < end) find(base + kPositions);
+        }
+        if (t < live_tiles) to_score[t] = split_query<kKeyType, DIM>(x, a.scale, query[t]);
         __builtin_amdgcn_sched_barrier(0);  // a tile's queries at a time, for the registers
-        const int query_row = first_row + 64 * t + column, new_row = a.new_row(query_row);
-        const bool live = query_row < job.rows;
-        const float* const from =
-            a.queries + (live ? int64_t(job.first + new_row) * a.query_stride +
-                                    (job.head * a.group + query_row - new_row * a.group) * DIM
-                              : 0);
-        float x[kSteps][8], top = 0.f;
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-            const float4_a4 lo = *reinterpret_cast<const float4_a4*>(from + 32 * k + 8 * part);
-            const float4_a4 hi = *reinterpret_cast<const float4_a4*>(from + 32 * k + 8 * part + 4);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[k][e] = live ? lo[e] : 0.f, x[k][4 + e] = live ? hi[e] : 0.f;
-        }
-        // Above 0, so that minus infinity stays that: a scale's sign goes into the queries.
-        to_score[t] = fmaxf(__builtin_fabsf(a.scale), 1e-37f);
-        const float sign = a.scale == 0.f ? 0.f : __builtin_copysignf(1.f, a.scale);
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[k][e] *= sign;
-        if constexpr (kKeyType == kPagedF16) {
-            // An exact power of two brings a row's largest query to [2^14, 2^15), so that neither term leaves
-            // FP16's range; non-finite ones stay so.
-#pragma unroll
-            for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) top = fmaxf(top, __builtin_fabsf(x[k][e]));
-            top = fmaxf(top, dev::xor_lanes<16>(top));
-            top = fmaxf(top, dev::xor_lanes<32>(top));
-            const int up = 14 - max(int(__builtin_bit_cast(unsigned, top) >> 23) - 127, -100);
-#pragma unroll
-            for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[k][e] *= pow2(up);
-            to_score[t] = fmaxf(to_score[t] * pow2(-up), 0x1p-149f);
-        }
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                unsigned words[kTerms];
-                Terms<kKeyType, false>::split(x[k][2 * e], x[k][2 * e + 1], false, words);
-#pragma unroll
-                for (int p = 0; p < kTerms; ++p) query[t][k][p][e] = words[p];
-            }
     }
-    load(base);
-    if (base + kPositions < end) find(base + kPositions);
 
     // The loop has no branches around a tile's products, which would wait for every piece of LDS by itself.
     auto go = [&](auto live) {
@@ -696,50 +629,25 @@ __device__ __forceinline__ void shared_attend_wide(const PagedView& v, const Sha
                 for (int t = 0; t < LIVE; ++t) {
                     if (!whole)
 #pragma unroll
-                        for (int u = 0; u < 2; ++u)
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) s[t][u][r] = hidden >> (4 * u + r) & 1 ? -kInf : s[t][u][r];
-                    float high, factor[2][4];
+                        for (int i = 0; i < 8; ++i)
+                            if (hidden >> i & 1) s[t][i / 4][i % 4] = -kInf;
+                    float weights[2][4], high = -kInf;
                     if constexpr (kScaled) {
-                        high = -kInf;
+                        float factor[2][4];
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             factor[i / 4][i % 4] = fmaxf(to_score[t] * powers[i / 4][i % 4], 0x1p-149f);
                             high = fmaxf(high, s[t][i / 4][i % 4] * factor[i / 4][i % 4]);
                         }
+                        soften<TYPE>(s[t], [&](int u, int r) { return factor[u][r]; }, high, reference[t], sum[t], acc[t],
+                                     weights);
                     } else {
-                        high = s[t][0][0];
 #pragma unroll
-                        for (int i = 1; i < 8; ++i) high = fmaxf(high, s[t][i / 4][i % 4]);
-                        high *= to_score[t];
+                        for (int i = 0; i < 8; ++i) high = fmaxf(high, s[t][i / 4][i % 4]);
+                        soften<TYPE>(s[t], [&](int, int) { return to_score[t]; }, high * to_score[t], reference[t], sum[t],
+                                     acc[t], weights);
                     }
-                    if (__any(high > reference[t] + (kHead + kGrow))) {
-                        high = fmaxf(high, dev::xor_lanes<16>(high));
-                        high = fmaxf(high, dev::xor_lanes<32>(high));
-                        const float moved = fmaxf(reference[t], high - kHead);
-                        const float shrink = reference[t] == moved ? 1.f : exp2_fast(reference[t] - moved);
-                        reference[t] = moved;
-                        sum[t] *= shrink;
-#pragma unroll
-                        for (int o = 0; o < kOut; ++o) acc[t][o] *= shrink;
-                    }
-                    const float from = reference[t] == -kInf ? 0.f : reference[t];
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        float p[4];
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            p[r] = exp2_fast(__builtin_fmaf(s[t][u][r], kScaled ? factor[u][r] : to_score[t], -from));
-                            sum[t] += p[r];
-                        }
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            unsigned words[kProducts];
-                            Terms<TYPE, false>::split(p[2 * e], p[2 * e + 1], false, words);
-#pragma unroll
-                            for (int q = 0; q < kProducts; ++q) weight[t][q][2 * u + e] = words[q];
-                        }
-                    }
+                    split_weights<TYPE>(weights, weight[t]);
                 }
 #pragma unroll
                 for (int o = 0; o < kOut; ++o) {
@@ -848,7 +756,7 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void shared_attent
         if constexpr (WIDE)
             shared_attend_wide<TYPE, DIM, WIDE>(v, a, job, space.wide);
         else
-            shared_attend<TYPE, DIM, 1, false>(v, a, job, space.narrow);
+            shared_attend<TYPE, DIM, false>(v, a, job, space.narrow);
     } else {
         if (block >= a.rest_jobs) return;
         // First parts first: of ragged lengths, the last parts are those that some sequences do not have.
@@ -869,7 +777,7 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void shared_attent
         job.to = index == a.rest_parts - 1 ? length : min(length, job.from + a.rest_part);
         job.sees = length - n + 1;
         job.slot = a.parts + index;
-        shared_attend<TYPE, DIM, 1, true>(v, a, job, space.narrow);
+        shared_attend<TYPE, DIM, true>(v, a, job, space.narrow);
     }
 }
 
