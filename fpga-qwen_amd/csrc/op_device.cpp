@@ -60,7 +60,7 @@ void check_arrays(const OpArray* arrays, int count) {
         if (!a.written || !a.at) continue;
         for (int j = 0; j < count; ++j) {
             const OpArray& b = arrays[j];
-            if (j == i || !b.at || (a.at == b.at && (a.in_place_of == b.at || b.in_place_of == a.at))) continue;
+            if (j == i || !b.at || (a.at == b.at && a.in_place_of == b.at && !b.written)) continue;
             if (!apart(a.at, a.bytes, b.at, b.bytes))
                 throw std::runtime_error(std::string(a.name) + " overlaps " + b.name);
         }

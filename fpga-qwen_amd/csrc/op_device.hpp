@@ -23,7 +23,7 @@ private:
 };
 
 // An argument of a call. Arrays that are written overlap no others, but for
-// the one whose place they may take, from its start.
+// the one that is only read whose place they may take, from its start.
 struct OpArray {
     const char* name;
     const void* at;

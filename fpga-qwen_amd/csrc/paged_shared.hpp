@@ -753,7 +753,7 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void shared_attent
             }
             before = __builtin_amdgcn_readlane(upto, 63);
         }
-        if (g < 0) return;
+        if (g < 0 || index < 0 || tiles <= 0 || most <= 0) return;  // (the last three only where offsets fall)
         const int of_eight = index / (8 * tiles), within = index - of_eight * 8 * tiles;
         const int pair = of_eight * 8 + (within & 7);
         // Tiles of equal size, of whole 16 rows.

@@ -143,12 +143,13 @@ __global__ __launch_bounds__(THREADS) void reserve_kernel(ReserveView v, bool ma
     __shared__ int upto[THREADS * EACH], start[THREADS * EACH];
     const int tid = threadIdx.x, n = v.sequences;
     const int free_count = min(max(v.free_count[0], 0), v.pages);
-    int length[EACH], change[EACH], held[EACH], needed[EACH], keep[EACH];
+    int length[EACH], seen[EACH], change[EACH], held[EACH], needed[EACH], keep[EACH];
     unsigned need[EACH], surplus[EACH], sums[2] = {0, 0}, before[2], all[2];
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {  // all loads first; sequences that are not there count as empty ones
         const int s = min(EACH * tid + i, n - 1);
         length[i] = v.lengths[s];
+        seen[i] = v.seen ? v.seen[s] : 0;
         held[i] = v.held[s];
         change[i] = v.changes[s];
         keep[i] = v.shared ? v.shared[s] : 0;
@@ -163,7 +164,7 @@ __global__ __launch_bounds__(THREADS) void reserve_kernel(ReserveView v, bool ma
         const PageSlot end = page_slot(unsigned(length[i] + change[i]), v.page_size, v.magic);
         needed[i] = end.page + (end.slot > 0);
         keep[i] = min(held[i], max(needed[i], keep[i]));
-        need[i] = max(0, needed[i] - held[i]);
+        need[i] = change[i] > 0 ? max(0, needed[i] - held[i]) : 0;
         surplus[i] = held[i] - keep[i];
         sums[0] = limited(sums[0], surplus[i]);
         sums[1] = limited(sums[1], need[i]);
@@ -217,7 +218,7 @@ __global__ __launch_bounds__(THREADS) void reserve_kernel(ReserveView v, bool ma
         if (s < n) {
             const int delta = change[i] > 0 && !granted ? 0 : change[i];
             v.new_lengths[s] = length[i] + delta;
-            if (v.new_seen) v.new_seen[s] = v.seen[s] + delta;
+            if (v.new_seen) v.new_seen[s] = seen[i] + delta;
             v.new_held[s] = granted && need[i] ? needed[i] : keep[i];
         }
     }

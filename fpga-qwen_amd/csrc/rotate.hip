@@ -2,9 +2,9 @@
 #include "rotate.hpp"
 
 #include <cmath>
-#include <cstdlib>
 #include <string>
 #include <type_traits>
+#include <utility>
 
 #include "half_split.hpp"
 #include "op_device.hpp"
@@ -58,7 +58,6 @@ struct RotateArgs {
     const int32_t* positions;
     int rows, group;       // all, and of a workgroup
     int pairs, turned;     // of a head; those that turn are the first
-    int dims;
     int lanes;             // of a head, a power of two
     float magnitude, epsilon, over_dim;
 };
@@ -341,7 +340,6 @@ void launch_rotate(const qwen_gpu_rotary& rotary, const qwen_gpu_rotary_heads& q
     a.group = rows >= 4096 ? kMaxRows : 1;
     a.pairs = rotary.head_dim / 2;
     a.turned = rotary.dims / 2;
-    a.dims = rotary.dims;
     a.magnitude = rotary.magnitude;
     a.epsilon = rotary.epsilon;
     a.over_dim = 1.f / rotary.head_dim;

@@ -456,13 +456,15 @@ typedef struct qwen_gpu_paged_growth {
  * takes them from the stack's end, until one needs more than there are, and
  * from there on only those that need none are granted; and no sequence
  * whose rows, with those granted before, pass total_rows, nor any with new rows behind
- * it. One that is not granted keeps its length and has no rows in `offsets`.
+ * it. One that is not granted keeps its length and has no rows in `offsets`;
+ * one that has fewer pages than the rows it has need takes those too, when it
+ * grows.
  * A wish that the table has no entries for (length + change above
  * table_stride * page_size) counts as a change of 0; a change never takes
  * back more than there is. The lengths, seen, held and changes of one call
  * are read before the results are written, so new_lengths may be lengths,
- * new_seen seen, new_held held and new_free_count free_count; otherwise the
- * arrays must not overlap. What the arrays hold is bounded: held into 0 ..
+ * new_seen seen, new_held held and new_free_count free_count; otherwise
+ * nothing that is written may overlap another array. What the arrays hold is bounded: held into 0 ..
  * table_stride, lengths into 0 .. table_stride * page_size (at most 2^30), free_count into 0
  * .. pages; pages given back beyond `pages` free ones are dropped. Tables and
  * slots of pages outside 0 .. pages - 1 (which only a wrong stack can hold)

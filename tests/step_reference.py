@@ -74,7 +74,8 @@ def reserve(table, held, free, lengths, changes, page_size, pages, room, seen=No
     wished_rows = 0  # of the sequences that have pages, whether there is room for them or not
     left = len(free)
     for s in range(n):
-        change, need = wished[s], max(0, -(-(lengths[s] + wished[s]) // page_size) - before[s])
+        change = wished[s]
+        need = max(0, -(-(lengths[s] + change) // page_size) - before[s]) if change > 0 else 0
         short = short or need > left
         if change > 0 and need and short:
             change = 0

@@ -287,6 +287,40 @@ def test_reserve_bounds_what_the_device_holds(qpkg):
         assert on['stack'].to_array(np.int32, 5)[4] == -55
 
 
+@pytest.mark.parametrize('n', [2, 30, 1500])
+def test_reserve_with_fewer_pages_than_rows(qpkg, n):
+    """A sequence that has fewer pages than its rows need takes them all when it grows, and none before."""
+    rng = np.random.default_rng(n)
+    given = state(rng, n, 4, 30, 3 * n)
+    given['held'] = np.maximum(0, given['held'] - rng.integers(0, 3, n))
+    given['changes'] = rng.integers(-2, 4, n)
+    expect_reserved(qpkg.paged_reserve(**given, room=4 * n), ref.reserve(**given, room=4 * n))
+
+
+def test_reserve_with_one_array_as_lengths_and_seen(qpkg):
+    """Lengths that are the text's positions as well, and their results in the place of one of them."""
+    rng, q = np.random.default_rng(5), qpkg
+    given = state(rng, 30, 4, 30, 60)
+    changes = rng.integers(-6, 6, 30)
+    want = ref.reserve(**given, changes=changes, room=0)
+    stack = np.full(given['pages'], -1, np.int32)
+    stack[:len(given['free'])] = given['free']
+    for in_place in ('lengths', 'seen'):
+        on = {name: q.DeviceBuffer.from_array(np.asarray(x, np.int32)) for name, x in dict(
+            table=given['table'], held=given['held'], lengths=given['lengths'], changes=changes, stack=stack,
+            count=[len(given['free'])], other=[0] * 30, offsets=[0] * 31).items()}
+        at = {name: buffer.ptr for name, buffer in on.items()}
+        pool = q.PagedPool(at['table'], at['stack'], at['held'], at['count'], None, given['pages'], 4, 30,
+                           np.asarray(given['table']).shape[1])
+        results = (at['lengths'], at['other']) if in_place == 'lengths' else (at['other'], at['lengths'])
+        growth = q.PagedGrowth(at['lengths'], at['lengths'], at['changes'], *results, at['held'], at['count'], at['offsets'],
+                               None, None, None, 0)
+        ok(q, q.load_library().qwen_gpu_op_paged_reserve(pool, growth, None))
+        q.synchronize()
+        for name in ('lengths', 'other'):
+            assert np.array_equal(on[name].to_array(np.int32, 30), want['lengths']), (in_place, name)
+
+
 def test_reserve_results_apart_from_what_is_given(qpkg):
     """Results in arrays of their own: what was given stays, and the call can be made again."""
     rng, q = np.random.default_rng(4), qpkg

@@ -185,6 +185,15 @@ def test_growths_in_place_are_accepted(qpkg):
     refused(qpkg, 'Not device memory: table', qpkg.load_library().qwen_gpu_op_paged_reserve(pool(qpkg), in_place, None))
 
 
+@pytest.mark.parametrize('message,fields', [
+    ('new_lengths overlaps new_seen', dict(seen=AT + 4 * FAR, new_seen=AT + 4 * FAR, new_lengths=AT + 4 * FAR)),
+    ('new_lengths overlaps new_held', dict(new_lengths=AT + 4 * FAR, new_held=AT + 4 * FAR)),
+    ('new_lengths overlaps held', dict(new_lengths=AT + 2 * FAR))])
+def test_results_share_no_place(qpkg, message, fields):
+    """Two results in the place of one array, also where that array is given twice."""
+    refused(qpkg, message, qpkg.load_library().qwen_gpu_op_paged_reserve(pool(qpkg), growth(qpkg, **fields), None))
+
+
 def test_reserve_oracle():
     """Worked by hand: pages of 4; sequence 0 grows into its page, 1 ends, 2 takes three pages, 3 wants more than are left,
     4 needs none, 5 has no entries."""
@@ -194,6 +203,11 @@ def test_reserve_oracle():
     assert got['table'][2].tolist() == [2, 1, 10, -1] and got['free'].tolist() == [9]
     assert got['offsets'].tolist() == [0, 1, 1, 11, 11, 13, 13]
     assert got['slots'][:13].tolist() == [3, 8, 9, 10, 11, 4, 5, 6, 7, 40, 41, 17, 18]
+    # Pages that a sequence lacks for the rows that it has are taken when it grows, not before.
+    got = ref.reserve([[-1, -1], [7, -1]], [0, 1], [5, 6], [6, 4], [0, 1], 4, 8, 4)
+    assert got['held'].tolist() == [0, 2] and got['table'].tolist() == [[-1, -1], [7, 6]] and got['free'].tolist() == [5]
+    got = ref.reserve([[-1, -1], [7, -1]], [0, 1], [5, 6], [6, 4], [1, 1], 4, 8, 4)
+    assert got['held'].tolist() == [2, 1] and got['table'].tolist() == [[6, 5], [7, -1]] and got['free'].tolist() == []
 
 
 # ---- drafts ----
