@@ -85,7 +85,6 @@ void launch_paged_attention_shared(const qwen_gpu_paged_cache& cache, const qwen
                        int(plan.rest_part),
                        int(plan.jobs),
                        int(plan.rest_jobs),
-                       plan.part < 2 * plan.rest_part,
                        plan.compact,
                        reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.state_bytes),
                        static_cast<float2*>(workspace)};

@@ -23,7 +23,6 @@ struct SharedArgs {
     int parts, rest_parts;      // of a prefix, of what is behind it, at most
     int part, rest_part;        // positions of each
     int jobs, rest_jobs;        // workgroups of the prefixes (a multiple of 8), of what is behind them
-    bool in_turn;               // workgroups of both kinds
     bool compact;               // behind the prefixes only those with work come first
     float* sums;                // [parts + rest_parts][total_rows][query_heads][DIM]
     float2* states;             // [parts + rest_parts][total_rows][query_heads]: reference, sum
@@ -481,7 +480,9 @@ __device__ __forceinline__ void widen_f16(uint4_t raw, uint4_t (&out)[2]) {
 }
 
 // LDS of a workgroup whose waves share its positions: two steps' keys and
-// values, 16-bit whatever the cache's type, and which of them exist.
+// values, 16-bit whatever the cache's type, and which of them exist. (64
+// positions a step instead of 32 took 46 us, not 42, for 8192 F16 positions,
+// and 132, not 120, for 4 times 24 BF16 sequences.)
 template <int DIM>
 struct WideSpace {
     static constexpr int kPositions = DIM == 64 ? 64 : 32, kPitch = DIM * 2 + 32;
@@ -497,6 +498,15 @@ struct WideSpace {
 // into LDS together, a step ahead, widened to 16 bits once. A wave's part of the loads
 // takes a quarter of the registers, so that two workgroups fit a CU and one's
 // products run beside the other's exponentials.
+//
+// A prefix is read once from memory, but multiplied with every query row, in
+// two or three terms: 65000 E4M3 positions by 128 rows are 38 us of products
+// at the rate of a large matrix product (a score's two and a weight's three
+// terms), 11 of its bytes. The kernel takes 105, as LDS, exponentials and
+// products wait for each other at two waves a SIMD; tiles that every wave
+// reads for itself, without LDS, took 1020. Of 64 rows (TILES 1) 8192 positions
+// and what 64 users have behind them take 48 us, of 128 40; heads of 256 have
+// registers for 64.
 template <int TYPE, int DIM, int TILES>
 __device__ __forceinline__ void shared_attend_wide(const PagedView& v, const SharedArgs& a, const SharedJob& job,
                                                    WideSpace<DIM>& space) {
@@ -718,18 +728,8 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void shared_attent
         WideSpace<DIM> wide;
     } space;
     const SharedGroups groups(v, a);
-    // Both kinds in turn, 8 workgroups at a time (one an XCD) and 256 of them the other way round, so that a CU gets
-    // one of each: a prefix's products run beside the loads of what is behind it.
     int block = blockIdx.x;
-    bool of_prefix;
-    const int both = a.in_turn ? 2 * min(a.jobs, (a.rest_jobs + 7) / 8 * 8) : 0;
-    if (block < both) {
-        of_prefix = !((block / 8 + block / 256) & 1);
-        block = block / 16 * 8 + block % 8;
-    } else {
-        of_prefix = block - both / 2 < a.jobs;
-        block -= of_prefix ? both / 2 : both ? both / 2 : a.jobs;
-    }
+    const bool of_prefix = block < a.jobs;
     SharedJob job;
     if (of_prefix) {
         // Each group has its tiles for each head and part of its prefix. Those of one head and part are 8 workgroups
@@ -777,6 +777,7 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void shared_attent
         else
             shared_attend<TYPE, DIM, false>(v, a, job, space.narrow);
     } else {
+        block -= a.jobs;
         if (block >= a.rest_jobs) return;
         int at = block, parts = 0, index = 0, of_head = 0;
         if (a.compact) {
@@ -920,31 +921,41 @@ struct SharedPlan {
                int query_heads) {
         const int64_t group = query_heads / c.kv_heads, rows = group * b.total_rows;
         const int64_t of_group = rows / p.groups;  // a group has as many of them if all have the same
-        wide = of_group <= 16 ? 0 : of_group <= 64 || c.head_dim == 256 ? 1 : 2;
+        // (16 query rows behind 8192 positions: 20.3 us, or 21 as a wide tile; 24 of them 26.4, or 21.5; E4M3 17.7 or 20.5,
+        // and 23.5 or 21.5.)
+        wide = of_group <= 16 ? 0 : c.head_dim == 256 ? 1 : 2;
         const int64_t tile = rows_of_wide(wide);
         tiles = (rows + p.groups * (tile - 1)) / tile;  // however the groups share them
         rest_tiles = (group * b.rows + 15) / 16;
-        // Parts for as many workgroups as the GPU holds at once, of 256 positions or more, and of 768 at most behind
-        // the prefixes, where ragged lengths would keep a few workgroups long (96 sequences of up to 1500 positions
-        // 84 us, 79 with it, 83 with 384).
+        // Parts for as many workgroups as the GPU holds at once, of 256 positions or more (8192 positions and 64 users 40 us;
+        // of 128 51, of 512 44), and of 640 at most behind the prefixes, where ragged lengths would keep a few workgroups
+        // long (64 sequences of up to 3000 90 us, with 1024 98, without 122; of 4 times 24 of up to 1500 100, 99 and 114).
         const int64_t held = c.head_dim == 256 ? 256 : 512;
-        auto split = [&](int64_t units, int64_t positions, int64_t longest, int64_t& count, int64_t& size) {
+        auto split = [&](int64_t units, int64_t places, int64_t positions, int64_t longest, int64_t& count, int64_t& size) {
             const int64_t most = std::max<int64_t>(1, (positions + 255) / 256);
             const int64_t least = std::max<int64_t>(1, (positions + longest - 1) / longest);
-            count = std::clamp<int64_t>(held / std::max<int64_t>(1, units), least, most);
+            count = std::clamp<int64_t>(places / std::max<int64_t>(1, units), least, most);
             size = (positions + count - 1) / count;
             size = std::max<int64_t>(kBlock, (size + kBlock - 1) / kBlock * kBlock);
             count = std::max<int64_t>(1, (positions + size - 1) / size);
         };
-        split(std::max<int64_t>(1, (rows + tile - 1) / tile) * c.kv_heads, p.max_length, kPagedMaxLength, parts, part);
         // (A sequence has a row at least where it has work.)
-        const int64_t working = std::min<int64_t>(b.sequences, b.total_rows);
-        split(rest_tiles * working * c.kv_heads, p.max_rest, 768, rest_parts, rest_part);
+        const int64_t working = std::min<int64_t>(b.sequences, b.total_rows), units = rest_tiles * working * c.kv_heads;
+        split(units, held, p.max_rest, 640, rest_parts, rest_part);
+        // The prefixes have as many of the places as their share of the work, and a third more, so that none of their
+        // workgroups is the last one: 85 ns a position of theirs, 65 (E4M3 45) behind them, where half of the most are
+        // taken for ragged ones' mean. (All places, as if there were nothing behind them: 4 times 24 sequences 120 us,
+        // not 98, as each workgroup of theirs has its start and its sums.)
+        const int64_t of_prefixes = std::max<int64_t>(1, tiles) * c.kv_heads;
+        const int64_t ahead = of_prefixes * p.max_length * (c.type == kPagedE4M3 ? 17 : 12), behind = units * p.max_rest / 2 * 9;
+        const int64_t places = held * 4 / 3 * ahead / (ahead + behind + 1) + of_prefixes - 1;
+        split(of_prefixes, std::min(held, places), p.max_length, kPagedMaxLength, parts, part);
         jobs = p.max_length ? (parts * c.kv_heads + 7) / 8 * 8 * tiles : 0;
         rest_jobs = rest_parts * rest_tiles * b.sequences * c.kv_heads;
-        // Where all workgroups start at once, those without work cost nothing.
+        // Where all workgroups start at once, those without work cost nothing; where they do not, 4 times 24 ragged
+        // sequences take 127 us with them, 116 without.
         compact = b.sequences <= 256 && p.groups < 64 && rest_jobs > held;
-        if (compact) rest_jobs = rest_parts * rest_tiles * working * c.kv_heads;
+        if (compact) rest_jobs = rest_parts * units;
         slots = parts + rest_parts;
         state_bytes = (size_t(slots) * b.total_rows * query_heads * 8 + 15) / 16 * 16;
         sum_bytes = size_t(slots) * b.total_rows * query_heads * c.head_dim * 4;
@@ -963,8 +974,7 @@ void shared_launch(int dim, const PagedView& v, const SharedArgs& a, const Share
     auto run = [&](auto of_dim) {
         constexpr int kDim = decltype(of_dim)::value;
         if (plan.wide == 0) return shared_run<TYPE, kDim, 0>(v, a, plan, stream);
-        if (plan.wide == 1) return shared_run<TYPE, kDim, 1>(v, a, plan, stream);
-        if constexpr (kDim < 256) shared_run<TYPE, kDim, 2>(v, a, plan, stream);
+        shared_run<TYPE, kDim, kDim == 256 ? 1 : 2>(v, a, plan, stream);
     };
     if (dim == 64) return run(std::integral_constant<int, 64>{});
     if (dim == 128) return run(std::integral_constant<int, 128>{});

@@ -16,7 +16,9 @@ namespace {
 
 constexpr int kMost = 4096;  // sequences of a call
 constexpr int kMaxRow = 1 << 30;
-constexpr int kFewRows = 1024;  // up to which they are mapped without a launch of their own
+// Rows up to which they are mapped without a launch of their own: 64 sequences' 480 take 4.7 us, 5.7 with one, 960 of them
+// 6.2 and 6.0.
+constexpr int kFewRows = 768;
 
 struct ReserveView {
     int32_t* table;

@@ -42,7 +42,7 @@ void rotary_frequencies(int scaling, int dims, double base, double factor, doubl
 
 namespace {
 
-constexpr int kThreads = 256, kMaxRows = 4, kMaxDim = 512;
+constexpr int kThreads = 256, kMaxDim = 512;
 
 struct Side {
     const char* rows;
@@ -56,7 +56,6 @@ struct RotateArgs {
     Side sides[2];
     const double* frequencies;
     const int32_t* positions;
-    int rows, group;       // all, and of a workgroup
     int pairs, turned;     // of a head; those that turn are the first
     int lanes;             // of a head, a power of two
     float magnitude, epsilon, over_dim;
@@ -103,21 +102,29 @@ __device__ __forceinline__ void store(T* to, const float* from) {
     }
 }
 
-// A workgroup has up to 4 rows. Its threads first find the rows' angles, one
-// pair each: position * frequency in turns and FP64, less the nearest quarter,
+// A workgroup has a row. Its threads first find the row's angles, one pair
+// each: position * frequency in turns and FP64, less the nearest quarter,
 // which leaves an eighth of a turn at most, so that rounding it to FP32 costs
 // half a step of sine and cosine. Then a head at a time goes through `lanes`
 // lanes of a wave, each with V pairs (K times V where there are more): both
 // channels of a pair are in one lane, so the rotation moves nothing between
 // lanes and the norm is one sum over them. Channels behind the turned ones
 // count as pairs that stay.
+//
+// Memory bounds it: 8191 rows of 40 BF16 heads of 128 (168 MB read and written)
+// take 37.8 us, 4.4 TB/s, where a copy of 1 GiB reaches 5.16; 512 rows of 24
+// FP32 heads 5.6, 8 rows 4.3, a launch's latency with the angles' FP64 in it.
+// Four rows a workgroup, for fewer of them, took 9.7 and 8.6 us for those, two
+// 6.4 and 5.4, and no less for many (16384: 70 us with one row, 70 with two, 74
+// with four).
 template <typename T, int V, int K, bool INTERLEAVED>
 __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs a) {
-    __shared__ float2 turns[kMaxRows * kMaxDim / 2];
-    const int row0 = blockIdx.x * a.group, rows = min(a.group, a.rows - row0);
-    for (int i = threadIdx.x; i < rows * a.turned; i += kThreads) {
-        const int r = i / a.turned, pair = i - r * a.turned;
-        const int position = a.positions[row0 + r];
+    __shared__ float2 turns[kMaxDim / 2];
+    static_assert(kMaxDim / 2 <= kThreads, "a pair each");
+    const int64_t row = blockIdx.x;
+    const int position = a.positions[row];
+    if (position < 0) return;
+    if (const int pair = threadIdx.x; pair < a.turned) {
         double turn = position * (a.frequencies[pair] * 0.159154943091895335769);  // 1 / (2 pi)
         const double quarters = rint(4 * turn);
         turn -= quarters / 4;
@@ -130,18 +137,15 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs a) {
             s = x;
         }
         if (quarter & 2) c = -c, s = -s;
-        turns[i] = float2{c * a.magnitude, s * a.magnitude};
+        turns[pair] = float2{c * a.magnitude, s * a.magnitude};
     }
     __syncthreads();
     const int heads = a.sides[0].heads + a.sides[1].heads, slots = kThreads / a.lanes;
     const int lane = threadIdx.x & (a.lanes - 1);
-    for (int item = threadIdx.x / a.lanes; item < rows * heads; item += slots) {
-        const int r = item / heads, of_all = item - r * heads;
-        const bool second = of_all >= a.sides[0].heads;
+    for (int item = threadIdx.x / a.lanes; item < heads; item += slots) {
+        const bool second = item >= a.sides[0].heads;
         const Side& side = a.sides[second];
-        const int head = second ? of_all - a.sides[0].heads : of_all;
-        const int64_t row = row0 + r;
-        if (a.positions[row] < 0) continue;  // the same for all lanes of the head
+        const int head = second ? item - a.sides[0].heads : item;
         const T* const from = reinterpret_cast<const T*>(side.rows) + row * side.row_stride + head * side.head_stride;
         T* const to = reinterpret_cast<T*>(side.out) + row * side.out_row_stride + head * side.out_head_stride;
         float x[K][2 * V];
@@ -184,7 +188,7 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs a) {
             if (pair < a.turned) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const float2 t = turns[r * a.turned + pair + i];
+                    const float2 t = turns[pair + i];
                     const int one = INTERLEAVED ? 2 * i : i, two = INTERLEAVED ? 2 * i + 1 : V + i;
                     const float p = x[k][one], q = x[k][two];
                     x[k][one] = __builtin_fmaf(p, t.x, -(q * t.y));
@@ -198,27 +202,27 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs a) {
 }
 
 template <typename T, int V>
-void rotate_run(const RotateArgs& args, bool interleaved, hipStream_t stream) {
+void rotate_run(const RotateArgs& args, unsigned rows, bool interleaved, hipStream_t stream) {
     constexpr int K = V >= 4 ? 1 : 4 / V;  // 512 channels are 256 pairs
     RotateArgs a = args;
     a.lanes = 1;
     while (a.lanes < 64 && a.lanes * V < a.pairs) a.lanes *= 2;
-    const unsigned grid = unsigned((a.rows + a.group - 1) / a.group);
     if (interleaved)
-        rotate_kernel<T, V, K, true><<<grid, kThreads, 0, stream>>>(a);
+        rotate_kernel<T, V, K, true><<<rows, kThreads, 0, stream>>>(a);
     else
-        rotate_kernel<T, V, K, false><<<grid, kThreads, 0, stream>>>(a);
+        rotate_kernel<T, V, K, false><<<rows, kThreads, 0, stream>>>(a);
 }
 
-// 16 bytes a load, or fewer where the turned and the other pairs do not come in such groups.
+// 16 bytes a load, or fewer where the turned and the other pairs do not come in such groups (of the 8191 BF16 rows above:
+// 8 bytes 43 us, 4 68, 2 120).
 template <typename T>
-void rotate_of(const RotateArgs& a, bool interleaved, hipStream_t stream) {
+void rotate_of(const RotateArgs& a, unsigned rows, bool interleaved, hipStream_t stream) {
     auto fits = [&](int v) { return a.turned % v == 0 && a.pairs % v == 0; };
     if constexpr (sizeof(T) == 2)
-        if (fits(8)) return rotate_run<T, 8>(a, interleaved, stream);
-    if (fits(4)) return rotate_run<T, 4>(a, interleaved, stream);
-    if (fits(2)) return rotate_run<T, 2>(a, interleaved, stream);
-    rotate_run<T, 1>(a, interleaved, stream);
+        if (fits(8)) return rotate_run<T, 8>(a, rows, interleaved, stream);
+    if (fits(4)) return rotate_run<T, 4>(a, rows, interleaved, stream);
+    if (fits(2)) return rotate_run<T, 2>(a, rows, interleaved, stream);
+    rotate_run<T, 1>(a, rows, interleaved, stream);
 }
 
 // Where the heads of a side lie, in bytes: [outer][inner] pieces of `piece`.
@@ -336,8 +340,6 @@ void launch_rotate(const qwen_gpu_rotary& rotary, const qwen_gpu_rotary_heads& q
                           sides[i]->heads};
     a.frequencies = rotary.frequencies;
     a.positions = positions;
-    a.rows = rows;
-    a.group = rows >= 4096 ? kMaxRows : 1;
     a.pairs = rotary.head_dim / 2;
     a.turned = rotary.dims / 2;
     a.magnitude = rotary.magnitude;
@@ -345,11 +347,11 @@ void launch_rotate(const qwen_gpu_rotary& rotary, const qwen_gpu_rotary_heads& q
     a.over_dim = 1.f / rotary.head_dim;
     const bool interleaved = rotary.layout == QWEN_GPU_ROTARY_INTERLEAVED;
     if (rotary.type == QWEN_GPU_F32)
-        rotate_of<float>(a, interleaved, stream);
+        rotate_of<float>(a, unsigned(rows), interleaved, stream);
     else if (rotary.type == QWEN_GPU_F16)
-        rotate_of<_Float16>(a, interleaved, stream);
+        rotate_of<_Float16>(a, unsigned(rows), interleaved, stream);
     else
-        rotate_of<__bf16>(a, interleaved, stream);
+        rotate_of<__bf16>(a, unsigned(rows), interleaved, stream);
 }
 
 }  // namespace qwen_hip
