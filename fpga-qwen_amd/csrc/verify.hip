@@ -371,7 +371,7 @@ struct Drawn {
 };
 __device__ __forceinline__ Drawn drawn_from(const VerifyArgs& a, const Powers& powers, const Verdict& v, double heat) {
     const bool judged = v.accepted < v.drafted;
-    return {uniform(v.top), heat, judged ? 1. / v.z : 1., judged, judged && a.draft ? a.draft + v.row * a.draft_stride : nullptr, v.token,
+    return {uniform(v.top), heat, judged && a.draft ? 1. / v.z : 1., judged, judged && a.draft ? a.draft + v.row * a.draft_stride : nullptr, v.token,
             powers};
 }
 
@@ -398,8 +398,8 @@ __device__ __forceinline__ double sum_before(double x, double* waves, double& al
     return base + before;
 }
 
-// The lowest of the threads' numbers, or the highest of `others` where none is below `none`.
-__device__ __forceinline__ int lowest_or_last(int number, int none, int other, int* waves) {
+// The lowest of the threads' numbers, and the highest of their others.
+__device__ __forceinline__ int lowest(int number, int& other, int* waves) {
     number = wave_min(number);
     other = -wave_min(-other);
     if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = number, waves[kWaves + (threadIdx.x >> 6)] = other;
@@ -407,7 +407,7 @@ __device__ __forceinline__ int lowest_or_last(int number, int none, int other, i
     number = min(min(waves[0], waves[1]), min(waves[2], waves[3]));
     other = max(max(waves[4], waves[5]), max(waves[6], waves[7]));
     __syncthreads();
-    return number < none ? number : other;
+    return number;
 }
 
 // What a sequence's rows come to: the first row whose drafted token is not
@@ -460,9 +460,9 @@ __device__ __forceinline__ double posted(const double* p) {
 
 // Every workgroup of a sequence judges its rows (from sums, which takes no
 // longer than to wait for another's word) and adds the weights that the token
-// is drawn from up over its own chunks; the last one to do so draws: the
-// chunk in which the sum of the weights passes sample times the whole, then
-// the token in it. Sums of one range in two orders may differ in their last
+// is drawn from up over its own chunks, unless they are a row's own, whose
+// sums are there; the last one to do so draws: the chunk (or range) in which
+// the sum of the weights passes sample times the whole, then the token in it. Sums of one range in two orders may differ in their last
 // place, so that a border can lie between them: the last token with a weight
 // stands for what lies behind all. Latency bounds it: 12 us for a sequence of
 // two rows, 15 for eight of five, 21 for 64 of up to seven, a chain of loads
@@ -485,23 +485,37 @@ __global__ __launch_bounds__(kThreads, 4) void verify_draw_kernel(VerifyArgs a) 
     int token = draws || v.row < 0 || !(v.z > 0.) ? -1 : v.best;
     Drawn drawn = drawn_from(a, powers, v, heat);
     double* const rest = a.rest + int64_t(s) * a.chunks;
-    if (!draws && own) return;
+    // Without a q to subtract, the ranges' sums are those of the first kernel, but for the drafted token's range. (A token
+    // for each of 64 sequences 27 us, 41 without this; 64 sequences of up to seven BF16 rows, whose ranges have eight chunks, 48 us
+    // with it, 42 without.)
+    const bool known = !(drawn.judged && drawn.q) && a.chunks <= a.ranges * max(2, a.draw_chunks);
+    if ((!draws || known) && own) return;
     if (draws) {
-        double all = 0.;
-        // Up to 8 chunks' sums, the next one's tokens on their way; wave 0 posts them.
-        auto add_up = [&](int c0, int c1) {
+        // The weights of chunks, the next one's tokens on their way, until f says that it is enough.
+        auto walk = [&](int c0, int c1, bool together, auto f) {
             Drawn::Chunk<T> ahead;
-            drawn.load<T>(a, v.row, c0 * kChunk, false, ahead);
+            drawn.load<T>(a, v.row, c0 * kChunk, together, ahead);
             for (int c = c0; c < c1; ++c) {
                 const Drawn::Chunk<T> here = ahead;
-                if (c + 1 < c1) drawn.load<T>(a, v.row, (c + 1) * kChunk, false, ahead);
-                double w[kEach], sum = 0.;
-                drawn.weigh<T>(here, c * kChunk, false, w);
-#pragma unroll
-                for (int i = 0; i < kEach; ++i) sum += w[i];
-                sum = dev::wave_sum(sum);
-                if ((tid & 63) == 0) chunk_sums[c - c0][tid >> 6] = sum;
+                if (c + 1 < c1) drawn.load<T>(a, v.row, (c + 1) * kChunk, together, ahead);
+                double w[kEach];
+                drawn.weigh<T>(here, c * kChunk, together, w);
+                if (f(c, w)) break;
             }
+        };
+        auto sum_of = [](const double (&w)[kEach]) {
+            double sum = 0.;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) sum += w[i];
+            return sum;
+        };
+        // Up to 8 chunks' sums; wave 0 posts them.
+        auto add_up = [&](int c0, int c1) {
+            walk(c0, c1, false, [&](int c, const double (&w)[kEach]) {
+                const double sum = dev::wave_sum(sum_of(w));
+                if ((tid & 63) == 0) chunk_sums[c - c0][tid >> 6] = sum;
+                return false;
+            });
             __syncthreads();
             if (tid < c1 - c0) {
                 const double* const of = chunk_sums[tid];
@@ -510,55 +524,79 @@ __global__ __launch_bounds__(kThreads, 4) void verify_draw_kernel(VerifyArgs a) 
             if (tid < 64) posted_stores_done();
             __syncthreads();
         };
-        add_up(own * a.draw_chunks, min((own + 1) * a.draw_chunks, a.chunks));
-        if (tid == 0)
-            last_one = __hip_atomic_fetch_add(a.done + s, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == groups - 1;
-        __syncthreads();
-        if (!last_one) return;
-        const int each = (a.chunks + kThreads - 1) / kThreads, c0 = min(tid * each, a.chunks), c1 = min(c0 + each, a.chunks);
-        double before = 0., only = 0.;  // only: of up to 256 chunks, the thread's
+        // Pieces of the row whose sums are at hand: ranges, or chunks.
+        const int pieces = known ? a.ranges : a.chunks;
+        auto first_chunk = [&](int piece) { return known ? int(int64_t(a.chunks) * piece / a.ranges) : piece; };
+        double all = 0., without = 0.;
+        int spared = -1;  // the drafted token's range, whose sum is `without`
+        if (known && drawn.judged && v.token >= 0 && v.token < a.vocabulary) {
+            spared = int((int64_t(v.token / kChunk + 1) * a.ranges - 1) / a.chunks);
+            double sum = 0.;
+            walk(first_chunk(spared), first_chunk(spared + 1), false, [&](int, const double (&w)[kEach]) {
+                sum += sum_of(w);
+                return false;
+            });
+            (void)sum_before(sum, waves, without);
+        } else if (!known) {
+            add_up(own * a.draw_chunks, min((own + 1) * a.draw_chunks, a.chunks));
+            if (tid == 0)
+                last_one = __hip_atomic_fetch_add(a.done + s, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == groups - 1;
+            __syncthreads();
+            if (!last_one) return;
+        }
+        auto piece_sum = [&](int i) {
+            if (!known) return posted(rest + i);
+            const Part part = a.parts[int64_t(v.row) * a.ranges + i];
+            return i == spared ? without : part.sum * (part.top == v.top ? 1. : powers.weight(part.top, v.top, heat));
+        };
+        const int each = (pieces + kThreads - 1) / kThreads, i0 = min(tid * each, pieces), i1 = min(i0 + each, pieces);
+        double before = 0., only = 0.;  // only: of up to 256 pieces, the thread's
         for (;;) {
             double sum = 0.;
-            for (int c = c0; c < c1; ++c) sum += only = posted(rest + c);
+            for (int i = i0; i < i1; ++i) sum += only = piece_sum(i);
             before = sum_before(sum, waves, all);
             if (!drawn.judged || all > 0.) break;
             drawn.judged = false;  // q is p or more throughout
             drawn.by = 1.;
-            for (int c = 0; c < a.chunks; c += kMostChunks) add_up(c, min(c + kMostChunks, a.chunks));
+            spared = -1;
+            if (!known)
+                for (int c = 0; c < a.chunks; c += kMostChunks) add_up(c, min(c + kMostChunks, a.chunks));
         }
         const double target = double(a.sample[s]) * all;
-        int chunk = a.chunks, last = -1;
+        int piece = pieces, last = -1;
         double upto = before, base = before, last_base = before;
-        for (int c = c0; c < c1; ++c) {
-            const double sum = each == 1 ? only : posted(rest + c);
-            if (sum > 0.) last = c, last_base = upto;
-            if (chunk == a.chunks && upto + sum > target && sum > 0.) chunk = c, base = upto;
+        for (int i = i0; i < i1; ++i) {
+            const double sum = each == 1 ? only : piece_sum(i);
+            if (sum > 0.) last = i, last_base = upto;
+            if (piece == pieces && upto + sum > target && sum > 0.) piece = i, base = upto;
             upto += sum;
         }
-        const int found = max(0, lowest_or_last(chunk, a.chunks, last, picks));
-        if (found == chunk)
+        int last_of_all = last;
+        const int first = lowest(piece, last_of_all, picks), found = first < pieces ? first : max(0, last_of_all);
+        if (found == piece)
             base_of = base;
-        else if (found == last && found >= c0 && found < c1)
+        else if (first == pieces && found == last)
             base_of = last_base;
         __syncthreads();
-        double w[kEach], sum = 0.;
-        Drawn::Chunk<T> here;
-        drawn.load<T>(a, v.row, found * kChunk, true, here);
-        drawn.weigh<T>(here, found * kChunk, true, w);
+        double from = base_of;  // the sum before a chunk
+        walk(first_chunk(found), first_chunk(found + 1), true, [&](int c, const double (&w)[kEach]) {
+            double whole;
+            double upto = from + sum_before(sum_of(w), waves, whole);
+            int pick = a.vocabulary, end = -1;
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) sum += w[i];
-        upto = base_of + sum_before(sum, waves, all);
-        int pick = a.vocabulary, end = -1;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const int at = found * kChunk + tid * kEach + i;
-            upto += w[i];
-            if (w[i] > 0.) {
-                end = at;
-                if (pick == a.vocabulary && upto > target) pick = at;
+            for (int i = 0; i < kEach; ++i) {
+                const int at = c * kChunk + tid * kEach + i;
+                upto += w[i];
+                if (w[i] > 0.) {
+                    end = at;
+                    if (pick == a.vocabulary && upto > target) pick = at;
+                }
             }
-        }
-        token = lowest_or_last(pick, a.vocabulary, end, picks);
+            pick = lowest(pick, end, picks);
+            token = pick < a.vocabulary ? pick : max(token, end);
+            from += whole;
+            return pick < a.vocabulary;
+        });
     }
     if (tid) return;
     a.next[s] = token;

@@ -431,6 +431,38 @@ def test_verify(qpkg, kind, n, rows, vocabulary, ragged, draft, filtered):
     assert np.array_equal(back, want[0] - (given['counts'] - 1))
 
 
+@pytest.mark.parametrize('kind', ['f32', 'bf16'])
+@pytest.mark.parametrize('n,rows,vocabulary', [(1, 1, 151936), (1, 2, 151936), (3, 4, 20000), (64, 7, 20000), (200, 8, 12289),
+                                               (385, 2, 32769)])
+def test_verify_certain_drafts(qpkg, kind, n, rows, vocabulary):
+    """Without probabilities of their own: a row's sums are added once, in ranges of one chunk, of several, and of more than
+    a workgroup goes through."""
+    rng = np.random.default_rng(n + vocabulary)
+    given = random_drafts(rng, n, rows, vocabulary, draft=False)
+    raw = ref.encode(given['logits'], kind)
+    given['logits'] = ref.decode(raw, kind)
+    temperature = (0.3 + rng.random(n)).astype(np.float32)
+    want = ref.verify(**given, temperature=temperature)
+    given['logits'] = raw
+    accepted, following, _ = Drafts(qpkg, **given, temperature=temperature, kind=kind)()
+    assert np.array_equal(accepted, want[0]) and np.array_equal(following, want[1])
+
+
+@pytest.mark.parametrize('many', [1, 50])
+def test_verify_certain_drafts_at_borders(qpkg, many):
+    """Equal logits again, the drafted token refused: the others' weights are whole numbers on either side of it. Rows
+    of 400 sequences are one range, of three chunks."""
+    vocabulary, token = 8192 + 1, 5000
+    share = np.array([0, 1, 4095, 4096, 4999, 5000, 8191, 8190])
+    n, sample = 8 * many, np.tile(share / 8192, many).astype(np.float32)
+    logits = np.full((2 * n, vocabulary), -2.5, np.float32)
+    tokens = np.zeros(2 * n, int)
+    tokens[1::2] = token
+    accepted, following, _ = Drafts(qpkg, logits, tokens, np.full(2 * n, 0.5, np.float32), sample)()
+    want = np.tile(share + (share >= token), n // 8)
+    assert not accepted.any() and np.array_equal(following, want)
+
+
 def test_verify_wrapper(qpkg):
     rng = np.random.default_rng(9)
     given = random_drafts(rng, 6, 4, 500, ragged=True)
