@@ -948,9 +948,10 @@ struct SharedPlan {
         // taken for ragged ones' mean. (All places, as if there were nothing behind them: 4 times 24 sequences 120 us,
         // not 98, as each workgroup of theirs has its start and its sums.)
         const int64_t of_prefixes = std::max<int64_t>(1, tiles) * c.kv_heads;
-        const int64_t ahead = of_prefixes * p.max_length * (c.type == kPagedE4M3 ? 17 : 12), behind = units * p.max_rest / 2 * 9;
-        const int64_t places = held * 4 / 3 * ahead / (ahead + behind + 1) + of_prefixes - 1;
-        split(of_prefixes, std::min(held, places), p.max_length, kPagedMaxLength, parts, part);
+        const double ahead = double(of_prefixes) * p.max_length * (c.type == kPagedE4M3 ? 85. / 45 : 85. / 65);
+        const double share = ahead / (ahead + double(units) * p.max_rest / 2 + 1);
+        split(of_prefixes, std::min(held, int64_t(held * 4 / 3 * share) + of_prefixes - 1), p.max_length, kPagedMaxLength, parts,
+              part);
         jobs = p.max_length ? (parts * c.kv_heads + 7) / 8 * 8 * tiles : 0;
         rest_jobs = rest_parts * rest_tiles * b.sequences * c.kv_heads;
         // Where all workgroups start at once, those without work cost nothing; where they do not, 4 times 24 ragged
