@@ -86,8 +86,10 @@ __device__ __forceinline__ int owner(const int* upto, int n, int k) {
 }
 
 // Pages k below `count`, whose sequences' sums are `upto`: f(s, k) gives a
-// place to read and one to write. Of many, a thread has eight in a row, so it
-// looks for the first one's sequence alone, and all its loads are in flight.
+// place to read and one to write. Of many, a thread has four in a row, so it
+// looks for the first one's sequence alone, and all its loads are in flight
+// (1000 sequences with 21600 pages to move, maps and all, 21.3 us; two in a row
+// 23.3, eight 25.9, four that lie 64 apart with a search each 30.2).
 template <int THREADS, class F>
 __device__ __forceinline__ void move_pages(const int* upto, int n, int count, F f) {
     if (count <= THREADS) {
@@ -99,7 +101,7 @@ __device__ __forceinline__ void move_pages(const int* upto, int n, int count, F 
         *to = *from;
         return;
     }
-    constexpr int kRow = 8;
+    constexpr int kRow = 4;
     for (int k0 = kRow * threadIdx.x; k0 < count; k0 += kRow * THREADS) {
         int s = owner(upto, n, k0), page[kRow];
         int32_t* to[kRow];
@@ -141,7 +143,7 @@ __device__ __forceinline__ void map_row(const ReserveView& v, const int* upto, i
 // are no more threads than they need. A step of 64 sequences takes 3.8 us (4.7
 // with 1024 threads, 6.3 with four sequences a thread as well), of 1000 6.2
 // (8.0 with four each); 1000 sequences with prompts of up to 1000 tokens among
-// them, 12000 pages given back and 9600 taken, 21 us, and their 150000 rows' maps
+// them, 12000 pages given back and 9600 taken, 17 us, and their 150000 rows' maps
 // another 4.6.
 template <int THREADS, int EACH>
 __global__ __launch_bounds__(THREADS) void reserve_kernel(ReserveView v, bool maps) {
