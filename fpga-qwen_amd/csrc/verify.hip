@@ -464,8 +464,8 @@ __device__ __forceinline__ double posted(const double* p) {
 // sums are there; the last one to do so draws: the chunk (or range) in which
 // the sum of the weights passes sample times the whole, then the token in it. Sums of one range in two orders may differ in their last
 // place, so that a border can lie between them: the last token with a weight
-// stands for what lies behind all. Latency bounds it: 12 us for a sequence of
-// two rows, 15 for eight of five, 21 for 64 of up to seven, a chain of loads
+// stands for what lies behind all. Latency bounds it: 11 us for a sequence of
+// two rows, 15 for eight of five, 22 for 64 of up to seven, a chain of loads
 // (offsets, tokens, the row's parts, its logits, the posted sums, the chosen
 // chunk) with a launch before it.
 template <typename T>
