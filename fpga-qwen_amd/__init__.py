@@ -88,7 +88,7 @@ class RotaryHeads(ctypes.Structure):
 
 
 class Draft(ctypes.Structure):
-    """qwen_gpu_draft: drafted tokens and the logits that judge them."""
+    """qwen_gpu_draft: drafted tokens and the logits that decide on them."""
     _fields_ = [('logits', ctypes.c_void_p), ('draft', ctypes.c_void_p), ('tokens', ctypes.c_void_p),
                 ('offsets', ctypes.c_void_p), ('temperature', ctypes.c_void_p), ('accept', ctypes.c_void_p),
                 ('sample', ctypes.c_void_p), ('logit_stride', ctypes.c_int64), ('draft_stride', ctypes.c_int64),

@@ -474,8 +474,10 @@ __device__ __forceinline__ void shared_attend(const PagedView& v, const SharedAr
 __device__ __forceinline__ void widen_f16(uint4_t raw, uint4_t (&out)[2]) {
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-        out[w / 2][2 * (w % 2)] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(raw[w], 1.f, false));
-        out[w / 2][2 * (w % 2) + 1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(raw[w], 1.f, true));
+        const auto low = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(raw[w], 1.f, false);
+        const auto high = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(raw[w], 1.f, true);
+        out[w / 2][2 * (w % 2)] = __builtin_bit_cast(unsigned, low);
+        out[w / 2][2 * (w % 2) + 1] = __builtin_bit_cast(unsigned, high);
     }
 }
 
@@ -950,8 +952,8 @@ struct SharedPlan {
         const int64_t of_prefixes = std::max<int64_t>(1, tiles) * c.kv_heads;
         const double ahead = double(of_prefixes) * p.max_length * (c.type == kPagedE4M3 ? 85. / 45 : 85. / 65);
         const double share = ahead / (ahead + double(units) * p.max_rest / 2 + 1);
-        split(of_prefixes, std::min(held, int64_t(held * 4 / 3 * share) + of_prefixes - 1), p.max_length, kPagedMaxLength, parts,
-              part);
+        const int64_t places = std::min(held, int64_t(held * 4 / 3 * share) + of_prefixes - 1);
+        split(of_prefixes, places, p.max_length, kPagedMaxLength, parts, part);
         jobs = p.max_length ? (parts * c.kv_heads + 7) / 8 * 8 * tiles : 0;
         rest_jobs = rest_parts * rest_tiles * b.sequences * c.kv_heads;
         // Where all workgroups start at once, those without work cost nothing; where they do not, 4 times 24 ragged

@@ -64,7 +64,8 @@ __device__ __forceinline__ void scan_block(const unsigned (&x)[N], unsigned (*wa
     for (int i = 0; i < N; ++i) {
         const unsigned of_lane = scan_wave(lane < THREADS / 64 ? waves[i][lane] : 0u);
         all[i] = __builtin_amdgcn_readlane(of_lane, 63);
-        const unsigned base = wave ? __builtin_amdgcn_readlane(of_lane, __builtin_amdgcn_readfirstlane(max(wave - 1, 0))) : 0u;
+        const int wave_before = __builtin_amdgcn_readfirstlane(max(wave - 1, 0));
+        const unsigned base = wave ? __builtin_amdgcn_readlane(of_lane, wave_before) : 0u;
         // The sum up to the lane before, which the limit keeps from being a difference.
         const unsigned one_less = __shfl_up(upto[i], 1);
         before[i] = limited(base, lane ? one_less : 0u);

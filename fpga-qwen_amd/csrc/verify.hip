@@ -32,12 +32,12 @@ struct Part {
 };
 
 // What the rows of a sequence come to.
-struct Verdict {
+struct Outcome {
     double z;        // of the row that the token is drawn from
     float top;
     int best;        // lowest token of the largest logit
     int row;         // -1: there is none
-    int token;       // the drafted one that the row judges, -1: none
+    int token;       // the drafted one that the row decides on, -1: none
     int accepted, drafted;
 };
 
@@ -264,11 +264,13 @@ __global__ __launch_bounds__(kThreads) void verify_parts_kernel(VerifyArgs a) {
         }
 #pragma unroll
         for (int i = 0; i < kEach; i += 4)
-            if (const float four = fmaxf(fmaxf(x[i], x[i + 1]), fmaxf(x[i + 2], x[i + 3])); __any(four > -kInf && four >= top - span))
+            if (const float four = fmaxf(fmaxf(x[i], x[i + 1]), fmaxf(x[i + 2], x[i + 3]));
+                __any(four > -kInf && four >= top - span))
 #pragma unroll
                 for (int j = 0; j < 4; ++j) sum += powers.summand(x[i + j], top, heat);
     }
-    // All lanes' by the largest of all (a lane without tokens has added 2^-1000 up at most); where it wins, its sum is 1 and the token the lowest that has it.
+    // All lanes' by the largest of all (a lane without tokens has added 2^-1000 up at most); where the largest wins, the sum
+    // is 1 and the token the lowest that has it.
     auto weigh = [&](float of, float whole) { return of == whole ? 1. : powers.weight(of, whole, heat); };
     float whole = dev::wave_max(top);
     if (lane == 0) tops[wave] = whole;
@@ -313,7 +315,7 @@ __device__ __forceinline__ Part whole_row(const VerifyArgs& a, const Powers& pow
 struct Drawn {
     float top;
     double heat, by;   // by: 1 / Z where there is a q, 1 elsewhere
-    bool judged;       // less q
+    bool refused;       // less q
     const float* q;    // of the row, or NULL: all at the token
     int token;
     const Powers& powers;
@@ -327,7 +329,7 @@ struct Drawn {
     template <typename T>
     __device__ __forceinline__ void load(const VerifyArgs& a, int row, int from, bool together, Chunk<T>& c) const {
         c.logits.load(reinterpret_cast<const T*>(a.logits) + row * a.logit_stride, from, a.vocabulary, together, T(-kInf));
-        if (!judged || !q) return;
+        if (!refused || !q) return;
         if (from + kChunk <= a.vocabulary) {
             typedef float float4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 #pragma unroll
@@ -361,18 +363,18 @@ struct Drawn {
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                if (judged && q)
+                if (refused && q)
                     w[i + j] = fmax(w[i + j] - fmax(double(c.of_q[i + j]), 0.), 0.);
-                else if (judged && from + Tokens<T>::at(i + j, together) == token)
+                else if (refused && from + Tokens<T>::at(i + j, together) == token)
                     w[i + j] = 0.;
             }
         }
     }
 };
-__device__ __forceinline__ Drawn drawn_from(const VerifyArgs& a, const Powers& powers, const Verdict& v, double heat) {
-    const bool judged = v.accepted < v.drafted;
-    return {uniform(v.top), heat, judged && a.draft ? 1. / v.z : 1., judged, judged && a.draft ? a.draft + v.row * a.draft_stride : nullptr, v.token,
-            powers};
+__device__ __forceinline__ Drawn drawn_from(const VerifyArgs& a, const Powers& powers, const Outcome& v, double heat) {
+    const bool refused = v.accepted < v.drafted;
+    const float* const q = refused && a.draft ? a.draft + v.row * a.draft_stride : nullptr;
+    return {uniform(v.top), heat, q ? 1. / v.z : 1., refused, q, v.token, powers};
 }
 
 // The sum over the threads before this one, and over all.
@@ -411,14 +413,14 @@ __device__ __forceinline__ int lowest(int number, int& other, int* waves) {
 }
 
 // What a sequence's rows come to: the first row whose drafted token is not
-// accepted, or the last. A wave judges a row, so a workgroup four at a time.
+// accepted, or the last. A wave checks a row, so a workgroup four at a time.
 template <typename T>
-__device__ __forceinline__ Verdict judge(const VerifyArgs& a, const Powers& powers, int s, double heat, bool greedy,
-                                         Verdict (&of_wave)[kWaves], int (&fits)[kWaves]) {
+__device__ __forceinline__ Outcome check_rows(const VerifyArgs& a, const Powers& powers, int s, double heat, bool greedy,
+                                              Outcome (&of_wave)[kWaves], int (&fits)[kWaves]) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int first;
     const int n = a.rows_of(s, first);
-    Verdict v{0., -kInf, -1, -1, -1, 0, max(n - 1, 0)};
+    Outcome v{0., -kInf, -1, -1, -1, 0, max(n - 1, 0)};
     for (int i0 = 0; i0 < n && v.row < 0; i0 += kWaves) {
         const int i = i0 + wave;
         if (i < n) {
@@ -458,12 +460,12 @@ __device__ __forceinline__ double posted(const double* p) {
                                                         __HIP_MEMORY_SCOPE_AGENT));
 }
 
-// Every workgroup of a sequence judges its rows (from sums, which takes no
+// Every workgroup of a sequence checks its rows (from sums, which takes no
 // longer than to wait for another's word) and adds the weights that the token
 // is drawn from up over its own chunks, unless they are a row's own, whose
 // sums are there; the last one to do so draws: the chunk (or range) in which
-// the sum of the weights passes sample times the whole, then the token in it. Sums of one range in two orders may differ in their last
-// place, so that a border can lie between them: the last token with a weight
+// the sum of the weights passes sample times the whole, then the token in it.
+// Sums of one range in two orders may differ in their last place, so that a border can lie between them: the last token with a weight
 // stands for what lies behind all. Latency bounds it: 11 us for a sequence of
 // two rows, 15 for eight of five, 22 for 64 of up to seven, a chain of loads
 // (offsets, tokens, the row's parts, its logits, the posted sums, the chosen
@@ -472,7 +474,7 @@ template <typename T>
 __global__ __launch_bounds__(kThreads, 4) void verify_draw_kernel(VerifyArgs a) {
     __shared__ Powers powers;
     __shared__ double waves[kWaves], base_of, chunk_sums[kMostChunks][kWaves];
-    __shared__ Verdict of_wave[kWaves];
+    __shared__ Outcome of_wave[kWaves];
     __shared__ int fits[kWaves], picks[2 * kWaves], last_one;
     const int groups = (a.chunks + a.draw_chunks - 1) / a.draw_chunks;
     const int s = blockIdx.x / groups, own = blockIdx.x - s * groups, tid = threadIdx.x;
@@ -480,15 +482,15 @@ __global__ __launch_bounds__(kThreads, 4) void verify_draw_kernel(VerifyArgs a) 
     __syncthreads();
     const double heat = a.heat(s);
     const bool greedy = a.greedy(s);
-    const Verdict v = judge<T>(a, powers, s, heat, greedy, of_wave, fits);
+    const Outcome v = check_rows<T>(a, powers, s, heat, greedy, of_wave, fits);
     const bool draws = v.row >= 0 && v.z > 0. && !greedy;
     int token = draws || v.row < 0 || !(v.z > 0.) ? -1 : v.best;
     Drawn drawn = drawn_from(a, powers, v, heat);
     double* const rest = a.rest + int64_t(s) * a.chunks;
     // Without a q to subtract, the ranges' sums are those of the first kernel, but for the drafted token's range. (A token
-    // for each of 64 sequences 27 us, 41 without this; 64 sequences of up to seven BF16 rows, whose ranges have eight chunks, 48 us
-    // with it, 42 without.)
-    const bool known = !(drawn.judged && drawn.q) && a.chunks <= a.ranges * max(2, a.draw_chunks);
+    // for each of 64 sequences 27 us, 41 without this; 64 sequences of up to seven BF16 rows, whose ranges have eight
+    // chunks, 48 us with it, 42 without.)
+    const bool known = !(drawn.refused && drawn.q) && a.chunks <= a.ranges * max(2, a.draw_chunks);
     if ((!draws || known) && own) return;
     if (draws) {
         // The weights of chunks, the next one's tokens on their way, until f says that it is enough.
@@ -529,7 +531,7 @@ __global__ __launch_bounds__(kThreads, 4) void verify_draw_kernel(VerifyArgs a) 
         auto first_chunk = [&](int piece) { return known ? int(int64_t(a.chunks) * piece / a.ranges) : piece; };
         double all = 0., without = 0.;
         int spared = -1;  // the drafted token's range, whose sum is `without`
-        if (known && drawn.judged && v.token >= 0 && v.token < a.vocabulary) {
+        if (known && drawn.refused && v.token >= 0 && v.token < a.vocabulary) {
             spared = int((int64_t(v.token / kChunk + 1) * a.ranges - 1) / a.chunks);
             double sum = 0.;
             walk(first_chunk(spared), first_chunk(spared + 1), false, [&](int, const double (&w)[kEach]) {
@@ -555,8 +557,8 @@ __global__ __launch_bounds__(kThreads, 4) void verify_draw_kernel(VerifyArgs a) 
             double sum = 0.;
             for (int i = i0; i < i1; ++i) sum += only = piece_sum(i);
             before = sum_before(sum, waves, all);
-            if (!drawn.judged || all > 0.) break;
-            drawn.judged = false;  // q is p or more throughout
+            if (!drawn.refused || all > 0.) break;
+            drawn.refused = false;  // q is p or more throughout
             drawn.by = 1.;
             spared = -1;
             if (!known)
@@ -679,7 +681,8 @@ void launch_verify_draft(const qwen_gpu_draft& d, int32_t* accepted, int32_t* ne
     char* const space = static_cast<char*>(workspace);
     const VerifyArgs a{static_cast<const char*>(d.logits), d.draft, d.tokens, d.offsets, d.temperature, d.accept, d.sample,
                        d.total_rows > 1 ? d.logit_stride : 0, d.total_rows > 1 ? d.draft_stride : 0, d.vocabulary,
-                       int(plan.chunks), d.sequences, d.rows, d.total_rows, int(plan.ranges), int(plan.draw_chunks), reinterpret_cast<Part*>(space),
+                       int(plan.chunks), d.sequences, d.rows, d.total_rows, int(plan.ranges), int(plan.draw_chunks),
+                       reinterpret_cast<Part*>(space),
                        reinterpret_cast<double*>(space + plan.parts),
                        reinterpret_cast<int*>(space + plan.parts + plan.rest), accepted, next, back};
     if (d.type == QWEN_GPU_F32)

@@ -396,8 +396,9 @@ int qwen_gpu_op_paged_evict(const qwen_gpu_paged_cache* cache, const qwen_gpu_pa
  * offsets[g] .. offsets[g + 1] - 1 (bounded to 0 .. sequences on the device;
  * offsets must not fall), which hold the same keys and values in their first
  * lengths[g] slots; those are read through the table of its first sequence
- * with new rows. The prefix is taken no longer than the rows that each of the group's sequences
- * with new rows cached before them, and a sequence of no group has none, so
+ * with new rows. The prefix is taken no longer than what each of the group's
+ * sequences with new rows had cached before them, and a sequence of no group
+ * has none, so
  * every row attends what qwen_gpu_op_paged_attention gives it. max_length
  * and max_rest size the launch: what a sequence has beyond them is attended
  * too, by fewer workgroups. Weights are not tracked: batch->weights and
@@ -455,8 +456,8 @@ typedef struct qwen_gpu_paged_growth {
  * emptied. Then sequences get their new rows, in order: one that needs pages
  * takes them from the stack's end, until one needs more than there are, and
  * from there on only those that need none are granted; and no sequence
- * whose rows, with those granted before, pass total_rows, nor any with new rows behind
- * it. One that is not granted keeps its length and has no rows in `offsets`;
+ * whose rows, with those granted before, pass total_rows, nor any with new
+ * rows behind it. One that is not granted keeps its length and has no rows in `offsets`;
  * one that has fewer pages than the rows it has need takes those too, when it
  * grows.
  * A wish that the table has no entries for (length + change above
@@ -464,9 +465,9 @@ typedef struct qwen_gpu_paged_growth {
  * back more than there is. The lengths, seen, held and changes of one call
  * are read before the results are written, so new_lengths may be lengths,
  * new_seen seen, new_held held and new_free_count free_count; otherwise
- * nothing that is written may overlap another array. What the arrays hold is bounded: held into 0 ..
- * table_stride, lengths into 0 .. table_stride * page_size (at most 2^30), free_count into 0
- * .. pages; pages given back beyond `pages` free ones are dropped. Tables and
+ * nothing that is written may overlap another array. What the arrays hold is
+ * bounded: held into 0 .. table_stride, lengths into 0 .. table_stride *
+ * page_size (at most 2^30), free_count into 0 .. pages; pages given back beyond `pages` free ones are dropped. Tables and
  * slots of pages outside 0 .. pages - 1 (which only a wrong stack can hold)
  * get -1 as their slots. Streams as for the paged cache; the device is that
  * of `table`. */
@@ -537,7 +538,7 @@ int qwen_gpu_op_rotate(const qwen_gpu_rotary* rotary, const qwen_gpu_rotary_head
 /* ---- Verification of drafted tokens (no reference counterpart) ----
  *
  * Sequence s has n rows of logits: row i is the target's for the token behind
- * the row's own, so that row i of the first n - 1 judges the drafted token
+ * the row's own, so that row i of the first n - 1 decides on the drafted token
  * tokens[first + i + 1] and the last one is for the token after all drafts. A
  * sequence of one row has no drafts: a token is drawn for it. */
 typedef struct qwen_gpu_draft {
@@ -547,7 +548,8 @@ typedef struct qwen_gpu_draft {
     const int32_t* tokens;      /* [total_rows]: the rows' own tokens */
     const int32_t* offsets;     /* [sequences + 1]: as a paged batch's; NULL: `rows` rows each */
     const float* temperature;   /* [sequences], NULL: 1 */
-    const float* accept;        /* [total_rows]: numbers of [0, 1), one for each drafted token, at its judge's row */
+    const float* accept;        /* [total_rows]: numbers of [0, 1), one for each drafted token, at the row that
+                                 * decides on it */
     const float* sample;        /* [sequences]: numbers of [0, 1), for the token that is drawn */
     int64_t logit_stride;       /* elements */
     int64_t draft_stride;
