@@ -930,21 +930,22 @@ struct SharedPlan {
         const int64_t tile = rows_of_wide(wide);
         tiles = (rows + p.groups * (tile - 1)) / tile;  // however the groups share them
         rest_tiles = (group * b.rows + 15) / 16;
-        // Parts for as many workgroups as the GPU holds at once, of 256 positions or more (8192 positions and 64 users 40 us;
-        // of 128 51, of 512 44), and of 640 at most behind the prefixes, where ragged lengths would keep a few workgroups
+        // Parts for as many workgroups as the GPU holds at once, of 256 positions or more (two sequences behind 4000 14.2
+        // us, of 128 16.1, of 512 17.5), and of 640 at most behind the prefixes, where ragged lengths would keep a few workgroups
         // long (64 sequences of up to 3000 90 us, with 1024 98, without 122; of 4 times 24 of up to 1500 100, 99 and 114).
         const int64_t held = c.head_dim == 256 ? 256 : 512;
-        auto split = [&](int64_t units, int64_t places, int64_t positions, int64_t longest, int64_t& count, int64_t& size) {
-            const int64_t most = std::max<int64_t>(1, (positions + 255) / 256);
+        auto split = [&](int64_t units, int64_t places, int64_t positions, int64_t shortest, int64_t longest, int64_t step,
+                         int64_t& count, int64_t& size) {
+            const int64_t most = std::max<int64_t>(1, (positions + shortest - 1) / shortest);
             const int64_t least = std::max<int64_t>(1, (positions + longest - 1) / longest);
             count = std::clamp<int64_t>(places / std::max<int64_t>(1, units), least, most);
             size = (positions + count - 1) / count;
-            size = std::max<int64_t>(kBlock, (size + kBlock - 1) / kBlock * kBlock);
+            size = std::max<int64_t>(step, (size + step - 1) / step * step);
             count = std::max<int64_t>(1, (positions + size - 1) / size);
         };
         // (A sequence has a row at least where it has work.)
         const int64_t working = std::min<int64_t>(b.sequences, b.total_rows), units = rest_tiles * working * c.kv_heads;
-        split(units, held, p.max_rest, 640, rest_parts, rest_part);
+        split(units, held, p.max_rest, 256, 640, kBlock, rest_parts, rest_part);
         // The prefixes have as many of the places as their share of the work, and a third more, so that none of their
         // workgroups is the last one: 85 ns a position of theirs, 65 (E4M3 45) behind them, where half of the most are
         // taken for ragged ones' mean. (All places, as if there were nothing behind them: 4 times 24 sequences 120 us,
@@ -953,7 +954,14 @@ struct SharedPlan {
         const double ahead = double(of_prefixes) * p.max_length * (c.type == kPagedE4M3 ? 85. / 45 : 85. / 65);
         const double share = ahead / (ahead + double(units) * p.max_rest / 2 + 1);
         const int64_t places = std::min(held, int64_t(held * 4 / 3 * share) + of_prefixes - 1);
-        split(of_prefixes, places, p.max_length, kPagedMaxLength, parts, part);
+        // Wide tiles' workgroups go 32 positions a step (64 with heads of 64) and may be short, up to 128 parts: 14
+        // sequences of 16 query heads on one KV head behind 3616 positions 18 us, of 256 positions at least 25; with 503
+        // parts of 60000 positions instead of 235 44 us, not 36.
+        if (wide)
+            split(of_prefixes, places, p.max_length, std::clamp<int64_t>(p.max_length / 128, 64, 256), kPagedMaxLength,
+                  c.head_dim == 64 ? 64 : 32, parts, part);
+        else
+            split(of_prefixes, places, p.max_length, 256, kPagedMaxLength, kBlock, parts, part);
         jobs = p.max_length ? (parts * c.kv_heads + 7) / 8 * 8 * tiles : 0;
         rest_jobs = rest_parts * rest_tiles * b.sequences * c.kv_heads;
         // Where all workgroups start at once, those without work cost nothing; where they do not, 4 times 24 ragged
