@@ -930,9 +930,11 @@ struct SharedPlan {
         const int64_t tile = rows_of_wide(wide);
         tiles = (rows + p.groups * (tile - 1)) / tile;  // however the groups share them
         rest_tiles = (group * b.rows + 15) / 16;
-        // Parts for as many workgroups as the GPU holds at once, of 256 positions or more (two sequences behind 4000 14.2
-        // us, of 128 16.1, of 512 17.5), and of 640 at most behind the prefixes, where ragged lengths would keep a few workgroups
-        // long (64 sequences of up to 3000 90 us, with 1024 98, without 122; of 4 times 24 of up to 1500 100, 99 and 114).
+        // Parts for as many workgroups as the GPU holds at once, half of that where each has 16 query rows, which is one a
+        // CU (8 sequences behind 512 positions 19.4 us, 20.3 with two, 4 with up to 3000 more 25.1 and 29.7), of 256
+        // positions or more (two sequences behind 4000 14.2 us, of 128 16.1, of 512 17.5), and of 640 at most behind the
+        // prefixes, where ragged lengths would keep a few workgroups long (64 sequences of up to 3000 90 us, with 1024 98,
+        // without 122; 4 times 24 of up to 1500 100, 99 and 114).
         const int64_t held = c.head_dim == 256 ? 256 : 512;
         auto split = [&](int64_t units, int64_t places, int64_t positions, int64_t shortest, int64_t longest, int64_t step,
                          int64_t& count, int64_t& size) {
@@ -945,7 +947,7 @@ struct SharedPlan {
         };
         // (A sequence has a row at least where it has work.)
         const int64_t working = std::min<int64_t>(b.sequences, b.total_rows), units = rest_tiles * working * c.kv_heads;
-        split(units, held, p.max_rest, 256, 640, kBlock, rest_parts, rest_part);
+        split(units, 256, p.max_rest, 256, 640, kBlock, rest_parts, rest_part);
         // The prefixes have as many of the places as their share of the work, and a third more, so that none of their
         // workgroups is the last one: 85 ns a position of theirs, 65 (E4M3 45) behind them, where half of the most are
         // taken for ragged ones' mean. (All places, as if there were nothing behind them: 4 times 24 sequences 120 us,
@@ -960,8 +962,8 @@ struct SharedPlan {
         if (wide)
             split(of_prefixes, places, p.max_length, std::clamp<int64_t>(p.max_length / 128, 64, 256), kPagedMaxLength,
                   c.head_dim == 64 ? 64 : 32, parts, part);
-        else
-            split(of_prefixes, places, p.max_length, 256, kPagedMaxLength, kBlock, parts, part);
+        else  // a workgroup a CU: 8 sequences behind 16000 positions 22.8 us, with two 27.8, behind 60000 54 and 56
+            split(of_prefixes, std::min<int64_t>(places, 256), p.max_length, 256, kPagedMaxLength, kBlock, parts, part);
         jobs = p.max_length ? (parts * c.kv_heads + 7) / 8 * 8 * tiles : 0;
         rest_jobs = rest_parts * rest_tiles * b.sequences * c.kv_heads;
         // Where all workgroups start at once, those without work cost nothing; where they do not, 4 times 24 ragged
