@@ -256,7 +256,8 @@ __global__ __launch_bounds__(kThreads) void verify_parts_kernel(VerifyArgs a) {
             sum = high == kInf || top == -kInf ? 0. : sum * powers.weight<true>(top, high, heat);
             top = high;
         }
-        if (!__any(high > -kInf && high >= top - span)) continue;
+        // (Not `high >= top - span`: with an infinite span an infinite top leaves no number there, and counts.)
+        if (!__any(high > -kInf && !(high < top - span))) continue;
         if (__any(top == kInf)) {
 #pragma unroll
             for (int i = 0; i < kEach; ++i) sum += powers.weight(x[i], top, heat);

@@ -622,3 +622,36 @@ def test_host_memory_is_refused(qpkg):
     call.given.sample = host.ctypes.data
     with pytest.raises(RuntimeError, match='Not device memory: sample'):
         call()
+
+
+@pytest.mark.parametrize('kind', ref.TYPES)
+@pytest.mark.parametrize('vocabulary', [1, 6, 300, 70000])
+def test_verify_infinite_temperatures(qpkg, kind, vocabulary):
+    """At temperatures at which all finite logits are as likely, infinite ones still have all of p, also where no other
+    token of their row is left: alone, at both ends, throughout, beside finite ones and beside NaN."""
+    inf, v = np.inf, vocabulary
+    rng = np.random.default_rng(v)
+    rows = [np.full(v, x, np.float32) for x in (-inf, -inf, -inf, inf, 0.0, np.nan, -inf, -inf)]
+    rows[0][0] = rows[1][-1] = rows[2][0] = rows[2][-1] = rows[4][v // 2] = rows[5][v // 3] = inf
+    rows[6][v // 2] = 3.0  # the last one has no token
+    logits, tokens, accept, sample, heat = [], [], [], [], []
+    for row in rows:
+        for token in (0, v - 1, v // 2):
+            for t in (inf, 3.4e38, 6e36, 5e36, 1.0):
+                logits += [row, rng.standard_normal(v).astype(np.float32)]
+                tokens += [0, token]
+                accept += [0.25, 0.5]
+                sample.append(rng.choice([0, 0.51237, 0.99917]))  # on no border between equal weights
+                heat.append(t)
+    raw = ref.encode(np.asarray(logits, np.float32), kind)
+    given = dict(logits=ref.decode(raw, kind), tokens=np.asarray(tokens), accept=np.asarray(accept, np.float32),
+                 sample=np.asarray(sample, np.float32))
+    heat = np.asarray(heat, np.float32)
+    draft = np.full(raw.shape, 1 / v, np.float32)
+    for q in (None, draft):
+        with np.errstate(all='ignore'):
+            want = ref.verify(**given, draft=q, temperature=heat)
+        accepted, following, _ = Drafts(qpkg, raw, given['tokens'], given['accept'], given['sample'], q, temperature=heat,
+                                        kind=kind)()
+        assert np.array_equal(accepted, want[0])
+        assert np.array_equal(following, want[1]), np.flatnonzero(following != want[1])[:5]
