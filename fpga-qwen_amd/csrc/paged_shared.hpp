@@ -794,7 +794,10 @@ __global__ __launch_bounds__(kWaves * 64, DIM == 256 ? 1 : 2) void shared_attent
                 int row;
                 const int n = v.new_rows(min(s, v.sequences - 1), row), positions = v.length(min(s, v.sequences - 1));
                 const int of = groups.rest_parts(positions, n, groups.nominal_of_lane(s));
-                if (s < v.sequences) counts[c] = of * ((n * a.group + 15) / 16);
+                // (The launch has workgroups for no more sequences than there are rows.)
+                int there, past;
+                v.existing(row, n, there, past);
+                if (s < v.sequences && there < past) counts[c] = of * ((n * a.group + 15) / 16);
                 of_head += __builtin_amdgcn_readlane(scan_lanes(counts[c]), 63);
             }
             if (!of_head) return;

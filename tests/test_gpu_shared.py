@@ -514,3 +514,36 @@ def test_captured_steps(qpkg):
         hip.hipGraphExecDestroy(run)
         hip.hipGraphDestroy(graph)
         hip.hipStreamDestroy(stream)
+
+
+class Poisoned(Shared):
+    """A call whose workspace holds NaN, so that whatever nobody wrote shows."""
+
+    def workspace(self, heads):
+        return self.q.DeviceBuffer.from_array(np.full(super().workspace(heads).nbytes, 0xff, np.uint8))
+
+
+@pytest.fixture
+def poisoned(monkeypatch):
+    monkeypatch.setattr(sys.modules[__name__], 'Shared', Poisoned)
+
+
+@pytest.mark.parametrize('kind', ['f16', 'bf16', 'e4m3'])
+@pytest.mark.parametrize('below,total,rows,sequences', [(0, 50, 1, 200), (0, 1, 1, 256), (70, 50, 1, 200), (130, 77, 3, 130)])
+def test_offsets_past_the_rows(qpkg, poisoned, kind, below, total, rows, sequences):
+    """Many sequences whose offsets rise past total_rows, from below 0 too: the rows that are there get all of their KV
+    heads, of the prefix and of what is behind it, and all others stay."""
+    rng = np.random.default_rng(41)
+    prefix, kv, group, dim = 16, 8, 2, 64
+    counts = np.full(sequences, rows)
+    offsets = np.concatenate(([0], np.cumsum(counts))) - below
+    lengths = [prefix + rows + int(x) for x in rng.integers(0, 40, sequences)]
+    cache, table = made(rng, kind, kv, dim, 16, 'head', [0, sequences], lengths, [prefix])
+    queries = rng.standard_normal((total + 3, kv * group * dim)).astype(np.float32)
+    out = np.full(queries.shape, 7.5, np.float32)
+    call = Shared(qpkg, cache, table, lengths, [prefix], rows=rows, offsets=offsets, total=total, max_rest=64, max_prefix=16)
+    got = call(queries, kv * group, 0.125, out)
+    want, tolerance, _, _ = ref.attention(cache, table, lengths, rows, offsets, queries[:total].reshape(total, -1, dim), 0.125,
+                                          out[:total].reshape(total, -1, dim))
+    assert (np.abs(got[:total].reshape(want.shape) - want) <= tolerance).all()
+    assert (got[total:] == 7.5).all()
