@@ -2,6 +2,7 @@
 #include "paged_shared.hpp"
 
 #include <cmath>
+#include <string>
 
 #include "paged.hpp"
 #include "qwen_common.hpp"
@@ -27,10 +28,12 @@ SharedPlan plan_of(const qwen_gpu_paged_cache& cache, const qwen_gpu_paged_batch
             "The prefixes' max_length must be in 0..max_length");
     require(prefix.max_rest >= 1 && prefix.max_rest <= batch.max_length, "max_rest must be in 1..max_length");
     const char* const too_many = "Too many new rows or positions for one call";
-    // Query rows fit 31 bits, and so do workgroups; the first check keeps the plan's products within 64 bits.
+    // Query rows fit 31 bits, which keeps the plan's products within 64. A launch counts its threads in 32 bits, so
+    // each has fewer than 2^24 workgroups of 256: those of the attention, and one for each new row to join its parts.
     require(int64_t(query_heads) * std::max(batch.rows, batch.total_rows) < int64_t(1) << 31, too_many);
     const SharedPlan plan(cache, batch, prefix, query_heads);
-    require(plan.jobs < int64_t(1) << 30 && plan.rest_jobs < int64_t(1) << 30, too_many);
+    constexpr int64_t kMostGroups = int64_t(1) << 24;
+    require(plan.groups() < kMostGroups && batch.total_rows < kMostGroups, too_many);
     return plan;
 }
 
@@ -94,6 +97,9 @@ void launch_paged_attention_shared(const qwen_gpu_paged_cache& cache, const qwen
         shared_launch<kPagedBF16>(cache.head_dim, v, a, plan, stream);
     else
         shared_launch<kPagedE4M3>(cache.head_dim, v, a, plan, stream);
+    // (Without the parts there is nothing to join.)
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess)
+        throw std::runtime_error(std::string("HIP error: ") + hipGetErrorString(e));
     // A workgroup for each piece of few rows; of many, it finds its row's parts once for several pieces.
     const int64_t pieces = (row / 4 + kJoinItems - 1) / kJoinItems;
     const dim3 grid(unsigned(batch.total_rows), unsigned(std::clamp<int64_t>(2048 / batch.total_rows, 1, pieces)));

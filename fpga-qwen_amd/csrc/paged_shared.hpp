@@ -977,13 +977,14 @@ struct SharedPlan {
         state_bytes = (size_t(slots) * b.total_rows * query_heads * 8 + 15) / 16 * 16;
         sum_bytes = size_t(slots) * b.total_rows * query_heads * c.head_dim * 4;
     }
+    int64_t groups() const { return jobs + (rest_jobs + 7) / 8 * 8; }
     size_t bytes() const { return sum_bytes + state_bytes; }
 };
 
 template <int TYPE, int DIM, int WIDE>
 void shared_run(const PagedView& v, const SharedArgs& a, const SharedPlan& plan, hipStream_t stream) {
     shared_attention_kernel<TYPE, DIM, WIDE>
-        <<<unsigned(plan.jobs + (plan.rest_jobs + 7) / 8 * 8), kWaves * 64, 0, stream>>>(v, a);
+        <<<unsigned(plan.groups()), kWaves * 64, 0, stream>>>(v, a);
 }
 
 template <int TYPE>

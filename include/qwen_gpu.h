@@ -401,7 +401,8 @@ int qwen_gpu_op_paged_evict(const qwen_gpu_paged_cache* cache, const qwen_gpu_pa
  * has none, so
  * every row attends what qwen_gpu_op_paged_attention gives it. max_length
  * and max_rest size the launch: what a sequence has beyond them is attended
- * too, by fewer workgroups. Weights are not tracked: batch->weights and
+ * too, by fewer workgroups. Sizes that come to 2^24 workgroups or more, or to
+ * 2^24 rows, are refused. Weights are not tracked: batch->weights and
  * batch->positions must be NULL. The workspace (device memory, aligned to 16)
  * needs no zeroing and keeps nothing between calls. */
 typedef struct qwen_gpu_paged_prefix {

@@ -80,6 +80,25 @@ def test_workspace(qpkg, sequences, rows, heads, max_length, max_rest, dim):
     assert need.value == (2 * sequences * rows * heads * 8 + 15) // 16 * 16 + 2 * sequences * rows * heads * dim * 4
 
 
+@pytest.mark.parametrize('kv,heads,batch_fields', [
+    (256, 256, dict(sequences=4096, rows=256, total_rows=4096, offsets=AT)),  # workgroups behind the prefixes
+    (1024, 1024, dict(sequences=1, rows=32, total_rows=(1 << 21) - 1, offsets=AT)),  # of the prefixes
+    (8, 8, dict(sequences=1, rows=1 << 24, total_rows=1 << 24))])  # a workgroup for each new row
+def test_launches_that_cannot_be(qpkg, kv, heads, batch_fields):
+    """A launch has less than 2^32 threads, 2^24 workgroups of 256; what is a little smaller is accepted."""
+    need, lib = ctypes.c_size_t(), qpkg.load_library()
+    c = cache(qpkg, kv_heads=kv, page_stride=kv * 16 * 128)
+    p = prefix(qpkg, max_rest=1)
+    given = dict(c=c, p=p, heads=heads, q_stride=heads * 128, out_stride=heads * 128, bytes=1 << 60)
+    b = untracked(qpkg, **batch_fields)
+    assert lib.qwen_gpu_op_paged_shared_workspace(c, b, p, heads, ctypes.byref(need)) == 1 and need.value == 0
+    refused(qpkg, 'Too many new rows or positions', b=b, **given)
+    fewer = dict(batch_fields, rows=batch_fields['rows'] * 15 // 16, total_rows=batch_fields['total_rows'] * 15 // 16)
+    b = untracked(qpkg, **fewer)
+    assert lib.qwen_gpu_op_paged_shared_workspace(c, b, p, heads, ctypes.byref(need)) == 0 and need.value
+    refused(qpkg, 'Not device memory', b=b, **given)
+
+
 def test_wrapper_checks(qpkg):
     paged = object.__new__(qpkg.PagedKV)
     paged.lengths, paged._counts, paged.head_dim = np.zeros(3, np.int32), np.array([1, 0, 2]), 64
