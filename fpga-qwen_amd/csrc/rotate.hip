@@ -42,7 +42,7 @@ void rotary_frequencies(int scaling, int dims, double base, double factor, doubl
 
 namespace {
 
-constexpr int kThreads = 256, kMaxDim = 512;
+constexpr int kThreads = 256, kMaxDim = 512, kMaxRows = 1 << 24;
 
 struct Side {
     const char* rows;
@@ -121,7 +121,7 @@ template <typename T, int V, int K, bool INTERLEAVED>
 __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs a) {
     __shared__ float2 turns[kMaxDim / 2];
     static_assert(kMaxDim / 2 <= kThreads, "a pair each");
-    const int64_t row = blockIdx.x;
+    const int64_t row = blockIdx.y * gridDim.x + blockIdx.x;
     const int position = a.positions[row];
     if (position < 0) return;
     if (const int pair = threadIdx.x; pair < a.turned) {
@@ -207,10 +207,12 @@ void rotate_run(const RotateArgs& args, unsigned rows, bool interleaved, hipStre
     RotateArgs a = args;
     a.lanes = 1;
     while (a.lanes < 64 && a.lanes * V < a.pairs) a.lanes *= 2;
+    // The threads of a grid's axis are counted in 32 bits: the most rows there are need one more.
+    const dim3 grid = rows == kMaxRows ? dim3(kMaxRows / 2, 2) : dim3(rows);
     if (interleaved)
-        rotate_kernel<T, V, K, true><<<rows, kThreads, 0, stream>>>(a);
+        rotate_kernel<T, V, K, true><<<grid, kThreads, 0, stream>>>(a);
     else
-        rotate_kernel<T, V, K, false><<<rows, kThreads, 0, stream>>>(a);
+        rotate_kernel<T, V, K, false><<<grid, kThreads, 0, stream>>>(a);
 }
 
 // 16 bytes a load, or fewer where the turned and the other pairs do not come in such groups (of the 8191 BF16 rows above:
@@ -289,7 +291,7 @@ void launch_rotate(const qwen_gpu_rotary& rotary, const qwen_gpu_rotary_heads& q
     require(rotary.epsilon > 0 && std::isfinite(rotary.epsilon), "The norm's epsilon must be above 0");
     require(rotary.frequencies || !rotary.dims, "Null argument: frequencies");
     require(positions, "Null argument: positions");
-    require(rows >= 0 && rows <= 1 << 24, "Rotary rows must be in 0..2^24");
+    require(rows >= 0 && rows <= kMaxRows, "Rotary rows must be in 0..2^24");
     check_side(queries, "queries", rotary.head_dim, rows);
     if (keys) check_side(*keys, "keys", rotary.head_dim, rows);
     const int size = rotary.type == QWEN_GPU_F32 ? 4 : 2;

@@ -655,3 +655,23 @@ def test_verify_infinite_temperatures(qpkg, kind, vocabulary):
                                         kind=kind)()
         assert np.array_equal(accepted, want[0])
         assert np.array_equal(following, want[1]), np.flatnonzero(following != want[1])[:5]
+
+
+@pytest.mark.parametrize('rows', [(1 << 24) - 1, 1 << 24])
+def test_rotate_the_most_rows(qpkg, rows):
+    """As many rows as a call has at most, of which a few are there; all others, of negative positions, stay."""
+    rng = np.random.default_rng(25)
+    live = np.unique(np.concatenate(([0, 1, (1 << 23) - 1, 1 << 23, rows - 2, rows - 1], rng.integers(0, rows, 2000))))
+    positions = np.full(rows, -1, np.int32)
+    positions[live] = rng.integers(0, 5000, live.size)
+    raw = np.full((rows, 2), 0x3c00, np.uint16)  # ones
+    raw[live] = ref.encode(rng.standard_normal((live.size, 2)), 'f16')
+    side = Heads(qpkg, raw, 1, 2, 0)
+    got, = rotate(qpkg, [side], [None], positions, np.array([0.37]), False, 1.0, 'f16')
+    x = ref.decode(raw[live], 'f16').reshape(-1, 1, 2)
+    want, tolerance = ref.rotate(x, positions[live], np.array([0.37]), False, np.float32(1), None, np.float32(1e-6), 'f16')
+    off = np.abs(ref.decode(got[live], 'f16').reshape(want.shape) - want)
+    assert (off <= tolerance).all(), (off / tolerance).max()
+    rest = got.copy()
+    rest[live] = raw[live]
+    assert np.array_equal(rest, raw)
