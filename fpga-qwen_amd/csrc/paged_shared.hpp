@@ -918,6 +918,12 @@ __global__ __launch_bounds__(kWaves * 64) void shared_join_kernel(PagedView v, S
 }
 
 // Sizes of a call: how its work is split, and what its workspace holds.
+// The sums behind the prefixes take 256 MiB at most, which the last level of
+// the caches holds, or one part's. 2048 new rows of 32 heads of 128 that may
+// have 32768 positions behind their prefix take 827 us with 260 MiB in all,
+// 1457 with parts of 640 and 1.7 GB; 64 sequences of 4 rows that may have 131072
+// 430 us with 252 MiB, 426 with 837.
+constexpr int64_t kRestBytes = int64_t(1) << 28;
 struct SharedPlan {
     int wide;
     bool compact;
@@ -950,7 +956,11 @@ struct SharedPlan {
         };
         // (A sequence has a row at least where it has work.)
         const int64_t working = std::min<int64_t>(b.sequences, b.total_rows), units = rest_tiles * working * c.kv_heads;
-        split(units, 256, p.max_rest, 256, 640, kBlock, rest_parts, rest_part);
+        // Parts of 640 only while their sums, which every row has for every part, fit kRestBytes.
+        const int64_t row_bytes = int64_t(query_heads) * (c.head_dim * 4 + 8);
+        const int64_t room = std::max<int64_t>(1, kRestBytes / std::max<int64_t>(1, b.total_rows * row_bytes));
+        const int64_t longest = std::max<int64_t>(640, (p.max_rest + room - 1) / room);
+        split(units, 256, p.max_rest, 256, longest, kBlock, rest_parts, rest_part);
         // The prefixes have as many of the places as their share of the work, and a third more, so that none of their
         // workgroups is the last one: 85 ns a position of theirs, 65 (E4M3 45) behind them, where half of the most are
         // taken for ragged ones' mean. (All places, as if there were nothing behind them: 4 times 24 sequences 120 us,

@@ -404,7 +404,11 @@ int qwen_gpu_op_paged_evict(const qwen_gpu_paged_cache* cache, const qwen_gpu_pa
  * too, by fewer workgroups. Sizes that come to 2^24 workgroups or more, or to
  * 2^24 rows, are refused. Weights are not tracked: batch->weights and
  * batch->positions must be NULL. The workspace (device memory, aligned to 16)
- * needs no zeroing and keeps nothing between calls. */
+ * needs no zeroing and keeps nothing between calls. A part of the positions
+ * takes 4 * head_dim + 8 bytes of it for each new row and query head; it holds
+ * one part of the prefixes and one behind them at least, more where few rows
+ * leave room on the GPU (tens of MiB), and behind the prefixes as long as all
+ * of theirs fit 256 MiB. */
 typedef struct qwen_gpu_paged_prefix {
     const int32_t* lengths;     /* [groups] */
     const int32_t* offsets;     /* [groups + 1]; NULL: one group of all sequences */

@@ -547,3 +547,16 @@ def test_offsets_past_the_rows(qpkg, poisoned, kind, below, total, rows, sequenc
                                           out[:total].reshape(total, -1, dim))
     assert (np.abs(got[:total].reshape(want.shape) - want) <= tolerance).all()
     assert (got[total:] == 7.5).all()
+
+
+@pytest.mark.parametrize('kind', ['f16', 'e4m3'])
+def test_rests_far_shorter_than_they_may_be(qpkg, poisoned, kind):
+    """A launch sized for rests of 131072 positions, whose parts the workspace bounds: one that has three of them, others of
+    a few positions."""
+    rng = np.random.default_rng(42)
+    prefix, kv, group, dim, rows, page = 100, 2, 16, 64, 4, 16
+    lengths = [prefix + 3000] + [prefix + rows + int(x) for x in rng.integers(0, 40, 63)]
+    cache, table = made(rng, kind, kv, dim, page, 'head', [0, 64], lengths, [prefix])
+    table = np.pad(table, ((0, 0), (0, 131072 // page)), constant_values=-1)
+    call, _ = attend(qpkg, cache, table, lengths, [prefix], kv * group, rows=rows, rng=rng, max_rest=131072)
+    assert 200 << 20 < call.workspace(kv * group).nbytes < 300 << 20

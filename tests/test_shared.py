@@ -80,6 +80,19 @@ def test_workspace(qpkg, sequences, rows, heads, max_length, max_rest, dim):
     assert need.value == (2 * sequences * rows * heads * 8 + 15) // 16 * 16 + 2 * sequences * rows * heads * dim * 4
 
 
+@pytest.mark.parametrize('sequences,rows,total,heads,max_rest', [
+    (16, 128, 2048, 32, 32768), (1, 8192, 8192, 16, 1 << 17), (64, 4, 256, 32, 131072), (4096, 1, 4096, 32, 131072),
+    (64, 4096, 4159, 16, 65536), (1, 1 << 16, 1 << 16, 16, 1 << 20), (3, 5, 0, 16, 1 << 24)])
+def test_workspace_of_long_rests(qpkg, sequences, rows, total, heads, max_rest):
+    """However long the rests may be, their parts' sums take 256 MiB, or one part's: a prefix of one part here."""
+    need, lib = ctypes.c_size_t(), qpkg.load_library()
+    b = untracked(qpkg, sequences=sequences, rows=rows, total_rows=total, offsets=AT, max_length=max_rest, table_stride=1 << 20)
+    status = lib.qwen_gpu_op_paged_shared_workspace(cache(qpkg), b, prefix(qpkg, max_rest=max_rest), heads, ctypes.byref(need))
+    assert status == 0, lib.qwen_gpu_last_error()
+    part = total * heads * (128 * 4 + 8)
+    assert need.value <= part + max(part, 1 << 28) + 16
+
+
 @pytest.mark.parametrize('kv,heads,batch_fields', [
     (256, 256, dict(sequences=4096, rows=256, total_rows=4096, offsets=AT)),  # workgroups behind the prefixes
     (1024, 1024, dict(sequences=1, rows=32, total_rows=(1 << 21) - 1, offsets=AT)),  # of the prefixes
