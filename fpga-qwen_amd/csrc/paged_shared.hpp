@@ -859,7 +859,8 @@ __global__ __launch_bounds__(kWaves * 64) void shared_join_kernel(PagedView v, S
     if (s < 0) return;
     int first, reads;
     const int n = v.new_rows(s, first);
-    if (row - first >= n) return;
+    // (first may be as low as -2^31, and above the row where offsets fall)
+    if (const int64_t rank = int64_t(row) - first; rank < 0 || rank >= n) return;
     const int g = groups.of(s), shared = a.parts_of(groups.prefix(g, reads), a.part, a.parts);
     const int count = shared + groups.rest_parts(v.length(s), n, groups.nominal(g));
     for (int piece = blockIdx.y; piece * kJoinItems < a.query_heads * (DIM / 4); piece += gridDim.y) {

@@ -560,3 +560,27 @@ def test_rests_far_shorter_than_they_may_be(qpkg, poisoned, kind):
     table = np.pad(table, ((0, 0), (0, 131072 // page)), constant_values=-1)
     call, _ = attend(qpkg, cache, table, lengths, [prefix], kv * group, rows=rows, rng=rng, max_rest=131072)
     assert 200 << 20 < call.workspace(kv * group).nbytes < 300 << 20
+
+
+def test_rows_of_no_sequence(qpkg, poisoned):
+    """Rows between a first sequence's, which lie as far below 0 as they can, and the next one's stay."""
+    rng, dim = np.random.default_rng(44), 64
+    lengths, offsets = [40, 50, 60], np.array([-2 ** 31, 4, 7, 10])
+    cache, table = made(rng, 'f16', 2, dim, 16, 'head', [0, 3], lengths, [30])
+    queries = rng.standard_normal((12, 4 * dim)).astype(np.float32)
+    out = np.full_like(queries, 7.5)
+    got = Shared(qpkg, cache, table, lengths, [30], rows=3, offsets=offsets, total=12)(queries, 4, 0.125, out)
+    want, tolerance, _, _ = ref.attention(cache, table, lengths, 3, offsets, queries.reshape(12, 4, dim), 0.125,
+                                          out.reshape(12, 4, dim))
+    assert (np.abs(got.reshape(want.shape) - want) <= tolerance).all()
+    assert (got[:4] == 7.5).all() and (got[10:] == 7.5).all()
+
+
+@pytest.mark.parametrize('kind', ['f16', 'bf16', 'e4m3'])
+def test_reads_nothing_that_nobody_wrote(qpkg, poisoned, kind):
+    """Ragged rows, many groups, launches of other sizes and what the device may hold, again, where every place of the
+    workspace that a call does not write is NaN."""
+    test_groups_and_ragged_rows(qpkg, kind, 2, 3, 128)
+    test_many_groups(qpkg, kind)
+    test_long_prefix(qpkg, kind)
+    test_bounds_what_the_device_holds(qpkg)
