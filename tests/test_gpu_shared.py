@@ -584,3 +584,27 @@ def test_reads_nothing_that_nobody_wrote(qpkg, poisoned, kind):
     test_many_groups(qpkg, kind)
     test_long_prefix(qpkg, kind)
     test_bounds_what_the_device_holds(qpkg)
+
+
+def test_calls_on_streams(qpkg):
+    """Three calls of other sizes on streams of their own, each with its workspace, all in flight at once, give what each
+    gives alone."""
+    hip, rng, calls = Hip(), np.random.default_rng(43), []
+    for kind, sequences, rows, heads in (('f16', 64, 1, 16), ('bf16', 9, 5, 8), ('e4m3', 2, 1, 8)):
+        prefix = 700
+        lengths = [prefix + rows + 30 * s for s in range(sequences)]
+        cache, table = made(rng, kind, 2, 128, 16, 'head', [0, sequences], lengths, [prefix])
+        call = Shared(qpkg, cache, table, lengths, [prefix], rows=rows)
+        queries = rng.standard_normal((sequences * rows, heads * 128)).astype(np.float32)
+        want = call(queries, heads, 0.1, np.zeros_like(queries))
+        stream = ctypes.c_void_p()
+        hip.hipStreamCreate(ctypes.byref(stream))
+        calls.append((call, stream, want, heads, call.workspace(heads), qpkg.DeviceBuffer.from_array(queries),
+                      qpkg.DeviceBuffer.from_array(np.zeros_like(queries))))
+    for _ in range(8):
+        for call, stream, want, heads, space, queries, out in calls:
+            call.enqueue(queries.ptr, heads * 128, heads, 0.1, out.ptr, heads * 128, space, stream)
+    for call, stream, want, heads, space, queries, out in calls:
+        hip.hipStreamSynchronize(stream)
+        assert np.array_equal(out.to_array(np.float32, want.size).view(np.uint32), want.reshape(-1).view(np.uint32))
+        hip.hipStreamDestroy(stream)

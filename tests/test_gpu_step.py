@@ -675,3 +675,48 @@ def test_rotate_the_most_rows(qpkg, rows):
     rest = got.copy()
     rest[live] = raw[live]
     assert np.array_equal(rest, raw)
+
+
+def test_reservations_on_streams(qpkg):
+    """Pages of two pools reserved on streams of their own, beside rotations and verifications, step after step."""
+    q, hip, rng = qpkg, Hip(), np.random.default_rng(26)
+    lib, n, streams, pools, want = q.load_library(), 300, [], [], []
+    for _ in range(2):
+        streams.append(ctypes.c_void_p())
+        hip.hipStreamCreate(ctypes.byref(streams[-1]))
+        given = state(rng, n, 4, 30, 2000, width=40)
+        steps = [rng.integers(-5, 6, n) for _ in range(6)]
+        on = {name: q.DeviceBuffer.from_array(np.asarray(x, np.int32)) for name, x in dict(
+            table=given['table'], held=given['held'], lengths=given['lengths'], count=[len(given['free'])],
+            stack=np.pad(given['free'], (0, given['pages'] - len(given['free'])), constant_values=-1),
+            offsets=np.zeros(n + 1), positions=np.zeros(3000)).items()}
+        changes = [q.DeviceBuffer.from_array(np.asarray(x, np.int32)) for x in steps]
+        pools.append((on, changes, q.PagedPool(on['table'].ptr, on['stack'].ptr, on['held'].ptr, on['count'].ptr, None,
+                                               given['pages'], 4, n, 40)))
+        for x in steps:
+            there = ref.reserve(**given, changes=x, room=3000)
+            given.update({name: there[name] for name in ('table', 'held', 'free', 'lengths')})
+        want.append(there)
+    draft = Drafts(q, **random_drafts(rng, 5, 4, 9000, ragged=True))
+    alone = draft()
+    turned = q.DeviceBuffer.from_array(rng.standard_normal((200, 384)).astype(np.float32))
+    place, turns = q.DeviceBuffer.from_array(np.full(200, 7, np.int32)), q.DeviceBuffer.from_array(np.full(32, 0.3))
+    for i in range(6):
+        for stream, (on, changes, pool) in zip(streams, pools):
+            growth = q.PagedGrowth(on['lengths'].ptr, None, changes[i].ptr, on['lengths'].ptr, None, on['held'].ptr,
+                                   on['count'].ptr, on['offsets'].ptr, None, on['positions'].ptr, None, 3000)
+            ok(q, lib.qwen_gpu_op_paged_reserve(pool, growth, stream))
+        draft.enqueue(streams[0])
+        heads = q.RotaryHeads(turned.ptr, turned.ptr, None, 384, 64, 384, 64, 6)
+        ok(q, lib.qwen_gpu_op_rotate(q.Rotary(turns.ptr, 64, 0, 64, 0, 1, 1e-6), heads, None, place.ptr, 200, streams[1]))
+    for stream in streams:
+        hip.hipStreamSynchronize(stream)
+    assert all(np.array_equal(a, b) for a, b in zip(draft.results(), alone))
+    for (on, _, _), there in zip(pools, want):
+        for name in ('held', 'lengths', 'offsets', 'positions'):
+            assert np.array_equal(on[name].to_array(np.int32, there[name].size), there[name]), name
+        assert np.array_equal(on['table'].to_array(np.int32, n * 40).reshape(n, 40), there['table'])
+        count = int(on['count'].to_array(np.int32, 1)[0])
+        assert np.array_equal(on['stack'].to_array(np.int32, on['stack'].nbytes // 4)[:count], there['free'])
+    for stream in streams:
+        hip.hipStreamDestroy(stream)
