@@ -27,6 +27,7 @@ void rotary_frequencies(int scaling, int dims, double base, double factor, doubl
                                                 std::isfinite(fast)),
             "A rotary ramp needs trained positions and 0 < slow < fast");
     if (scaling == QWEN_GPU_ROTARY_BASE) base *= std::pow(factor, double(dims) / (dims - 2));
+    require(std::isfinite(base), "The rotary base must be finite, scaled too");  // its last pair would not turn
     constexpr double kTurn = 6.283185307179586476925;
     for (int i = 0; i < dims / 2; ++i) {
         const double f = std::pow(base, -2.0 * i / dims);

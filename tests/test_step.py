@@ -101,6 +101,13 @@ def test_frequencies_refused(qpkg, message, call):
     refused(qpkg, message, qpkg.load_library().qwen_gpu_rotary_frequencies(*call, to, None))
 
 
+@pytest.mark.parametrize('dims,base,factor', [(4, 1e10, 1e150), (4, 1e300, 1e5), (512, 1e300, 1e9)])
+def test_scaled_bases_that_no_number_holds(qpkg, dims, base, factor):
+    """Their last pair would not turn at all, instead of by 1 / factor of its angle."""
+    to = (ctypes.c_double * 256)()
+    refused(qpkg, 'base must be finite', qpkg.load_library().qwen_gpu_rotary_frequencies(2, dims, base, factor, 0, 0, 0, to, None))
+
+
 def test_frequencies_need_room(qpkg):
     refused(qpkg, 'Null argument', qpkg.load_library().qwen_gpu_rotary_frequencies(0, 8, 1e4, 1, 0, 0, 0, None, None))
 
