@@ -502,12 +502,13 @@ struct WideSpace {
 // products run beside the other's exponentials.
 //
 // A prefix is read once from memory, but multiplied with every query row, in
-// two or three terms: 65000 E4M3 positions by 128 rows are 38 us of products
-// at the rate of a large matrix product (a score's two and a weight's three
-// terms), 11 of its bytes. The kernel takes 105, as LDS, exponentials and
-// products wait for each other at two waves a SIMD; tiles that every wave
-// reads for itself, without LDS, took 1020. Of 64 rows (TILES 1) 8192 positions
-// and what 64 users have behind them take 48 us, of 128 40; heads of 256 have
+// two or three terms: 65000 E4M3 positions of 8 heads by 128 rows are 30 us of
+// products at the rate of a large matrix product, 74 in terms (a score's two
+// and a weight's three), 26 of their bytes. The kernel takes 105 to 111, a call
+// of both kernels among others 103, as LDS, exponentials and products wait for
+// each other at two waves a SIMD; tiles that every wave reads for itself,
+// without LDS, took 1020. Of 64 rows (TILES 1) 8192 positions and what 64 users
+// have behind them took 48 us a call in a graph, of 128 40; heads of 256 have
 // registers for 64.
 template <int TYPE, int DIM, int TILES>
 __device__ __forceinline__ void shared_attend_wide(const PagedView& v, const SharedArgs& a, const SharedJob& job,

@@ -94,9 +94,9 @@ __device__ __forceinline__ double series(double z) {
 }
 
 // Weights of tokens. 2^z as 2^n * 2^(j / 64) * 2^r with the 64 powers in LDS
-// and |r| <= 1 / 128, where four terms of the series are 4e-14 off: the FP64
-// operations of a token bound the kernel, 13 of them here, 21 with the
-// series alone (260 rows of 151936 BF16 logits took 47 us with that).
+// and |r| <= 1 / 128, where four terms of the series are 4e-14 off: a token
+// takes 13 FP64 operations, and 21 with the series alone (260 rows of 151936
+// BF16 logits took 47 us with that).
 struct Powers {
     double at[64];
 
@@ -194,8 +194,13 @@ __device__ __forceinline__ int wave_min(int x) {
 // weights, each lane by itself until the end, with the next chunk's logits on
 // their way. The largest is wanted as a token where it wins. Memory bounds it
 // where rows are many and filtered (263 rows of 151936 BF16 logits, 80 MB, 21
-// us, 3.8 TB/s), FP64 where they are not, latency where they are few (two rows
-// 4.3 us, of which the launch has most; 40 FP32 rows, 24 MB, 10 us).
+// us, 3.8 TB/s), latency where they are few (two rows 4.6 us, of which the
+// launch has most; 40 FP32 rows, 24 MB, 10 us). Unfiltered, those 263 rows take
+// 45 us as BF16 and as FP32, twice the bytes, so memory does not: 27 vector
+// instructions a token, the 13 of FP64 among them, keep a SIMD busy for 67 of
+// the 82 thousand cycles that its CU has work, of 115 that the kernel takes
+// (starts and ends of five workgroups a CU are the rest); the table's reads
+// from LDS take 10.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void verify_parts_kernel(VerifyArgs a) {
     __shared__ Powers powers;

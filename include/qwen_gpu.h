@@ -398,23 +398,26 @@ int qwen_gpu_op_paged_evict(const qwen_gpu_paged_cache* cache, const qwen_gpu_pa
  * lengths[g] slots; those are read through the table of its first sequence
  * with new rows. The prefix is taken no longer than what each of the group's
  * sequences with new rows had cached before them, and a sequence of no group
- * has none, so
- * every row attends what qwen_gpu_op_paged_attention gives it. max_length
- * and max_rest size the launch: what a sequence has beyond them is attended
- * too, by fewer workgroups. Sizes that come to 2^24 workgroups or more, or to
- * 2^24 rows, are refused. Weights are not tracked: batch->weights and
- * batch->positions must be NULL. The workspace (device memory, aligned to 16)
- * needs no zeroing and keeps nothing between calls. A part of the positions
- * takes 4 * head_dim + 8 bytes of it for each new row and query head; it holds
- * one part of the prefixes and one behind them at least, more where few rows
- * leave room on the GPU (tens of MiB), and behind the prefixes as long as all
- * of theirs fit 256 MiB. */
+ * has none, so every row attends what qwen_gpu_op_paged_attention gives it.
+ * max_length and max_rest size the launch and share the GPU out between the
+ * prefixes and what is behind them; what a sequence has beyond them is attended
+ * too, by fewer workgroups. Give max_rest what sequences have as a rule, not
+ * the most that they may reach, which would leave few workgroups to the prefix:
+ * 64 sequences behind 8192 positions with up to 500 more take 42 us with a
+ * max_rest of 500, 49 with 128, 408 with 32768. Sizes that come to 2^24
+ * workgroups or more, or to 2^24 rows, are refused. Weights are not tracked:
+ * batch->weights and batch->positions must be NULL. The workspace (device
+ * memory, aligned to 16) needs no zeroing and keeps nothing between calls. A
+ * part of the positions takes 4 * head_dim + 8 bytes of it for each new row and
+ * query head; it holds one part of the prefixes and one behind them at least,
+ * more where few rows leave room on the GPU (tens of MiB), and behind the
+ * prefixes as long as all of theirs fit 256 MiB. */
 typedef struct qwen_gpu_paged_prefix {
     const int32_t* lengths;     /* [groups] */
     const int32_t* offsets;     /* [groups + 1]; NULL: one group of all sequences */
     int groups;                 /* 1..sequences; 1 where offsets is NULL */
     int max_length;             /* 0..batch->max_length: most positions of a prefix */
-    int max_rest;               /* 1..batch->max_length: most positions of a sequence behind its prefix */
+    int max_rest;               /* 1..batch->max_length: positions of a sequence behind its prefix, as a rule */
 } qwen_gpu_paged_prefix;
 
 int qwen_gpu_op_paged_shared_workspace(const qwen_gpu_paged_cache* cache, const qwen_gpu_paged_batch* batch,
@@ -524,7 +527,10 @@ typedef struct qwen_gpu_rotary_heads {
  *         positions, f_i / factor where it makes `slow` or fewer, in between
  *         their mean weighted by where the turns lie between the two;
  *         magnitude 0.1 ln(factor) + 1.
- * The magnitude of the others is 1. */
+ * The magnitude of the others is 1, and a base that grows past all numbers is
+ * refused. RAMP goes by turns. Checkpoints scaled by a ramp over the pairs'
+ * indices, between two borders that are rounded to whole pairs, or run with
+ * another magnitude, have other frequencies: give qwen_gpu_op_rotate those. */
 int qwen_gpu_rotary_frequencies(int scaling, int dims, double base, double factor, double trained, double slow,
                                 double fast, double* frequencies, float* magnitude);
 /* Every head of every row, normed (x / sqrt(mean x^2 + epsilon) * norm) and
