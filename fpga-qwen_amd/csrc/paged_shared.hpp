@@ -919,13 +919,14 @@ __global__ __launch_bounds__(kWaves * 64) void shared_join_kernel(PagedView v, S
     }
 }
 
-// Sizes of a call: how its work is split, and what its workspace holds.
 // The sums behind the prefixes take 256 MiB at most, which the last level of
 // the caches holds, or one part's. 2048 new rows of 32 heads of 128 that may
 // have 32768 positions behind their prefix take 827 us with 260 MiB in all,
 // 1457 with parts of 640 and 1.7 GB; 64 sequences of 4 rows that may have 131072
 // 430 us with 252 MiB, 426 with 837.
 constexpr int64_t kRestBytes = int64_t(1) << 28;
+
+// Sizes of a call: how its work is split, and what its workspace holds.
 struct SharedPlan {
     int wide;
     bool compact;
